@@ -436,6 +436,33 @@ int mg_delta_step_heads(int dtype, const void* H_in, const float* P, const float
                         void* H_out, float* y, int64_t B, int H, int nh, int dk, int dv,
                         mg_stream_t stream);
 
+/* ---- the norms around a block, with its gate and residual scale --------------------
+ * No reference kernels: the reference's blocks run torch's LayerNorm and an addition
+ * (src/mingru/min_gru.py:3819-3872).  Per row of D <= 8192 elements:
+ *   p = post(h); u = p act(gate); r = x + scale u (u without x); y = pre(r)
+ * post, pre: 0 none, 1 LayerNorm, 2 RMS norm, with their weights and biases (D), NULL for 1
+ * and 0; act: 0 no gate, 1 sigmoid, 2 silu; scale (D), or scale_const where it is NULL.
+ * dtype (0 fp32, 1 bf16) is the rows' type, pdtype (0, or dtype) the row vectors'.  ld*:
+ * elements between rows of an input, at least D; outputs are dense.  stats (rows, 4) fp32,
+ * 16-byte aligned, is what the backward reads of the forward; NULL if there is none.  r may
+ * be NULL if pre is not 0.
+ * Backward: any output may be NULL, and dr or dy where that gradient is zero; the workspace
+ * is needed for the row vectors' gradients alone. */
+size_t mg_residual_norm_workspace_bytes(int64_t rows, int64_t D);
+int mg_residual_norm_fwd(int dtype, int pdtype, int post, int act, int pre, const void* h,
+                         int64_t ldh, const void* x, int64_t ldx, const void* gate, int64_t ldg,
+                         const void* scale, float scale_const, const void* post_w,
+                         const void* post_b, const void* pre_w, const void* pre_b, void* r,
+                         void* y, float* stats, int64_t rows, int64_t D, float eps,
+                         mg_stream_t stream);
+int mg_residual_norm_bwd(int dtype, int pdtype, int post, int act, int pre, const void* h,
+                         int64_t ldh, const void* x, int64_t ldx, const void* gate, int64_t ldg,
+                         const void* scale, float scale_const, const void* post_w,
+                         const void* post_b, const void* pre_w, const float* stats,
+                         const void* dr, int64_t lddr, const void* dy, int64_t lddy, void* dh,
+                         void* dx, void* dgate, void* dscale, void* dpost_w, void* dpost_b,
+                         void* dpre_w, void* dpre_b, int64_t rows, int64_t D, float eps, void* ws,
+                         size_t ws_bytes, mg_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -5,6 +5,9 @@ Public surface (same names and signatures as chris-santiago/minGRU,
 ``MinGRUStack`` and the scan primitives ``parallel_scan_log``, ``linear_scan``,
 ``matrix_scan``, ``matrix_affine_scan``.
 
+Beside them stand the operators of :mod:`mingru_amd.sequence_ops`, which the reference
+does not have.
+
 The GPU backend, :mod:`mingru_amd.hip_scans`, is never imported by
 ``import mingru_amd``: its public names resolve lazily (PEP 562) on first
 access, and the ``MINGRU_SCAN`` seam imports it only for GPU tensors.
@@ -12,6 +15,8 @@ access, and the ``MINGRU_SCAN`` seam imports it only for GPU tensors.
 
 from .min_gru import *  # noqa: F401,F403
 from .min_gru import __all__ as _min_gru_all
+from .sequence_ops import *  # noqa: F401,F403
+from .sequence_ops import __all__ as _sequence_all
 
 __version__ = "0.2.1+mi355x"
 
@@ -23,7 +28,7 @@ _BACKEND_EXPORTS = (
     "delta_scan_impl",
 )
 
-__all__ = [*_min_gru_all, "__version__"]
+__all__ = [*_min_gru_all, *_sequence_all, "__version__"]
 
 
 def __getattr__(name: str) -> object:

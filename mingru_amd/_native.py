@@ -128,6 +128,15 @@ _SIGNATURES = {
     "mg_delta_gated_bwd": (
         _I32, [_P] * 14 + [_I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _P, _SZ, _P],
     ),
+    "mg_residual_norm_workspace_bytes": (_SZ, [_I64, _I64]),
+    "mg_residual_norm_fwd": (
+        _I32, [_I32] * 5 + [_P, _I64] * 3 + [_P, _F32] + [_P] * 7 + [_I64, _I64, _F32, _P],
+    ),
+    "mg_residual_norm_bwd": (
+        _I32,
+        [_I32] * 5 + [_P, _I64] * 3 + [_P, _F32] + [_P] * 4 + [_P, _I64] * 2 + [_P] * 8
+        + [_I64, _I64, _F32, _P, _SZ, _P],
+    ),
 }
 
 _lib = None

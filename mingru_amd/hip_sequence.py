@@ -1,0 +1,137 @@
+"""HIP backend of :mod:`mingru_amd.sequence_ops`.
+
+Same manners as :mod:`mingru_amd.hip_scans`: ``*_impl`` functions take the public
+function's checked arguments, run on torch's current stream with outputs and workspaces
+from torch's caching allocator, differentiate through ``torch.autograd.Function`` wrappers
+(no double backward), and raise ``ScanFallback`` for a call they decline.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .hip_scans import ScanFallback, _call, _funnel, _ptr, _size, _stream, _workspace
+
+__all__ = ["residual_norm_impl"]
+
+_DTYPE_TAG = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _half_to_float(*ts):
+    """fp16 inputs run the fp32 kernels on upcast copies; float64 declines."""
+    out = []
+    for t in ts:
+        if t is not None and t.dtype not in _DTYPE_TAG:
+            if t.dtype != torch.float16:
+                raise ScanFallback(f"the kernels compute in fp32; {t.dtype} stays on the eager path")
+            t = t.float()
+        out.append(t)
+    return out
+
+
+# ---------------------------------------------------------------------------
+# residual_norm
+# ---------------------------------------------------------------------------
+
+_NORM_MAX_D = 8192
+_NORM_TAG = {"none": 0, "layer": 1, "rms": 2}
+_GATE_TAG = {"none": 0, "sigmoid": 1, "silu": 2}
+
+
+def _rows(t, D):
+    """``t`` as rows of ``D`` consecutive elements and the elements between them."""
+    if t is None:
+        return None, 0
+    if t.stride(-1) != 1 and D > 1:
+        t = t.contiguous()
+    t = t.reshape(-1, D)
+    if t.shape[0] == 1:
+        return t, D
+    if t.stride(0) < D:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+class _ResidualNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, x, gate, scale, post_w, post_b, pre_w, pre_b, kinds, number, eps):
+        ctx.set_materialize_grads(False)
+        D = h.shape[-1]
+        h2, ldh = _rows(h, D)
+        x2, ldx = _rows(x, D)
+        g2, ldg = _rows(gate, D)
+        vectors = [t if t is None else t.contiguous()
+                   for t in (scale, post_w, post_b, pre_w, pre_b)]
+        first = next((t for t in vectors if t is not None), h2)
+        rows = h2.shape[0]
+        r = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+        y = torch.empty_like(r) if kinds[2] else None
+        stats = None
+        if any(ctx.needs_input_grad) and (kinds[0] or kinds[2]):
+            stats = torch.empty(rows, 4, dtype=torch.float32, device=h.device)
+        tags = (_DTYPE_TAG[h.dtype], _DTYPE_TAG[first.dtype], *kinds)
+        scale, post_w, post_b, pre_w, pre_b = vectors
+        _call("mg_residual_norm_fwd", *tags, _ptr(h2), ldh, _ptr(x2), ldx, _ptr(g2), ldg,
+              _ptr(scale), number, _ptr(post_w), _ptr(post_b), _ptr(pre_w), _ptr(pre_b), _ptr(r),
+              _ptr(y), _ptr(stats), rows, D, eps, _stream(h))
+        ctx.save_for_backward(h, x, gate, stats, *vectors)
+        ctx.tags, ctx.number, ctx.eps = tags, number, eps
+        return (r, y) if kinds[2] else r
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dr, dy=None):
+        h, x, gate, stats, scale, post_w, post_b, pre_w, pre_b = ctx.saved_tensors
+        D, dev = h.shape[-1], h.device
+        if dr is None and dy is None:
+            return (None,) * 11
+        need = ctx.needs_input_grad
+        post, act, _ = ctx.tags[2:]
+        h2, ldh = _rows(h, D)
+        x2, ldx = _rows(x, D)
+        g2, ldg = _rows(gate, D)
+        dr2, lddr = _rows(dr, D)
+        dy2, lddy = _rows(dy, D)
+        rows = h2.shape[0]
+
+        def like(i):
+            return torch.empty(h.shape, dtype=h.dtype, device=dev) if need[i] else None
+
+        # The block's part of a plain sum has the stream's own gradient.
+        same = bool(need[1]) and not (post or act) and scale is None and ctx.number == 1.0
+        dx, dgate = like(1), like(2)
+        dh = None if same else like(0)
+        vectors = [torch.empty(D, dtype=t.dtype, device=dev) if need[3 + i] else None
+                   for i, t in enumerate((scale, post_w, post_b, pre_w, pre_b))]
+        ws = None
+        if any(v is not None for v in vectors):
+            ws = _workspace(_size("mg_residual_norm_workspace_bytes", rows, D), dev)
+        _call("mg_residual_norm_bwd", *ctx.tags, _ptr(h2), ldh, _ptr(x2), ldx, _ptr(g2), ldg,
+              _ptr(scale), ctx.number, _ptr(post_w), _ptr(post_b), _ptr(pre_w), _ptr(stats),
+              _ptr(dr2), lddr, _ptr(dy2), lddy, _ptr(dh), _ptr(dx), _ptr(dgate),
+              *[_ptr(v) for v in vectors], rows, D, ctx.eps, _ptr(ws),
+              0 if ws is None else ws.numel(),
+              _stream(h))
+        return (dx if same and need[0] else dh, dx, dgate, *vectors, None, None, None)
+
+
+def residual_norm_impl(h, x, gate, scale, post_w, post_b, pre_w, pre_b, post, act, pre, number,
+                       eps):
+    """``residual_norm`` on checked arguments (``number``: the scale where ``scale`` is None)."""
+    if h.shape[-1] > _NORM_MAX_D:
+        raise ScanFallback(f"residual_norm kernels hold rows of at most {_NORM_MAX_D} elements "
+                           f"(got {h.shape[-1]})")
+    dtype = h.dtype if x is None else torch.promote_types(h.dtype, x.dtype)
+    h, x, gate, *vectors = _half_to_float(h, x, gate, scale, post_w, post_b, pre_w, pre_b)
+    if any(t is not None and t.dtype != h.dtype for t in (x, gate)):
+        h, x, gate = (t if t is None else t.float() for t in (h, x, gate))
+    if any(t is not None and t.dtype != torch.bfloat16 for t in vectors) or \
+            h.dtype == torch.float32:
+        vectors = [t if t is None else t.float() for t in vectors]
+    kinds = (_NORM_TAG[post], _GATE_TAG[act], _NORM_TAG[pre])
+    out = _funnel("residual_norm", _ResidualNormFn.apply, h, x, gate, *vectors, kinds, number,
+                  float(eps))
+    if h.dtype == dtype:
+        return out
+    return tuple(t.to(dtype) for t in out) if kinds[2] else out.to(dtype)
