@@ -464,6 +464,39 @@ int mg_residual_norm_bwd(int dtype, int pdtype, int post, int act, int pre, cons
                          void* dpre_w, void* dpre_b, int64_t rows, int64_t D, float eps, void* ws,
                          size_t ws_bytes, mg_stream_t stream);
 
+/* ---- linear attention with a decay for each head -----------------------------------
+ * No reference kernels (the reference's matrix-state mixer is the delta rule).
+ *   S_t = exp(g_t) S_{t-1} + k_t v_t^T;  o_t = scale S_t^T q_t
+ * q, k (B, T, Hk, dk), v and o (B, T, H, dv) in dtype (0 fp32, 1 bf16), Hk dividing H; g (log
+ * decay, (B, T, H)) and the states (B, H, dk, dv) fp32; 1 <= dk, dv <= 128.  A g whose factor
+ * is below the smallest normal float starts the state over.  strides: a host array of element
+ * strides (batch, token, head) of q, k, v, g and, for the backward, the output's gradient;
+ * their last dimension is dense.  lengths (B) or NULL: tokens of right-padded sequences.  h0
+ * NULL for 0.
+ * state: what the forward leaves for the backward (states between the segments of a
+ * sequence); needed by the forward in any case.  Backward: dhT NULL for 0, dh0 may be NULL;
+ * dg is (B, T, H) dense whatever g's strides; other gradients are dense in their inputs'
+ * shapes. */
+size_t mg_linear_attention_state_bytes(int dtype, int64_t B, int64_t T, int H, int Hk, int dk,
+                                       int dv);
+size_t mg_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int H, int Hk, int dk,
+                                           int dv);
+int mg_linear_attention_fwd(int dtype, const void* q, const void* k, const void* v, const float* g,
+                            const int64_t* strides, const int* lengths, const float* h0, void* o,
+                            float* hT, void* state, size_t state_bytes, int64_t B, int64_t T,
+                            int H, int Hk, int dk, int dv, float scale, mg_stream_t stream);
+int mg_linear_attention_bwd(int dtype, const void* q, const void* k, const void* v, const float* g,
+                            const void* dout, const int64_t* strides, const int* lengths,
+                            const float* h0, const float* hT, const void* state, const float* dhT,
+                            void* dq, void* dk_, void* dv_, float* dg, float* dh0, int64_t B,
+                            int64_t T, int H, int Hk, int dk, int dv, float scale, void* ws,
+                            size_t ws_bytes, mg_stream_t stream);
+/* One token: strides (batch, head) of q, k, v, g; h_out may be h.  Any dk, dv. */
+int mg_linear_attention_step(int dtype, const void* q, const void* k, const void* v, const float* g,
+                             const int64_t* strides, const float* h, void* o, float* h_out,
+                             int64_t B, int H, int Hk, int dk, int dv, float scale,
+                             mg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

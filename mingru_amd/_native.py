@@ -29,6 +29,7 @@ _I64 = ctypes.c_int64
 _I32 = ctypes.c_int
 _F32 = ctypes.c_float
 _SZ = ctypes.c_size_t
+_PI64 = ctypes.POINTER(ctypes.c_int64)
 
 _SIGNATURES = {
     "mg_linear_scan_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
@@ -127,6 +128,20 @@ _SIGNATURES = {
     ),
     "mg_delta_gated_bwd": (
         _I32, [_P] * 14 + [_I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _P, _SZ, _P],
+    ),
+    "mg_linear_attention_state_bytes": (_SZ, [_I32, _I64, _I64] + [_I32] * 4),
+    "mg_linear_attention_workspace_bytes": (_SZ, [_I32, _I64, _I64] + [_I32] * 4),
+    "mg_linear_attention_fwd": (
+        _I32,
+        [_I32] + [_P] * 4 + [_PI64] + [_P] * 5 + [_SZ, _I64, _I64] + [_I32] * 4 + [_F32, _P],
+    ),
+    "mg_linear_attention_bwd": (
+        _I32,
+        [_I32] + [_P] * 5 + [_PI64] + [_P] * 10 + [_I64, _I64] + [_I32] * 4
+        + [_F32, _P, _SZ, _P],
+    ),
+    "mg_linear_attention_step": (
+        _I32, [_I32] + [_P] * 4 + [_PI64] + [_P] * 3 + [_I64] + [_I32] * 4 + [_F32, _P],
     ),
     "mg_residual_norm_workspace_bytes": (_SZ, [_I64, _I64]),
     "mg_residual_norm_fwd": (

@@ -8,12 +8,23 @@ from torch's caching allocator, differentiate through ``torch.autograd.Function`
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 from torch.autograd.function import once_differentiable
 
-from .hip_scans import ScanFallback, _call, _funnel, _ptr, _size, _stream, _workspace
+from .hip_scans import (
+    ScanFallback,
+    _call,
+    _funnel,
+    _ptr,
+    _size,
+    _stream,
+    _workspace,
+    column_sums,
+)
 
-__all__ = ["residual_norm_impl"]
+__all__ = ["linear_attention_impl", "linear_attention_step_impl", "residual_norm_impl"]
 
 _DTYPE_TAG = {torch.float32: 0, torch.bfloat16: 1}
 
@@ -135,3 +146,100 @@ def residual_norm_impl(h, x, gate, scale, post_w, post_b, pre_w, pre_b, post, ac
     if h.dtype == dtype:
         return out
     return tuple(t.to(dtype) for t in out) if kinds[2] else out.to(dtype)
+
+
+# ---------------------------------------------------------------------------
+# linear_attention
+# ---------------------------------------------------------------------------
+
+_ATTENTION_MAX_D = 128
+
+
+def _last_dense(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _decay_strides(g, n):
+    """Strides of ``g`` over ``n`` leading dimensions and the heads; a decay for each head has none."""
+    return (0,) * n + (g.stride(0),) if g.dim() == 1 else g.stride()
+
+
+def _array(values):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+class _LinearAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, h0, lengths, scale):
+        ctx.set_materialize_grads(False)
+        q, k, v = (_last_dense(t) for t in (q, k, v))
+        (B, T, Hk, dk), (H, dv) = q.shape, v.shape[2:]
+        tag, dev = _DTYPE_TAG[q.dtype], q.device
+        size = (tag, B, T, H, Hk, dk, dv)
+        o = torch.empty(B, T, H, dv, dtype=q.dtype, device=dev)
+        h = torch.empty(B, H, dk, dv, dtype=torch.float32, device=dev)
+        state = _workspace(_size("mg_linear_attention_state_bytes", *size), dev)
+        strides = (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_decay_strides(g, 2))
+        _call("mg_linear_attention_fwd", tag, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _array(strides),
+              _ptr(lengths), _ptr(h0), _ptr(o), _ptr(h), _ptr(state), state.numel(), B, T, H, Hk,
+              dk, dv, scale, _stream(q))
+        if any(ctx.needs_input_grad):
+            ctx.save_for_backward(q, k, v, g, h0, lengths, h, state)
+            ctx.size, ctx.strides, ctx.scale = size, strides, scale
+        return o, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do, dh):
+        if do is None and dh is None:
+            return (None,) * 7
+        q, k, v, g, h0, lengths, h, state = ctx.saved_tensors
+        tag, B, T, H, Hk, dk, dv = ctx.size
+        dev = q.device
+        if do is None:
+            do = torch.zeros(B, T, H, dv, dtype=q.dtype, device=dev)
+        do = _last_dense(do)
+        if dh is not None:
+            dh = dh.contiguous()
+        dq, dk_, dv_ = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        dg = torch.empty(B, T, H, dtype=torch.float32, device=dev)
+        dh0 = torch.empty_like(h) if ctx.needs_input_grad[4] else None
+        ws = _workspace(_size("mg_linear_attention_workspace_bytes", *ctx.size), dev)
+        _call("mg_linear_attention_bwd", tag, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(do),
+              _array((*ctx.strides, *do.stride()[:3])), _ptr(lengths), _ptr(h0), _ptr(h),
+              _ptr(state), _ptr(dh), _ptr(dq), _ptr(dk_), _ptr(dv_), _ptr(dg), _ptr(dh0), B, T, H,
+              Hk, dk, dv, ctx.scale, _ptr(ws), ws.numel(), _stream(q))
+        if g.dim() == 1 and ctx.needs_input_grad[3]:
+            dg = column_sums(dg.view(B * T, H))
+        return dq, dk_, dv_, dg, dh0, None, None
+
+
+def linear_attention_impl(q, k, v, g, h0, lengths, scale):
+    """``linear_attention`` on checked arguments of one type."""
+    if max(q.shape[-1], v.shape[-1]) > _ATTENTION_MAX_D:
+        raise ScanFallback(f"linear_attention kernels take head sizes up to {_ATTENTION_MAX_D} "
+                           f"(got {q.shape[-1]} and {v.shape[-1]})")
+    dtype = q.dtype
+    q, k, v, g, h0 = _half_to_float(q, k, v, g, h0)
+    if h0 is not None:
+        h0 = h0.contiguous()
+    if lengths is not None:
+        lengths = lengths.to(torch.int32).contiguous()
+    o, h = _funnel("linear_attention", _LinearAttentionFn.apply, q, k, v, g, h0, lengths, scale)
+    return o.to(dtype), h
+
+
+def linear_attention_step_impl(q, k, v, g, h, scale):
+    """``linear_attention_step`` on checked arguments of one type."""
+    dtype = q.dtype
+    q, k, v, g, h = _half_to_float(q, k, v, g, h)
+    q, k, v = (_last_dense(t) for t in (q, k, v))
+    h = h.contiguous()
+    (B, Hk, dk), (H, dv) = q.shape, v.shape[1:]
+    o = torch.empty(B, H, dv, dtype=q.dtype, device=q.device)
+    h_out = torch.empty_like(h)
+    strides = (*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *_decay_strides(g, 1))
+    _funnel("linear_attention_step", _call, "mg_linear_attention_step", _DTYPE_TAG[q.dtype],
+            _ptr(q), _ptr(k), _ptr(v), _ptr(g), _array(strides), _ptr(h), _ptr(o), _ptr(h_out), B,
+            H, Hk, dk, dv, scale, _stream(q))
+    return o if o.dtype == dtype else o.to(dtype), h_out

@@ -17,7 +17,7 @@ import torch
 
 from .min_gru import _resolve_native_dispatch, _resolve_scan_mode
 
-__all__ = ["residual_norm"]
+__all__ = ["linear_attention", "linear_attention_step", "residual_norm"]
 
 _warned: set = set()
 
@@ -153,3 +153,156 @@ def residual_norm(h, x=None, *, post="none", post_weight=None, post_bias=None, g
     if pre == "none":
         return u.to(dtype)
     return u.to(dtype), _eager_one_norm(u, pre, pre_weight, pre_bias, eps).to(dtype)
+
+
+# ---------------------------------------------------------------------------
+# linear_attention
+# ---------------------------------------------------------------------------
+
+_EAGER_CHUNK = 64
+
+
+def _over(g: torch.Tensor) -> torch.Tensor:
+    """Steps whose factor is below the smallest normal float start over."""
+    return g.double() * 1.4426950408889634 < -126.0
+
+
+def _spans(total, count, lower):
+    """``exp`` of the sums between two tokens, 0 where a step in between starts over."""
+    diff = total[..., :, None] - total[..., None, :]
+    keep = lower & (count[..., :, None] == count[..., None, :])
+    return torch.exp(torch.where(keep, diff, torch.full_like(diff, -torch.inf)))
+
+
+def _eager_linear_attention(q, k, v, g, h, lengths, scale):
+    """Heads repeated, every input in the computing type; one chunk after another."""
+    B, T, H, _ = q.shape
+    if lengths is not None:
+        live = torch.arange(T, device=q.device) < lengths[:, None].to(q.device)
+        q, k, v = (torch.where(live[..., None, None], t, torch.zeros_like(t)) for t in (q, k, v))
+        g = torch.where(live[..., None], g, torch.zeros_like(g))
+    q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+    g = g.transpose(1, 2)
+    out = []
+    for at in range(0, T, _EAGER_CHUNK):
+        qc, kc, vc, gc = (t[:, :, at : at + _EAGER_CHUNK] for t in (q, k, v, g))
+        over = _over(gc)
+        count = over.cumsum(-1)
+        total = torch.where(over, torch.zeros_like(gc), gc).double().cumsum(-1)
+        lower = torch.ones(gc.shape[-1], gc.shape[-1], dtype=torch.bool, device=q.device).tril()
+        D = _spans(total, count, lower).to(q.dtype)
+        carried = torch.where(count == 0, total.exp(), torch.zeros_like(total)).to(q.dtype)
+        o = carried[..., None] * (qc @ h) + ((qc @ kc.transpose(-1, -2)) * D) @ vc
+        out.append(scale * o)
+        h = carried[..., -1, None, None] * h + (kc * D[..., -1, :, None]).transpose(-1, -2) @ vc
+    return torch.cat(out, 2).transpose(1, 2), h
+
+
+def _attention_checks(what, q, k, v, log_decay, h, lead):
+    """Shared argument checks; ``lead``: the dimensions before the heads."""
+    _check_floats(what, q=q, k=k, v=v, log_decay=log_decay, h=h)
+    n = len(lead)
+    if q.dim() != n + 2 or k.shape != q.shape or v.dim() != n + 2 or v.shape[:n] != q.shape[:n]:
+        raise ValueError(
+            f"{what}: q and k are {(*lead, 'Hk', 'dk')}, v is {(*lead, 'H', 'dv')} (got "
+            f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)})")
+    Hk, dk = q.shape[n:]
+    H, dv = v.shape[n:]
+    if Hk < 1 or H < 1 or H % Hk or dk < 1 or dv < 1:
+        raise ValueError(f"{what}: the {H} heads of v are not a multiple of the {Hk} of q and k, "
+                         "or a size is 0")
+    if log_decay.shape != (*q.shape[:n], H) and log_decay.shape != (H,):
+        raise ValueError(f"{what}: log_decay is {(*lead, 'H')} or (H,) (got "
+                         f"{tuple(log_decay.shape)})")
+    if h is not None and h.shape != (q.shape[0], H, dk, dv):
+        raise ValueError(f"{what}: the state is (B, H, dk, dv) = {(q.shape[0], H, dk, dv)} (got "
+                         f"{tuple(h.shape)})")
+
+
+def _attention_types(q, k, v, log_decay, h):
+    """Inputs in one type, decays and state in 32 bits (64 where an input has them)."""
+    dtype = torch.promote_types(torch.promote_types(q.dtype, k.dtype), v.dtype)
+    wide = torch.float64 if torch.float64 in (dtype, log_decay.dtype) else torch.float32
+    if wide == torch.float64:
+        dtype = wide
+    return (q.to(dtype), k.to(dtype), v.to(dtype), log_decay.to(wide),
+            None if h is None else h.to(wide))
+
+
+def linear_attention(q, k, v, log_decay, h_0=None, lengths=None, scale=None):
+    """Attention through a state that decays: a prompt's or a training batch's whole pass.
+
+    ``S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T`` and ``o_t = scale * S_t^T q_t`` for each
+    sequence and head.
+
+    Parameters
+    ----------
+    q, k : (B, T, Hk, dk)
+    v : (B, T, H, dv)
+        ``Hk`` divides ``H``; each query and key head serves ``H / Hk`` heads in a row.
+    log_decay : (B, T, H), or (H) for one decay a head
+        At most 0.  ``-inf``, and any value whose factor is below the smallest normal float,
+        starts a new document: nothing of the state before is seen after it.
+    h_0 : (B, H, dk, dv), optional
+        The state to start from, 0 by default.
+    lengths : (B) integers, optional
+        Tokens of right-padded sequences.  The rest is not read; its outputs and gradients are
+        0, and the final state is the one after a sequence's last token.
+    scale : float, optional
+        ``dk ** -0.5`` by default.
+
+    Returns
+    -------
+    ``o`` (B, T, H, dv) in the inputs' type and the final state (B, H, dk, dv) in 32 bits (64
+    for float64 inputs).  Differentiable in every floating input.
+    """
+    what = "linear_attention"
+    _attention_checks(what, q, k, v, log_decay, h_0, ("B", "T"))
+    if lengths is not None:
+        if not torch.is_tensor(lengths) or lengths.dtype.is_floating_point or \
+                lengths.dtype == torch.bool:
+            raise TypeError(f"{what}: lengths must be a tensor of integers")
+        if lengths.shape != q.shape[:1] or lengths.device != q.device:
+            raise ValueError(f"{what}: lengths is (B,) on the inputs' device (got "
+                             f"{tuple(lengths.shape)} on {lengths.device})")
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    q, k, v, log_decay, h_0 = _attention_types(q, k, v, log_decay, h_0)
+    if q.numel() and v.numel():
+        out = _dispatch(what, q.is_cuda, lambda backend: backend.linear_attention_impl(
+            q, k, v, log_decay, h_0, lengths, scale))
+        if out is not None:
+            return out
+    (B, T, Hk, dk), (H, dv) = q.shape, v.shape[2:]
+    wide = log_decay.dtype
+    h = q.new_zeros(B, H, dk, dv, dtype=wide) if h_0 is None else h_0
+    if T == 0 or B == 0:
+        return q.new_zeros(B, T, H, dv), h.clone()
+    rep = H // Hk
+    o, h = _eager_linear_attention(
+        q.to(wide).repeat_interleave(rep, 2), k.to(wide).repeat_interleave(rep, 2), v.to(wide),
+        log_decay.expand(B, T, H), h, lengths, scale)
+    return o.to(q.dtype), h
+
+
+@torch.no_grad()
+def linear_attention_step(q_t, k_t, v_t, log_decay_t, h_prev=None, scale=None):
+    """One token of :func:`linear_attention`: ``q_t``, ``k_t`` (B, Hk, dk), ``v_t`` (B, H, dv),
+    ``log_decay_t`` (B, H) or (H), ``h_prev`` (B, H, dk, dv).  Returns ``o_t`` (B, H, dv) and the
+    new state; no gradients."""
+    what = "linear_attention_step"
+    _attention_checks(what, q_t, k_t, v_t, log_decay_t, h_prev, ("B",))
+    scale = q_t.shape[-1] ** -0.5 if scale is None else float(scale)
+    q, k, v, g, h = _attention_types(q_t, k_t, v_t, log_decay_t, h_prev)
+    (B, Hk, dk), (H, dv) = q.shape, v.shape[1:]
+    if h is None:
+        h = torch.zeros(B, H, dk, dv, dtype=g.dtype, device=q.device)
+    if B:
+        out = _dispatch(what, q.is_cuda, lambda backend: backend.linear_attention_step_impl(
+            q, k, v, g, h, scale))
+        if out is not None:
+            return out
+    rep = H // Hk
+    kw, qw = (t.to(g.dtype).repeat_interleave(rep, 1) for t in (k, q))
+    a = torch.where(_over(g), torch.zeros_like(g), g.exp()).expand(B, H)
+    h = a[..., None, None] * h + kw[..., None] * v.to(g.dtype)[..., None, :]
+    return (scale * (qw[..., None, :] @ h)[..., 0, :]).to(q.dtype), h
