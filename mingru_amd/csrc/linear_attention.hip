@@ -37,7 +37,8 @@
 // the slow one a bf16 fragment comes from two ds_read_b64_tr_b16.  Rounding, bf16: inputs are
 // exact.  What only feeds bf16 outputs (the C x C matrices, the state in o and dv) is rounded
 // to bf16 once; what feeds fp32 outputs (decayed keys and queries into the states, the states
-// into the gradient of g) is held as hi + lo, 16 significant bits, at twice the products.
+// into the gradient of g) is split into three bf16 planes, 24 significant bits, at three times
+// the products: with two planes the states were 2.4e-6 off and the gradient of g 7e-6.
 //
 // Bound: LDS reads of operand fragments, then memory.
 #include "mg_common.h"
@@ -71,29 +72,53 @@ struct LaArgs {
   float* decay;         // (BH, segs - 1)
   void *out, *out2;     // o; dq; dk and dv
   float *part;          // (B, T, H, dk) fp32 in place of out where heads share it
-  float* e;             // (BH, T)
+  float* e;             // (BH, T): what the queries (keys) add to the gradient of G
 };
 
 // ---- operands ------------------------------------------------------------------------
+// A matrix in LDS has rows of D elements without padding; the 16-byte chunk c of row r lies
+// at chunk c ^ swz(r).  swz spreads both kinds of fragment reads over all banks: one chunk of
+// 8 or 16 consecutive rows (near), and 16 columns of 4 rows in turn (far).
 template <typename T>
 struct Op;
+
+template <typename T, int D>
+__device__ __forceinline__ int place(int r, int c) {
+  constexpr int CE = Op<T>::VE;
+  return r * D + (((c / CE) ^ (Op<T>::swz(r) & (D / CE - 1))) * CE | c % CE);
+}
 
 template <>
 struct Op<u16> {
   typedef bf16x8 Frag;
-  static constexpr int KB = 32, VE = 8, PAD = 8, PLANES = 2;
-  // Rows of the free index, the contracted one consecutive.
-  static __device__ __forceinline__ Frag near(const u16* m, int ld, int r0, int k0) {
+  static constexpr int KB = 32, VE = 8, PLANES = 3, HALVES = 2;
+  static __device__ __forceinline__ int swz(int r) {
+    return ((r & 3) << 1) | ((r >> 2) & 1) | (r & 8);
+  }
+  // Lane offsets of fragment reads; row and column of the tile and k0 are added by frag_*.
+  template <int D>
+  static __device__ __forceinline__ int near_base() {
     const int l = threadIdx.x & 63;
-    return *reinterpret_cast<const bf16x8*>(m + (r0 + (l & 15)) * ld + k0 + 8 * (l >> 4));
+    return place<u16, D>(l & 15, 8 * (l >> 4));
+  }
+  template <int D>
+  static __device__ __forceinline__ int far_base() {
+    const int l = threadIdx.x & 63;
+    return place<u16, D>(8 * (l >> 4) + ((l & 15) >> 2), 4 * (l & 3));
+  }
+  // Rows of the free index, the contracted one consecutive.
+  template <int D>
+  static __device__ __forceinline__ Frag near(const u16* m, int base, int r0, int k0) {
+    return *reinterpret_cast<const bf16x8*>(m + (base ^ k0) + r0 * D);
   }
   // Rows of the contracted index: 16 lanes fetch 4 rows x 16 columns and get a column each.
-  static __device__ __forceinline__ Frag far(const u16* m, int ld, int c0, int k0) {
-    const int l = threadIdx.x & 63;
-    const u16* p = m + (k0 + 8 * (l >> 4) + ((l & 15) >> 2)) * ld + c0 + 4 * (l & 3);
+  template <int D>
+  static __device__ __forceinline__ Frag far(const u16* m, int base, int c0, int k0) {
     typedef __attribute__((address_space(3))) s16x4* lds_t;
+    const u16* p = m + (base ^ c0) + k0 * D;
+    const u16* p4 = m + (base ^ c0 ^ 8) + (k0 + 4) * D;
     const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)p);
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(p + 4 * ld));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)p4);
     const s16x8 x = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     return __builtin_bit_cast(bf16x8, x);
   }
@@ -105,15 +130,27 @@ struct Op<u16> {
 template <>
 struct Op<float> {
   typedef f32x4 Frag;
-  static constexpr int KB = 16, VE = 4, PAD = 4, PLANES = 1;
-  static __device__ __forceinline__ Frag near(const float* m, int ld, int r0, int k0) {
+  static constexpr int KB = 16, VE = 4, PLANES = 1, HALVES = 1;
+  static __device__ __forceinline__ int swz(int r) { return r & 15; }
+  template <int D>
+  static __device__ __forceinline__ int near_base() {
     const int l = threadIdx.x & 63;
-    return *reinterpret_cast<const f32x4*>(m + (r0 + (l & 15)) * ld + k0 + 4 * (l >> 4));
+    return place<float, D>(l & 15, 4 * (l >> 4));
   }
-  static __device__ __forceinline__ Frag far(const float* m, int ld, int c0, int k0) {
+  template <int D>
+  static __device__ __forceinline__ int far_base() {
     const int l = threadIdx.x & 63;
-    const float* p = m + (k0 + 4 * (l >> 4)) * ld + c0 + (l & 15);
-    const f32x4 x = {p[0], p[ld], p[2 * ld], p[3 * ld]};
+    return place<float, D>(4 * (l >> 4), l & 15);
+  }
+  template <int D>
+  static __device__ __forceinline__ Frag near(const float* m, int base, int r0, int k0) {
+    return *reinterpret_cast<const f32x4*>(m + (base ^ k0) + r0 * D);
+  }
+  template <int D>
+  static __device__ __forceinline__ Frag far(const float* m, int base, int c0, int k0) {
+    f32x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = m[(base ^ c0 ^ (4 * i)) + (k0 + i) * D];
     return x;
   }
   static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
@@ -136,36 +173,38 @@ struct Tiling {
   static __device__ __forceinline__ int n0(int t) { return 16 * (wn() * TN + t); }
 };
 
-// acc[tm][tn] += A B over K contracted elements: A (free index M) and B (free index N) each
-// near or far, in AP and BP planes of hi and lo (their lo lo product is below fp32's rounding
-// of the sum and left out).
-template <typename T, typename Ti, int K, bool AFAR, bool BFAR, int AP, int BP>
-__device__ __forceinline__ void product(f32x4 (&acc)[Ti::TM][Ti::TN], const T* A, int lda, int pa,
-                                        const T* B, int ldb, int pb) {
+// acc[tm][tn] += A B over K contracted elements.  A (free index M) and B (free index N) are
+// each near (rows of K elements) or far (rows of LA or LB elements), and come in planes: A[0]
+// to A[AP - 1] times B[0], and A[0] times the other planes of B.
+template <typename T, typename Ti, int K, bool AFAR, bool BFAR, int LA, int LB, int AP, int BP>
+__device__ __forceinline__ void product(f32x4 (&acc)[Ti::TM][Ti::TN], const T* const (&A)[AP],
+                                        const T* const (&B)[BP]) {
   if (!Ti::live()) return;
+  typedef Op<T> O;
+  const int ab = AFAR ? O::template far_base<LA>() : O::template near_base<LA>();
+  const int bb = BFAR ? O::template far_base<LB>() : O::template near_base<LB>();
 #pragma unroll
-  for (int k0 = 0; k0 < K; k0 += Op<T>::KB) {
-    typename Op<T>::Frag a[AP][Ti::TM], b[BP][Ti::TN];
+  for (int k0 = 0; k0 < K; k0 += O::KB) {
+    typename O::Frag a[AP][Ti::TM], b[BP][Ti::TN];
 #pragma unroll
     for (int p = 0; p < AP; ++p)
 #pragma unroll
       for (int t = 0; t < Ti::TM; ++t)
-        a[p][t] = AFAR ? Op<T>::far(A + p * pa, lda, Ti::m0(t), k0)
-                       : Op<T>::near(A + p * pa, lda, Ti::m0(t), k0);
+        a[p][t] = AFAR ? O::template far<LA>(A[p], ab, Ti::m0(t), k0)
+                       : O::template near<LA>(A[p], ab, Ti::m0(t), k0);
 #pragma unroll
     for (int p = 0; p < BP; ++p)
 #pragma unroll
       for (int t = 0; t < Ti::TN; ++t)
-        b[p][t] = BFAR ? Op<T>::far(B + p * pb, ldb, Ti::n0(t), k0)
-                       : Op<T>::near(B + p * pb, ldb, Ti::n0(t), k0);
+        b[p][t] = BFAR ? O::template far<LB>(B[p], bb, Ti::n0(t), k0)
+                       : O::template near<LB>(B[p], bb, Ti::n0(t), k0);
 #pragma unroll
-    for (int i = 0; i < Ti::TM; ++i)
+    for (int p = 0; p < AP + BP - 1; ++p)
 #pragma unroll
-      for (int j = 0; j < Ti::TN; ++j) {
-        acc[i][j] = Op<T>::mma(a[0][i], b[0][j], acc[i][j]);
-        if constexpr (AP > 1) acc[i][j] = Op<T>::mma(a[1][i], b[0][j], acc[i][j]);
-        if constexpr (BP > 1) acc[i][j] = Op<T>::mma(a[0][i], b[1][j], acc[i][j]);
-      }
+      for (int i = 0; i < Ti::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < Ti::TN; ++j)
+          acc[i][j] = O::mma(a[p < AP ? p : 0][i], b[p < AP ? 0 : p - AP + 1][j], acc[i][j]);
   }
 }
 
@@ -180,47 +219,53 @@ __device__ __forceinline__ void clear(f32x4 (&acc)[Ti::TM][Ti::TN]) {
 // ---- elements --------------------------------------------------------------------------
 __device__ __forceinline__ float to_f(u16 x) { return __uint_as_float((unsigned)x << 16); }
 __device__ __forceinline__ float to_f(float x) { return x; }
+// Two values rounded to bf16 by one packed conversion; the empty asm keeps it one.
 __device__ __forceinline__ unsigned pack2(float x, float y) {
   const bf16x2 h = {(__bf16)x, (__bf16)y};
-  return __builtin_bit_cast(unsigned, h);
+  unsigned u = __builtin_bit_cast(unsigned, h);
+  asm("" : "+v"(u));
+  return u;
 }
-// x = hi + lo, both rounded to nearest, two values at a time.
-__device__ __forceinline__ void split2(float x, float y, unsigned& hi, unsigned& lo) {
-  hi = pack2(x, y);
-  lo = pack2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
-}
+__device__ __forceinline__ float low(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
 
-// Four consecutive elements into LDS, in PL planes `plane` elements apart.
-template <int PL>
-__device__ __forceinline__ void put4(u16* p, int plane, f32x4 x) {
-  if constexpr (PL == 2) {
-    unsigned h0, l0, h1, l1;
-    split2(x[0], x[1], h0, l0);
-    split2(x[2], x[3], h1, l1);
-    *reinterpret_cast<uint2*>(p) = make_uint2(h0, h1);
-    *reinterpret_cast<uint2*>(p + plane) = make_uint2(l0, l1);
-  } else {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
+// x in planes of 8 bits each, from plane FIRST on: what is left after each rounding is exact.
+template <int FIRST, int PL>
+__device__ __forceinline__ void put4(u16* const (&to)[PL], int at, f32x4 x) {
+  static_assert(FIRST >= 0 && PL >= 1, "planes");
+#pragma unroll
+  for (int p = 0; p < FIRST + PL; ++p) {
+    const unsigned a = pack2(x[0], x[1]), b = pack2(x[2], x[3]);
+    if (p >= FIRST) *reinterpret_cast<uint2*>(to[p < FIRST ? 0 : p - FIRST] + at) = make_uint2(a, b);
+    x[0] -= low(a), x[1] -= high(a), x[2] -= low(b), x[3] -= high(b);
   }
 }
-template <int PL>
-__device__ __forceinline__ void put4(float* p, int, f32x4 x) {
-  *reinterpret_cast<f32x4*>(p) = x;
+template <int FIRST, int PL>
+__device__ __forceinline__ void put4(float* const (&to)[PL], int at, f32x4 x) {
+  *reinterpret_cast<f32x4*>(to[0] + at) = x;
 }
+__device__ __forceinline__ f32x4 get4(const u16* p) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  return f32x4{low(u.x), high(u.x), low(u.y), high(u.y)};
+}
+__device__ __forceinline__ f32x4 get4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
 
-// Four consecutive elements from column c of a row of d, to memory.
+// Four consecutive elements from column c of a row of d, to memory.  WIDE: d and the row's
+// start are multiples of 4 elements.
+template <bool WIDE>
 __device__ __forceinline__ void store4(u16* p, int c, int d, f32x4 x) {
-  if (c + 4 <= d && (((uintptr_t)(p + c)) & 7) == 0) {
-    *reinterpret_cast<uint2*>(p + c) = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
+  if constexpr (WIDE) {
+    if (c < d) *reinterpret_cast<uint2*>(p + c) = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (c + i < d) p[c + i] = __builtin_bit_cast(u16, (__bf16)x[i]);
   }
 }
+template <bool WIDE>
 __device__ __forceinline__ void store4(float* p, int c, int d, f32x4 x) {
-  if (c + 4 <= d && (((uintptr_t)(p + c)) & 15) == 0) {
-    *reinterpret_cast<f32x4*>(p + c) = x;
+  if constexpr (WIDE) {
+    if (c < d) *reinterpret_cast<f32x4*>(p + c) = x;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -229,10 +274,12 @@ __device__ __forceinline__ void store4(float* p, int c, int d, f32x4 x) {
 }
 
 // A chunk's (C, D) block on its way from memory to LDS, 16 bytes a vector; 0 outside the
-// sequence and the d columns.
-template <typename T, int C, int D>
+// sequence and the d columns.  WIDE: vectors are aligned and lie inside a row or outside it;
+// they are loaded from a place inside the block in any case and cleared when they are used,
+// since a load under a condition is waited for where the branches meet.
+template <typename T, int C, int D, bool WIDE>
 struct Block {
-  static constexpr int VE = Op<T>::VE, N = C * D / VE / NT, LD = D + Op<T>::PAD;
+  static constexpr int VE = Op<T>::VE, N = C * D / VE / NT;
   static_assert(C * D % (VE * NT) == 0, "whole vectors for every thread");
   uint4 x[N];
 
@@ -240,45 +287,50 @@ struct Block {
   static __device__ __forceinline__ int col(int n) {
     return (threadIdx.x + n * NT) % (D / VE) * VE;
   }
-  // src: the chunk's first row; ld: elements between rows; wide: 16-byte vectors are aligned
-  // and lie inside the row or outside it.
-  __device__ __forceinline__ void load(const T* src, int64_t ld, int rows, int d, bool wide) {
+  // src: the chunk's first row; ld: elements between rows.
+  __device__ __forceinline__ void load(const T* src, int64_t ld, int rows, int d) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      x[n] = make_uint4(0u, 0u, 0u, 0u);
       const int r = row(n), c = col(n);
-      if (r >= rows) continue;
-      const T* p = src + r * ld + c;
-      if (wide) {
-        if (c < d) x[n] = *reinterpret_cast<const uint4*>(p);
+      if constexpr (WIDE) {
+        const unsigned at = (unsigned)(r < rows ? r : rows - 1) * (unsigned)ld + (c < d ? c : 0);
+        x[n] = *reinterpret_cast<const uint4*>(src + at);
       } else {
         T e[VE];
 #pragma unroll
-        for (int i = 0; i < VE; ++i) e[i] = c + i < d ? p[i] : (T)0;
+        for (int i = 0; i < VE; ++i) e[i] = r < rows && c + i < d ? src[r * ld + c + i] : (T)0;
         __builtin_memcpy(&x[n], e, 16);
       }
     }
   }
+  __device__ __forceinline__ void mask(int rows, int d) {
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (row(n) >= rows || col(n) >= d) x[n] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
   __device__ __forceinline__ void put(T* m) const {
 #pragma unroll
-    for (int n = 0; n < N; ++n) *reinterpret_cast<uint4*>(m + row(n) * LD + col(n)) = x[n];
+    for (int n = 0; n < N; ++n) *reinterpret_cast<uint4*>(m + place<T, D>(row(n), col(n))) = x[n];
   }
   __device__ __forceinline__ void get(const T* m) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) x[n] = *reinterpret_cast<const uint4*>(m + row(n) * LD + col(n));
+    for (int n = 0; n < N; ++n) x[n] = *reinterpret_cast<const uint4*>(m + place<T, D>(row(n), col(n)));
   }
-  // Rows times w[row], in all planes.
-  __device__ __forceinline__ void put_scaled(T* m, const float* w) const {
+  // Rows times weight(row), in all planes.
+  template <int PL, typename W>
+  __device__ __forceinline__ void put_scaled(T* const (&m)[PL], W&& weight) const {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const float s = w[row(n)];
+      const float s = weight(row(n));
       T e[VE];
       __builtin_memcpy(e, &x[n], 16);
 #pragma unroll
       for (int i = 0; i < VE; i += 4) {
         const f32x4 y = {s * to_f(e[i]), s * to_f(e[i + 1]), s * to_f(e[i + 2]),
                          s * to_f(e[i + 3])};
-        put4<Op<T>::PLANES>(m + row(n) * LD + col(n) + i, C * LD, y);
+        put4<0, PL>(m, place<T, D>(row(n), col(n)) + i, y);
       }
     }
   }
@@ -296,52 +348,68 @@ __device__ __forceinline__ float span0(const Gate& i) {
   return __builtin_amdgcn_exp2f(fmaf(-1e6f, i.n, i.hi + i.lo));
 }
 
-// One wave: lane i forms the chunk's i-th gate from its g (0 past the sequence).
+template <int CTRL>
+__device__ __forceinline__ double dpp0(double x) {
+  const int2 u = __builtin_bit_cast(int2, x);
+  return __builtin_bit_cast(double,
+                            make_int2(__builtin_amdgcn_update_dpp(0, u.x, CTRL, 0xf, 0xf, false),
+                                      __builtin_amdgcn_update_dpp(0, u.y, CTRL, 0xf, 0xf, false)));
+}
+__device__ __forceinline__ double lane_of(double x, int l) {
+  const int2 u = __builtin_bit_cast(int2, x);
+  return __builtin_bit_cast(
+      double, make_int2(__builtin_amdgcn_readlane(u.x, l), __builtin_amdgcn_readlane(u.y, l)));
+}
+
+// One wave: lane i forms the chunk's i-th gate from its g (0 past the sequence).  The prefix
+// sums take steps of 1, 2, 4 and 8 lanes in each row of 16, then the rows' totals.
 template <int C>
 __device__ __forceinline__ void make_gates(Gate* out, float g) {
-  const int l = threadIdx.x & 63;
+  const int l = threadIdx.x & 63, row = l >> 4;
   constexpr double LOG2E = 1.4426950408889634;
   double s = (double)g * LOG2E;
   const bool over = s < -126.0;
-  float n = over ? 1.f : 0.f;
+  const float n = mg_wave_prefix_sum(over ? 1.f : 0.f);
   s = over ? 0.0 : s;
-#pragma unroll
-  for (int d = 1; d < C; d *= 2) {
-    const double t = __shfl_up(s, d);
-    const float u = __shfl_up(n, d);
-    if (l >= d) s += t, n += u;
-  }
+  s += dpp0<0x111>(s);
+  s += dpp0<0x112>(s);
+  s += dpp0<0x114>(s);
+  s += dpp0<0x118>(s);
+  const double a = lane_of(s, 15), b = lane_of(s, 31), c = lane_of(s, 47);
+  s += (row > 0 ? a : 0.0) + (row > 1 ? b : 0.0) + (row > 2 ? c : 0.0);
   const float hi = (float)s;
   if (l < C) out[l] = Gate{hi, (float)(s - (double)hi), n, 0.f};
 }
 
 // ---- the sweep -------------------------------------------------------------------------------
+// LDS, in elements.  In the gradients' sweeps the two leading planes of the state lie in S[0],
+// S[1]; once they are read the third lies in S[0] and the decayed rows' leading planes in
+// S[1], their third one in place of the rows themselves.
 template <typename T, int C, int DK, int DV, int MODE>
 struct Lds {
-  static constexpr int E = sizeof(T), PAD = Op<T>::PAD, PL = Op<T>::PLANES;
-  static constexpr int LK = DK + PAD, LV = DV + PAD, LC = C + PAD;
+  static constexpr int PL = Op<T>::PLANES, HV = Op<T>::HALVES;
   static constexpr bool GRAD = MODE == LA_DQ || MODE == LA_DKV;
   static constexpr bool BARE = MODE == LA_STATE || MODE == LA_RSTATE;
   static constexpr int Q = 0;  // queries
-  static constexpr int K = Q + (BARE ? 0 : C * LK);
-  static constexpr int V = K + (BARE ? 0 : C * LK);
-  static constexpr int O = V + C * LV;  // output gradients
-  static constexpr int P = O + (GRAD ? C * LV : 0);
-  static constexpr int P2 = P + (BARE ? 0 : C * LC);
-  static constexpr int S = P2 + (MODE == LA_DKV ? C * LC : 0);  // state
-  static constexpr int SPLANES = GRAD ? PL : 1;
-  static constexpr int SSIZE = BARE ? 0 : DK * LV * SPLANES;
-  // decayed keys (queries): in the state's place where it has been read by then
-  static constexpr int W = GRAD ? S : S + SSIZE;
-  static constexpr int WSIZE = C * LK * PL;
-  static constexpr int END = GRAD ? S + (SSIZE > WSIZE ? SSIZE : WSIZE) : W + WSIZE;
-  static constexpr int BYTES = (END * E + 15) / 16 * 16;
+  static constexpr int K = Q + (BARE ? 0 : C * DK);
+  static constexpr int V = K + (BARE ? 0 : C * DK);
+  static constexpr int O = V + C * DV;  // output gradients
+  static constexpr int P = O + (GRAD ? C * DV : 0);
+  static constexpr int P2 = P + (BARE ? 0 : C * C);
+  static constexpr int S = P2 + (MODE == LA_DKV ? C * C : 0);
+  static constexpr int S1 = S + (BARE ? 0 : DK * DV);
+  static constexpr int STATE = DK * DV * (HV - 1), ROWS = C * DK * HV;
+  static constexpr int W = GRAD && PL == 1 ? S : S1;  // decayed keys or queries
+  static constexpr int END =
+      GRAD ? (PL == 1 ? S + (DK * DV > C * DK ? DK * DV : C * DK) : S1 + (STATE > ROWS ? STATE : ROWS))
+           : W + C * DK * PL;
+  static constexpr int BYTES = END * (int)sizeof(T);
 };
 
-template <typename T, int C, int DK, int DV, int MODE>
+template <typename T, int C, int DK, int DV, int MODE, bool WIDE>
 __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
   typedef Lds<T, C, DK, DV, MODE> L;
-  constexpr int PL = L::PL, LK = L::LK, LV = L::LV, LC = L::LC;
+  constexpr int PL = L::PL;
   constexpr bool REV = MODE == LA_RSTATE || MODE == LA_DKV, BARE = L::BARE, GRAD = L::GRAD;
   typedef Tiling<DV / 16, DK / 16, 2> TS;  // the state, transposed: M = dv, N = dk
   typedef Tiling<C / 16, C / 16, 4> TC;    // chunk matrices
@@ -349,18 +417,19 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
   typedef Tiling<DV / 16, C / 16, 4> TV;   // (dv, token)
   __shared__ __align__(16) char raw[L::BYTES];
   __shared__ Gate gates[2][C];
-  __shared__ float s_w[C];
   // Sums over the chunk matrices' rows and columns, and rows' products with dq or dk, by wave.
   __shared__ float s_row[4][C], s_col[4][C], s_dot[4][C];
-  T* lds = reinterpret_cast<T*>(raw);
-  T *sQ = lds + L::Q, *sK = lds + L::K, *sV = lds + L::V, *sO = lds + L::O, *sP = lds + L::P,
-    *sP2 = lds + L::P2, *sS = lds + L::S, *sW = lds + L::W;
+  T* const lds = reinterpret_cast<T*>(raw);
+  T *const sQ = lds + L::Q, *const sK = lds + L::K, *const sV = lds + L::V, *const sO = lds + L::O;
+  T *const sP = lds + L::P, *const sP2 = lds + L::P2, *const sS = lds + L::S, *const sW = lds + L::W;
+  T* const sS1 = lds + L::S1;
 
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int wave = mg_uniform(tid >> 6);
   const int64_t bh = blockIdx.x;
-  const int seg = blockIdx.y;  // bare passes: the last (first) segment's state isn't needed
-  const int b = (int)(bh / a.H), h = (int)(bh % a.H), kh = h / a.group;
+  const int seg = blockIdx.y;
+  const int64_t b = bh / a.H;
+  const int h = (int)(bh % a.H), kh = h / a.group;
   const int dk = a.dk, dv = a.dv;
   const int64_t T_ = a.T;
   int64_t len = T_;
@@ -379,13 +448,6 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
   const T* v = (const T*)a.v + b * a.vs[0] + h * a.vs[2];
   const T* dout = (const T*)a.dout + b * a.ds[0] + h * a.ds[2];
   const float* g = a.g + b * a.gs[0] + h * a.gs[2];
-  const auto wide = [&](const void* p, const int64_t (&s)[3], int d) {
-    constexpr int VE = Op<T>::VE;
-    return (((uintptr_t)p) & 15) == 0 && d % VE == 0 && s[0] % VE == 0 && s[1] % VE == 0 &&
-           s[2] % VE == 0;
-  };
-  const bool wq = MODE == LA_STATE || wide(a.q, a.qs, dk), wk = wide(a.k, a.ks, dk),
-             wv = wide(a.v, a.vs, dv), wo = wide(a.dout, a.ds, dv);
 
   // The state: lane (lg, lr) of tile (i, j) holds S[n0 + lr][m0 + 4 lg .. + 3].
   f32x4 S[TS::TM][TS::TN];
@@ -395,8 +457,35 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
 #pragma unroll
     for (int i = 0; i < TS::TM; ++i)
 #pragma unroll
-      for (int j = 0; j < TS::TN; ++j) f(S[i][j], TS::n0(j) + lr, TS::m0(i) + 4 * lg);
+      for (int j = 0; j < TS::TN; ++j)
+        if (TS::live()) f(S[i][j], TS::n0(j) + lr, TS::m0(i) + 4 * lg);
   };
+
+  Block<T, C, DK, WIDE> bq, bk;
+  Block<T, C, DV, WIDE> bv, bo;
+  const auto at = [&](int n) { return t0 + (int64_t)(REV ? chunks - 1 - n : n) * C; };
+  const auto rows_at = [&](int64_t t) { return (int)(e1 - t < C ? e1 - t : C); };
+  const auto fetch = [&](int64_t t) {
+    const int rows = rows_at(t);
+    if constexpr (MODE != LA_STATE) bq.load(q + t * a.qs[1], a.qs[1], rows, dk);
+    if constexpr (MODE != LA_RSTATE) bk.load(k + t * a.ks[1], a.ks[1], rows, dk);
+    if constexpr (MODE != LA_RSTATE) bv.load(v + t * a.vs[1], a.vs[1], rows, dv);
+    if constexpr (GRAD || MODE == LA_RSTATE) bo.load(dout + t * a.ds[1], a.ds[1], rows, dv);
+  };
+  // Wave 0 forms the gates one chunk ahead, from decays loaded two chunks ahead.
+  const auto decays = [&](int n) {
+    const int64_t t = at(n);
+    return lane < rows_at(t) ? g[(t + lane) * a.gs[1]] : 0.f;
+  };
+  float g_next = 0.f;
+  if (chunks > 0) {
+    fetch(at(0));
+    if (wave == 0) {
+      const float g0 = decays(0);
+      if (chunks > 1) g_next = decays(1);
+      make_gates<C>(gates[0], g0);
+    }
+  }
   if constexpr (!BARE) {
     const float* from;
     if constexpr (REV)
@@ -407,31 +496,16 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
                       : a.bound + (bh * (a.segs - 1) + seg - 1) * ss;
     if (from)
       each_state([&](f32x4& x, int r, int c) {
-        if (r < dk) {
+        if constexpr (WIDE) {
+          const bool in = r < dk && c < dv;
+          const f32x4 y = *reinterpret_cast<const f32x4*>(from + (in ? r * dv + c : 0));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = c + i < dv ? from[(int64_t)r * dv + c + i] : 0.f;
+          for (int i = 0; i < 4; ++i) x[i] = in ? y[i] : 0.f;
+        } else if (r < dk) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = c + i < dv ? from[r * dv + c + i] : 0.f;
         }
       });
-  }
-
-  Block<T, C, DK> bq, bk;
-  Block<T, C, DV> bv, bo;
-  const auto at = [&](int n) { return t0 + (int64_t)(REV ? chunks - 1 - n : n) * C; };
-  const auto rows_at = [&](int64_t t) { return (int)(e1 - t < C ? e1 - t : C); };
-  const auto fetch = [&](int64_t t) {
-    const int rows = rows_at(t);
-    if constexpr (MODE != LA_STATE) bq.load(q + t * a.qs[1], a.qs[1], rows, dk, wq);
-    if constexpr (MODE != LA_RSTATE) bk.load(k + t * a.ks[1], a.ks[1], rows, dk, wk);
-    if constexpr (MODE != LA_RSTATE) bv.load(v + t * a.vs[1], a.vs[1], rows, dv, wv);
-    if constexpr (GRAD || MODE == LA_RSTATE) bo.load(dout + t * a.ds[1], a.ds[1], rows, dv, wo);
-  };
-  const auto gates_of = [&](int n) {
-    const int64_t t = at(n);
-    make_gates<C>(gates[n & 1], lane < rows_at(t) ? g[(t + lane) * a.gs[1]] : 0.f);
-  };
-  if (chunks > 0) {
-    fetch(at(0));
-    if (wave == 0) gates_of(0);
   }
   float fall = 1.f;  // the segment's decay so far
 
@@ -440,40 +514,75 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
     const int rows = rows_at(t);
     const Gate* ga = gates[n & 1];
     __syncthreads();  // the gates; and the last chunk's operands are read
+    const Gate end = ga[C - 1];
+    const float keep = span0(end);
+    const auto weight = [&](int r) { return REV ? a.scale * span0(ga[r]) : span(end, ga[r]); };
+    if constexpr (MODE != LA_STATE) bq.mask(rows, dk);
+    if constexpr (MODE != LA_RSTATE) bk.mask(rows, dk), bv.mask(rows, dv);
+    if constexpr (GRAD || MODE == LA_RSTATE) bo.mask(rows, dv);
     if constexpr (!BARE) {
       bq.put(sQ);
       bk.put(sK);
       if constexpr (GRAD) bo.put(sO);
-      each_state([&](f32x4& x, int r, int c) { put4<L::SPLANES>(sS + r * LV + c, DK * LV, x); });
+      each_state([&](f32x4& x, int r, int c) {
+        const int p = place<T, DV>(r, c);
+        if constexpr (GRAD && PL > 1) {
+          T* const to[2] = {sS, sS1};
+          put4<0, 2>(to, p, x);
+        } else {
+          T* const to[1] = {sS};
+          put4<0, 1>(to, p, x);
+        }
+      });
     }
-    const Gate end = ga[C - 1];
-    const float keep = span0(end);
-    if (tid < C) s_w[tid] = REV ? a.scale * span0(ga[tid]) : span(end, ga[tid]);
     if constexpr (MODE == LA_RSTATE) bo.put(sV);
     else bv.put(sV);
     if constexpr (!GRAD) {
-      __syncthreads();  // s_w
-      if constexpr (MODE == LA_RSTATE) bq.put_scaled(sW, s_w);
-      else bk.put_scaled(sW, s_w);
+      T* to[PL];
+#pragma unroll
+      for (int p = 0; p < PL; ++p) to[p] = sW + p * C * DK;
+      if constexpr (MODE == LA_RSTATE) bq.put_scaled(to, weight);
+      else bk.put_scaled(to, weight);
     }
     __syncthreads();
     if (n + 1 < chunks) {
       fetch(at(n + 1));
-      if (wave == 0) gates_of(n + 1);
+      if (wave == 0) {
+        make_gates<C>(gates[(n + 1) & 1], g_next);
+        if (n + 2 < chunks) g_next = decays(n + 2);
+      }
+    }
+    const auto update = [&](const T* rows_v, const T* const (&w)[PL]) {
+#pragma unroll
+      for (int i = 0; i < TS::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TS::TN; ++j) S[i][j] *= keep;
+      const T* const av[1] = {rows_v};
+      product<T, TS, C, true, true, DV, DK, 1, PL>(S, av, w);
+      fall *= keep;
+    };
+    if constexpr (!GRAD) {
+      const T* w[PL];
+#pragma unroll
+      for (int p = 0; p < PL; ++p) w[p] = sW + p * C * DK;
+      update(sV, w);
     }
 
+    f32x4 ack[TK::TM][TK::TN], acv[TV::TM][TV::TN];
     if constexpr (!BARE) {
       // Chunk matrices, M the token that is contracted next, N the other: (j, i) towards the
       // queries' side, (i, j) towards the keys'.
       f32x4 A[TC::TM][TC::TN], B[TC::TM][TC::TN];
       clear<TC>(A);
       clear<TC>(B);
+      const T *const pq[1] = {sQ}, *const pk[1] = {sK}, *const pv[1] = {sV}, *const po[1] = {sO};
+      const T *const ps[1] = {sS};
       if constexpr (REV) {
-        product<T, TC, DK, false, false, 1, 1>(A, sQ, LK, 0, sK, LK, 0);
-        product<T, TC, DV, false, false, 1, 1>(B, sO, LV, 0, sV, LV, 0);
+        product<T, TC, DK, false, false, DK, DK, 1, 1>(A, pq, pk);
+        product<T, TC, DV, false, false, DV, DV, 1, 1>(B, po, pv);
       } else {
-        product<T, TC, DK, false, false, 1, 1>(A, sK, LK, 0, sQ, LK, 0);
-        if constexpr (GRAD) product<T, TC, DV, false, false, 1, 1>(B, sV, LV, 0, sO, LV, 0);
+        product<T, TC, DK, false, false, DK, DK, 1, 1>(A, pk, pq);
+        if constexpr (GRAD) product<T, TC, DV, false, false, DV, DV, 1, 1>(B, pv, po);
       }
       if (TC::live()) {
         float col[TC::TM][4];
@@ -495,8 +604,8 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
               const int i = REV ? mm + x : nn, j = REV ? nn : mm + x;
               const float d = j <= i ? a.scale * (REV ? span(ga[mm + x], gn) : span(gn, ga[mm + x]))
                                      : 0.f;
-              const float pa = A[im][jn][x] * d, pb = B[im][jn][x] * d;
-              p[x] = MODE == LA_DQ ? pb : pa;
+              const float pb = B[im][jn][x] * d;
+              p[x] = MODE == LA_DQ ? pb : A[im][jn][x] * d;
               p2[x] = pb;
               if constexpr (MODE == LA_DQ) {
                 const float xs = j < i ? A[im][jn][x] * pb : 0.f;
@@ -504,8 +613,9 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
                 col[im][x] += xs;
               }
             }
-            put4<1>(sP + nn * LC + mm, 0, p);
-            if constexpr (MODE == LA_DKV) put4<1>(sP2 + nn * LC + mm, 0, p2);
+            T *const to[1] = {sP}, *const to2[1] = {sP2};
+            put4<0, 1>(to, place<T, C>(nn, mm), p);
+            if constexpr (MODE == LA_DKV) put4<0, 1>(to2, place<T, C>(nn, mm), p2);
           }
           if constexpr (MODE == LA_DQ) {
             row = mg_pair_sum<32>(mg_pair_sum<16>(row));
@@ -522,109 +632,113 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
             }
         }
       }
-      __syncthreads();
+      // What comes through the state: o's, dq's or dk's and dv's.
+      if constexpr (MODE != LA_DQ) {
+        clear<TV>(acv);
+        product<T, TV, DK, true, false, DV, DK, 1, 1>(acv, ps, REV ? pk : pq);
+      }
+      if constexpr (GRAD) {
+        clear<TK>(ack);
+        if constexpr (PL > 1) {
+          const T* const two[2] = {sS, sS1};
+          product<T, TK, DV, false, false, DV, DV, 2, 1>(ack, two, REV ? pv : po);
+        } else {
+          product<T, TK, DV, false, false, DV, DV, 1, 1>(ack, ps, REV ? pv : po);
+        }
+      }
+      __syncthreads();  // the chunk matrices are there, the state's leading planes are read
     }
 
-    if constexpr (MODE == LA_OUT) {
-      f32x4 in[TV::TM][TV::TN], ac[TV::TM][TV::TN];
+    const auto out_v = [&](T* to, const T* far, auto&& factor) {
+      f32x4 in[TV::TM][TV::TN];
       clear<TV>(in);
-      clear<TV>(ac);
-      product<T, TV, DK, true, false, 1, 1>(ac, sS, LV, 0, sQ, LK, 0);
-      product<T, TV, C, true, false, 1, 1>(in, sV, LV, 0, sP, LC, 0);
+      const T *const af[1] = {far}, *const pp[1] = {sP};
+      product<T, TV, C, true, false, DV, C, 1, 1>(in, af, pp);
       if (TV::live()) {
+        T* const base = to + ((b * T_ + t) * a.H + h) * (int64_t)dv;
 #pragma unroll
         for (int j = 0; j < TV::TN; ++j) {
           const int i = TV::n0(j) + lr;
-          const float f = a.scale * span0(ga[i]);
+          const float f = factor(i);
           if (i < rows) {
-            T* o = (T*)a.out + ((b * T_ + t + i) * a.H + h) * (int64_t)dv;
+            T* const p = base + (int64_t)i * a.H * dv;
 #pragma unroll
             for (int m = 0; m < TV::TM; ++m)
-              store4(o, TV::m0(m) + 4 * lg, dv, in[m][j] + f * ac[m][j]);
+              store4<WIDE>(p, TV::m0(m) + 4 * lg, dv, in[m][j] + f * acv[m][j]);
           }
         }
       }
-    }
+    };
+    if constexpr (MODE == LA_OUT)
+      out_v((T*)a.out, sV, [&](int i) { return a.scale * span0(ga[i]); });
+    if constexpr (MODE == LA_DKV)
+      out_v((T*)a.out2, sO, [&](int i) { return span(end, ga[i]); });
     if constexpr (GRAD) {
-      // dq or dk: the part through the state, then the chunk's own.
-      f32x4 in[TK::TM][TK::TN], ac[TK::TM][TK::TN];
+      // dq or dk of the chunk itself, then the state's third plane.
+      f32x4 in[TK::TM][TK::TN];
       clear<TK>(in);
-      clear<TK>(ac);
-      product<T, TK, DV, false, false, PL, 1>(ac, sS, LV, DK * LV, REV ? sV : sO, LV, 0);
-      product<T, TK, C, true, false, 1, 1>(in, REV ? sQ : sK, LK, 0, REV ? sP2 : sP, LC, 0);
+      const T *const rk[1] = {REV ? sQ : sK}, *const pp[1] = {REV ? sP2 : sP};
+      product<T, TK, C, true, false, DK, C, 1, 1>(in, rk, pp);
+      if constexpr (PL > 1) {
+        each_state([&](f32x4& x, int r, int c) {
+          T* const to[1] = {sS};
+          put4<2, 1>(to, place<T, DV>(r, c), x);
+        });
+      }
+      __syncthreads();  // the chunk's rows are read, the third plane is there
+      if constexpr (PL > 1) {
+        const T *const third[1] = {sS}, *const rv[1] = {REV ? sV : sO};
+        product<T, TK, DV, false, false, DV, DV, 1, 1>(ack, third, rv);
+      }
       if (TK::live()) {
+        const int64_t base = ((b * T_ + t) * a.H + h) * (int64_t)dk;
 #pragma unroll
         for (int j = 0; j < TK::TN; ++j) {
           const int i = TK::n0(j) + lr;
           const float f = REV ? span(end, ga[i]) : a.scale * span0(ga[i]);
-          const T* x = (REV ? sK : sQ) + i * LK;
-          const int64_t row = ((b * T_ + t + i) * a.H + h) * (int64_t)dk;
+          const int64_t row = base + (int64_t)i * a.H * dk;
           float dot = 0.f;
 #pragma unroll
           for (int m = 0; m < TK::TM; ++m) {
             const int c = TK::m0(m) + 4 * lg;
-            const f32x4 y = f * ac[m][j];
+            const f32x4 y = f * ack[m][j], x = get4((REV ? sK : sQ) + place<T, DK>(i, c));
 #pragma unroll
-            for (int u = 0; u < 4; ++u) dot += y[u] * to_f(x[c + u]);
+            for (int u = 0; u < 4; ++u) dot += y[u] * x[u];
             if (i < rows) {
-              if (a.part) store4(a.part + row, c, dk, y + in[m][j]);
-              else store4((T*)a.out + row, c, dk, y + in[m][j]);
+              if (a.part) store4<WIDE>(a.part + row, c, dk, y + in[m][j]);
+              else store4<WIDE>((T*)a.out + row, c, dk, y + in[m][j]);
             }
           }
           dot = mg_pair_sum<32>(mg_pair_sum<16>(dot));
           if (lane < 16) s_dot[TK::wm()][i] = dot;
         }
       }
-    }
-    if constexpr (MODE == LA_DKV) {
-      f32x4 in[TV::TM][TV::TN], ac[TV::TM][TV::TN];
-      clear<TV>(in);
-      clear<TV>(ac);
-      product<T, TV, DK, true, false, 1, 1>(ac, sS, LV, 0, sK, LK, 0);
-      product<T, TV, C, true, false, 1, 1>(in, sO, LV, 0, sP, LC, 0);
-      if (TV::live()) {
+      // The rows the state takes up, decayed; the third plane in their own place.
+      Block<T, C, DK, WIDE> w;
+      w.get(REV ? sQ : sK);
+      T* to[PL];
+      const T* from[PL];
 #pragma unroll
-        for (int j = 0; j < TV::TN; ++j) {
-          const int i = TV::n0(j) + lr;
-          const float f = span(end, ga[i]);
-          if (i < rows) {
-            T* o = (T*)a.out2 + ((b * T_ + t + i) * a.H + h) * (int64_t)dv;
-#pragma unroll
-            for (int m = 0; m < TV::TM; ++m)
-              store4(o, TV::m0(m) + 4 * lg, dv, in[m][j] + f * ac[m][j]);
-          }
-        }
+      for (int p = 0; p < PL; ++p) {
+        to[p] = p == 2 ? (REV ? sQ : sK) : sW + p * C * DK;
+        from[p] = to[p];
       }
-    }
-    if constexpr (GRAD) {
-      __syncthreads();  // the state's copy is read, the sums are written
+      w.put_scaled(to, weight);
+      __syncthreads();
       if (tid < rows) {
         float x = 0.f;
 #pragma unroll
-        for (int w = 0; w < TK::WM; ++w) x += s_dot[w][tid];
-        float* e = a.e + bh * T_ + t + tid;
+        for (int u = 0; u < TK::WM; ++u) x += s_dot[u][tid];
         if constexpr (MODE == LA_DQ) {
 #pragma unroll
-          for (int w = 0; w < TC::WM; ++w) x += s_row[w][tid];
+          for (int u = 0; u < TC::WM; ++u) x += s_row[u][tid];
 #pragma unroll
-          for (int w = 0; w < TC::WN && w < C / 16; ++w) x -= s_col[w][tid];
-          *e = x;
-        } else {
-          *e -= x;
+          for (int u = 0; u < TC::WN && u < C / 16; ++u) x -= s_col[u][tid];
         }
+        a.e[bh * T_ + t + tid] = x;
       }
-      Block<T, C, DK> w;
-      w.get(REV ? sQ : sK);
-      w.put_scaled(sW, s_w);
-      __syncthreads();
+      update(REV ? sO : sV, from);
     }
-    // The state: its decay, then the chunk's own.
-#pragma unroll
-    for (int i = 0; i < TS::TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TS::TN; ++j) S[i][j] *= keep;
-    product<T, TS, C, true, true, 1, PL>(S, MODE == LA_DKV ? sO : sV, LV, 0, sW, LK, C * LK);
-    fall *= keep;
   }
 
   float* to = nullptr;
@@ -636,7 +750,7 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
   }
   if (to)
     each_state([&](f32x4& x, int r, int c) {
-      if (r < dk) store4(to + (int64_t)r * dv, c, dv, x);
+      if (r < dk) store4<WIDE>(to + r * dv, c, dv, x);
     });
   // Past a sequence's length.
   if constexpr (!BARE) {
@@ -649,10 +763,9 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
     if constexpr (GRAD) {
       if (a.part) zero(a.part, dk);
       else zero((T*)a.out, dk);
+      for (int64_t x = z0 + tid; x < t1; x += NT) a.e[bh * T_ + x] = 0.f;
     }
     if constexpr (MODE == LA_DKV) zero((T*)a.out2, dv);
-    if constexpr (MODE == LA_DQ)
-      for (int64_t x = z0 + tid; x < t1; x += NT) a.e[bh * T_ + x] = 0.f;
   }
 }
 
@@ -673,10 +786,11 @@ __global__ __launch_bounds__(256) void la_join(const float* __restrict__ first,
   }
 }
 
-// dg_t = sum of e from t to its segment's end + <R, S> there; 0 past a sequence's length and
+// e: the queries' side less the keys'.  dg_t = sum of e from t to its segment's end + <R, S> there; 0 past a sequence's length and
 // at steps that start over.
 __global__ __launch_bounds__(256) void la_decay_grad(LaArgs a, const float* states,
                                                      const float* adjoints, const float* last_r,
+                                                     const float* __restrict__ keys,
                                                      float* __restrict__ dg, int C) {
   __shared__ double s_e[4];
   __shared__ float s_t[4];
@@ -706,7 +820,7 @@ __global__ __launch_bounds__(256) void la_decay_grad(LaArgs a, const float* stat
   const float* g = a.g + b * a.gs[0] + h * a.gs[2];
   for (int64_t hi = t1; hi > t0; hi -= 256) {
     const int64_t t = hi - 256 + tid;
-    const float e = t >= t0 ? a.e[bh * a.T + t] : 0.f;
+    const float e = t >= t0 ? a.e[bh * a.T + t] - keys[bh * a.T + t] : 0.f;
     float s = mg_wave_suffix_sum(e);
     if (lane == 0) s_t[w] = s;
     __syncthreads();
@@ -842,29 +956,43 @@ size_t la_decay_bytes(const Plan& p, int64_t BH) {
   return mg_align_up((size_t)BH * (p.segs - 1) * sizeof(float), 256);
 }
 
-template <typename T, int C, int DK, int DV>
+template <typename T, int C, int DK, int DV, bool WIDE>
 int la_modes(const LaArgs& a, int mode, int64_t BH, hipStream_t stream) {
   const bool bare = mode == LA_STATE || mode == LA_RSTATE;
   const dim3 grid((unsigned)BH, (unsigned)(a.segs - (bare ? 1 : 0)));
   switch (mode) {
-    case LA_STATE: hipLaunchKernelGGL((la_sweep<T, C, DK, DV, LA_STATE>), grid, dim3(NT), 0, stream, a); break;
-    case LA_OUT: hipLaunchKernelGGL((la_sweep<T, C, DK, DV, LA_OUT>), grid, dim3(NT), 0, stream, a); break;
-    case LA_RSTATE: hipLaunchKernelGGL((la_sweep<T, C, DK, DV, LA_RSTATE>), grid, dim3(NT), 0, stream, a); break;
-    case LA_DQ: hipLaunchKernelGGL((la_sweep<T, C, DK, DV, LA_DQ>), grid, dim3(NT), 0, stream, a); break;
-    default: hipLaunchKernelGGL((la_sweep<T, C, DK, DV, LA_DKV>), grid, dim3(NT), 0, stream, a);
+    case LA_STATE: hipLaunchKernelGGL((la_sweep<T, C, DK, DV, LA_STATE, WIDE>), grid, dim3(NT), 0, stream, a); break;
+    case LA_OUT: hipLaunchKernelGGL((la_sweep<T, C, DK, DV, LA_OUT, WIDE>), grid, dim3(NT), 0, stream, a); break;
+    case LA_RSTATE: hipLaunchKernelGGL((la_sweep<T, C, DK, DV, LA_RSTATE, WIDE>), grid, dim3(NT), 0, stream, a); break;
+    case LA_DQ: hipLaunchKernelGGL((la_sweep<T, C, DK, DV, LA_DQ, WIDE>), grid, dim3(NT), 0, stream, a); break;
+    default: hipLaunchKernelGGL((la_sweep<T, C, DK, DV, LA_DKV, WIDE>), grid, dim3(NT), 0, stream, a);
   }
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
-template <typename T, int C>
+template <typename T, int C, bool WIDE>
 int la_sizes(const LaArgs& a, int mode, int64_t BH, hipStream_t stream) {
   if (a.dk <= 64)
-    return a.dv <= 64 ? la_modes<T, C, 64, 64>(a, mode, BH, stream)
-                      : la_modes<T, C, 64, 128>(a, mode, BH, stream);
-  return a.dv <= 64 ? la_modes<T, C, 128, 64>(a, mode, BH, stream)
-                    : la_modes<T, C, 128, 128>(a, mode, BH, stream);
+    return a.dv <= 64 ? la_modes<T, C, 64, 64, WIDE>(a, mode, BH, stream)
+                      : la_modes<T, C, 64, 128, WIDE>(a, mode, BH, stream);
+  return a.dv <= 64 ? la_modes<T, C, 128, 64, WIDE>(a, mode, BH, stream)
+                    : la_modes<T, C, 128, 128, WIDE>(a, mode, BH, stream);
+}
+// Rows made of whole aligned 16-byte vectors, close enough that a chunk's offsets fit 32 bits.
+bool la_wide(const void* p, const int64_t (&s)[3], int d, int ve) {
+  return !p || ((((uintptr_t)p) & 15) == 0 && d % ve == 0 && s[0] % ve == 0 && s[1] % ve == 0 &&
+                s[2] % ve == 0 && s[1] >= 0 && s[1] < (1 << 24));
 }
 int la_run(int dtype, const LaArgs& a, int mode, int64_t BH, hipStream_t stream) {
-  return dtype ? la_sizes<u16, 64>(a, mode, BH, stream) : la_sizes<float, 32>(a, mode, BH, stream);
+  const int ve = dtype ? 8 : 4;
+  const auto al = [](const void* p) { return (((uintptr_t)p) & 15) == 0; };
+  const bool wide = la_wide(a.q, a.qs, a.dk, ve) && la_wide(a.k, a.ks, a.dk, ve) &&
+                    la_wide(a.v, a.vs, a.dv, ve) && la_wide(a.dout, a.ds, a.dv, ve) &&
+                    al(a.first) && al(a.last) && al(a.bound) && al(a.out) && al(a.out2) && al(a.part);
+  if (dtype)
+    return wide ? la_sizes<u16, 64, true>(a, mode, BH, stream)
+                : la_sizes<u16, 64, false>(a, mode, BH, stream);
+  return wide ? la_sizes<float, 32, true>(a, mode, BH, stream)
+              : la_sizes<float, 32, false>(a, mode, BH, stream);
 }
 
 void la_strides(int64_t (&to)[3], const int64_t* from) {
@@ -904,7 +1032,7 @@ size_t mg_linear_attention_workspace_bytes(int dtype, int64_t B, int64_t T, int 
                                            int dv) {
   if (!la_ok(dtype, B, T, H, Hk, dk, dv)) return 0;
   size_t n = mg_linear_attention_state_bytes(dtype, B, T, H, Hk, dk, dv);
-  n += mg_align_up((size_t)B * H * T * sizeof(float), 256);
+  n += 2 * mg_align_up((size_t)B * H * T * sizeof(float), 256);
   if (H != Hk) n += (size_t)B * T * H * dk * sizeof(float);
   return n;
 }
@@ -962,13 +1090,15 @@ int mg_linear_attention_bwd(int dtype, const void* q, const void* k, const void*
   at += la_bound_bytes(p, BH, dk, dv);
   a.decay = (float*)at;
   at += la_decay_bytes(p, BH) + 256;
-  a.e = (float*)at;
+  float* const queries = (float*)at;
+  at += mg_align_up((size_t)BH * T * sizeof(float), 256);
+  float* const keys = (float*)at;
   at += mg_align_up((size_t)BH * T * sizeof(float), 256);
   float* const part = a.group > 1 ? (float*)at : nullptr;
   // dq, and the queries' side of e, from the first segment on
   a.bound = (float*)state;
   a.first = h0, a.last = nullptr;
-  a.out = dq, a.part = part;
+  a.out = dq, a.part = part, a.e = queries;
   int rc = la_run(dtype, a, LA_DQ, BH, stream);
   if (rc == MG_OK && part) rc = la_sum_run(dtype, part, dq, B * T * Hk * dk, a.group, dk, stream);
   // dk, dv, and the keys' side, from the last one back
@@ -978,13 +1108,13 @@ int mg_linear_attention_bwd(int dtype, const void* q, const void* k, const void*
     if (rc == MG_OK) rc = la_join_run(dhT, adjoints, a.decay, BH, ss, p.segs - 1, 1, stream);
   }
   a.first = dhT, a.last = dh0;
-  a.out = dk_, a.out2 = dv_;
+  a.out = dk_, a.out2 = dv_, a.e = keys;
   if (rc == MG_OK) rc = la_run(dtype, a, LA_DKV, BH, stream);
   if (rc == MG_OK && part) rc = la_sum_run(dtype, part, dk_, B * T * Hk * dk, a.group, dk, stream);
   if (rc != MG_OK) return rc;
-  a.first = hT;
+  a.first = hT, a.e = queries;
   hipLaunchKernelGGL(la_decay_grad, dim3((unsigned)BH, (unsigned)p.segs), dim3(256), 0, stream, a,
-                     (const float*)state, (const float*)adjoints, dhT, dg, p.C);
+                     (const float*)state, (const float*)adjoints, dhT, keys, dg, p.C);
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
 
