@@ -75,26 +75,47 @@ struct LaArgs {
   float* e;             // (BH, T): what the queries (keys) add to the gradient of G
 };
 
+// ---- elements --------------------------------------------------------------------------
+__device__ __forceinline__ float to_f(u16 x) { return __uint_as_float((unsigned)x << 16); }
+__device__ __forceinline__ float to_f(float x) { return x; }
+// Two values rounded to bf16 by one packed conversion; the empty asm keeps it one.
+__device__ __forceinline__ unsigned pack2(float x, float y) {
+  const bf16x2 h = {(__bf16)x, (__bf16)y};
+  unsigned u = __builtin_bit_cast(unsigned, h);
+  asm("" : "+v"(u));
+  return u;
+}
+__device__ __forceinline__ float low(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+
 // ---- operands ------------------------------------------------------------------------
 // A matrix in LDS has rows of D elements without padding; the 16-byte chunk c of row r lies
-// at chunk c ^ swz(r).  swz spreads both kinds of fragment reads over all banks: one chunk of
-// 8 or 16 consecutive rows (near), and 16 columns of 4 rows in turn (far).
+// at chunk c ^ swz(r).  swz spreads both kinds of fragment reads over all 64 banks: 16 bytes of
+// 16 rows (near), which the LDS serves 16 lanes at a time -- 0-3, 12-15, 20-23 and 24-27
+// together, then 4-11, 16-19 and 28-31, then the same of the upper half --, and 16 columns of 4
+// rows in turn (far), 32 lanes at a time.
 template <typename T>
 struct Op;
 
 template <typename T, int D>
 __device__ __forceinline__ int place(int r, int c) {
   constexpr int CE = Op<T>::VE;
-  return r * D + (((c / CE) ^ (Op<T>::swz(r) & (D / CE - 1))) * CE | c % CE);
+  return r * D + (((c / CE) ^ Op<T>::template swz<D / CE>(r)) * CE | c % CE);
 }
 
 template <>
 struct Op<u16> {
   typedef bf16x8 Frag;
   static constexpr int KB = 32, VE = 8, PLANES = 3, HALVES = 2;
+  template <int CHUNKS>
   static __device__ __forceinline__ int swz(int r) {
-    return ((r & 3) << 1) | ((r >> 2) & 1) | (r & 8);
+    const int x = ((r >> 2) ^ (r >> 3)) & 1;
+    if constexpr (CHUNKS >= 16) return ((r & 3) << 1) | ((r >> 3) & 1) | (x << 3);
+    else return (r & 2) | (x << 2) | ((r >> 2) & 1);
   }
+  // swz(r) ^ swz(r + 4) of a row r whose bit 2 is clear, in elements.
+  template <int D>
+  static constexpr int FOUR = (D / VE >= 16 ? 8 : 5) * VE;
   // Lane offsets of fragment reads; row and column of the tile and k0 are added by frag_*.
   template <int D>
   static __device__ __forceinline__ int near_base() {
@@ -116,7 +137,7 @@ struct Op<u16> {
   static __device__ __forceinline__ Frag far(const u16* m, int base, int c0, int k0) {
     typedef __attribute__((address_space(3))) s16x4* lds_t;
     const u16* p = m + (base ^ c0) + k0 * D;
-    const u16* p4 = m + (base ^ c0 ^ 8) + (k0 + 4) * D;
+    const u16* p4 = m + (base ^ c0 ^ FOUR<D>) + (k0 + 4) * D;
     const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)p);
     const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)p4);
     const s16x8 x = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -125,13 +146,34 @@ struct Op<u16> {
   static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
+  // A fragment times w[contracted index], in planes.
+  static __device__ __forceinline__ void scaled(Frag b, const float* w, Frag (&to)[PLANES]) {
+    const uint4 u = __builtin_bit_cast(uint4, b);
+    const unsigned v[4] = {u.x, u.y, u.z, u.w};
+    unsigned o[PLANES][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x = low(v[i]) * w[2 * i], y = high(v[i]) * w[2 * i + 1];
+#pragma unroll
+      for (int p = 0; p < PLANES; ++p) {
+        o[p][i] = pack2(x, y);
+        x -= low(o[p][i]), y -= high(o[p][i]);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p)
+      to[p] = __builtin_bit_cast(Frag, make_uint4(o[p][0], o[p][1], o[p][2], o[p][3]));
+  }
 };
 
 template <>
 struct Op<float> {
   typedef f32x4 Frag;
   static constexpr int KB = 16, VE = 4, PLANES = 1, HALVES = 1;
-  static __device__ __forceinline__ int swz(int r) { return r & 15; }
+  template <int CHUNKS>
+  static __device__ __forceinline__ int swz(int r) {
+    return r & 15 & (CHUNKS - 1);
+  }
   template <int D>
   static __device__ __forceinline__ int near_base() {
     const int l = threadIdx.x & 63;
@@ -157,6 +199,10 @@ struct Op<float> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
     return c;
+  }
+  static __device__ __forceinline__ void scaled(Frag b, const float* w, Frag (&to)[PLANES]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[0][i] = b[i] * w[i];
   }
 };
 
@@ -208,6 +254,33 @@ __device__ __forceinline__ void product(f32x4 (&acc)[Ti::TM][Ti::TN], const T* c
   }
 }
 
+// acc += V^T (w K): rows of the contracted index both, K's (free index N) times w in all planes.
+template <typename T, typename Ti, int C, int LV, int LK>
+__device__ __forceinline__ void take_up(f32x4 (&acc)[Ti::TM][Ti::TN], const T* V, const T* K,
+                                        const float* w) {
+  typedef Op<T> O;
+  constexpr int PL = O::PLANES, KL = O::KB / 4;  // contracted elements of a lane
+  const int ab = O::template far_base<LV>(), bb = O::template far_base<LK>();
+  const float* const wl = w + KL * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+  for (int k0 = 0; k0 < C; k0 += O::KB) {
+    typename O::Frag a[Ti::TM], b[Ti::TN][PL];
+    float x[KL];
+#pragma unroll
+    for (int i = 0; i < KL; ++i) x[i] = wl[k0 + i];
+#pragma unroll
+    for (int t = 0; t < Ti::TN; ++t) O::scaled(O::template far<LK>(K, bb, Ti::n0(t), k0), x, b[t]);
+#pragma unroll
+    for (int t = 0; t < Ti::TM; ++t) a[t] = O::template far<LV>(V, ab, Ti::m0(t), k0);
+#pragma unroll
+    for (int p = 0; p < PL; ++p)
+#pragma unroll
+      for (int i = 0; i < Ti::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < Ti::TN; ++j) acc[i][j] = O::mma(a[i], b[j][p], acc[i][j]);
+  }
+}
+
 template <typename Ti>
 __device__ __forceinline__ void clear(f32x4 (&acc)[Ti::TM][Ti::TN]) {
 #pragma unroll
@@ -215,19 +288,6 @@ __device__ __forceinline__ void clear(f32x4 (&acc)[Ti::TM][Ti::TN]) {
 #pragma unroll
     for (int j = 0; j < Ti::TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
-
-// ---- elements --------------------------------------------------------------------------
-__device__ __forceinline__ float to_f(u16 x) { return __uint_as_float((unsigned)x << 16); }
-__device__ __forceinline__ float to_f(float x) { return x; }
-// Two values rounded to bf16 by one packed conversion; the empty asm keeps it one.
-__device__ __forceinline__ unsigned pack2(float x, float y) {
-  const bf16x2 h = {(__bf16)x, (__bf16)y};
-  unsigned u = __builtin_bit_cast(unsigned, h);
-  asm("" : "+v"(u));
-  return u;
-}
-__device__ __forceinline__ float low(unsigned u) { return __uint_as_float(u << 16); }
-__device__ __forceinline__ float high(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
 
 // x in planes of 8 bits each, from plane FIRST on: what is left after each rounding is exact.
 template <int FIRST, int PL>
@@ -304,7 +364,7 @@ struct Block {
     }
   }
   __device__ __forceinline__ void mask(int rows, int d) {
-    if constexpr (WIDE) {
+    if (WIDE && (rows < C || d < D)) {
 #pragma unroll
       for (int n = 0; n < N; ++n)
         if (row(n) >= rows || col(n) >= d) x[n] = make_uint4(0u, 0u, 0u, 0u);
@@ -313,26 +373,6 @@ struct Block {
   __device__ __forceinline__ void put(T* m) const {
 #pragma unroll
     for (int n = 0; n < N; ++n) *reinterpret_cast<uint4*>(m + place<T, D>(row(n), col(n))) = x[n];
-  }
-  __device__ __forceinline__ void get(const T* m) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) x[n] = *reinterpret_cast<const uint4*>(m + place<T, D>(row(n), col(n)));
-  }
-  // Rows times weight(row), in all planes.
-  template <int PL, typename W>
-  __device__ __forceinline__ void put_scaled(T* const (&m)[PL], W&& weight) const {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const float s = weight(row(n));
-      T e[VE];
-      __builtin_memcpy(e, &x[n], 16);
-#pragma unroll
-      for (int i = 0; i < VE; i += 4) {
-        const f32x4 y = {s * to_f(e[i]), s * to_f(e[i + 1]), s * to_f(e[i + 2]),
-                         s * to_f(e[i + 3])};
-        put4<0, PL>(m, place<T, D>(row(n), col(n)) + i, y);
-      }
-    }
   }
 };
 
@@ -361,10 +401,12 @@ __device__ __forceinline__ double lane_of(double x, int l) {
       double, make_int2(__builtin_amdgcn_readlane(u.x, l), __builtin_amdgcn_readlane(u.y, l)));
 }
 
-// One wave: lane i forms the chunk's i-th gate from its g (0 past the sequence).  The prefix
-// sums take steps of 1, 2, 4 and 8 lanes in each row of 16, then the rows' totals.
-template <int C>
-__device__ __forceinline__ void make_gates(Gate* out, float g) {
+// One wave: lane i forms the chunk's i-th gate from its g (0 past the sequence), and the
+// factor that its row is taken up into the state with: exp(G_C - G_i) for keys, scale exp(G_i)
+// for queries.  The prefix sums take steps of 1, 2, 4 and 8 lanes in each row of 16, then the
+// rows' totals.
+template <int C, bool REV>
+__device__ __forceinline__ void make_gates(Gate* out, float* w, float g, float scale) {
   const int l = threadIdx.x & 63, row = l >> 4;
   constexpr double LOG2E = 1.4426950408889634;
   double s = (double)g * LOG2E;
@@ -378,51 +420,58 @@ __device__ __forceinline__ void make_gates(Gate* out, float g) {
   const double a = lane_of(s, 15), b = lane_of(s, 31), c = lane_of(s, 47);
   s += (row > 0 ? a : 0.0) + (row > 1 ? b : 0.0) + (row > 2 ? c : 0.0);
   const float hi = (float)s;
-  if (l < C) out[l] = Gate{hi, (float)(s - (double)hi), n, 0.f};
+  const Gate me = {hi, (float)(s - (double)hi), n, 0.f};
+  if constexpr (REV) {
+    if (l < C) w[l] = scale * span0(me);
+  } else {
+    const auto last = [](float x) {
+      return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), C - 1));
+    };
+    const Gate end = {last(me.hi), last(me.lo), last(me.n), 0.f};
+    if (l < C) w[l] = span(end, me);
+  }
+  if (l < C) out[l] = me;
 }
 
 // ---- the sweep -------------------------------------------------------------------------------
-// LDS, in elements.  In the gradients' sweeps the two leading planes of the state lie in S[0],
-// S[1]; once they are read the third lies in S[0] and the decayed rows' leading planes in
-// S[1], their third one in place of the rows themselves.
+// LDS, in elements.  The plain sweeps have two sets of a chunk's operands where they fit, one
+// being filled while the other is used (TWO).  The gradients' have one; the state's two leading planes lie in S
+// and S1, and once they are read the third lies in S.
 template <typename T, int C, int DK, int DV, int MODE>
 struct Lds {
-  static constexpr int PL = Op<T>::PLANES, HV = Op<T>::HALVES;
+  static constexpr int HV = Op<T>::HALVES;
   static constexpr bool GRAD = MODE == LA_DQ || MODE == LA_DKV;
   static constexpr bool BARE = MODE == LA_STATE || MODE == LA_RSTATE;
-  static constexpr int Q = 0;  // queries
-  static constexpr int K = Q + (BARE ? 0 : C * DK);
-  static constexpr int V = K + (BARE ? 0 : C * DK);
-  static constexpr int O = V + C * DV;  // output gradients
-  static constexpr int P = O + (GRAD ? C * DV : 0);
+  static constexpr int K = 0;  // keys (LA_RSTATE: queries)
+  static constexpr int V = K + C * DK;  // values (LA_RSTATE: output gradients)
+  static constexpr int Q = V + C * DV;
+  static constexpr int O = Q + (BARE ? 0 : C * DK);
+  static constexpr int SET = O + (GRAD ? C * DV : 0);
+  static constexpr int REST = (BARE ? 0 : C * C + DK * DV);
+  static constexpr bool TWO = !GRAD && (2 * SET + REST) * (int)sizeof(T) <= 156 * 1024;
+  static constexpr int P = SET * (TWO ? 2 : 1);
   static constexpr int P2 = P + (BARE ? 0 : C * C);
-  static constexpr int S = P2 + (MODE == LA_DKV ? C * C : 0);
+  static constexpr int S = P2 + (MODE == LA_DKV ? C * C : 0);  // state
   static constexpr int S1 = S + (BARE ? 0 : DK * DV);
-  static constexpr int STATE = DK * DV * (HV - 1), ROWS = C * DK * HV;
-  static constexpr int W = GRAD && PL == 1 ? S : S1;  // decayed keys or queries
-  static constexpr int END =
-      GRAD ? (PL == 1 ? S + (DK * DV > C * DK ? DK * DV : C * DK) : S1 + (STATE > ROWS ? STATE : ROWS))
-           : W + C * DK * PL;
-  static constexpr int BYTES = END * (int)sizeof(T);
+  static constexpr int BYTES = (S1 + (GRAD ? DK * DV * (HV - 1) : 0)) * (int)sizeof(T);
 };
 
 template <typename T, int C, int DK, int DV, int MODE, bool WIDE>
 __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
   typedef Lds<T, C, DK, DV, MODE> L;
-  constexpr int PL = L::PL;
-  constexpr bool REV = MODE == LA_RSTATE || MODE == LA_DKV, BARE = L::BARE, GRAD = L::GRAD;
-  typedef Tiling<DV / 16, DK / 16, 2> TS;  // the state, transposed: M = dv, N = dk
+  constexpr int PL = Op<T>::PLANES;
+  constexpr bool REV = MODE == LA_RSTATE || MODE == LA_DKV, BARE = L::BARE, GRAD = L::GRAD, TWO = L::TWO;
+  typedef Tiling<DV / 16, DK / 16, DK >= 128 ? 1 : 2> TS;  // the state, transposed: M = dv, N = dk
   typedef Tiling<C / 16, C / 16, 4> TC;    // chunk matrices
   typedef Tiling<DK / 16, C / 16, 4> TK;   // (dk, token)
   typedef Tiling<DV / 16, C / 16, 4> TV;   // (dv, token)
   __shared__ __align__(16) char raw[L::BYTES];
   __shared__ Gate gates[2][C];
+  __shared__ __align__(16) float weights[2][C];
   // Sums over the chunk matrices' rows and columns, and rows' products with dq or dk, by wave.
   __shared__ float s_row[4][C], s_col[4][C], s_dot[4][C];
   T* const lds = reinterpret_cast<T*>(raw);
-  T *const sQ = lds + L::Q, *const sK = lds + L::K, *const sV = lds + L::V, *const sO = lds + L::O;
-  T *const sP = lds + L::P, *const sP2 = lds + L::P2, *const sS = lds + L::S, *const sW = lds + L::W;
-  T* const sS1 = lds + L::S1;
+  T *const sP = lds + L::P, *const sP2 = lds + L::P2, *const sS = lds + L::S, *const sS1 = lds + L::S1;
 
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int wave = mg_uniform(tid >> 6);
@@ -477,13 +526,16 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
     const int64_t t = at(n);
     return lane < rows_at(t) ? g[(t + lane) * a.gs[1]] : 0.f;
   };
+  const auto gates_of = [&](int n, float x) {
+    make_gates<C, REV>(gates[n & 1], weights[n & 1], x, a.scale);
+  };
   float g_next = 0.f;
   if (chunks > 0) {
     fetch(at(0));
     if (wave == 0) {
       const float g0 = decays(0);
       if (chunks > 1) g_next = decays(1);
-      make_gates<C>(gates[0], g0);
+      gates_of(0, g0);
     }
   }
   if constexpr (!BARE) {
@@ -507,67 +559,89 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
         }
       });
   }
+  // A fetched chunk, and the state in its leading planes, into LDS.
+  const auto put_chunk = [&](int n) {
+    T* const set = lds + (TWO ? (n & 1) * L::SET : 0);
+    const int rows = rows_at(at(n));
+    if constexpr (MODE != LA_RSTATE) {
+      bk.mask(rows, dk), bv.mask(rows, dv);
+      bk.put(set + L::K), bv.put(set + L::V);
+    }
+    if constexpr (MODE != LA_STATE) {
+      bq.mask(rows, dk);
+      bq.put(set + (MODE == LA_RSTATE ? L::K : L::Q));
+    }
+    if constexpr (GRAD || MODE == LA_RSTATE) {
+      bo.mask(rows, dv);
+      bo.put(set + (MODE == LA_RSTATE ? L::V : L::O));
+    }
+  };
+  const auto put_state = [&]() {
+    each_state([&](f32x4& x, int r, int c) {
+      const int p = place<T, DV>(r, c);
+      if constexpr (GRAD && PL > 1) {
+        T* const to[2] = {sS, sS1};
+        put4<0, 2>(to, p, x);
+      } else {
+        T* const to[1] = {sS};
+        put4<0, 1>(to, p, x);
+      }
+    });
+  };
+  // The finished chunk's part of the gradient of G, once its sums are there.
+  const auto put_e = [&](int n) {
+    const int64_t t = at(n);
+    if (tid < rows_at(t)) {
+      float x = 0.f;
+#pragma unroll
+      for (int u = 0; u < TK::WM; ++u) x += s_dot[u][tid];
+      if constexpr (MODE == LA_DQ) {
+#pragma unroll
+        for (int u = 0; u < TC::WM; ++u) x += s_row[u][tid];
+#pragma unroll
+        for (int u = 0; u < TC::WN && u < C / 16; ++u) x -= s_col[u][tid];
+      }
+      a.e[bh * T_ + t + tid] = x;
+    }
+  };
+  if constexpr (TWO)
+    if (chunks > 0) {
+      put_chunk(0);
+      if constexpr (!BARE) put_state();
+      if (chunks > 1) fetch(at(1));
+    }
   float fall = 1.f;  // the segment's decay so far
 
   for (int n = 0; n < chunks; ++n) {
     const int64_t t = at(n);
     const int rows = rows_at(t);
-    const Gate* ga = gates[n & 1];
-    __syncthreads();  // the gates; and the last chunk's operands are read
+    const Gate* const ga = gates[n & 1];
+    __syncthreads();  // the gates (and operands) are there; the last chunk's are read
+    if constexpr (!TWO) {
+      if constexpr (GRAD)
+        if (n > 0) put_e(n - 1);
+      put_chunk(n);
+      if constexpr (!BARE) put_state();
+      __syncthreads();
+      if (n + 1 < chunks) fetch(at(n + 1));
+    }
+    const T* const set = lds + (TWO ? (n & 1) * L::SET : 0);
+    const T *const sK = set + L::K, *const sV = set + L::V, *const sQ = set + L::Q,
+            *const sO = set + L::O;
     const Gate end = ga[C - 1];
     const float keep = span0(end);
-    const auto weight = [&](int r) { return REV ? a.scale * span0(ga[r]) : span(end, ga[r]); };
-    if constexpr (MODE != LA_STATE) bq.mask(rows, dk);
-    if constexpr (MODE != LA_RSTATE) bk.mask(rows, dk), bv.mask(rows, dv);
-    if constexpr (GRAD || MODE == LA_RSTATE) bo.mask(rows, dv);
-    if constexpr (!BARE) {
-      bq.put(sQ);
-      bk.put(sK);
-      if constexpr (GRAD) bo.put(sO);
-      each_state([&](f32x4& x, int r, int c) {
-        const int p = place<T, DV>(r, c);
-        if constexpr (GRAD && PL > 1) {
-          T* const to[2] = {sS, sS1};
-          put4<0, 2>(to, p, x);
-        } else {
-          T* const to[1] = {sS};
-          put4<0, 1>(to, p, x);
-        }
-      });
-    }
-    if constexpr (MODE == LA_RSTATE) bo.put(sV);
-    else bv.put(sV);
-    if constexpr (!GRAD) {
-      T* to[PL];
-#pragma unroll
-      for (int p = 0; p < PL; ++p) to[p] = sW + p * C * DK;
-      if constexpr (MODE == LA_RSTATE) bq.put_scaled(to, weight);
-      else bk.put_scaled(to, weight);
-    }
-    __syncthreads();
-    if (n + 1 < chunks) {
-      fetch(at(n + 1));
-      if (wave == 0) {
-        make_gates<C>(gates[(n + 1) & 1], g_next);
-        if (n + 2 < chunks) g_next = decays(n + 2);
-      }
-    }
-    const auto update = [&](const T* rows_v, const T* const (&w)[PL]) {
+    const auto update = [&](const T* rows_v, const T* rows_k) {
 #pragma unroll
       for (int i = 0; i < TS::TM; ++i)
 #pragma unroll
         for (int j = 0; j < TS::TN; ++j) S[i][j] *= keep;
-      const T* const av[1] = {rows_v};
-      product<T, TS, C, true, true, DV, DK, 1, PL>(S, av, w);
+      take_up<T, TS, C, DV, DK>(S, rows_v, rows_k, weights[n & 1]);
       fall *= keep;
     };
-    if constexpr (!GRAD) {
-      const T* w[PL];
-#pragma unroll
-      for (int p = 0; p < PL; ++p) w[p] = sW + p * C * DK;
-      update(sV, w);
+    if (wave == 0 && n + 1 < chunks) {
+      gates_of(n + 1, g_next);
+      if (n + 2 < chunks) g_next = decays(n + 2);
     }
-
     f32x4 ack[TK::TM][TK::TN], acv[TV::TM][TV::TN];
     if constexpr (!BARE) {
       // Chunk matrices, M the token that is contracted next, N the other: (j, i) towards the
@@ -646,8 +720,9 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
           product<T, TK, DV, false, false, DV, DV, 1, 1>(ack, ps, REV ? pv : po);
         }
       }
-      __syncthreads();  // the chunk matrices are there, the state's leading planes are read
     }
+    if constexpr (!GRAD) update(sV, sK);
+    if constexpr (!BARE) __syncthreads();  // the chunk matrices are there, the state is read
 
     const auto out_v = [&](T* to, const T* far, auto&& factor) {
       f32x4 in[TV::TM][TV::TN];
@@ -655,13 +730,13 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
       const T *const af[1] = {far}, *const pp[1] = {sP};
       product<T, TV, C, true, false, DV, C, 1, 1>(in, af, pp);
       if (TV::live()) {
-        T* const base = to + ((b * T_ + t) * a.H + h) * (int64_t)dv;
+        T* const base = to + ((b * T_ + t) * a.H + h) * dv;
 #pragma unroll
         for (int j = 0; j < TV::TN; ++j) {
           const int i = TV::n0(j) + lr;
           const float f = factor(i);
           if (i < rows) {
-            T* const p = base + (int64_t)i * a.H * dv;
+            T* const p = base + (unsigned)i * (unsigned)(a.H * dv);
 #pragma unroll
             for (int m = 0; m < TV::TM; ++m)
               store4<WIDE>(p, TV::m0(m) + 4 * lg, dv, in[m][j] + f * acv[m][j]);
@@ -691,12 +766,14 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
         product<T, TK, DV, false, false, DV, DV, 1, 1>(ack, third, rv);
       }
       if (TK::live()) {
-        const int64_t base = ((b * T_ + t) * a.H + h) * (int64_t)dk;
+        const int64_t base = ((b * T_ + t) * a.H + h) * dk;
+        float* const part = a.part + base;
+        T* const out = (T*)a.out + base;
 #pragma unroll
         for (int j = 0; j < TK::TN; ++j) {
           const int i = TK::n0(j) + lr;
           const float f = REV ? span(end, ga[i]) : a.scale * span0(ga[i]);
-          const int64_t row = base + (int64_t)i * a.H * dk;
+          const unsigned row = (unsigned)i * (unsigned)(a.H * dk);
           float dot = 0.f;
 #pragma unroll
           for (int m = 0; m < TK::TM; ++m) {
@@ -705,41 +782,27 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) dot += y[u] * x[u];
             if (i < rows) {
-              if (a.part) store4<WIDE>(a.part + row, c, dk, y + in[m][j]);
-              else store4<WIDE>((T*)a.out + row, c, dk, y + in[m][j]);
+              if (a.part) store4<WIDE>(part + row, c, dk, y + in[m][j]);
+              else store4<WIDE>(out + row, c, dk, y + in[m][j]);
             }
           }
           dot = mg_pair_sum<32>(mg_pair_sum<16>(dot));
           if (lane < 16) s_dot[TK::wm()][i] = dot;
         }
       }
-      // The rows the state takes up, decayed; the third plane in their own place.
-      Block<T, C, DK, WIDE> w;
-      w.get(REV ? sQ : sK);
-      T* to[PL];
-      const T* from[PL];
-#pragma unroll
-      for (int p = 0; p < PL; ++p) {
-        to[p] = p == 2 ? (REV ? sQ : sK) : sW + p * C * DK;
-        from[p] = to[p];
-      }
-      w.put_scaled(to, weight);
-      __syncthreads();
-      if (tid < rows) {
-        float x = 0.f;
-#pragma unroll
-        for (int u = 0; u < TK::WM; ++u) x += s_dot[u][tid];
-        if constexpr (MODE == LA_DQ) {
-#pragma unroll
-          for (int u = 0; u < TC::WM; ++u) x += s_row[u][tid];
-#pragma unroll
-          for (int u = 0; u < TC::WN && u < C / 16; ++u) x -= s_col[u][tid];
-        }
-        a.e[bh * T_ + t + tid] = x;
-      }
-      update(REV ? sO : sV, from);
+      update(REV ? sO : sV, REV ? sQ : sK);
+    }
+    if (TWO && n + 1 < chunks) {
+      if constexpr (!BARE) put_state();
+      put_chunk(n + 1);
+      if (n + 2 < chunks) fetch(at(n + 2));
     }
   }
+  if constexpr (GRAD)
+    if (chunks > 0) {
+      __syncthreads();
+      put_e(chunks - 1);
+    }
 
   float* to = nullptr;
   if constexpr (BARE) {
@@ -924,7 +987,7 @@ constexpr int LA_MAXD = 128;
 
 bool la_ok(int dtype, int64_t B, int64_t T, int H, int Hk, int dk, int dv) {
   return !(dtype & ~1) && B >= 1 && T >= 1 && H >= 1 && Hk >= 1 && H % Hk == 0 && dk >= 1 &&
-         dv >= 1 && dk <= LA_MAXD && dv <= LA_MAXD && H <= (1 << 20) &&
+         dv >= 1 && dk <= LA_MAXD && dv <= LA_MAXD && H <= (1 << 16) &&
          B * H <= (1ll << 24) && T <= (1ll << 32);
 }
 
