@@ -289,20 +289,22 @@ __device__ __forceinline__ void clear(f32x4 (&acc)[Ti::TM][Ti::TN]) {
     for (int j = 0; j < Ti::TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
-// x in planes of 8 bits each, from plane FIRST on: what is left after each rounding is exact.
-template <int FIRST, int PL>
-__device__ __forceinline__ void put4(u16* const (&to)[PL], int at, f32x4 x) {
-  static_assert(FIRST >= 0 && PL >= 1, "planes");
-#pragma unroll
-  for (int p = 0; p < FIRST + PL; ++p) {
-    const unsigned a = pack2(x[0], x[1]), b = pack2(x[2], x[3]);
-    if (p >= FIRST) *reinterpret_cast<uint2*>(to[p < FIRST ? 0 : p - FIRST] + at) = make_uint2(a, b);
-    x[0] -= low(a), x[1] -= high(a), x[2] -= low(b), x[3] -= high(b);
-  }
+// Four consecutive elements to LDS, rounded; in planes of 8 bits each, the third returned:
+// what is left after each rounding is exact.
+__device__ __forceinline__ void put4(u16* p, f32x4 x) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
 }
-template <int FIRST, int PL>
-__device__ __forceinline__ void put4(float* const (&to)[PL], int at, f32x4 x) {
-  *reinterpret_cast<f32x4*>(to[0] + at) = x;
+__device__ __forceinline__ void put4(float* p, f32x4 x) { *reinterpret_cast<f32x4*>(p) = x; }
+__device__ __forceinline__ uint2 put4_split(u16* p0, u16* p1, f32x4 x) {
+  uint2 u;
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+    u = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
+    if (p == 0) *reinterpret_cast<uint2*>(p0) = u;
+    if (p == 1) *reinterpret_cast<uint2*>(p1) = u;
+    if (p < 2) x[0] -= low(u.x), x[1] -= high(u.x), x[2] -= low(u.y), x[3] -= high(u.y);
+  }
+  return u;
 }
 __device__ __forceinline__ f32x4 get4(const u16* p) {
   const uint2 u = *reinterpret_cast<const uint2*>(p);
@@ -502,12 +504,15 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
   f32x4 S[TS::TM][TS::TN];
   clear<TS>(S);
   const int64_t ss = (int64_t)dk * dv;
-  const auto each_state = [&](auto&& f) {
+  const auto each_tile = [&](auto&& f) {
 #pragma unroll
     for (int i = 0; i < TS::TM; ++i)
 #pragma unroll
       for (int j = 0; j < TS::TN; ++j)
-        if (TS::live()) f(S[i][j], TS::n0(j) + lr, TS::m0(i) + 4 * lg);
+        if (TS::live()) f(i, j, TS::n0(j) + lr, TS::m0(i) + 4 * lg);
+  };
+  const auto each_state = [&](auto&& f) {
+    each_tile([&](int i, int j, int r, int c) { f(S[i][j], r, c); });
   };
 
   Block<T, C, DK, WIDE> bq, bk;
@@ -576,16 +581,12 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
       bo.put(set + (MODE == LA_RSTATE ? L::V : L::O));
     }
   };
+  uint2 third[TS::TM][TS::TN];  // the third plane, until there is room for it
   const auto put_state = [&]() {
-    each_state([&](f32x4& x, int r, int c) {
+    each_tile([&](int i, int j, int r, int c) {
       const int p = place<T, DV>(r, c);
-      if constexpr (GRAD && PL > 1) {
-        T* const to[2] = {sS, sS1};
-        put4<0, 2>(to, p, x);
-      } else {
-        T* const to[1] = {sS};
-        put4<0, 1>(to, p, x);
-      }
+      if constexpr (GRAD && PL > 1) third[i][j] = put4_split(sS + p, sS1 + p, S[i][j]);
+      else put4(sS + p, S[i][j]);
     });
   };
   // The finished chunk's part of the gradient of G, once its sums are there.
@@ -687,9 +688,8 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
                 col[im][x] += xs;
               }
             }
-            T *const to[1] = {sP}, *const to2[1] = {sP2};
-            put4<0, 1>(to, place<T, C>(nn, mm), p);
-            if constexpr (MODE == LA_DKV) put4<0, 1>(to2, place<T, C>(nn, mm), p2);
+            put4(sP + place<T, C>(nn, mm), p);
+            if constexpr (MODE == LA_DKV) put4(sP2 + place<T, C>(nn, mm), p2);
           }
           if constexpr (MODE == LA_DQ) {
             row = mg_pair_sum<32>(mg_pair_sum<16>(row));
@@ -754,12 +754,10 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
       clear<TK>(in);
       const T *const rk[1] = {REV ? sQ : sK}, *const pp[1] = {REV ? sP2 : sP};
       product<T, TK, C, true, false, DK, C, 1, 1>(in, rk, pp);
-      if constexpr (PL > 1) {
-        each_state([&](f32x4& x, int r, int c) {
-          T* const to[1] = {sS};
-          put4<2, 1>(to, place<T, DV>(r, c), x);
+      if constexpr (PL > 1)
+        each_tile([&](int i, int j, int r, int c) {
+          *reinterpret_cast<uint2*>(sS + place<T, DV>(r, c)) = third[i][j];
         });
-      }
       __syncthreads();  // the chunk's rows are read, the third plane is there
       if constexpr (PL > 1) {
         const T *const third[1] = {sS}, *const rv[1] = {REV ? sV : sO};
@@ -851,27 +849,35 @@ __global__ __launch_bounds__(256) void la_join(const float* __restrict__ first,
 
 // e: the queries' side less the keys'.  dg_t = sum of e from t to its segment's end + <R, S> there; 0 past a sequence's length and
 // at steps that start over.
-__global__ __launch_bounds__(256) void la_decay_grad(LaArgs a, const float* states,
-                                                     const float* adjoints, const float* last_r,
-                                                     const float* __restrict__ keys,
-                                                     float* __restrict__ dg, int C) {
-  __shared__ double s_e[4];
-  __shared__ float s_t[4];
+// A workgroup of 16 waves takes a segment: at fewer the product's loads wait for one another
+// (4 waves: 35 us at 128 heads of 2048 tokens, 16: 9).
+constexpr int DG_NT = 1024, DG_W = DG_NT / MG_WAVE;
+__global__ __launch_bounds__(DG_NT) void la_decay_grad(LaArgs a, const float* states,
+                                                       const float* adjoints, const float* last_r,
+                                                       const float* __restrict__ keys,
+                                                       float* __restrict__ dg, int C) {
+  __shared__ double s_e[DG_W];
+  __shared__ float s_t[DG_W];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, seg = blockIdx.y;
-  const int64_t bh = blockIdx.x, ss = (int64_t)a.dk * a.dv;
-  const int b = (int)(bh / a.H), h = (int)(bh % a.H);
+  const int64_t bh = blockIdx.x;
+  const int ss = a.dk * a.dv;
+  const int64_t b = bh / a.H;
+  const int h = (int)(bh % a.H);
   const bool final = seg == a.segs - 1;
   const float* S = final ? a.first + bh * ss : states + (bh * (a.segs - 1) + seg) * ss;
   const float* R = final ? (last_r ? last_r + bh * ss : nullptr)
                          : adjoints + (bh * (a.segs - 1) + seg) * ss;
   double E = 0.0;
   if (R) {
-    for (int64_t x = tid; x < ss; x += 256) E += (double)S[x] * (double)R[x];
+#pragma unroll 4
+    for (int x = tid; x < ss; x += DG_NT) E += (double)S[x] * (double)R[x];
 #pragma unroll
     for (int d = 32; d; d /= 2) E += __shfl_xor(E, d);
     if (lane == 0) s_e[w] = E;
     __syncthreads();
-    E = (s_e[0] + s_e[1]) + (s_e[2] + s_e[3]);
+    E = 0.0;
+#pragma unroll
+    for (int i = 0; i < DG_W; ++i) E += s_e[i];
   }
   int64_t len = a.T;
   if (a.lengths) {
@@ -881,17 +887,21 @@ __global__ __launch_bounds__(256) void la_decay_grad(LaArgs a, const float* stat
   const int64_t t0 = (int64_t)seg * a.per * C;
   const int64_t t1 = t0 + (int64_t)a.per * C < a.T ? t0 + (int64_t)a.per * C : a.T;
   const float* g = a.g + b * a.gs[0] + h * a.gs[2];
-  for (int64_t hi = t1; hi > t0; hi -= 256) {
-    const int64_t t = hi - 256 + tid;
+  for (int64_t hi = t1; hi > t0; hi -= DG_NT) {
+    const int64_t t = hi - DG_NT + tid;
     const float e = t >= t0 ? a.e[bh * a.T + t] - keys[bh * a.T + t] : 0.f;
-    float s = mg_wave_suffix_sum(e);
+    const float gt = t >= t0 ? g[t * a.gs[1]] : 0.f;
+    const float s = mg_wave_suffix_sum(e);
     if (lane == 0) s_t[w] = s;
     __syncthreads();
     double later = E;
-    for (int i = w + 1; i < 4; ++i) later += (double)s_t[i];
-    E += ((double)s_t[0] + (double)s_t[1]) + ((double)s_t[2] + (double)s_t[3]);
+#pragma unroll
+    for (int i = 0; i < DG_W; ++i) {
+      if (i > w) later += (double)s_t[i];
+      E += (double)s_t[i];
+    }
     if (t >= t0) {
-      const bool off = t >= len || (double)g[t * a.gs[1]] * 1.4426950408889634 < -126.0;
+      const bool off = t >= len || (double)gt * 1.4426950408889634 < -126.0;
       dg[(b * a.T + t) * a.H + h] = off ? 0.f : (float)(later + (double)s);
     }
     __syncthreads();
@@ -1176,7 +1186,7 @@ int mg_linear_attention_bwd(int dtype, const void* q, const void* k, const void*
   if (rc == MG_OK && part) rc = la_sum_run(dtype, part, dk_, B * T * Hk * dk, a.group, dk, stream);
   if (rc != MG_OK) return rc;
   a.first = hT, a.e = queries;
-  hipLaunchKernelGGL(la_decay_grad, dim3((unsigned)BH, (unsigned)p.segs), dim3(256), 0, stream, a,
+  hipLaunchKernelGGL(la_decay_grad, dim3((unsigned)BH, (unsigned)p.segs), dim3(DG_NT), 0, stream, a,
                      (const float*)state, (const float*)adjoints, dhT, keys, dg, p.C);
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
