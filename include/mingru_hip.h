@@ -497,6 +497,26 @@ int mg_linear_attention_step(int dtype, const void* q, const void* k, const void
                              int64_t B, int H, int Hk, int dk, int dv, float scale,
                              mg_stream_t stream);
 
+/* ---- softmax cross entropy over a vocabulary ----------------------------------------
+ * No reference kernels.  l = x w^T + bias; loss_n = log sum_v exp(l_nv) - l_n[target_n]; the
+ * logits are formed in tiles and never kept.  x (N, D) with ldx elements between rows, w (V, D)
+ * 16-byte aligned, bias (V) or NULL in dtype (0 fp32, 1 bf16).  Rows whose target is
+ * ignore_index are left out; another target outside the vocabulary gives a NaN.  reduction: 0
+ * none (loss (N)), 1 mean over the counted rows (0 if there are none), 2 sum.
+ * state: what the forward leaves for the backward.  Backward: dloss is (N) or a scalar; dx
+ * (N, D) and dw (V, D) with db (V) may be NULL, db only together with dw.  Sizes up to 2^30
+ * rows and entries and D up to 2^20. */
+size_t mg_vocab_loss_state_bytes(int dtype, int64_t N, int64_t V, int64_t D);
+size_t mg_vocab_loss_fwd_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D);
+size_t mg_vocab_loss_bwd_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D);
+int mg_vocab_loss_fwd(int dtype, const void* x, int64_t ldx, const void* w, const void* bias,
+                      const int64_t* target, int64_t ignore_index, int reduction, float* loss,
+                      int64_t N, int64_t V, int64_t D, void* state, size_t state_bytes, void* ws,
+                      size_t ws_bytes, mg_stream_t stream);
+int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* dloss,
+                      int reduction, void* dx, void* dw, void* db, int64_t N, int64_t V, int64_t D,
+                      const void* state, void* ws, size_t ws_bytes, mg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

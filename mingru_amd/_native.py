@@ -143,6 +143,16 @@ _SIGNATURES = {
     "mg_linear_attention_step": (
         _I32, [_I32] + [_P] * 4 + [_PI64] + [_P] * 3 + [_I64] + [_I32] * 4 + [_F32, _P],
     ),
+    "mg_vocab_loss_state_bytes": (_SZ, [_I32, _I64, _I64, _I64]),
+    "mg_vocab_loss_fwd_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64]),
+    "mg_vocab_loss_bwd_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64]),
+    "mg_vocab_loss_fwd": (
+        _I32,
+        [_I32, _P, _I64, _P, _P, _P, _I64, _I32, _P, _I64, _I64, _I64, _P, _SZ, _P, _SZ, _P],
+    ),
+    "mg_vocab_loss_bwd": (
+        _I32, [_I32, _P, _P, _P, _I32, _P, _P, _P, _I64, _I64, _I64, _P, _P, _SZ, _P],
+    ),
     "mg_residual_norm_workspace_bytes": (_SZ, [_I64, _I64]),
     "mg_residual_norm_fwd": (
         _I32, [_I32] * 5 + [_P, _I64] * 3 + [_P, _F32] + [_P] * 7 + [_I64, _I64, _F32, _P],

@@ -1,0 +1,804 @@
+// Softmax cross entropy over a vocabulary, logits never kept (gfx950).
+//
+//   l_n = W x_n + b,  loss_n = log sum_v exp(l_nv) - l_n[t_n]
+//   d_nv = g_n (exp(l_nv - lse_n) - [v = t_n]),  dx = d W,  dW = d^T x,  db = sum_n d_n
+//
+// Rows whose target is the ignored one are left out at the start: the others are packed one
+// after another (their values are never read, so a NaN there stays there), and every launch
+// ends at the packed count, which stays on the device.
+//
+// Forward: one product whose epilogue keeps, for each row and 128 columns of the vocabulary,
+// the largest logit and the sum of exponentials against it, and the target's logit; a second
+// launch joins them.  Backward, in pieces of the vocabulary: the product again, whose epilogue
+// turns the logits into d; then dx's share and dW's piece as products over d.  So 8 N V D
+// operations in place of 6 with kept logits: at D = 1024 a logit's recomputation costs less
+// than writing and reading it in fp32.
+//
+// Products: 256 x 256 tiles of the result, 4 waves of 128 x 128 each (v_mfma_f32_32x32x16_bf16,
+// all 256 accumulator registers), 64 contracted elements a step through two LDS buffers.  Wave
+// tiles that large keep the operands' LDS reads (16 KB for 32 K MFMA cycles of a wave) below
+// the matrix cores' time.  Operands are rows of the free index with the contracted one
+// consecutive (near), or the other way round (far, read with ds_read_b64_tr_b16): x, W and d
+// all lie in memory once, and each is near in one product and far in another.
+//
+// fp32 inputs are split into three bf16 planes (24 significant bits, exact) and a product takes
+// the six pairs of planes that reach 2^-24: six times the work of bf16, against sixteen times
+// for fp32's own matrix instruction.  bf16 inputs: d is rounded to bf16 once, sums are fp32.
+// With a bias, x has a column of ones behind its own, which makes db one more column of dW.
+#include "mg_common.h"
+
+namespace {
+
+typedef uint16_t u16;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int TILE = 256, BK = 64, NT = 256;
+constexpr int STAGE = TILE * BK;  // elements of one operand's step
+
+// ---- elements --------------------------------------------------------------------------
+__device__ __forceinline__ float to_f(u16 x) { return __uint_as_float((unsigned)x << 16); }
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ u16 to_bf(float x) { return __builtin_bit_cast(u16, (__bf16)x); }
+__device__ __forceinline__ unsigned pack2(float x, float y) {
+  const bf16x2 h = {(__bf16)x, (__bf16)y};
+  unsigned u = __builtin_bit_cast(unsigned, h);
+  asm("" : "+v"(u));
+  return u;
+}
+__device__ __forceinline__ float low(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+// What a plane leaves for the next ones; an infinity or NaN is the first plane's alone.
+__device__ __forceinline__ float rest(float x, u16 plane) {
+  const float r = x - to_f(plane);
+  return r == r ? r : 0.f;
+}
+
+// ---- packing ----------------------------------------------------------------------------
+// Counted rows in order: idx[j] the j-th one's row, pos[i] a row's place or -1, tgt[j] its
+// target, -1 where that lies outside the vocabulary.  One workgroup.
+__global__ __launch_bounds__(1024) void vl_index(const int64_t* __restrict__ target,
+                                                 int64_t ignore, int64_t V, int* __restrict__ idx,
+                                                 int* __restrict__ pos, int* __restrict__ tgt,
+                                                 int* __restrict__ count, int N) {
+  __shared__ int s_n[16];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  int base = 0;
+  for (int i0 = 0; i0 < N; i0 += 1024) {
+    const int i = i0 + tid;
+    const int64_t t = i < N ? target[i] : ignore;
+    const bool in = i < N && t != ignore;
+    const unsigned long long m = __ballot(in);
+    __syncthreads();
+    if (lane == 0) s_n[w] = __popcll(m);
+    __syncthreads();
+    int at = base, all = 0;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      at += u < w ? s_n[u] : 0;
+      all += s_n[u];
+    }
+    at += __popcll(m & ((1ull << lane) - 1));
+    if (in) idx[at] = i, tgt[at] = t >= 0 && t < V ? (int)t : -1;
+    if (i < N) pos[i] = in ? at : -1;
+    base += all;
+  }
+  if (tid == 0) *count = base;
+}
+
+// Rows of `cols` elements in PL planes of bf16, `ld` elements a row, 0 past the columns except
+// a 1 at `ones`.  idx: the counted rows, padded with rows of 0 to a whole tile; null: all rows.
+template <typename E, int PL>
+__global__ __launch_bounds__(256) void vl_pack(const E* __restrict__ src, int64_t lds_, int cols,
+                                               u16* __restrict__ dst, int ld, int64_t plane,
+                                               const int* __restrict__ idx,
+                                               const int* __restrict__ count, int64_t rows,
+                                               int ones) {
+  const int64_t j = blockIdx.x;
+  const int64_t n = count ? *count : rows;
+  if (j >= (n + TILE - 1) / TILE * TILE) return;
+  const bool live = j < n;
+  const E* s = src + (live ? (idx ? (int64_t)idx[j] : j) * lds_ : 0);
+  for (int c = threadIdx.x * 2; c < ld; c += 512) {
+    float x = live && c < cols ? to_f(s[c]) : 0.f, y = live && c + 1 < cols ? to_f(s[c + 1]) : 0.f;
+    if (live && c == ones) x = 1.f;
+    if (live && c + 1 == ones) y = 1.f;
+#pragma unroll
+    for (int p = 0; p < PL; ++p) {
+      const u16 a = to_bf(x), b = to_bf(y);
+      *reinterpret_cast<unsigned*>(dst + p * plane + j * ld + c) = a | ((unsigned)b << 16);
+      x = rest(x, a), y = rest(y, b);
+    }
+  }
+}
+
+// ---- products -----------------------------------------------------------------------------
+enum { VL_LSE = 0, VL_D = 1, VL_OUT = 2 };
+
+struct VlArgs {
+  const u16 *A, *B;        // M's and N's operands
+  int64_t pa, pb;          // elements between their planes
+  int lda, ldb;            // elements between rows
+  int m_rows, n_rows;      // rows (near) or columns (far) that exist; read places are clamped
+  const int* m_count;      // on the device, in their place, if not null
+  const int* n_count;
+  const int* k_count;      // contracted elements on the device, or K
+  int K;                   // a multiple of the step
+  int ka;                  // of them that a far A has rows for
+  int mt, nt, splits;      // tiles, and parts of the contracted axis
+  // LSE and D: M the vocabulary from column v0 on, N the packed rows
+  int v0, V;               // piece's first column; vocabulary
+  const void* bias;
+  const int* tgt;
+  float2* part;            // LSE: (2 mt, n_ld) largest logit and sum of exponentials
+  float* tlogit;           // LSE: the target's logit
+  const float2* soft;      // D: of each row, its largest logit and 1 / its sum of exponentials
+  const float* g;          // D: of each row, the upstream gradient
+  u16* d;                  // D: (planes, n_ld, ldd)
+  int64_t pd;
+  int ldd, n_ld;
+  // OUT: out[n][m]
+  void* out;
+  int64_t ldo, po;         // elements between rows, between the splits' results
+  int m_out, n_out;        // what of it is written
+  void* extra;             // column m_out in a vector of its own
+  int out_f32;
+  int64_t pe;              // extra: elements between the splits'
+};
+
+// Fragment of 32 rows (near) or columns (far) x 16 contracted elements.  LDS: near rows of 64
+// elements, 16-byte chunk c of row r at c ^ ((r >> 1) & 7); far rows of 256, at
+// c ^ ((r & 3) << 2).  Both read all 64 banks evenly.
+__device__ __forceinline__ int near_place(int r, int c) { return r * BK + ((c ^ ((r >> 1) & 7)) << 3); }
+__device__ __forceinline__ int far_place(int r, int c) { return r * TILE + ((c ^ ((r & 3) << 2)) << 3); }
+
+template <bool FAR>
+__device__ __forceinline__ int frag_base() {
+  const int l = threadIdx.x & 63;
+  if constexpr (FAR)
+    return far_place(8 * (l >> 5) + ((l & 15) >> 2), 2 * ((l >> 4) & 1) + ((l & 3) >> 1)) + 4 * (l & 1);
+  else
+    return near_place(l & 31, l >> 5);
+}
+// r0: multiple of 32; k0: multiple of 16.
+template <bool FAR>
+__device__ __forceinline__ bf16x8 frag(const u16* m, int base, int r0, int k0) {
+  if constexpr (FAR) {
+    typedef __attribute__((address_space(3))) s16x4* lds_t;
+    const u16* p = m + (base ^ r0) + k0 * TILE;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)p);
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(p + 4 * TILE));
+    const s16x8 x = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    return __builtin_bit_cast(bf16x8, x);
+  } else {
+    return *reinterpret_cast<const bf16x8*>(m + (base ^ k0) + r0 * BK);
+  }
+}
+
+// One operand's step on its way to LDS: 8 vectors of 16 bytes a thread, at element offsets
+// from the step's first element that hold for every step.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+template <bool FAR>
+__device__ __forceinline__ void step_places(unsigned (&at)[8], int r0, int rows, int ld) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int v = threadIdx.x + i * NT;
+    if constexpr (FAR) {
+      const int c = r0 + (v & 31) * 8;
+      at[i] = (unsigned)(v >> 5) * (unsigned)ld + (unsigned)(c + 8 <= rows ? c : 0);
+    } else {
+      const int r = r0 + (v >> 3);
+      at[i] = (unsigned)((r < rows ? r : rows - 1) - r0) * (unsigned)ld + (v & 7) * 8;
+    }
+  }
+}
+// left: contracted elements from p on.  A far operand's rows past them are the last one again:
+// the other operand is 0 there.
+template <bool FAR>
+__device__ __forceinline__ void step_load(u32x4 (&x)[8], const u16* p, const unsigned (&at)[8],
+                                          int left, int ld) {
+  if (FAR && left < BK) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = (threadIdx.x + i * NT) >> 5;
+      x[i] = *reinterpret_cast<const u32x4*>(p + at[i] - (unsigned)(r < left ? 0 : r - left + 1) * (unsigned)ld);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const u32x4*>(p + at[i]);
+  }
+}
+template <bool FAR>
+__device__ __forceinline__ void step_put(u16* m, const u32x4 (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int v = threadIdx.x + i * NT;
+    *reinterpret_cast<u32x4*>(m + (FAR ? far_place(v >> 5, v & 31) : near_place(v >> 3, v & 7))) = x[i];
+  }
+}
+
+// Pairs of planes whose product is not below 2^-24 of the whole, smallest first.
+template <int PL>
+__device__ __forceinline__ void pair_of(int i, int& a, int& b) {
+  if constexpr (PL == 1) {
+    a = b = 0;
+  } else {
+    a = (0x001102 >> (4 * (5 - i))) & 15;  // 0 2 1 1 0 0 from the last digit on
+    b = (0x010120 >> (4 * (5 - i))) & 15;
+  }
+}
+
+template <int EPI, bool AFAR, bool BFAR, int PL, typename E>
+__global__ __launch_bounds__(NT, 1) void vl_gemm(VlArgs a) {
+  __shared__ __align__(16) u16 lds[2][2][STAGE];
+  __shared__ __align__(16) float s_bias[TILE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = mg_uniform(tid >> 6);
+  const int wm = wave & 1, wn = wave >> 1;
+  // Tiles in bands of 8 along N, so that neighbours share operands; each XCD takes a run.
+  const int tiles = a.mt * a.nt, work = tiles * a.splits;
+  int id = blockIdx.x;
+  {
+    const int per = (work + 7) / 8, x = id & 7, y = id >> 3;
+    id = x * per + y;
+    if (y >= per || id >= work) return;
+  }
+  const int split = id / tiles;
+  id -= split * tiles;
+  const int band = id / (8 * a.mt), in = id - band * 8 * a.mt;
+  const int wide = a.nt - band * 8 < 8 ? a.nt - band * 8 : 8;
+  const int nt = band * 8 + in % wide, mt = in / wide;
+  const int m0 = mt * TILE, n0 = nt * TILE;
+  const int m_rows = a.m_count ? *a.m_count : a.m_rows, n_rows = a.n_count ? *a.n_count : a.n_rows;
+  const int K = a.k_count ? (*a.k_count + BK - 1) / BK * BK : a.K;
+  if (m0 >= m_rows || n0 >= n_rows) return;
+
+  constexpr int PAIRS = PL == 1 ? 1 : 6;
+  const int ksteps = K / BK;
+  const int per = (ksteps + a.splits - 1) / a.splits;
+  const int s0 = split * per, s1 = s0 + per < ksteps ? s0 + per : ksteps;
+  const int steps = s1 > s0 ? (s1 - s0) * PAIRS : 0;
+
+  u32x4 xa[8], xb[8];
+  unsigned oa[8], ob[8];
+  step_places<AFAR>(oa, m0, m_rows, a.lda);
+  step_places<BFAR>(ob, n0, n_rows, a.ldb);
+  const u16* const A0 = a.A + (AFAR ? 0 : (int64_t)m0 * a.lda);
+  const u16* const B0 = a.B + (BFAR ? 0 : (int64_t)n0 * a.ldb);
+  const auto fetch = [&](int s) {
+    int k = s0 + s, p = 0, q = 0;
+    if constexpr (PL > 1) {
+      const int pair = s / (s1 - s0);
+      k = s0 + s - pair * (s1 - s0);
+      pair_of<PL>(pair, p, q);
+    }
+    step_load<AFAR>(xa, A0 + p * a.pa + (AFAR ? (int64_t)k * BK * a.lda : (int64_t)k * BK), oa,
+                    a.ka - k * BK, a.lda);
+    step_load<BFAR>(xb, B0 + q * a.pb + (BFAR ? (int64_t)k * BK * a.ldb : (int64_t)k * BK), ob,
+                    1 << 30, a.ldb);
+  };
+  f32x16 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+  if constexpr (EPI != VL_OUT) {
+    const int m = m0 + tid;
+    s_bias[tid] = a.bias && m < m_rows ? to_f(((const E*)a.bias)[a.v0 + m]) : 0.f;
+  }
+  const int ab = frag_base<AFAR>(), bb = frag_base<BFAR>();
+  if (steps > 0) {
+    fetch(0);
+    step_put<AFAR>(lds[0][0], xa);
+    step_put<BFAR>(lds[0][1], xb);
+  }
+  __syncthreads();
+  for (int s = 0; s < steps; ++s) {
+    const u16* const la = lds[s & 1][0];
+    const u16* const lb = lds[s & 1][1];
+    if (s + 1 < steps) fetch(s + 1);
+#pragma unroll
+    for (int k0 = 0; k0 < BK; k0 += 16) {
+      bf16x8 fa[4], fb[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fa[i] = frag<AFAR>(la, ab, wm * 128 + i * 32, k0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fb[j] = frag<BFAR>(lb, bb, wn * 128 + j * 32, k0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+    }
+    if (s + 1 < steps) {
+      step_put<AFAR>(lds[(s + 1) & 1][0], xa);
+      step_put<BFAR>(lds[(s + 1) & 1][1], xb);
+    }
+    __syncthreads();
+  }
+
+  // Lane: column n = n0 + 128 wn + 32 j + (lane & 31) of the result; rows m = m0 + 128 wm +
+  // 32 i + 8 q + 4 (lane >> 5) + x in acc[i][j][4 q + x].
+  const int half = lane >> 5, mw = m0 + wm * 128 + 4 * half, nw = n0 + wn * 128 + (lane & 31);
+  // Logits of a row's 64 columns of this lane, -inf past the vocabulary.
+  const float* const bw = s_bias + wm * 128 + 4 * half;
+  const bool ragged = m0 + TILE > m_rows;
+  if constexpr (EPI == VL_LSE) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = nw + 32 * j;
+      const int t = a.tgt[n < n_rows ? n : n_rows - 1] - a.v0 - mw;
+      float l[64], top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        const float4 b = *reinterpret_cast<const float4*>(bw + 32 * (c >> 2) + 8 * (c & 3));
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int m = 32 * (c >> 2) + 8 * (c & 3) + x;
+          float v = acc[c >> 2][j][4 * (c & 3) + x] + (x == 0 ? b.x : x == 1 ? b.y : x == 2 ? b.z : b.w);
+          if (ragged && mw + m >= m_rows) v = -INFINITY;
+          l[4 * c + x] = v;
+          top = fmaxf(top, v);
+        }
+      }
+      if (__ballot(t >= 0 && t < 128 && n < n_rows)) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (t == 8 * (c >> 2) + (c & 3) && n < n_rows) a.tlogit[n] = l[c];
+      }
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float ref = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 64; ++c) sum += __expf(l[c] - ref);
+      sum += __shfl_xor(sum, 32);
+      // fmaxf drops a NaN; the sum keeps it.
+      if (half == 0 && n < n_rows) a.part[(int64_t)(2 * mt + wm) * a.n_ld + n] = make_float2(top, sum);
+    }
+  }
+  if constexpr (EPI == VL_D) {
+    // In four rounds of 64 rows, (planes, 64 rows n, 256 columns m) in LDS with chunk c of row r
+    // at c ^ (r & 31), then whole rows out.  Rows up to the next multiple of the contracted step
+    // are written, as 0.
+    u16* const stage = &lds[0][0][0];
+    const int rows = (n_rows + BK - 1) / BK * BK;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = nw + 32 * j, r = n < n_rows ? n : n_rows - 1;
+      const float2 soft = a.soft[r];
+      const float g = n < n_rows ? a.g[r] : 0.f;
+      const int t = a.tgt[r] - a.v0 - mw;
+      const int sr = wn * 32 + (lane & 31);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        const float4 b = *reinterpret_cast<const float4*>(bw + 32 * (c >> 2) + 8 * (c & 3));
+        float p[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int m = 32 * (c >> 2) + 8 * (c & 3) + x;
+          const float v = acc[c >> 2][j][4 * (c & 3) + x] + (x == 0 ? b.x : x == 1 ? b.y : x == 2 ? b.z : b.w);
+          p[x] = (__expf(v - soft.x) * soft.y - (t == m ? 1.f : 0.f)) * g;
+          if ((ragged && mw + m >= m_rows) || n >= n_rows) p[x] = 0.f;
+        }
+        u16* const to = stage + sr * TILE + (((wm * 16 + c) ^ (sr & 31)) << 3) + 4 * half;
+#pragma unroll
+        for (int q = 0; q < PL; ++q) {
+          const unsigned u0 = pack2(p[0], p[1]), u1 = pack2(p[2], p[3]);
+          *reinterpret_cast<uint2*>(to + q * 64 * TILE) = make_uint2(u0, u1);
+          p[0] -= low(u0), p[1] -= high(u0), p[2] -= low(u1), p[3] -= high(u1);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < PL * 8; ++u) {
+        const int v = tid + u * NT, q = v >> 11, r2 = (v >> 5) & 63, c = v & 31;
+        const int n2 = n0 + (r2 >> 5) * 128 + 32 * j + (r2 & 31);
+        if (n2 < rows && m0 + c * 8 < a.ldd)
+          *reinterpret_cast<u32x4*>(a.d + q * a.pd + (int64_t)n2 * a.ldd + m0 + c * 8) =
+              *reinterpret_cast<const u32x4*>(stage + q * 64 * TILE + r2 * TILE + ((c ^ (r2 & 31)) << 3));
+      }
+      __syncthreads();
+    }
+  }
+  if constexpr (EPI == VL_OUT) {
+    const bool f32 = a.out_f32;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = nw + 32 * j;
+      if (n >= a.n_out) continue;
+      const int64_t row = split * a.po + n * a.ldo;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int m = mw + 32 * i + 8 * q;
+          float v[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) v[x] = acc[i][j][4 * q + x];
+          if (m + 4 <= a.m_out && (a.ldo & 3) == 0) {
+            if (f32) *reinterpret_cast<float4*>((float*)a.out + row + m) = make_float4(v[0], v[1], v[2], v[3]);
+            else *reinterpret_cast<uint2*>((u16*)a.out + row + m) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+          } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              if (m + x < a.m_out) {
+                if (f32) ((float*)a.out)[row + m + x] = v[x];
+                else ((u16*)a.out)[row + m + x] = to_bf(v[x]);
+              } else if (m + x == a.m_out && a.extra) {
+                if (f32) ((float*)a.extra)[split * a.pe + n] = v[x];
+                else ((u16*)a.extra)[n] = to_bf(v[x]);
+              }
+            }
+          }
+        }
+    }
+  }
+}
+
+// ---- joins ----------------------------------------------------------------------------------
+// Rows' largest logits and sums from their parts, and their losses.  64 rows a workgroup, 16 threads each.
+__global__ __launch_bounds__(1024) void vl_join(const float2* __restrict__ part,
+                                                const float* __restrict__ tlogit,
+                                                const int* __restrict__ tgt,
+                                                const int* __restrict__ idx,
+                                                const int* __restrict__ count, int parts, int ld,
+                                                float2* __restrict__ soft,
+                                                float* __restrict__ loss) {
+  __shared__ float2 s[16][64];
+  const int r = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int n = blockIdx.x * 64 + r, rows = *count;
+  if (blockIdx.x * 64 >= rows) return;
+  const float2* p = part + (n < rows ? n : rows - 1);
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+  for (int i = w; i < parts; i += 16) {
+    const float2 v = p[(int64_t)i * ld];
+    const float m = fmaxf(top, v.x), ref = m == -INFINITY ? 0.f : m;
+    sum = sum * __expf(top - ref) + v.y * __expf(v.x - ref);
+    top = m;
+  }
+  s[w][r] = make_float2(top, sum);
+  __syncthreads();
+  if (w != 0 || n >= rows) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) {
+    const float2 v = s[i][r];
+    const float m = fmaxf(top, v.x), ref = m == -INFINITY ? 0.f : m;
+    sum = sum * __expf(top - ref) + v.y * __expf(v.x - ref);
+    top = m;
+  }
+  // The largest logit and the sum stay apart: their log sum would round at the logits' size.
+  const bool in = tgt[n] >= 0;
+  soft[n] = make_float2(in ? top : __builtin_nanf(""), 1.f / sum);
+  loss[idx[n]] = in ? (top - tlogit[n]) + logf(sum) : __builtin_nanf("");
+}
+
+// The rows' losses, 0 where they are left out; or their sum, over the count if `mean`, in a
+// fixed order.  One workgroup.
+__global__ __launch_bounds__(1024) void vl_total(const float* __restrict__ loss,
+                                                 const int* __restrict__ pos,
+                                                 const int* __restrict__ count, int N, int mean,
+                                                 float* __restrict__ out) {
+  __shared__ double s[16];
+  double a[4] = {0.0, 0.0, 0.0, 0.0};
+  for (int i = threadIdx.x; i < N; i += 4096) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int x = i + u * 1024;
+      if (x < N && pos[x] >= 0) a[u] += (double)loss[x];
+    }
+  }
+  double t = (a[0] + a[1]) + (a[2] + a[3]);
+#pragma unroll
+  for (int d = 32; d; d /= 2) t += __shfl_xor(t, d);
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    t = 0.0;
+    for (int i = 0; i < 16; ++i) t += s[i];
+    *out = (float)(mean ? t / (*count > 0 ? *count : 1) : t);
+  }
+}
+__global__ __launch_bounds__(256) void vl_left_out(const int* __restrict__ pos, int N,
+                                                   float* __restrict__ loss) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < N && pos[i] < 0) loss[i] = 0.f;
+}
+// Upstream gradients of the counted rows.  reduction: 0 each row's own, 1 mean, 2 sum.
+__global__ __launch_bounds__(256) void vl_upstream(const float* __restrict__ up,
+                                                   const int* __restrict__ idx,
+                                                   const int* __restrict__ count, int reduction,
+                                                   float* __restrict__ g) {
+  const int j = blockIdx.x * 256 + threadIdx.x, n = *count;
+  if (j >= n) return;
+  g[j] = reduction == 0 ? up[idx[j]] : reduction == 1 ? up[0] / (float)n : up[0];
+}
+// out[i][c] = sum of the parts' rows, pos[i] if given (0 where that is negative).
+template <typename E>
+__global__ __launch_bounds__(256) void vl_sum(const float* __restrict__ part, int64_t po,
+                                              int parts, const int* __restrict__ pos, int64_t n,
+                                              int cols, E* __restrict__ out) {
+  const int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (x >= n) return;
+  if ((cols & 3) == 0) {
+    const int64_t i = x / cols, j = pos ? pos[i] : i;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (j >= 0)
+      for (int p = 0; p < parts; ++p) {
+        const float4 v = *reinterpret_cast<const float4*>(part + p * po + j * cols + x % cols);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+      }
+    if constexpr (sizeof(E) == 4) *reinterpret_cast<float4*>(out + x) = s;
+    else *reinterpret_cast<uint2*>(out + x) = make_uint2(pack2(s.x, s.y), pack2(s.z, s.w));
+    return;
+  }
+  for (int64_t y = x; y < x + 4 && y < n; ++y) {
+    const int64_t i = y / cols, j = pos ? pos[i] : i;
+    float s = 0.f;
+    if (j >= 0)
+      for (int p = 0; p < parts; ++p) s += part[p * po + j * cols + y % cols];
+    if constexpr (sizeof(E) == 4) out[y] = s;
+    else out[y] = to_bf(s);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------
+constexpr int64_t up_to(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+
+struct Shape {
+  int64_t N, V, D, np, kp, dx;  // padded rows, contracted columns, columns of packed x
+  int planes;
+  bool own_w;                    // W is packed too
+};
+bool vl_shape(int dtype, int64_t N, int64_t V, int64_t D, Shape* s) {
+  if ((dtype & ~1) || N < 1 || V < 1 || D < 1 || N > (1 << 30) || V > (1 << 30) || D > (1 << 20))
+    return false;
+  s->N = N, s->V = V, s->D = D;
+  s->np = up_to(N, TILE), s->kp = up_to(D, BK), s->dx = up_to(D + 1, BK);
+  s->planes = dtype ? 1 : 3;
+  s->own_w = dtype == 0 || D % BK != 0;
+  return true;
+}
+struct State {
+  int *idx, *pos, *tgt, *count;
+  float2* soft;
+  u16 *xc, *wc;
+  size_t bytes;
+};
+State vl_state(const Shape& s, void* base) {
+  char* p = (char*)base;
+  const auto take = [&](int64_t n) {
+    char* at = p;
+    p += up_to(n, 256);
+    return at;
+  };
+  State t;
+  t.count = (int*)take(256);
+  t.idx = (int*)take(s.N * 4), t.pos = (int*)take(s.N * 4), t.tgt = (int*)take(s.N * 4);
+  t.soft = (float2*)take(s.N * 8);
+  t.xc = (u16*)take(s.planes * s.np * s.dx * 2);
+  t.wc = s.own_w ? (u16*)take(s.planes * s.V * s.kp * 2) : nullptr;
+  t.bytes = p - (char*)base;
+  return t;
+}
+
+// Parts of the contracted axis for `tiles` result tiles on 256 CUs: the fewest steps in a row.
+int vl_splits(int64_t tiles, int64_t steps) {
+  int best = 1;
+  double least = 1e300;
+  for (int s = 1; s <= 16 && (s == 1 || steps / s >= 8); ++s) {
+    const double cost = (double)((tiles * s + 255) / 256) * ((steps + s - 1) / s + 4) + 2.0 * (s - 1);
+    if (cost < least) least = cost, best = s;
+  }
+  return best;
+}
+
+// Pieces of the vocabulary: as few as keep d in half a gigabyte.
+constexpr int64_t VL_D_BYTES = 512ll << 20;
+struct Back {
+  int64_t vp, pieces;   // columns of a piece
+  int dx_splits, dw_splits;
+  float *g, *dx_part, *dw_part, *db_part;
+  u16* d;
+  size_t bytes;
+};
+Back vl_back(const Shape& s, void* base) {
+  Back b;
+  const int64_t most = VL_D_BYTES / (s.np * 2 * s.planes);
+  b.pieces = (s.V + (most > TILE ? most : TILE) - 1) / (most > TILE ? most : TILE);
+  b.vp = up_to((s.V + b.pieces - 1) / b.pieces, TILE);
+  b.pieces = (s.V + b.vp - 1) / b.vp;
+  const int64_t steps = s.planes == 1 ? 1 : 6;
+  b.dx_splits = vl_splits((s.np / TILE) * ((s.D + TILE - 1) / TILE), b.vp / BK * steps);
+  b.dw_splits = vl_splits((b.vp / TILE) * ((s.D + 1 + TILE - 1) / TILE), s.np / BK * steps);
+  char* p = (char*)base;
+  const auto take = [&](int64_t n) {
+    char* at = p;
+    p += up_to(n, 256);
+    return at;
+  };
+  b.g = (float*)take(s.N * 4);
+  b.d = (u16*)take(s.planes * s.np * b.vp * 2);
+  b.dx_part = (float*)take(b.pieces * b.dx_splits * s.N * s.D * 4);
+  b.dw_part = b.dw_splits > 1 ? (float*)take(b.dw_splits * b.vp * s.D * 4) : nullptr;
+  b.db_part = b.dw_splits > 1 ? (float*)take(b.dw_splits * b.vp * 4) : nullptr;
+  b.bytes = p - (char*)base;
+  return b;
+}
+
+template <int EPI, bool AFAR, bool BFAR>
+int vl_run(int dtype, VlArgs& a, hipStream_t stream) {
+  const int64_t work = (int64_t)a.mt * a.nt * a.splits;
+  if (work > (1ll << 30)) return MG_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)((work + 7) / 8 * 8));
+  if (dtype) hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 1, u16>), grid, dim3(NT), 0, stream, a);
+  else hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 3, float>), grid, dim3(NT), 0, stream, a);
+  return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
+}
+
+// The logits' product: M the vocabulary's columns v0 .. v0 + cols - 1, N the packed rows.
+VlArgs vl_logits(const Shape& s, const State& t, const void* w, const void* bias, int64_t v0,
+                 int64_t cols) {
+  VlArgs a = {};
+  a.A = (s.own_w ? t.wc : (const u16*)w) + v0 * s.kp;
+  a.lda = (int)s.kp, a.pa = s.V * s.kp;
+  a.B = t.xc, a.ldb = (int)s.dx, a.pb = s.np * s.dx;
+  a.m_rows = (int)cols, a.n_count = t.count;
+  a.K = (int)s.kp, a.ka = 1 << 30;
+  a.mt = (int)((cols + TILE - 1) / TILE), a.nt = (int)(s.np / TILE), a.splits = 1;
+  a.v0 = (int)v0, a.V = (int)s.V, a.bias = bias, a.tgt = t.tgt, a.n_ld = (int)s.np;
+  return a;
+}
+
+int64_t vl_part_rows(const Shape& s) { return 2 * ((s.V + TILE - 1) / TILE); }
+
+template <typename E, int PL>
+void vl_pack_run(const void* src, int64_t ld, int64_t cols, u16* dst, int64_t dld, int64_t plane,
+                 const int* idx, const int* count, int64_t rows, int64_t grid, int ones,
+                 hipStream_t stream) {
+  hipLaunchKernelGGL((vl_pack<E, PL>), dim3((unsigned)grid), dim3(256), 0, stream, (const E*)src, ld,
+                     (int)cols, dst, (int)dld, plane, idx, count, rows, ones);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mg_vocab_loss_state_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
+  Shape s;
+  return vl_shape(dtype, N, V, D, &s) ? vl_state(s, nullptr).bytes : 0;
+}
+
+size_t mg_vocab_loss_fwd_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
+  Shape s;
+  if (!vl_shape(dtype, N, V, D, &s)) return 0;
+  return vl_part_rows(s) * s.np * sizeof(float2) + s.np * sizeof(float) + s.N * sizeof(float);
+}
+
+size_t mg_vocab_loss_bwd_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
+  Shape s;
+  return vl_shape(dtype, N, V, D, &s) ? vl_back(s, nullptr).bytes : 0;
+}
+
+int mg_vocab_loss_fwd(int dtype, const void* x, int64_t ldx, const void* w, const void* bias,
+                      const int64_t* target, int64_t ignore_index, int reduction, float* loss,
+                      int64_t N, int64_t V, int64_t D, void* state, size_t state_bytes, void* ws,
+                      size_t ws_bytes, hipStream_t stream) {
+  Shape s;
+  if (!x || !w || !target || !loss || !state || !ws || reduction < 0 || reduction > 2 || ldx < D ||
+      !vl_shape(dtype, N, V, D, &s))
+    return MG_ERR_ARG;
+  const State t = vl_state(s, state);
+  if (state_bytes < t.bytes || ws_bytes < mg_vocab_loss_fwd_workspace_bytes(dtype, N, V, D))
+    return MG_ERR_WORKSPACE;
+  float2* const part = (float2*)ws;
+  float* const tlogit = (float*)(part + vl_part_rows(s) * s.np);
+  float* const rows = reduction ? tlogit + s.np : loss;
+  hipLaunchKernelGGL(vl_index, dim3(1), dim3(1024), 0, stream, target, ignore_index, V, t.idx,
+                     t.pos, t.tgt, t.count, (int)N);
+  if (dtype) {
+    vl_pack_run<u16, 1>(x, ldx, D, t.xc, s.dx, 0, t.idx, t.count, N, s.np, (int)D, stream);
+    if (s.own_w) vl_pack_run<u16, 1>(w, D, D, t.wc, s.kp, 0, nullptr, nullptr, V, V, -1, stream);
+  } else {
+    vl_pack_run<float, 3>(x, ldx, D, t.xc, s.dx, s.np * s.dx, t.idx, t.count, N, s.np, (int)D, stream);
+    vl_pack_run<float, 3>(w, D, D, t.wc, s.kp, s.V * s.kp, nullptr, nullptr, V, V, -1, stream);
+  }
+  VlArgs a = vl_logits(s, t, w, bias, 0, V);
+  a.part = part, a.tlogit = tlogit;
+  const int rc = vl_run<VL_LSE, false, false>(dtype, a, stream);
+  if (rc != MG_OK) return rc;
+  hipLaunchKernelGGL(vl_join, dim3((unsigned)((N + 63) / 64)), dim3(1024), 0, stream, part, tlogit,
+                     t.tgt, t.idx, t.count, (int)vl_part_rows(s), (int)s.np, t.soft, rows);
+  if (reduction)
+    hipLaunchKernelGGL(vl_total, dim3(1), dim3(1024), 0, stream, rows, t.pos, t.count, (int)N,
+                       (int)(reduction == 1), loss);
+  else
+    hipLaunchKernelGGL(vl_left_out, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, stream, t.pos,
+                       (int)N, loss);
+  return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
+}
+
+int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* dloss,
+                      int reduction, void* dx, void* dw, void* db, int64_t N, int64_t V, int64_t D,
+                      const void* state, void* ws, size_t ws_bytes, hipStream_t stream) {
+  Shape s;
+  if (!w || !dloss || !state || !ws || reduction < 0 || reduction > 2 || (db && !dw) ||
+      !vl_shape(dtype, N, V, D, &s))
+    return MG_ERR_ARG;
+  const State t = vl_state(s, const_cast<void*>(state));
+  const Back b = vl_back(s, ws);
+  if (ws_bytes < b.bytes) return MG_ERR_WORKSPACE;
+  const int e = dtype ? 2 : 4;
+  hipLaunchKernelGGL(vl_upstream, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, stream, dloss,
+                     t.idx, t.count, reduction, b.g);
+  for (int64_t v0 = 0, piece = 0; v0 < V; v0 += b.vp, ++piece) {
+    const int64_t cols = V - v0 < b.vp ? V - v0 : b.vp, kc = up_to(cols, BK);
+    VlArgs a = vl_logits(s, t, w, bias, v0, cols);
+    a.soft = t.soft, a.g = b.g;
+    a.d = b.d, a.pd = s.np * b.vp, a.ldd = (int)kc;
+    int rc = vl_run<VL_D, false, false>(dtype, a, stream);
+    if (rc == MG_OK && dx) {
+      VlArgs c = {};
+      c.A = a.A, c.lda = a.lda, c.pa = a.pa, c.m_rows = (int)s.kp;
+      c.B = b.d, c.ldb = (int)kc, c.pb = a.pd, c.n_count = t.count;
+      c.K = (int)kc, c.ka = (int)cols;
+      c.mt = (int)((D + TILE - 1) / TILE), c.nt = (int)(s.np / TILE), c.splits = b.dx_splits;
+      c.out = b.dx_part + piece * b.dx_splits * N * D;
+      c.ldo = D, c.po = N * D, c.m_out = (int)D, c.n_out = (int)N, c.out_f32 = 1;
+      rc = vl_run<VL_OUT, true, false>(dtype, c, stream);
+    }
+    if (rc == MG_OK && dw) {
+      VlArgs c = {};
+      c.A = t.xc, c.lda = (int)s.dx, c.pa = s.np * s.dx, c.m_rows = (int)s.dx;
+      c.B = b.d, c.ldb = (int)kc, c.pb = a.pd, c.n_rows = (int)kc;
+      c.k_count = t.count, c.ka = 1 << 30;
+      c.mt = (int)((D + (db ? 1 : 0) + TILE - 1) / TILE), c.nt = (int)((cols + TILE - 1) / TILE);
+      c.splits = b.dw_splits;
+      c.ldo = D, c.m_out = (int)D, c.n_out = (int)cols;
+      void* const to = (char*)dw + v0 * D * e;
+      void* const to_b = db ? (char*)db + v0 * e : nullptr;
+      if (b.dw_splits > 1) {
+        c.out = b.dw_part, c.po = cols * D, c.out_f32 = 1;
+        c.extra = db ? b.db_part : nullptr, c.pe = cols;
+      } else {
+        c.out = to, c.out_f32 = dtype ? 0 : 1, c.extra = to_b;
+      }
+      rc = vl_run<VL_OUT, true, true>(dtype, c, stream);
+      if (rc == MG_OK && b.dw_splits > 1) {
+        for (int k = 0; k < (db ? 2 : 1); ++k) {
+          const int64_t n = k ? cols : cols * D;
+          const float* const from = k ? b.db_part : b.dw_part;
+          const int wide = k ? 1 : (int)D;
+          const dim3 grid((unsigned)((n / 4 + 256) / 256));
+          if (dtype)
+            hipLaunchKernelGGL(vl_sum<u16>, grid, dim3(256), 0, stream, from, n, b.dw_splits,
+                               (const int*)nullptr, n, wide, (u16*)(k ? to_b : to));
+          else
+            hipLaunchKernelGGL(vl_sum<float>, grid, dim3(256), 0, stream, from, n, b.dw_splits,
+                               (const int*)nullptr, n, wide, (float*)(k ? to_b : to));
+        }
+      }
+    }
+    if (rc != MG_OK) return rc;
+  }
+  if (dx) {
+    const int64_t n = N * D;
+    const int parts = (int)(b.pieces * b.dx_splits);
+    const dim3 grid((unsigned)((n / 4 + 256) / 256));
+    if (dtype)
+      hipLaunchKernelGGL(vl_sum<u16>, grid, dim3(256), 0, stream, b.dx_part, n, parts, t.pos, n,
+                         (int)D, (u16*)dx);
+    else
+      hipLaunchKernelGGL(vl_sum<float>, grid, dim3(256), 0, stream, b.dx_part, n, parts, t.pos, n,
+                         (int)D, (float*)dx);
+  }
+  return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
+}
+
+}  // extern "C"

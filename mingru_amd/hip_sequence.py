@@ -24,7 +24,12 @@ from .hip_scans import (
     column_sums,
 )
 
-__all__ = ["linear_attention_impl", "linear_attention_step_impl", "residual_norm_impl"]
+__all__ = [
+    "linear_attention_impl",
+    "linear_attention_step_impl",
+    "linear_cross_entropy_impl",
+    "residual_norm_impl",
+]
 
 _DTYPE_TAG = {torch.float32: 0, torch.bfloat16: 1}
 
@@ -243,3 +248,60 @@ def linear_attention_step_impl(q, k, v, g, h, scale):
             _ptr(q), _ptr(k), _ptr(v), _ptr(g), _array(strides), _ptr(h), _ptr(o), _ptr(h_out), B,
             H, Hk, dk, dv, scale, _stream(q))
     return o if o.dtype == dtype else o.to(dtype), h_out
+
+
+# ---------------------------------------------------------------------------
+# linear_cross_entropy
+# ---------------------------------------------------------------------------
+
+_REDUCTION_TAG = {"none": 0, "mean": 1, "sum": 2}
+
+
+class _VocabLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, target, ignore_index, reduction):
+        x2, ldx = _rows(x, x.shape[-1])
+        w = w.contiguous()
+        if w.data_ptr() % 16:
+            w = w.clone()
+        N, (V, D) = x2.shape[0], w.shape
+        tag, dev = _DTYPE_TAG[x.dtype], x.device
+        state = _workspace(_size("mg_vocab_loss_state_bytes", tag, N, V, D), dev)
+        ws = _workspace(_size("mg_vocab_loss_fwd_workspace_bytes", tag, N, V, D), dev)
+        loss = torch.empty(N if reduction == 0 else (), dtype=torch.float32, device=dev)
+        bias = bias if bias is None else bias.contiguous()
+        _call("mg_vocab_loss_fwd", tag, _ptr(x2), ldx, _ptr(w), _ptr(bias), _ptr(target),
+              ignore_index, reduction, _ptr(loss), N, V, D, _ptr(state), state.numel(), _ptr(ws),
+              ws.numel(), _stream(x))
+        if any(ctx.needs_input_grad):
+            ctx.save_for_backward(w, bias, state)
+            ctx.size, ctx.shape, ctx.reduction = (tag, N, V, D), x.shape, reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        w, bias, state = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = torch.empty(ctx.shape, dtype=w.dtype, device=w.device) if need[0] else None
+        db = torch.empty_like(bias) if need[2] else None
+        dw = torch.empty_like(w) if need[1] or db is not None else None
+        ws = _workspace(_size("mg_vocab_loss_bwd_workspace_bytes", *ctx.size), w.device)
+        tag, N, V, D = ctx.size
+        _call("mg_vocab_loss_bwd", tag, _ptr(w), _ptr(bias), _ptr(dloss.contiguous()),
+              ctx.reduction, _ptr(dx), _ptr(dw), _ptr(db), N, V, D, _ptr(state), _ptr(ws),
+              ws.numel(), _stream(w))
+        return dx, dw if need[1] else None, db, None, None, None
+
+
+def linear_cross_entropy_impl(x, weight, target, bias, ignore_index, reduction):
+    """``linear_cross_entropy`` on checked arguments of one type."""
+    x, weight, bias = _half_to_float(x, weight, bias)
+    N, (V, D) = target.numel(), weight.shape
+    if not _size("mg_vocab_loss_state_bytes", _DTYPE_TAG[x.dtype], N, V, D):
+        raise ScanFallback(f"linear_cross_entropy kernels take fewer than 2^30 rows and "
+                           f"vocabulary entries and rows of at most 2^20 (got {N}, {V}, {D})")
+    t = target.reshape(-1).to(torch.int64).contiguous()
+    loss = _funnel("linear_cross_entropy", _VocabLossFn.apply, x, weight, bias, t,
+                   int(ignore_index), _REDUCTION_TAG[reduction])
+    return loss.view(target.shape) if reduction == "none" else loss

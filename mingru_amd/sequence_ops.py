@@ -17,7 +17,7 @@ import torch
 
 from .min_gru import _resolve_native_dispatch, _resolve_scan_mode
 
-__all__ = ["linear_attention", "linear_attention_step", "residual_norm"]
+__all__ = ["linear_attention", "linear_attention_step", "linear_cross_entropy", "residual_norm"]
 
 _warned: set = set()
 
@@ -306,3 +306,72 @@ def linear_attention_step(q_t, k_t, v_t, log_decay_t, h_prev=None, scale=None):
     a = torch.where(_over(g), torch.zeros_like(g), g.exp()).expand(B, H)
     h = a[..., None, None] * h + kw[..., None] * v.to(g.dtype)[..., None, :]
     return (scale * (qw[..., None, :] @ h)[..., 0, :]).to(q.dtype), h
+
+
+# ---------------------------------------------------------------------------
+# linear_cross_entropy
+# ---------------------------------------------------------------------------
+
+_REDUCTIONS = ("none", "mean", "sum")
+
+
+def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of ``x @ weight.T + bias`` against ``target``, without keeping the
+    logits: on the GPU they are formed tile by tile, and again in the backward pass in pieces of
+    the vocabulary.
+
+    Parameters
+    ----------
+    x : (..., D)
+    weight : (V, D)
+    target : (...) integers
+        Rows with ``ignore_index`` are left out: they are not read, their losses and gradients
+        are 0.  Any other value outside the vocabulary raises ``IndexError`` on the CPU; on the
+        GPU, where looking would wait for it, that row's loss and all gradients that it is part
+        of are NaN.
+    bias : (V), optional
+    reduction : "mean", "sum" or "none"
+        "mean" is over the rows that count, 0 if there are none.
+
+    Returns the loss in 32 bits (64 for float64 inputs): a scalar, or each row's in ``target``'s
+    shape for "none".
+    """
+    what = "linear_cross_entropy"
+    _check_floats(what, x=x, weight=weight, bias=bias)
+    if not torch.is_tensor(target) or target.dtype.is_floating_point or \
+            target.dtype in (torch.bool, torch.complex64, torch.complex128):
+        raise TypeError(f"{what}: target must be a tensor of integers")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"{what}: reduction is one of {_REDUCTIONS} (got {reduction!r})")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"{what}: x is (..., D) and weight (V, D) (got {tuple(x.shape)} and "
+                         f"{tuple(weight.shape)})")
+    if target.shape != x.shape[:-1] or target.device != x.device:
+        raise ValueError(f"{what}: target has x's leading shape {tuple(x.shape[:-1])} and device "
+                         f"(got {tuple(target.shape)} on {target.device})")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"{what}: bias is (V,) = ({weight.shape[0]},) (got {tuple(bias.shape)})")
+    dtype = torch.promote_types(x.dtype, weight.dtype)
+    if bias is not None:
+        dtype = torch.promote_types(dtype, bias.dtype)
+        bias = bias.to(dtype)
+    x, weight = x.to(dtype), weight.to(dtype)
+    if target.numel():
+        out = _dispatch(what, x.is_cuda, lambda backend: backend.linear_cross_entropy_impl(
+            x, weight, target, bias, ignore_index, reduction))
+        if out is not None:
+            return out
+    t = target.reshape(-1)
+    rows = torch.nonzero(t != ignore_index)[:, 0]
+    at = t[rows].long()
+    outside = (at < 0) | (at >= weight.shape[0])
+    if bool(outside.any()):
+        raise IndexError(f"{what}: target {int(at[outside][0])} is outside the vocabulary of "
+                         f"{weight.shape[0]}")
+    logits = _wide(x.reshape(-1, x.shape[-1])[rows]) @ _wide(weight).t()
+    if bias is not None:
+        logits = logits + _wide(bias)
+    each = torch.logsumexp(logits, -1) - logits.gather(1, at[:, None])[:, 0]
+    if reduction == "none":
+        return each.new_zeros(t.shape).index_put((rows,), each).view(target.shape)
+    return each.sum() / max(1, rows.numel()) if reduction == "mean" else each.sum()
