@@ -127,7 +127,7 @@ struct VlArgs {
   const int* n_count;
   const int* k_count;      // contracted elements on the device, or K
   int K;                   // a multiple of the step
-  int ka;                  // of them that a far A has rows for
+  int ka;                  // of them that a far A has rows for, beside a near B
   int mt, nt, splits;      // tiles, and parts of the contracted axis
   // LSE and D: M the vocabulary from column v0 on, N the packed rows
   int v0, V;               // piece's first column; vocabulary
@@ -196,20 +196,19 @@ __device__ __forceinline__ void step_places(unsigned (&at)[8], int r0, int rows,
     }
   }
 }
-// left: contracted elements from p on.  A far operand's rows past them are the last one again:
-// the other operand is 0 there.
-template <bool FAR>
+// CLAMP: a far operand's rows past the `left` ones from p on are the last one again: the other
+// operand is 0 there.
+template <bool CLAMP>
 __device__ __forceinline__ void step_load(u32x4 (&x)[8], const u16* p, const unsigned (&at)[8],
                                           int left, int ld) {
-  if (FAR && left < BK) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = (threadIdx.x + i * NT) >> 5;
-      x[i] = *reinterpret_cast<const u32x4*>(p + at[i] - (unsigned)(r < left ? 0 : r - left + 1) * (unsigned)ld);
+  for (int i = 0; i < 8; ++i) {
+    unsigned o = at[i];
+    if constexpr (CLAMP) {
+      const int over = (int)((threadIdx.x + i * NT) >> 5) - (left - 1);
+      o -= (unsigned)(over > 0 ? over : 0) * (unsigned)ld;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const u32x4*>(p + at[i]);
+    x[i] = *reinterpret_cast<const u32x4*>(p + o);
   }
 }
 template <bool FAR>
@@ -229,6 +228,21 @@ __device__ __forceinline__ void pair_of(int i, int& a, int& b) {
   } else {
     a = (0x001102 >> (4 * (5 - i))) & 15;  // 0 2 1 1 0 0 from the last digit on
     b = (0x010120 >> (4 * (5 - i))) & 15;
+  }
+}
+
+// The order of a part: its LDS reads, writes and loads one by one between the 16 products, so
+// that the matrix cores do not wait while they are issued.
+template <int U, int READS, int WRITES, int LOADS>
+__device__ __forceinline__ void interleave() {
+  if constexpr (U < 16) {
+    if constexpr (U < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    if constexpr (U < WRITES) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+    if constexpr (U < LOADS) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    interleave<U + 1, READS, WRITES, LOADS>();
+  } else {
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -268,17 +282,21 @@ __global__ __launch_bounds__(NT, 1) void vl_gemm(VlArgs a) {
   step_places<BFAR>(ob, n0, n_rows, a.ldb);
   const u16* const A0 = a.A + (AFAR ? 0 : (int64_t)m0 * a.lda);
   const u16* const B0 = a.B + (BFAR ? 0 : (int64_t)n0 * a.ldb);
-  const auto fetch = [&](int s) {
-    int k = s0 + s, p = 0, q = 0;
-    if constexpr (PL > 1) {
-      const int pair = s / (s1 - s0);
-      k = s0 + s - pair * (s1 - s0);
-      pair_of<PL>(pair, p, q);
-    }
-    step_load<AFAR>(xa, A0 + p * a.pa + (AFAR ? (int64_t)k * BK * a.lda : (int64_t)k * BK), oa,
-                    a.ka - k * BK, a.lda);
-    step_load<BFAR>(xb, B0 + q * a.pb + (BFAR ? (int64_t)k * BK * a.ldb : (int64_t)k * BK), ob,
+  // The next step to fetch; past the last one it is fetched again, so that the loop has no
+  // branches.
+  int f_k = s0, f_pair = 0, f_left = steps;
+  const auto fetch = [&]() {
+    int p, q;
+    pair_of<PL>(f_pair, p, q);
+    step_load<AFAR && !BFAR>(xa, A0 + p * a.pa + (AFAR ? (int64_t)f_k * BK * a.lda : (int64_t)f_k * BK), oa,
+                    a.ka - f_k * BK, a.lda);
+    step_load<false>(xb, B0 + q * a.pb + (BFAR ? (int64_t)f_k * BK * a.ldb : (int64_t)f_k * BK), ob,
                     1 << 30, a.ldb);
+    if (--f_left > 0 && ++f_k == s1) f_k = s0, ++f_pair;
+  };
+  const auto put = [&](int s) {
+    step_put<AFAR>(lds[s & 1][0], xa);
+    step_put<BFAR>(lds[s & 1][1], xb);
   };
   f32x16 acc[4][4];
 #pragma unroll
@@ -287,41 +305,55 @@ __global__ __launch_bounds__(NT, 1) void vl_gemm(VlArgs a) {
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-
   if constexpr (EPI != VL_OUT) {
     const int m = m0 + tid;
     s_bias[tid] = a.bias && m < m_rows ? to_f(((const E*)a.bias)[a.v0 + m]) : 0.f;
   }
+  // Fragments one 16-element part ahead of the products that use them, a step's operands in LDS
+  // one step ahead, and in registers on their way there another.  The barrier of a step comes
+  // before its last part: the products of that part cover the first reads of the next step.
   const int ab = frag_base<AFAR>(), bb = frag_base<BFAR>();
+  bf16x8 fa[2][4], fb[2][4];
+  const auto read = [&](int s, int part, int to) {
+    const u16 *const la = lds[s & 1][0], *const lb = lds[s & 1][1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fa[to][i] = frag<AFAR>(la, ab, wm * 128 + i * 32, part * 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fb[to][j] = frag<BFAR>(lb, bb, wn * 128 + j * 32, part * 16);
+  };
+  const auto multiply = [&](int from) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[from][i], fb[from][j], acc[i][j], 0, 0, 0);
+  };
+  constexpr int READS = (AFAR ? 8 : 4) + (BFAR ? 8 : 4);
   if (steps > 0) {
-    fetch(0);
-    step_put<AFAR>(lds[0][0], xa);
-    step_put<BFAR>(lds[0][1], xb);
+    fetch();
+    put(0);
+    fetch();
+    __syncthreads();
+    read(0, 0, 0);
+    for (int s = 0; s < steps; ++s) {
+      read(s, 1, 1);
+      multiply(0);
+      interleave<0, READS, 0, 0>();
+      read(s, 2, 0);
+      multiply(1);
+      interleave<0, READS, 0, 0>();
+      read(s, 3, 1);
+      put(s + 1);
+      multiply(0);
+      interleave<0, READS, 16, 0>();
+      __syncthreads();
+      read(s + 1, 0, 0);
+      fetch();
+      multiply(1);
+      interleave<0, READS, 0, 16>();
+    }
   }
   __syncthreads();
-  for (int s = 0; s < steps; ++s) {
-    const u16* const la = lds[s & 1][0];
-    const u16* const lb = lds[s & 1][1];
-    if (s + 1 < steps) fetch(s + 1);
-#pragma unroll
-    for (int k0 = 0; k0 < BK; k0 += 16) {
-      bf16x8 fa[4], fb[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) fa[i] = frag<AFAR>(la, ab, wm * 128 + i * 32, k0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) fb[j] = frag<BFAR>(lb, bb, wn * 128 + j * 32, k0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
-    }
-    if (s + 1 < steps) {
-      step_put<AFAR>(lds[(s + 1) & 1][0], xa);
-      step_put<BFAR>(lds[(s + 1) & 1][1], xb);
-    }
-    __syncthreads();
-  }
 
   // Lane: column n = n0 + 128 wn + 32 j + (lane & 31) of the result; rows m = m0 + 128 wm +
   // 32 i + 8 q + 4 (lane >> 5) + x in acc[i][j][4 q + x].
