@@ -196,28 +196,22 @@ __device__ __forceinline__ void step_places(unsigned (&at)[8], int r0, int rows,
     }
   }
 }
-// CLAMP: a far operand's rows past the `left` ones from p on are the last one again: the other
-// operand is 0 there.
+// Vector i of a step.  CLAMP: a far operand's rows past the `left` ones from p on are the last
+// one again: the other operand is 0 there.
 template <bool CLAMP>
-__device__ __forceinline__ void step_load(u32x4 (&x)[8], const u16* p, const unsigned (&at)[8],
-                                          int left, int ld) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    unsigned o = at[i];
-    if constexpr (CLAMP) {
-      const int over = (int)((threadIdx.x + i * NT) >> 5) - (left - 1);
-      o -= (unsigned)(over > 0 ? over : 0) * (unsigned)ld;
-    }
-    x[i] = *reinterpret_cast<const u32x4*>(p + o);
+__device__ __forceinline__ u32x4 step_load(const u16* p, const unsigned (&at)[8], int i, int left,
+                                           int ld) {
+  unsigned o = at[i];
+  if constexpr (CLAMP) {
+    const int over = (int)((threadIdx.x + i * NT) >> 5) - (left - 1);
+    o -= (unsigned)(over > 0 ? over : 0) * (unsigned)ld;
   }
+  return *reinterpret_cast<const u32x4*>(p + o);
 }
 template <bool FAR>
-__device__ __forceinline__ void step_put(u16* m, const u32x4 (&x)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int v = threadIdx.x + i * NT;
-    *reinterpret_cast<u32x4*>(m + (FAR ? far_place(v >> 5, v & 31) : near_place(v >> 3, v & 7))) = x[i];
-  }
+__device__ __forceinline__ void step_put(u16* m, u32x4 x, int i) {
+  const int v = threadIdx.x + i * NT;
+  *reinterpret_cast<u32x4*>(m + (FAR ? far_place(v >> 5, v & 31) : near_place(v >> 3, v & 7))) = x;
 }
 
 // Pairs of planes whose product is not below 2^-24 of the whole, smallest first.
@@ -228,21 +222,6 @@ __device__ __forceinline__ void pair_of(int i, int& a, int& b) {
   } else {
     a = (0x001102 >> (4 * (5 - i))) & 15;  // 0 2 1 1 0 0 from the last digit on
     b = (0x010120 >> (4 * (5 - i))) & 15;
-  }
-}
-
-// The order of a part: its LDS reads, writes and loads one by one between the 16 products, so
-// that the matrix cores do not wait while they are issued.
-template <int U, int READS, int WRITES, int LOADS>
-__device__ __forceinline__ void interleave() {
-  if constexpr (U < 16) {
-    if constexpr (U < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    if constexpr (U < WRITES) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
-    if constexpr (U < LOADS) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    interleave<U + 1, READS, WRITES, LOADS>();
-  } else {
-    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -282,21 +261,27 @@ __global__ __launch_bounds__(NT, 1) void vl_gemm(VlArgs a) {
   step_places<BFAR>(ob, n0, n_rows, a.ldb);
   const u16* const A0 = a.A + (AFAR ? 0 : (int64_t)m0 * a.lda);
   const u16* const B0 = a.B + (BFAR ? 0 : (int64_t)n0 * a.ldb);
-  // The next step to fetch; past the last one it is fetched again, so that the loop has no
+  // The step being fetched; past the last one it is that one again, so that the loop has no
   // branches.
   int f_k = s0, f_pair = 0, f_left = steps;
-  const auto fetch = [&]() {
+  const u16 *fA = nullptr, *fB = nullptr;
+  const auto aim = [&]() {
     int p, q;
     pair_of<PL>(f_pair, p, q);
-    step_load<AFAR && !BFAR>(xa, A0 + p * a.pa + (AFAR ? (int64_t)f_k * BK * a.lda : (int64_t)f_k * BK), oa,
-                    a.ka - f_k * BK, a.lda);
-    step_load<false>(xb, B0 + q * a.pb + (BFAR ? (int64_t)f_k * BK * a.ldb : (int64_t)f_k * BK), ob,
-                    1 << 30, a.ldb);
-    if (--f_left > 0 && ++f_k == s1) f_k = s0, ++f_pair;
+    fA = A0 + p * a.pa + (AFAR ? (int64_t)f_k * BK * a.lda : (int64_t)f_k * BK);
+    fB = B0 + q * a.pb + (BFAR ? (int64_t)f_k * BK * a.ldb : (int64_t)f_k * BK);
   };
-  const auto put = [&](int s) {
-    step_put<AFAR>(lds[s & 1][0], xa);
-    step_put<BFAR>(lds[s & 1][1], xb);
+  const auto advance = [&]() {
+    if (--f_left > 0 && ++f_k == s1) f_k = s0, ++f_pair;
+    aim();
+  };
+  const auto load = [&](int v) {
+    xa[v] = step_load<AFAR && !BFAR>(fA, oa, v, a.ka - f_k * BK, a.lda);
+    xb[v] = step_load<false>(fB, ob, v, 0, a.ldb);
+  };
+  const auto put = [&](int s, int v) {
+    step_put<AFAR>(lds[s & 1][0], xa[v], v);
+    step_put<BFAR>(lds[s & 1][1], xb[v], v);
   };
   f32x16 acc[4][4];
 #pragma unroll
@@ -309,48 +294,57 @@ __global__ __launch_bounds__(NT, 1) void vl_gemm(VlArgs a) {
     const int m = m0 + tid;
     s_bias[tid] = a.bias && m < m_rows ? to_f(((const E*)a.bias)[a.v0 + m]) : 0.f;
   }
-  // Fragments one 16-element part ahead of the products that use them, a step's operands in LDS
-  // one step ahead, and in registers on their way there another.  The barrier of a step comes
-  // before its last part: the products of that part cover the first reads of the next step.
+  // A step has four parts of 16 contracted elements.  Fragments are read one part ahead of the
+  // products that use them; a step's operands go to LDS in quarters during the four parts
+  // before it is needed, and each quarter of the step after that is loaded into the registers
+  // it leaves: a whole step ahead, and never more than four loads at a time, since a wave whose
+  // loads queue up issues no products.  The barrier of a step comes before its last part, whose
+  // products cover the first reads of the next step.
   const int ab = frag_base<AFAR>(), bb = frag_base<BFAR>();
   bf16x8 fa[2][4], fb[2][4];
-  const auto read = [&](int s, int part, int to) {
-    const u16 *const la = lds[s & 1][0], *const lb = lds[s & 1][1];
+  const auto part = [&](const u16* la, const u16* lb, int k0, int from, int s, int quarter) {
+    const int to = from ^ 1;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) fa[to][i] = frag<AFAR>(la, ab, wm * 128 + i * 32, part * 16);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) fb[to][j] = frag<BFAR>(lb, bb, wn * 128 + j * 32, part * 16);
-  };
-  const auto multiply = [&](int from) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
+      fa[to][i] = frag<AFAR>(la, ab, wm * 128 + i * 32, k0);
+      fb[to][i] = frag<BFAR>(lb, bb, wn * 128 + i * 32, k0);
+      if (i & 1) {
+        put(s, 2 * quarter + (i >> 1));
+        if (quarter == 0 && i == 1) advance();
+        load(2 * quarter + (i >> 1));
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[from][i], fb[from][j], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
-  constexpr int READS = (AFAR ? 8 : 4) + (BFAR ? 8 : 4);
   if (steps > 0) {
-    fetch();
-    put(0);
-    fetch();
+    aim();
+#pragma unroll
+    for (int v = 0; v < 8; ++v) load(v);
+#pragma unroll
+    for (int v = 0; v < 8; ++v) put(0, v);
+    advance();
+#pragma unroll
+    for (int v = 0; v < 8; ++v) load(v);
     __syncthreads();
-    read(0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      fa[0][i] = frag<AFAR>(lds[0][0], ab, wm * 128 + i * 32, 0);
+      fb[0][i] = frag<BFAR>(lds[0][1], bb, wn * 128 + i * 32, 0);
+    }
+    put(1, 0), put(1, 1);
+    advance();
+    load(0), load(1);
     for (int s = 0; s < steps; ++s) {
-      read(s, 1, 1);
-      multiply(0);
-      interleave<0, READS, 0, 0>();
-      read(s, 2, 0);
-      multiply(1);
-      interleave<0, READS, 0, 0>();
-      read(s, 3, 1);
-      put(s + 1);
-      multiply(0);
-      interleave<0, READS, 16, 0>();
+      const u16 *const la = lds[s & 1][0], *const lb = lds[s & 1][1];
+      part(la, lb, 16, 0, s + 1, 1);
+      part(la, lb, 32, 1, s + 1, 2);
+      part(la, lb, 48, 0, s + 1, 3);
       __syncthreads();
-      read(s + 1, 0, 0);
-      fetch();
-      multiply(1);
-      interleave<0, READS, 0, 16>();
+      __builtin_amdgcn_sched_barrier(0);
+      part(lds[(s + 1) & 1][0], lds[(s + 1) & 1][1], 0, 1, s, 0);
     }
   }
   __syncthreads();
