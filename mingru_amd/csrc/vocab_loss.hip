@@ -14,10 +14,11 @@
 // operations in place of 6 with kept logits: at D = 1024 a logit's recomputation costs less
 // than writing and reading it in fp32.
 //
-// Products: 256 x 256 tiles of the result, 4 waves of 128 x 128 each (v_mfma_f32_32x32x16_bf16,
-// all 256 accumulator registers), 64 contracted elements a step through two LDS buffers.  Wave
-// tiles that large keep the operands' LDS reads (16 KB for 32 K MFMA cycles of a wave) below
-// the matrix cores' time.  Operands are rows of the free index with the contracted one
+// Products: 256 x 128 tiles of the result, 4 waves of 128 x 64 each with 32 x 32 x 16 matrix
+// instructions, 32 contracted elements a step through two LDS buffers (48 KB), so that a CU
+// holds two workgroups: one's epilogue, barriers and first loads pass under the other's
+// products.  (256 x 256 tiles, one workgroup a CU, spent a third of the logits' products'
+// time outside of them.)  Operands are rows of the free index with the contracted one
 // consecutive (near), or the other way round (far, read with ds_read_b64_tr_b16): x, W and d
 // all lie in memory once, and each is near in one product and far in another.
 //
@@ -36,8 +37,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int TILE = 256, BK = 64, NT = 256;
-constexpr int STAGE = TILE * BK;  // elements of one operand's step
+constexpr int TM = 256, TN = 128, BK = 32, NT = 256;
+constexpr int PADK = 64;  // packed rows are padded to this, and the contracted axis to it
 
 // ---- elements --------------------------------------------------------------------------
 __device__ __forceinline__ float to_f(u16 x) { return __uint_as_float((unsigned)x << 16); }
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(1024) void vl_index(const int64_t* __restrict__ tar
 }
 
 // Rows of `cols` elements in PL planes of bf16, `ld` elements a row, 0 past the columns except
-// a 1 at `ones`.  idx: the counted rows, padded with rows of 0 to a whole tile; null: all rows.
+// a 1 at `ones`.  idx: the counted rows, padded with rows of 0 to a multiple of the contracted step; null: all rows.
 template <typename E, int PL>
 __global__ __launch_bounds__(256) void vl_pack(const E* __restrict__ src, int64_t lds_, int cols,
                                                u16* __restrict__ dst, int ld, int64_t plane,
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(256) void vl_pack(const E* __restrict__ src, int64_
                                                int ones) {
   const int64_t j = blockIdx.x;
   const int64_t n = count ? *count : rows;
-  if (j >= (n + TILE - 1) / TILE * TILE) return;
+  if (j >= (n + PADK - 1) / PADK * PADK) return;
   const bool live = j < n;
   const E* s = src + (live ? (idx ? (int64_t)idx[j] : j) * lds_ : 0);
   for (int c = threadIdx.x * 2; c < ld; c += 512) {
@@ -149,28 +150,29 @@ struct VlArgs {
   int64_t pe;              // extra: elements between the splits'
 };
 
-// Fragment of 32 rows (near) or columns (far) x 16 contracted elements.  LDS: near rows of 64
-// elements, 16-byte chunk c of row r at c ^ ((r >> 1) & 7); far rows of 256, at
+// Fragment of 32 rows (near) or columns (far) x 16 contracted elements.  LDS: near rows of 32
+// elements, 16-byte chunk c of row r at c ^ ((r >> 2) & 3); far rows of W (256 or 128), at
 // c ^ ((r & 3) << 2).  Both read all 64 banks evenly.
-__device__ __forceinline__ int near_place(int r, int c) { return r * BK + ((c ^ ((r >> 1) & 7)) << 3); }
-__device__ __forceinline__ int far_place(int r, int c) { return r * TILE + ((c ^ ((r & 3) << 2)) << 3); }
+__device__ __forceinline__ int near_place(int r, int c) { return r * BK + ((c ^ ((r >> 2) & 3)) << 3); }
+template <int W>
+__device__ __forceinline__ int far_place(int r, int c) { return r * W + ((c ^ ((r & 3) << 2)) << 3); }
 
-template <bool FAR>
+template <bool FAR, int W>
 __device__ __forceinline__ int frag_base() {
   const int l = threadIdx.x & 63;
   if constexpr (FAR)
-    return far_place(8 * (l >> 5) + ((l & 15) >> 2), 2 * ((l >> 4) & 1) + ((l & 3) >> 1)) + 4 * (l & 1);
+    return far_place<W>(8 * (l >> 5) + ((l & 15) >> 2), 2 * ((l >> 4) & 1) + ((l & 3) >> 1)) + 4 * (l & 1);
   else
     return near_place(l & 31, l >> 5);
 }
-// r0: multiple of 32; k0: multiple of 16.
-template <bool FAR>
+// r0: multiple of 32; k0: 0 or 16.
+template <bool FAR, int W>
 __device__ __forceinline__ bf16x8 frag(const u16* m, int base, int r0, int k0) {
   if constexpr (FAR) {
     typedef __attribute__((address_space(3))) s16x4* lds_t;
-    const u16* p = m + (base ^ r0) + k0 * TILE;
+    const u16* p = m + (base ^ r0) + k0 * W;
     const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)p);
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(p + 4 * TILE));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(p + 4 * W));
     const s16x8 x = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     return __builtin_bit_cast(bf16x8, x);
   } else {
@@ -178,40 +180,40 @@ __device__ __forceinline__ bf16x8 frag(const u16* m, int base, int r0, int k0) {
   }
 }
 
-// One operand's step on its way to LDS: 8 vectors of 16 bytes a thread, at element offsets
+// One operand's step on its way to LDS: W / 64 vectors of 16 bytes a thread, at element offsets
 // from the step's first element that hold for every step.
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-template <bool FAR>
-__device__ __forceinline__ void step_places(unsigned (&at)[8], int r0, int rows, int ld) {
+template <bool FAR, int W>
+__device__ __forceinline__ void step_places(int (&at)[W / 64], int r0, int rows, int ld) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < W / 64; ++i) {
     const int v = threadIdx.x + i * NT;
     if constexpr (FAR) {
-      const int c = r0 + (v & 31) * 8;
-      at[i] = (unsigned)(v >> 5) * (unsigned)ld + (unsigned)(c + 8 <= rows ? c : 0);
+      const int c = r0 + (v % (W / 8)) * 8;
+      at[i] = v / (W / 8) * ld + (c + 8 <= rows ? c : 0);
     } else {
-      const int r = r0 + (v >> 3);
-      at[i] = (unsigned)((r < rows ? r : rows - 1) - r0) * (unsigned)ld + (v & 7) * 8;
+      const int r = r0 + (v >> 2);
+      at[i] = ((r < rows ? r : rows - 1) - r0) * ld + (v & 3) * 8;
     }
   }
 }
-// Vector i of a step.  CLAMP: a far operand's rows past the `left` ones from p on are the last
-// one again: the other operand is 0 there.
-template <bool CLAMP>
-__device__ __forceinline__ u32x4 step_load(const u16* p, const unsigned (&at)[8], int i, int left,
-                                           int ld) {
-  unsigned o = at[i];
+// Vector i of a step.  CLAMP: a far operand's rows past the `left` ones from p on (none or fewer
+// in a step that is padding alone) are the last one again: the other operand is 0 there.
+template <bool CLAMP, int W>
+__device__ __forceinline__ u32x4 step_load(const u16* p, const int (&at)[W / 64], int i,
+                                           int left, int ld) {
+  int o = at[i];
   if constexpr (CLAMP) {
-    const int over = (int)((threadIdx.x + i * NT) >> 5) - (left - 1);
-    o -= (unsigned)(over > 0 ? over : 0) * (unsigned)ld;
+    const int over = (int)(threadIdx.x + i * NT) / (W / 8) - (left - 1);
+    o -= (over > 0 ? over : 0) * ld;
   }
   return *reinterpret_cast<const u32x4*>(p + o);
 }
-template <bool FAR>
+template <bool FAR, int W>
 __device__ __forceinline__ void step_put(u16* m, u32x4 x, int i) {
   const int v = threadIdx.x + i * NT;
-  *reinterpret_cast<u32x4*>(m + (FAR ? far_place(v >> 5, v & 31) : near_place(v >> 3, v & 7))) = x;
+  *reinterpret_cast<u32x4*>(m + (FAR ? far_place<W>(v / (W / 8), v % (W / 8)) : near_place(v >> 2, v & 3))) = x;
 }
 
 // Pairs of planes whose product is not below 2^-24 of the whole, smallest first.
@@ -226,9 +228,9 @@ __device__ __forceinline__ void pair_of(int i, int& a, int& b) {
 }
 
 template <int EPI, bool AFAR, bool BFAR, int PL, typename E>
-__global__ __launch_bounds__(NT, 1) void vl_gemm(VlArgs a) {
-  __shared__ __align__(16) u16 lds[2][2][STAGE];
-  __shared__ __align__(16) float s_bias[TILE];
+__global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
+  __shared__ __align__(16) u16 lds[2][(TM + TN) * BK];  // the buffers: A, then B
+  __shared__ __align__(16) float s_bias[TM];
   const int tid = threadIdx.x, lane = tid & 63, wave = mg_uniform(tid >> 6);
   const int wm = wave & 1, wn = wave >> 1;
   // Tiles in bands of 8 along N, so that neighbours share operands; each XCD takes a run.
@@ -244,9 +246,9 @@ __global__ __launch_bounds__(NT, 1) void vl_gemm(VlArgs a) {
   const int band = id / (8 * a.mt), in = id - band * 8 * a.mt;
   const int wide = a.nt - band * 8 < 8 ? a.nt - band * 8 : 8;
   const int nt = band * 8 + in % wide, mt = in / wide;
-  const int m0 = mt * TILE, n0 = nt * TILE;
+  const int m0 = mt * TM, n0 = nt * TN;
   const int m_rows = a.m_count ? *a.m_count : a.m_rows, n_rows = a.n_count ? *a.n_count : a.n_rows;
-  const int K = a.k_count ? (*a.k_count + BK - 1) / BK * BK : a.K;
+  const int K = a.k_count ? (*a.k_count + PADK - 1) / PADK * PADK : a.K;
   if (m0 >= m_rows || n0 >= n_rows) return;
 
   constexpr int PAIRS = PL == 1 ? 1 : 6;
@@ -255,10 +257,11 @@ __global__ __launch_bounds__(NT, 1) void vl_gemm(VlArgs a) {
   const int s0 = split * per, s1 = s0 + per < ksteps ? s0 + per : ksteps;
   const int steps = s1 > s0 ? (s1 - s0) * PAIRS : 0;
 
-  u32x4 xa[8], xb[8];
-  unsigned oa[8], ob[8];
-  step_places<AFAR>(oa, m0, m_rows, a.lda);
-  step_places<BFAR>(ob, n0, n_rows, a.ldb);
+  constexpr int VA = TM / 64, VB = TN / 64;  // vectors of a thread
+  u32x4 xa[VA], xb[VB];
+  int oa[VA], ob[VB];
+  step_places<AFAR, TM>(oa, m0, m_rows, a.lda);
+  step_places<BFAR, TN>(ob, n0, n_rows, a.ldb);
   const u16* const A0 = a.A + (AFAR ? 0 : (int64_t)m0 * a.lda);
   const u16* const B0 = a.B + (BFAR ? 0 : (int64_t)n0 * a.ldb);
   // The step being fetched; past the last one it is that one again, so that the loop has no
@@ -275,167 +278,167 @@ __global__ __launch_bounds__(NT, 1) void vl_gemm(VlArgs a) {
     if (--f_left > 0 && ++f_k == s1) f_k = s0, ++f_pair;
     aim();
   };
-  const auto load = [&](int v) {
-    xa[v] = step_load<AFAR && !BFAR>(fA, oa, v, a.ka - f_k * BK, a.lda);
-    xb[v] = step_load<false>(fB, ob, v, 0, a.ldb);
+  // Half a step: the first or second of each thread's vectors.
+  const auto load = [&](int half) {
+#pragma unroll
+    for (int v = half * VA / 2; v < (half + 1) * VA / 2; ++v)
+      xa[v] = step_load<AFAR && !BFAR, TM>(fA, oa, v, a.ka - f_k * BK, a.lda);
+#pragma unroll
+    for (int v = half * VB / 2; v < (half + 1) * VB / 2; ++v)
+      xb[v] = step_load<false, TN>(fB, ob, v, 0, a.ldb);
   };
-  const auto put = [&](int s, int v) {
-    step_put<AFAR>(lds[s & 1][0], xa[v], v);
-    step_put<BFAR>(lds[s & 1][1], xb[v], v);
+  const auto put = [&](int s, int half) {
+#pragma unroll
+    for (int v = half * VA / 2; v < (half + 1) * VA / 2; ++v) step_put<AFAR, TM>(lds[s & 1], xa[v], v);
+#pragma unroll
+    for (int v = half * VB / 2; v < (half + 1) * VB / 2; ++v)
+      step_put<BFAR, TN>(lds[s & 1] + TM * BK, xb[v], v);
   };
-  f32x16 acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  // A row's bias is where its sum starts; past the vocabulary that is -inf, so that such a
+  // column's exponentials are 0.
+  f32x16 acc[4][2];
   if constexpr (EPI != VL_OUT) {
     const int m = m0 + tid;
-    s_bias[tid] = a.bias && m < m_rows ? to_f(((const E*)a.bias)[a.v0 + m]) : 0.f;
-  }
-  // A step has four parts of 16 contracted elements.  Fragments are read one part ahead of the
-  // products that use them; a step's operands go to LDS in quarters during the four parts
-  // before it is needed, and each quarter of the step after that is loaded into the registers
-  // it leaves: a whole step ahead, and never more than four loads at a time, since a wave whose
-  // loads queue up issues no products.  The barrier of a step comes before its last part, whose
-  // products cover the first reads of the next step.
-  const int ab = frag_base<AFAR>(), bb = frag_base<BFAR>();
-  bf16x8 fa[2][4], fb[2][4];
-  const auto part = [&](const u16* la, const u16* lb, int k0, int from, int s, int quarter) {
-    const int to = from ^ 1;
+    s_bias[tid] = m >= m_rows ? -INFINITY : a.bias ? to_f(((const E*)a.bias)[a.v0 + m]) : 0.f;
+    __syncthreads();
+    const float* const bw = s_bias + wm * 128 + 4 * (lane >> 5);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      fa[to][i] = frag<AFAR>(la, ab, wm * 128 + i * 32, k0);
-      fb[to][i] = frag<BFAR>(lb, bb, wn * 128 + i * 32, k0);
-      if (i & 1) {
-        put(s, 2 * quarter + (i >> 1));
-        if (quarter == 0 && i == 1) advance();
-        load(2 * quarter + (i >> 1));
+    for (int c = 0; c < 16; ++c) {
+      const float4 b = *reinterpret_cast<const float4*>(bw + 8 * c);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        acc[c >> 2][j][4 * (c & 3)] = b.x, acc[c >> 2][j][4 * (c & 3) + 1] = b.y;
+        acc[c >> 2][j][4 * (c & 3) + 2] = b.z, acc[c >> 2][j][4 * (c & 3) + 3] = b.w;
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[from][i], fb[from][j], acc[i][j], 0, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  }
+  // A step has two parts of 16 contracted elements.  Fragments are read one part ahead of the
+  // products that use them; a step's operands go to LDS in halves during the two parts before
+  // it is needed, and each half of the step after that is loaded into the registers it leaves.
+  // The barrier of a step comes before its last part, whose products cover the first reads of
+  // the next step.
+  const int ab = frag_base<AFAR, TM>(), bb = frag_base<BFAR, TN>();
+  bf16x8 fa[2][4], fb[2][2];
+  const auto read = [&](const u16* l, int k0, int to) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fa[to][i] = frag<AFAR, TM>(l, ab, wm * 128 + i * 32, k0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) fb[to][j] = frag<BFAR, TN>(l + TM * BK, bb, wn * 64 + j * 32, k0);
+  };
+  const auto part = [&](const u16* l, int k0, int from, int s, int half) {
+    read(l, k0, from ^ 1);
+    put(s, half);
+    if (half == 0) advance();
+    load(half);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[from][i], fb[from][j], acc[i][j], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
   };
   if (steps > 0) {
     aim();
-#pragma unroll
-    for (int v = 0; v < 8; ++v) load(v);
-#pragma unroll
-    for (int v = 0; v < 8; ++v) put(0, v);
-    advance();
-#pragma unroll
-    for (int v = 0; v < 8; ++v) load(v);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      fa[0][i] = frag<AFAR>(lds[0][0], ab, wm * 128 + i * 32, 0);
-      fb[0][i] = frag<BFAR>(lds[0][1], bb, wn * 128 + i * 32, 0);
-    }
-    put(1, 0), put(1, 1);
+    load(0), load(1);
+    put(0, 0), put(0, 1);
     advance();
     load(0), load(1);
+    __syncthreads();
+    read(lds[0], 0, 0);
+    put(1, 0);
+    advance();
+    load(0);
     for (int s = 0; s < steps; ++s) {
-      const u16 *const la = lds[s & 1][0], *const lb = lds[s & 1][1];
-      part(la, lb, 16, 0, s + 1, 1);
-      part(la, lb, 32, 1, s + 1, 2);
-      part(la, lb, 48, 0, s + 1, 3);
+      part(lds[s & 1], 16, 0, s + 1, 1);
       __syncthreads();
       __builtin_amdgcn_sched_barrier(0);
-      part(lds[(s + 1) & 1][0], lds[(s + 1) & 1][1], 0, 1, s, 0);
+      part(lds[(s + 1) & 1], 0, 1, s, 0);
     }
   }
   __syncthreads();
 
-  // Lane: column n = n0 + 128 wn + 32 j + (lane & 31) of the result; rows m = m0 + 128 wm +
+  // Lane: column n = n0 + 64 wn + 32 j + (lane & 31) of the result; rows m = m0 + 128 wm +
   // 32 i + 8 q + 4 (lane >> 5) + x in acc[i][j][4 q + x].
-  const int half = lane >> 5, mw = m0 + wm * 128 + 4 * half, nw = n0 + wn * 128 + (lane & 31);
-  // Logits of a row's 64 columns of this lane, -inf past the vocabulary.
-  const float* const bw = s_bias + wm * 128 + 4 * half;
-  const bool ragged = m0 + TILE > m_rows;
+  const int half = lane >> 5, mw = m0 + wm * 128 + 4 * half, nw = n0 + wn * 64 + (lane & 31);
   if constexpr (EPI == VL_LSE) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2; ++j) {
       const int n = nw + 32 * j;
       const int t = a.tgt[n < n_rows ? n : n_rows - 1] - a.v0 - mw;
-      float l[64], top = -INFINITY;
+      float top = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float4 b = *reinterpret_cast<const float4*>(bw + 32 * (c >> 2) + 8 * (c & 3));
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int m = 32 * (c >> 2) + 8 * (c & 3) + x;
-          float v = acc[c >> 2][j][4 * (c & 3) + x] + (x == 0 ? b.x : x == 1 ? b.y : x == 2 ? b.z : b.w);
-          if (ragged && mw + m >= m_rows) v = -INFINITY;
-          l[4 * c + x] = v;
-          top = fmaxf(top, v);
-        }
-      }
+      for (int c = 0; c < 64; ++c) top = fmaxf(top, acc[c >> 4][j][c & 15]);
       if (__ballot(t >= 0 && t < 128 && n < n_rows)) {
 #pragma unroll
         for (int c = 0; c < 64; ++c)
-          if (t == 8 * (c >> 2) + (c & 3) && n < n_rows) a.tlogit[n] = l[c];
+          if (t == 8 * (c >> 2) + (c & 3) && n < n_rows) a.tlogit[n] = acc[c >> 4][j][c & 15];
       }
       top = fmaxf(top, __shfl_xor(top, 32));
       const float ref = top == -INFINITY ? 0.f : top;
       float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < 64; ++c) sum += __expf(l[c] - ref);
+      for (int c = 0; c < 64; ++c) sum += __expf(acc[c >> 4][j][c & 15] - ref);
       sum += __shfl_xor(sum, 32);
       // fmaxf drops a NaN; the sum keeps it.
       if (half == 0 && n < n_rows) a.part[(int64_t)(2 * mt + wm) * a.n_ld + n] = make_float2(top, sum);
     }
   }
   if constexpr (EPI == VL_D) {
-    // In four rounds of 64 rows, (planes, 64 rows n, 256 columns m) in LDS with chunk c of row r
-    // at c ^ (r & 31), then whole rows out.  Rows up to the next multiple of the contracted step
-    // are written, as 0.
-    u16* const stage = &lds[0][0][0];
-    const int rows = (n_rows + BK - 1) / BK * BK;
+    // In two rounds of 64 rows and for each plane, (64 rows n, 256 columns m) in LDS with chunk
+    // c of row r at c ^ (r & 31), then whole rows out.  Rows up to the next multiple of the
+    // packing are written, as 0.
+    u16* const stage = &lds[0][0];
+    const int rows = (n_rows + PADK - 1) / PADK * PADK;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2; ++j) {
       const int n = nw + 32 * j, r = n < n_rows ? n : n_rows - 1;
       const float2 soft = a.soft[r];
-      const float g = n < n_rows ? a.g[r] : 0.f;
+      const float g = n < n_rows ? a.g[r] : 0.f, sg = soft.y * g;
       const int t = a.tgt[r] - a.v0 - mw;
+#pragma unroll
+      for (int c = 0; c < 64; ++c) {
+        acc[c >> 4][j][c & 15] = __expf(acc[c >> 4][j][c & 15] - soft.x) * sg;
+      }
+      if (__ballot(t >= 0 && t < 128)) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) acc[c >> 4][j][c & 15] -= t == 8 * (c >> 2) + (c & 3) ? g : 0.f;
+      }
       const int sr = wn * 32 + (lane & 31);
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float4 b = *reinterpret_cast<const float4*>(bw + 32 * (c >> 2) + 8 * (c & 3));
-        float p[4];
+      for (int q = 0; q < PL; ++q) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int m = 32 * (c >> 2) + 8 * (c & 3) + x;
-          const float v = acc[c >> 2][j][4 * (c & 3) + x] + (x == 0 ? b.x : x == 1 ? b.y : x == 2 ? b.z : b.w);
-          p[x] = (__expf(v - soft.x) * soft.y - (t == m ? 1.f : 0.f)) * g;
-          if ((ragged && mw + m >= m_rows) || n >= n_rows) p[x] = 0.f;
+        for (int c = 0; c < 16; ++c) {
+          f32x16& v = acc[c >> 2][j];
+          const int e = 4 * (c & 3);
+          const unsigned u0 = pack2(v[e], v[e + 1]), u1 = pack2(v[e + 2], v[e + 3]);
+          *reinterpret_cast<uint2*>(stage + sr * TM + (((wm * 16 + c) ^ (sr & 31)) << 3) + 4 * half) =
+              make_uint2(u0, u1);
+          if (q + 1 < PL) v[e] -= low(u0), v[e + 1] -= high(u0), v[e + 2] -= low(u1), v[e + 3] -= high(u1);
         }
-        u16* const to = stage + sr * TILE + (((wm * 16 + c) ^ (sr & 31)) << 3) + 4 * half;
+        __syncthreads();
 #pragma unroll
-        for (int q = 0; q < PL; ++q) {
-          const unsigned u0 = pack2(p[0], p[1]), u1 = pack2(p[2], p[3]);
-          *reinterpret_cast<uint2*>(to + q * 64 * TILE) = make_uint2(u0, u1);
-          p[0] -= low(u0), p[1] -= high(u0), p[2] -= low(u1), p[3] -= high(u1);
+        for (int u = 0; u < 8; ++u) {
+          const int v = tid + u * NT, r2 = v >> 5, c = v & 31;
+          const int n2 = n0 + (r2 >> 5) * 64 + 32 * j + (r2 & 31);
+          if (n2 < rows && m0 + c * 8 < a.ldd)
+            *reinterpret_cast<u32x4*>(a.d + q * a.pd + (int64_t)n2 * a.ldd + m0 + c * 8) =
+                *reinterpret_cast<const u32x4*>(stage + r2 * TM + ((c ^ (r2 & 31)) << 3));
         }
+        __syncthreads();
       }
-      __syncthreads();
-#pragma unroll
-      for (int u = 0; u < PL * 8; ++u) {
-        const int v = tid + u * NT, q = v >> 11, r2 = (v >> 5) & 63, c = v & 31;
-        const int n2 = n0 + (r2 >> 5) * 128 + 32 * j + (r2 & 31);
-        if (n2 < rows && m0 + c * 8 < a.ldd)
-          *reinterpret_cast<u32x4*>(a.d + q * a.pd + (int64_t)n2 * a.ldd + m0 + c * 8) =
-              *reinterpret_cast<const u32x4*>(stage + q * 64 * TILE + r2 * TILE + ((c ^ (r2 & 31)) << 3));
-      }
-      __syncthreads();
     }
   }
   if constexpr (EPI == VL_OUT) {
     const bool f32 = a.out_f32;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2; ++j) {
       const int n = nw + 32 * j;
       if (n >= a.n_out) continue;
       const int64_t row = split * a.po + n * a.ldo;
@@ -586,9 +589,9 @@ bool vl_shape(int dtype, int64_t N, int64_t V, int64_t D, Shape* s) {
   if ((dtype & ~1) || N < 1 || V < 1 || D < 1 || N > (1 << 30) || V > (1 << 30) || D > (1 << 20))
     return false;
   s->N = N, s->V = V, s->D = D;
-  s->np = up_to(N, TILE), s->kp = up_to(D, BK), s->dx = up_to(D + 1, BK);
+  s->np = up_to(N, PADK), s->kp = up_to(D, PADK), s->dx = up_to(D + 1, PADK);
   s->planes = dtype ? 1 : 3;
-  s->own_w = dtype == 0 || D % BK != 0;
+  s->own_w = dtype == 0 || D % PADK != 0;
   return true;
 }
 struct State {
@@ -614,12 +617,13 @@ State vl_state(const Shape& s, void* base) {
   return t;
 }
 
-// Parts of the contracted axis for `tiles` result tiles on 256 CUs: the fewest steps in a row.
+// Parts of the contracted axis for `tiles` result tiles on 256 CUs of two workgroups: the fewest
+// steps in a row.
 int vl_splits(int64_t tiles, int64_t steps) {
   int best = 1;
   double least = 1e300;
-  for (int s = 1; s <= 16 && (s == 1 || steps / s >= 8); ++s) {
-    const double cost = (double)((tiles * s + 255) / 256) * ((steps + s - 1) / s + 4) + 2.0 * (s - 1);
+  for (int s = 1; s <= 16 && (s == 1 || steps / s >= 16); ++s) {
+    const double cost = (double)((tiles * s + 511) / 512) * ((steps + s - 1) / s + 8) + 4.0 * (s - 1);
     if (cost < least) least = cost, best = s;
   }
   return best;
@@ -637,12 +641,12 @@ struct Back {
 Back vl_back(const Shape& s, void* base) {
   Back b;
   const int64_t most = VL_D_BYTES / (s.np * 2 * s.planes);
-  b.pieces = (s.V + (most > TILE ? most : TILE) - 1) / (most > TILE ? most : TILE);
-  b.vp = up_to((s.V + b.pieces - 1) / b.pieces, TILE);
+  b.pieces = (s.V + (most > TM ? most : TM) - 1) / (most > TM ? most : TM);
+  b.vp = up_to((s.V + b.pieces - 1) / b.pieces, TM);
   b.pieces = (s.V + b.vp - 1) / b.vp;
   const int64_t steps = s.planes == 1 ? 1 : 6;
-  b.dx_splits = vl_splits((s.np / TILE) * ((s.D + TILE - 1) / TILE), b.vp / BK * steps);
-  b.dw_splits = vl_splits((b.vp / TILE) * ((s.D + 1 + TILE - 1) / TILE), s.np / BK * steps);
+  b.dx_splits = vl_splits((s.np + TN - 1) / TN * ((s.D + TM - 1) / TM), b.vp / BK * steps);
+  b.dw_splits = vl_splits(b.vp / TN * ((s.D + TM) / TM), s.np / BK * steps);
   char* p = (char*)base;
   const auto take = [&](int64_t n) {
     char* at = p;
@@ -677,12 +681,12 @@ VlArgs vl_logits(const Shape& s, const State& t, const void* w, const void* bias
   a.B = t.xc, a.ldb = (int)s.dx, a.pb = s.np * s.dx;
   a.m_rows = (int)cols, a.n_count = t.count;
   a.K = (int)s.kp, a.ka = 1 << 30;
-  a.mt = (int)((cols + TILE - 1) / TILE), a.nt = (int)(s.np / TILE), a.splits = 1;
+  a.mt = (int)((cols + TM - 1) / TM), a.nt = (int)((s.np + TN - 1) / TN), a.splits = 1;
   a.v0 = (int)v0, a.V = (int)s.V, a.bias = bias, a.tgt = t.tgt, a.n_ld = (int)s.np;
   return a;
 }
 
-int64_t vl_part_rows(const Shape& s) { return 2 * ((s.V + TILE - 1) / TILE); }
+int64_t vl_part_rows(const Shape& s) { return 2 * ((s.V + TM - 1) / TM); }
 
 template <typename E, int PL>
 void vl_pack_run(const void* src, int64_t ld, int64_t cols, u16* dst, int64_t dld, int64_t plane,
@@ -764,7 +768,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
   hipLaunchKernelGGL(vl_upstream, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, stream, dloss,
                      t.idx, t.count, reduction, b.g);
   for (int64_t v0 = 0, piece = 0; v0 < V; v0 += b.vp, ++piece) {
-    const int64_t cols = V - v0 < b.vp ? V - v0 : b.vp, kc = up_to(cols, BK);
+    const int64_t cols = V - v0 < b.vp ? V - v0 : b.vp, kc = up_to(cols, PADK);
     VlArgs a = vl_logits(s, t, w, bias, v0, cols);
     a.soft = t.soft, a.g = b.g;
     a.d = b.d, a.pd = s.np * b.vp, a.ldd = (int)kc;
@@ -774,7 +778,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
       c.A = a.A, c.lda = a.lda, c.pa = a.pa, c.m_rows = (int)s.kp;
       c.B = b.d, c.ldb = (int)kc, c.pb = a.pd, c.n_count = t.count;
       c.K = (int)kc, c.ka = (int)cols;
-      c.mt = (int)((D + TILE - 1) / TILE), c.nt = (int)(s.np / TILE), c.splits = b.dx_splits;
+      c.mt = (int)((D + TM - 1) / TM), c.nt = (int)((s.np + TN - 1) / TN), c.splits = b.dx_splits;
       c.out = b.dx_part + piece * b.dx_splits * N * D;
       c.ldo = D, c.po = N * D, c.m_out = (int)D, c.n_out = (int)N, c.out_f32 = 1;
       rc = vl_run<VL_OUT, true, false>(dtype, c, stream);
@@ -784,7 +788,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
       c.A = t.xc, c.lda = (int)s.dx, c.pa = s.np * s.dx, c.m_rows = (int)s.dx;
       c.B = b.d, c.ldb = (int)kc, c.pb = a.pd, c.n_rows = (int)kc;
       c.k_count = t.count, c.ka = 1 << 30;
-      c.mt = (int)((D + (db ? 1 : 0) + TILE - 1) / TILE), c.nt = (int)((cols + TILE - 1) / TILE);
+      c.mt = (int)((D + (db ? 1 : 0) + TM - 1) / TM), c.nt = (int)((cols + TN - 1) / TN);
       c.splits = b.dw_splits;
       c.ldo = D, c.m_out = (int)D, c.n_out = (int)cols;
       void* const to = (char*)dw + v0 * D * e;
