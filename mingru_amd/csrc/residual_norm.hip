@@ -12,10 +12,10 @@
 //
 // Bound by memory: the forward reads h, x, gate and writes r, y; the backward reads h, x,
 // gate, dr, dy and writes dh, dx, dgate.  So a row is read once and stays in registers: a
-// group of TPR lanes holds it, K vectors of 8 consecutive elements a lane, and the groups
-// walk over rows with the row vectors (weights) loaded once.  The backward forms p, u and r
-// again from h, x and gate rather than reading them (r, rounded, would cost as many bytes as
-// x), from the forward's means and reciprocal deviations (16 bytes a row).
+// group of TPR lanes holds it, 8 consecutive elements a lane, and the groups walk over rows.
+// The backward forms p, u and r again from h, x and gate rather than reading them (r, rounded,
+// would cost as many bytes as x), from the forward's means and reciprocal deviations (16 bytes
+// a row).
 //
 // The row vectors' gradients are sums over all rows: every workgroup sums its rows in
 // registers, then over its groups in LDS in a fixed order, and writes one partial row; a
@@ -60,6 +60,7 @@ struct Vec8<float> {
     b = make_float4(v[4], v[5], v[6], v[7]);
   }
 };
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 template <>
 struct Vec8<u16> {
   uint4 q;
@@ -74,9 +75,11 @@ struct Vec8<u16> {
   __device__ __forceinline__ void set(const float (&v)[8]) {
     unsigned w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = (unsigned)__builtin_bit_cast(u16, (__bf16)v[2 * i]) |
-             ((unsigned)__builtin_bit_cast(u16, (__bf16)v[2 * i + 1]) << 16);
+    for (int i = 0; i < 4; ++i) {
+      const bf16x2 h = {(__bf16)v[2 * i], (__bf16)v[2 * i + 1]};
+      w[i] = __builtin_bit_cast(unsigned, h);
+      asm("" : "+v"(w[i]));  // keeps the pair one packed conversion
+    }
     q = make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
@@ -85,17 +88,20 @@ __device__ __forceinline__ float rn_ld1(const u16* p) { return __uint_as_float((
 __device__ __forceinline__ void rn_st1(float* p, float x) { *p = x; }
 __device__ __forceinline__ void rn_st1(u16* p, float x) { *p = __builtin_bit_cast(u16, (__bf16)x); }
 
-// Elements c .. c+7 of a row of D; past D they read as 0 and are not written.  VEC: D and
-// every row start are multiples of 16 bytes, so 8 elements lie inside or outside together.
+// Whether element c + i of a row of D is in it.  VEC: D and every row start are multiples of 16
+// bytes, so the 8 elements from c on are in the row or past it together.
+template <bool VEC>
+__device__ __forceinline__ bool rn_in(int c, int i, int D) {
+  return VEC ? c < D : c + i < D;
+}
+// Elements c .. c + 7 of a row; past it they read as 0 and are not written.
 template <typename E, bool VEC>
 __device__ __forceinline__ void rn_load(const E* row, int c, int D, float (&v)[8]) {
   if constexpr (VEC) {
-    if (c < D) {
-      reinterpret_cast<const Vec8<E>*>(row + c)->get(v);
-    } else {
+    // A load under no condition: one under it is waited for where the branches meet.
+    reinterpret_cast<const Vec8<E>*>(row + (c < D ? c : 0))->get(v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    }
+    for (int i = 0; i < 8; ++i) v[i] = c < D ? v[i] : 0.f;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = c + i < D ? rn_ld1(row + c + i) : 0.f;
@@ -115,6 +121,20 @@ __device__ __forceinline__ void rn_store(E* row, int c, int D, const float (&v)[
       if (c + i < D) rn_st1(row + c + i, v[i]);
   }
 }
+// Elements of a row vector, `other` where there is none.  They are read again for every row:
+// the caches hold them, registers for them would cost the waves that hide the rows' loads.
+template <typename P, bool VEC>
+__device__ __forceinline__ void rn_vector(const void* p, float other, int c, int D, float (&v)[8]) {
+  if (p) {
+    asm volatile("" : "+s"(p));  // or the compiler would load it once, before the loop
+    rn_load<P, VEC>((const P*)p, c, D, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = other;
+  }
+}
+
+constexpr int rn_threads(int tpr) { return tpr > 256 ? tpr : 256; }
 
 // A row's sums over its TPR lanes, in every one of them.  Past one wave the waves' sums meet
 // in LDS; `turn` alternates between two sets of slots, so one barrier is enough: a wave can
@@ -125,8 +145,8 @@ __device__ __forceinline__ void rn_sum(float (&s)[N], int& turn) {
   for (int i = 0; i < N; ++i) s[i] = mg_group_sum<(TPR < MG_WAVE ? TPR : MG_WAVE)>(s[i]);
   if constexpr (TPR > MG_WAVE) {
     constexpr int W = TPR / MG_WAVE;
-    __shared__ float slots[2][4][W];
-    const int w = threadIdx.x / MG_WAVE;
+    __shared__ float slots[2][N][rn_threads(TPR) / MG_WAVE];
+    const int w = mg_uniform(threadIdx.x / MG_WAVE), first = w / W * W;
     if ((threadIdx.x & (MG_WAVE - 1)) == 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i) slots[turn][i][w] = s[i];
@@ -136,7 +156,7 @@ __device__ __forceinline__ void rn_sum(float (&s)[N], int& turn) {
     for (int i = 0; i < N; ++i) {
       float t = 0.f;
 #pragma unroll
-      for (int j = 0; j < W; ++j) t += slots[turn][i][j];
+      for (int j = 0; j < W; ++j) t += slots[turn][i][first + j];
       s[i] = t;
     }
     turn ^= 1;
@@ -144,270 +164,206 @@ __device__ __forceinline__ void rn_sum(float (&s)[N], int& turn) {
 }
 
 // Mean and reciprocal deviation of a row held in v (elements past D are 0).
-template <int TPR, int K>
-__device__ __forceinline__ float2 rn_stats(const float (&v)[K][8], int kind, int c0, int D,
-                                           float eps, int& turn) {
+template <int TPR, bool VEC>
+__device__ __forceinline__ float2 rn_stats(const float (&v)[8], int kind, int c, int D, float eps,
+                                           int& turn) {
+  const float inv = 1.f / (float)D;
   float mean = 0.f;
   if (kind == RN_LAYER) {
-    float s[1] = {0.f};
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[0] += v[k][i];
+    float s[1] = {((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]))};
     rn_sum<TPR>(s, turn);
-    mean = s[0] / (float)D;
+    mean = s[0] * inv;
   }
   float q[1] = {0.f};
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float d = c0 + k * TPR * 8 + i < D ? v[k][i] - mean : 0.f;
-      q[0] += d * d;
-    }
-  rn_sum<TPR>(q, turn);
-  return make_float2(mean, 1.f / sqrtf(q[0] / (float)D + eps));
-}
-
-__device__ __forceinline__ float rn_sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
-
-template <int K, typename P, bool VEC, int TPR>
-__device__ __forceinline__ void rn_vector(const void* p, float other, int c0, int D,
-                                          float (&v)[K][8]) {
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (p) {
-      rn_load<P, VEC>((const P*)p, c0 + k * TPR * 8, D, v[k]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[k][i] = other;
-    }
+  for (int i = 0; i < 8; ++i) {
+    const float d = v[i] - mean;
+    q[0] += rn_in<VEC>(c, i, D) ? d * d : 0.f;
   }
+  rn_sum<TPR>(q, turn);
+  return make_float2(mean, 1.f / sqrtf(q[0] * inv + eps));
 }
 
-template <typename E, typename P, int TPR, int K, bool VEC>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_fwd(RnArgs a) {
-  constexpr int NT = TPR > 256 ? TPR : 256, ROWS = NT / TPR;
-  const int c0 = (threadIdx.x % TPR) * 8, D = a.D;
-  float scale[K][8], pw[K][8], pb[K][8], qw[K][8], qb[K][8];
-  rn_vector<K, P, VEC, TPR>(a.scale, a.scale_const, c0, D, scale);
-  rn_vector<K, P, VEC, TPR>(a.post_w, 1.f, c0, D, pw);
-  rn_vector<K, P, VEC, TPR>(a.post_b, 0.f, c0, D, pb);
-  rn_vector<K, P, VEC, TPR>(a.pre_w, 1.f, c0, D, qw);
-  rn_vector<K, P, VEC, TPR>(a.pre_b, 0.f, c0, D, qb);
+// 1 / (1 + e^-x) from the hardware's exponential and reciprocal, each 1 ulp off at most but for
+// the rounding of x log2 e: 1e-7 of the result for |x| < 1, 5e-7 at |x| = 10.
+__device__ __forceinline__ float rn_sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+}
+
+template <typename E, typename P, int TPR, bool VEC>
+__global__ __launch_bounds__(rn_threads(TPR)) void residual_norm_fwd(RnArgs a) {
+  constexpr int ROWS = rn_threads(TPR) / TPR;
+  const int c = (threadIdx.x % TPR) * 8, D = a.D;
   int turn = 0;
   // A group past the last row repeats it without storing, so that whole waves stay active.
   for (int64_t base = (int64_t)blockIdx.x * ROWS; base < a.rows; base += (int64_t)gridDim.x * ROWS) {
     const int64_t at = base + threadIdx.x / TPR;
     const bool live = at < a.rows;
     const int64_t row = live ? at : a.rows - 1;
-    float u[K][8], xv[K][8], gv[K][8];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = c0 + k * TPR * 8;
-      rn_load<E, VEC>((const E*)a.h + row * a.ldh, c, D, u[k]);
-      if (a.x) rn_load<E, VEC>((const E*)a.x + row * a.ldx, c, D, xv[k]);
-      if (a.act) rn_load<E, VEC>((const E*)a.gate + row * a.ldg, c, D, gv[k]);
-    }
+    float u[8], xv[8], gv[8], w[8], b[8];
+    rn_load<E, VEC>((const E*)a.h + row * a.ldh, c, D, u);
+    if (a.x) rn_load<E, VEC>((const E*)a.x + row * a.ldx, c, D, xv);
+    if (a.act) rn_load<E, VEC>((const E*)a.gate + row * a.ldg, c, D, gv);
     float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
     if (a.post) {
-      const float2 m = rn_stats<TPR, K>(u, a.post, c0, D, a.eps, turn);
+      rn_vector<P, VEC>(a.post_w, 1.f, c, D, w);
+      rn_vector<P, VEC>(a.post_b, 0.f, c, D, b);
+      const float2 m = rn_stats<TPR, VEC>(u, a.post, c, D, a.eps, turn);
       st.x = m.x, st.y = m.y;
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) u[k][i] = (u[k][i] - m.x) * m.y * pw[k][i] + pb[k][i];
+      for (int i = 0; i < 8; ++i) u[i] = (u[i] - m.x) * m.y * w[i] + b[i];
     }
-#pragma unroll
-    for (int k = 0; k < K; ++k)
+    if (a.act) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (a.act) {
-          const float s = rn_sigmoid(gv[k][i]);
-          u[k][i] *= a.act == RN_SILU ? s * gv[k][i] : s;
-        }
-        if (a.x) u[k][i] = xv[k][i] + scale[k][i] * u[k][i];
-        u[k][i] = c0 + k * TPR * 8 + i < D ? u[k][i] : 0.f;  // not the bias past the row
+        const float s = rn_sigmoid(gv[i]);
+        u[i] *= a.act == RN_SILU ? s * gv[i] : s;
       }
-    if (a.r && live) {
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-        rn_store<E, VEC>((E*)a.r + row * D, c0 + k * TPR * 8, D, u[k]);
     }
+    if (a.x) {
+      rn_vector<P, VEC>(a.scale, a.scale_const, c, D, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] = xv[i] + w[i] * u[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = rn_in<VEC>(c, i, D) ? u[i] : 0.f;  // not what a bias left
+    if (a.r && live) rn_store<E, VEC>((E*)a.r + row * D, c, D, u);
     if (a.pre) {
-      const float2 m = rn_stats<TPR, K>(u, a.pre, c0, D, a.eps, turn);
+      rn_vector<P, VEC>(a.pre_w, 1.f, c, D, w);
+      rn_vector<P, VEC>(a.pre_b, 0.f, c, D, b);
+      const float2 m = rn_stats<TPR, VEC>(u, a.pre, c, D, a.eps, turn);
       st.z = m.x, st.w = m.y;
       if (live) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          float y[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = (u[k][i] - m.x) * m.y * qw[k][i] + qb[k][i];
-          rn_store<E, VEC>((E*)a.y + row * D, c0 + k * TPR * 8, D, y);
-        }
+        for (int i = 0; i < 8; ++i) u[i] = (u[i] - m.x) * m.y * w[i] + b[i];
+        rn_store<E, VEC>((E*)a.y + row * D, c, D, u);
       }
     }
     if (a.stats && live && threadIdx.x % TPR == 0) a.stats[row] = st;
   }
 }
 
-template <typename E, typename P, int TPR, int K, bool VEC>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_bwd(RnArgs a) {
-  constexpr int NT = TPR > 256 ? TPR : 256, ROWS = NT / TPR;
-  const int c0 = (threadIdx.x % TPR) * 8, D = a.D;
+template <typename E, typename P, int TPR, bool VEC>
+__global__ __launch_bounds__(rn_threads(TPR)) void residual_norm_bwd(RnArgs a) {
+  constexpr int ROWS = rn_threads(TPR) / TPR;
+  const int c = (threadIdx.x % TPR) * 8, D = a.D;
   const float inv = 1.f / (float)D;
-  float scale[K][8], pw[K][8], pb[K][8], qw[K][8];
-  rn_vector<K, P, VEC, TPR>(a.scale, a.scale_const, c0, D, scale);
-  rn_vector<K, P, VEC, TPR>(a.post_w, 1.f, c0, D, pw);
-  rn_vector<K, P, VEC, TPR>(a.post_b, 0.f, c0, D, pb);
-  rn_vector<K, P, VEC, TPR>(a.pre_w, 1.f, c0, D, qw);
   // A row of one element: dn (1 - n^2) would cancel down to its rounding; 1 - n^2 = eps rstd^2.
   const auto lone = [&](int kind) { return D == 1 && kind == RN_RMS; };
-  float sum[RN_NPAR][K][8];
+  float sum[RN_NPAR][8];
 #pragma unroll
   for (int p = 0; p < RN_NPAR; ++p)
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum[p][k][i] = 0.f;
+    for (int i = 0; i < 8; ++i) sum[p][i] = 0.f;
   int turn = 0;
   for (int64_t base = (int64_t)blockIdx.x * ROWS; base < a.rows; base += (int64_t)gridDim.x * ROWS) {
     const int64_t at = base + threadIdx.x / TPR;
     const bool live = at < a.rows;
     const int64_t row = live ? at : a.rows - 1;
-    float n[K][8], xv[K][8], gv[K][8], g[K][8], dy[K][8];
+    float n[8], xv[8], gv[8], g[8], dy[8];
+    rn_load<E, VEC>((const E*)a.h + row * a.ldh, c, D, n);
+    if (a.dy && a.x) rn_load<E, VEC>((const E*)a.x + row * a.ldx, c, D, xv);
+    if (a.act) rn_load<E, VEC>((const E*)a.gate + row * a.ldg, c, D, gv);
+    if (a.dr) {
+      rn_load<E, VEC>((const E*)a.dr + row * a.lddr, c, D, g);
+    } else {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = c0 + k * TPR * 8;
-      rn_load<E, VEC>((const E*)a.h + row * a.ldh, c, D, n[k]);
-      if (a.x && a.pre) rn_load<E, VEC>((const E*)a.x + row * a.ldx, c, D, xv[k]);
-      if (a.act) rn_load<E, VEC>((const E*)a.gate + row * a.ldg, c, D, gv[k]);
-      if (a.dr) {
-        rn_load<E, VEC>((const E*)a.dr + row * a.lddr, c, D, g[k]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[k][i] = 0.f;
-      }
-      if (a.dy) rn_load<E, VEC>((const E*)a.dy + row * a.lddy, c, D, dy[k]);
+      for (int i = 0; i < 8; ++i) g[i] = 0.f;
     }
+    if (a.dy) rn_load<E, VEC>((const E*)a.dy + row * a.lddy, c, D, dy);
     const float4 st = a.stats ? a.stats[row] : make_float4(0.f, 1.f, 0.f, 1.f);
+    // n: the post norm's rows; p = n w + b; f = act(gate), slope = act'(gate); u = p f.
+    float p[8], f[8], slope[8], w[8], sc[8];
+    rn_vector<P, VEC>(a.scale, a.scale_const, c, D, sc);
     if (a.post) {
+      float b[8];
+      rn_vector<P, VEC>(a.post_w, 1.f, c, D, w);
+      rn_vector<P, VEC>(a.post_b, 0.f, c, D, b);
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+      for (int i = 0; i < 8; ++i) {
+        n[i] = (n[i] - st.x) * st.y;
+        p[i] = n[i] * w[i] + b[i];
+      }
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) n[k][i] = (n[k][i] - st.x) * st.y;
+      for (int i = 0; i < 8; ++i) w[i] = 1.f, p[i] = n[i];
     }
-    // n, p = n w + b, u = p act(gate), r = x + scale u, formed again where they are used.
-    const auto post = [&](int k, int i) { return a.post ? n[k][i] * pw[k][i] + pb[k][i] : n[k][i]; };
-    const auto act = [&](int k, int i) {
-      if (!a.act) return 1.f;
-      const float s = rn_sigmoid(gv[k][i]);
-      return a.act == RN_SILU ? s * gv[k][i] : s;
-    };
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[i] = 1.f, slope[i] = 0.f;
+      if (a.act) {
+        const float s = rn_sigmoid(gv[i]), ds = s * (1.f - s);
+        f[i] = a.act == RN_SILU ? s * gv[i] : s;
+        slope[i] = a.act == RN_SILU ? s + gv[i] * ds : ds;
+      }
+    }
     if (a.dy) {
-      float s[2] = {0.f, 0.f};
+      float qw[8], s[2] = {0.f, 0.f};
+      rn_vector<P, VEC>(a.pre_w, 1.f, c, D, qw);
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float u = post(k, i) * act(k, i);
-          const float r = a.x ? xv[k][i] + scale[k][i] * u : u;
-          xv[k][i] = (r - st.z) * st.w;  // the pre norm's rows
-          if (live) {
-            sum[RN_DPRE_W][k][i] += dy[k][i] * xv[k][i];
-            sum[RN_DPRE_B][k][i] += dy[k][i];
-          }
-          dy[k][i] *= qw[k][i];
-          s[0] += dy[k][i] * xv[k][i];  // dy is 0 past D
-          s[1] += dy[k][i];
-        }
+      for (int i = 0; i < 8; ++i) {
+        const float r = a.x ? xv[i] + sc[i] * (p[i] * f[i]) : p[i] * f[i];
+        xv[i] = (r - st.z) * st.w;  // the pre norm's rows
+        if (live) sum[RN_DPRE_W][i] += dy[i] * xv[i], sum[RN_DPRE_B][i] += dy[i];
+        dy[i] *= qw[i];
+        s[0] += dy[i] * xv[i];  // dy is 0 past D
+        s[1] += dy[i];
+      }
       rn_sum<TPR>(s, turn);
       const float m0 = s[0] * inv, m1 = a.pre == RN_LAYER ? s[1] * inv : 0.f;
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float d = dy[k][i] - xv[k][i] * m0 - m1;
-          g[k][i] += st.w * (lone(a.pre) ? dy[k][i] * (a.eps * st.w * st.w) : d);
-        }
+      for (int i = 0; i < 8; ++i) {
+        const float d = dy[i] - xv[i] * m0 - m1;
+        g[i] += st.w * (lone(a.pre) ? dy[i] * (a.eps * st.w * st.w) : d);
+      }
     }
-    if (a.dx && live) {
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-        rn_store<E, VEC>((E*)a.dx + row * D, c0 + k * TPR * 8, D, g[k]);
-    }
-    // g becomes dp; gv becomes the gate's gradient.
+    if (a.dx && live) rn_store<E, VEC>((E*)a.dx + row * D, c, D, g);
     float s[2] = {0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool in = c0 + k * TPR * 8 + i < D;
-        const float p = post(k, i);
-        float f = 1.f, slope = 0.f;
-        if (a.act) {
-          const float sg = rn_sigmoid(gv[k][i]);
-          const float ds = sg * (1.f - sg);
-          f = a.act == RN_SILU ? sg * gv[k][i] : sg;
-          slope = a.act == RN_SILU ? sg + gv[k][i] * ds : ds;
-        }
-        if (live) sum[RN_DSCALE][k][i] += g[k][i] * (p * f);
-        const float du = in ? (a.x ? g[k][i] * scale[k][i] : g[k][i]) : 0.f;
-        gv[k][i] = du * p * slope;
-        const float dp = du * f;
-        if (live) {
-          sum[RN_DPOST_W][k][i] += dp * n[k][i];
-          sum[RN_DPOST_B][k][i] += dp;
-        }
-        g[k][i] = a.post ? dp * pw[k][i] : dp;
-        s[0] += g[k][i] * n[k][i];
-        s[1] += g[k][i];
-      }
-    if (a.dgate && live) {
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-        rn_store<E, VEC>((E*)a.dgate + row * D, c0 + k * TPR * 8, D, gv[k]);
+    for (int i = 0; i < 8; ++i) {
+      if (live) sum[RN_DSCALE][i] += g[i] * (p[i] * f[i]);
+      const float du = rn_in<VEC>(c, i, D) ? (a.x ? g[i] * sc[i] : g[i]) : 0.f;
+      gv[i] = du * p[i] * slope[i];
+      const float dp = du * f[i];
+      if (live) sum[RN_DPOST_W][i] += dp * n[i], sum[RN_DPOST_B][i] += dp;
+      g[i] = dp * w[i];
+      s[0] += g[i] * n[i];
+      s[1] += g[i];
     }
+    if (a.dgate && live) rn_store<E, VEC>((E*)a.dgate + row * D, c, D, gv);
     if (a.post) {
       rn_sum<TPR>(s, turn);
       const float m0 = s[0] * inv, m1 = a.post == RN_LAYER ? s[1] * inv : 0.f;
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float d = g[k][i] - n[k][i] * m0 - m1;
-          g[k][i] = st.y * (lone(a.post) ? g[k][i] * (a.eps * st.y * st.y) : d);
-        }
+      for (int i = 0; i < 8; ++i) {
+        const float d = g[i] - n[i] * m0 - m1;
+        g[i] = st.y * (lone(a.post) ? g[i] * (a.eps * st.y * st.y) : d);
+      }
     }
-    if (a.dh && live) {
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-        rn_store<E, VEC>((E*)a.dh + row * D, c0 + k * TPR * 8, D, g[k]);
-    }
+    if (a.dh && live) rn_store<E, VEC>((E*)a.dh + row * D, c, D, g);
   }
   if (!a.part) return;
   // Over the workgroup's groups, then one partial row for each workgroup.
-  __shared__ float s[ROWS][TPR * 8];
   float* part = a.part + (int64_t)blockIdx.x * RN_NPAR * D;
+  if constexpr (ROWS == 1) {
 #pragma unroll
-  for (int p = 0; p < RN_NPAR; ++p) {
+    for (int p = 0; p < RN_NPAR; ++p)
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if constexpr (ROWS == 1) {
+      for (int i = 0; i < 8; ++i)
+        if (c + i < D) part[p * D + c + i] = sum[p][i];
+  } else {
+    __shared__ float s[ROWS][TPR * 8 + 4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c0 + k * TPR * 8 + i < D) part[p * D + c0 + k * TPR * 8 + i] = sum[p][k][i];
-      } else {
-        __syncthreads();
+    for (int p = 0; p < RN_NPAR; ++p) {
+      __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[threadIdx.x / TPR][c0 + i] = sum[p][k][i];
-        __syncthreads();
-        for (int c = threadIdx.x; c < TPR * 8; c += NT) {
-          float t = 0.f;
+      for (int i = 0; i < 8; ++i) s[threadIdx.x / TPR][c + i] = sum[p][i];
+      __syncthreads();
+      for (int x = threadIdx.x; x < TPR * 8 && x < D; x += rn_threads(TPR)) {
+        float t = 0.f;
 #pragma unroll
-          for (int j = 0; j < ROWS; ++j) t += s[j][c];
-          if (c + k * TPR * 8 < D) part[p * D + c + k * TPR * 8] = t;
-        }
+        for (int j = 0; j < ROWS; ++j) t += s[j][x];
+        part[p * D + x] = t;
       }
     }
   }
@@ -417,11 +373,13 @@ struct RnOut {
   void* p[RN_NPAR];
 };
 
-// out[c] = sum over the partial rows, in order: 4 waves take every fourth row of 64 columns.
+// out[c] = sum over the partial rows, in a fixed order: 16 waves take every sixteenth row of 64
+// columns.
+constexpr int RN_SUM_WAVES = 16;
 template <typename P>
-__global__ __launch_bounds__(256) void residual_norm_sums(const float* __restrict__ part,
-                                                          RnOut out, int parts, int D) {
-  __shared__ float s[4][MG_WAVE];
+__global__ __launch_bounds__(RN_SUM_WAVES* MG_WAVE) void residual_norm_sums(
+    const float* __restrict__ part, RnOut out, int parts, int D) {
+  __shared__ float s[RN_SUM_WAVES][MG_WAVE];
   const int lane = threadIdx.x & (MG_WAVE - 1), w = threadIdx.x / MG_WAVE;
   P* dst = (P*)out.p[blockIdx.y];
   if (!dst) return;
@@ -429,23 +387,32 @@ __global__ __launch_bounds__(256) void residual_norm_sums(const float* __restric
   const float* src = part + (int64_t)blockIdx.y * D + c;
   float a[4] = {0.f, 0.f, 0.f, 0.f};
   int r = w;
-  for (; r + 12 < parts; r += 16) {
+  for (; r + 3 * RN_SUM_WAVES < parts; r += 4 * RN_SUM_WAVES) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] += src[(int64_t)(r + 4 * i) * RN_NPAR * D];
+    for (int i = 0; i < 4; ++i) a[i] += src[(int64_t)(r + RN_SUM_WAVES * i) * RN_NPAR * D];
   }
-  for (; r < parts; r += 4) a[0] += src[(int64_t)r * RN_NPAR * D];
+  for (; r < parts; r += RN_SUM_WAVES) a[0] += src[(int64_t)r * RN_NPAR * D];
   s[w][lane] = (a[0] + a[1]) + (a[2] + a[3]);
   __syncthreads();
-  if (w == 0 && col < D) rn_st1(dst + col, (s[0][lane] + s[1][lane]) + (s[2][lane] + s[3][lane]));
+  if (w != 0 || col >= D) return;
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < RN_SUM_WAVES; ++i) t += s[i][lane];
+  rn_st1(dst + col, t);
 }
 
-// A row's lanes: the fewest that hold it with two vectors each, so that narrow rows share a
-// wave and a wide one has the registers of a workgroup.
-int rn_tpr(int64_t D) { return D <= 256 ? 16 : D <= 1024 ? 64 : D <= 4096 ? 256 : 512; }
+// A row's lanes: the fewest that hold it with 8 elements each, so that narrow rows share a wave
+// and a wide one has a workgroup.  (Wider rows at 16 elements a lane had one wave a SIMD in the
+// backward, 256 registers: 65536 rows of 1024 in bf16 took 670 us, at 8 elements a lane 0.)
+int rn_tpr(int64_t D) {
+  int n = 16;
+  while (n * 8 < D) n *= 2;
+  return n;
+}
 
 // Workgroups: enough to fill the chip several times over; each has partial sums to write, so
 // the backward takes no more than RN_PARTS.
-constexpr int64_t RN_GRID = 4096, RN_PARTS = 1024;
+constexpr int64_t RN_GRID = 8192, RN_PARTS = 1024;
 int64_t rn_grid(int64_t rows, int64_t D, int64_t most) {
   const int tpr = rn_tpr(D), per = tpr > 256 ? 1 : 256 / tpr;
   const int64_t n = (rows + per - 1) / per;
@@ -458,21 +425,18 @@ bool rn_vec(const void* p, int64_t ld, int esize) {
   return !p || (((uintptr_t)p & 15) == 0 && (ld * esize) % 16 == 0);
 }
 
-template <typename E, typename P, int TPR, int K, bool VEC>
+template <typename E, typename P, int TPR, bool VEC>
 void rn_launch(const RnArgs& a, bool bwd, unsigned grid, hipStream_t stream) {
-  const dim3 nt(TPR > 256 ? TPR : 256);
+  const dim3 nt(rn_threads(TPR));
   if (bwd)
-    hipLaunchKernelGGL((residual_norm_bwd<E, P, TPR, K, VEC>), dim3(grid), nt, 0, stream, a);
+    hipLaunchKernelGGL((residual_norm_bwd<E, P, TPR, VEC>), dim3(grid), nt, 0, stream, a);
   else
-    hipLaunchKernelGGL((residual_norm_fwd<E, P, TPR, K, VEC>), dim3(grid), nt, 0, stream, a);
+    hipLaunchKernelGGL((residual_norm_fwd<E, P, TPR, VEC>), dim3(grid), nt, 0, stream, a);
 }
 template <typename E, typename P, int TPR>
 void rn_pick(const RnArgs& a, bool vec, bool bwd, unsigned grid, hipStream_t stream) {
-  const bool one = a.D <= TPR * 8;
-  if (vec && one) rn_launch<E, P, TPR, 1, true>(a, bwd, grid, stream);
-  if (vec && !one) rn_launch<E, P, TPR, 2, true>(a, bwd, grid, stream);
-  if (!vec && one) rn_launch<E, P, TPR, 1, false>(a, bwd, grid, stream);
-  if (!vec && !one) rn_launch<E, P, TPR, 2, false>(a, bwd, grid, stream);
+  if (vec) rn_launch<E, P, TPR, true>(a, bwd, grid, stream);
+  else rn_launch<E, P, TPR, false>(a, bwd, grid, stream);
 }
 template <typename E, typename P>
 int rn_run(const RnArgs& a, bool bwd, unsigned grid, hipStream_t stream) {
@@ -485,9 +449,12 @@ int rn_run(const RnArgs& a, bool bwd, unsigned grid, hipStream_t stream) {
                    rn_vec(a.dh, a.D, e) && rn_vec(a.dx, a.D, e) && rn_vec(a.dgate, a.D, e);
   switch (rn_tpr(a.D)) {
     case 16: rn_pick<E, P, 16>(a, vec, bwd, grid, stream); break;
+    case 32: rn_pick<E, P, 32>(a, vec, bwd, grid, stream); break;
     case 64: rn_pick<E, P, 64>(a, vec, bwd, grid, stream); break;
+    case 128: rn_pick<E, P, 128>(a, vec, bwd, grid, stream); break;
     case 256: rn_pick<E, P, 256>(a, vec, bwd, grid, stream); break;
-    default: rn_pick<E, P, 512>(a, vec, bwd, grid, stream);
+    case 512: rn_pick<E, P, 512>(a, vec, bwd, grid, stream); break;
+    default: rn_pick<E, P, 1024>(a, vec, bwd, grid, stream);
   }
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
@@ -559,10 +526,10 @@ int mg_residual_norm_bwd(int dtype, int pdtype, int post, int act, int pre, cons
   const RnOut out = {{dscale, dpost_w, dpost_b, dpre_w, dpre_b}};
   const dim3 g((unsigned)((D + MG_WAVE - 1) / MG_WAVE), RN_NPAR);
   if (pdtype)
-    hipLaunchKernelGGL(residual_norm_sums<u16>, g, dim3(256), 0, stream, a.part, out, (int)grid,
+    hipLaunchKernelGGL(residual_norm_sums<u16>, g, dim3(RN_SUM_WAVES * MG_WAVE), 0, stream, a.part, out, (int)grid,
                        (int)D);
   else
-    hipLaunchKernelGGL(residual_norm_sums<float>, g, dim3(256), 0, stream, a.part, out, (int)grid,
+    hipLaunchKernelGGL(residual_norm_sums<float>, g, dim3(RN_SUM_WAVES * MG_WAVE), 0, stream, a.part, out, (int)grid,
                        (int)D);
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
