@@ -121,6 +121,30 @@ __device__ __forceinline__ void rn_store(E* row, int c, int D, const float (&v)[
       if (c + i < D) rn_st1(row + c + i, v[i]);
   }
 }
+// 8 elements as they lie in memory (VEC) or widened, loaded now and looked at later.
+template <typename E, bool VEC>
+struct RnRaw {
+  Vec8<E> q;
+  __device__ __forceinline__ void load(const E* row, int c, int D) {
+    q = *reinterpret_cast<const Vec8<E>*>(row + (c < D ? c : 0));
+  }
+  __device__ __forceinline__ void get(int c, int D, float (&v)[8]) const {
+    q.get(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c < D ? v[i] : 0.f;
+  }
+};
+template <typename E>
+struct RnRaw<E, false> {
+  float q[8];
+  __device__ __forceinline__ void load(const E* row, int c, int D) {
+    rn_load<E, false>(row, c, D, q);
+  }
+  __device__ __forceinline__ void get(int, int, float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = q[i];
+  }
+};
 // Elements of a row vector, `other` where there is none.  They are read again for every row:
 // the caches hold them, registers for them would cost the waves that hide the rows' loads.
 template <typename P, bool VEC>
@@ -256,22 +280,43 @@ __global__ __launch_bounds__(rn_threads(TPR)) void residual_norm_bwd(RnArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[p][i] = 0.f;
   int turn = 0;
+  // A row's loads are issued while the row before it is worked on: the sums leave registers for
+  // two or three waves a SIMD only, whose loads would otherwise come in bursts.
+  struct Rows {
+    RnRaw<E, VEC> h, x, g, dr, dy;
+    float4 st;
+  };
+  const auto fetch = [&](int64_t base) {
+    const int64_t at = base + threadIdx.x / TPR, row = at < a.rows ? at : a.rows - 1;
+    Rows r;
+    r.h.load((const E*)a.h + row * a.ldh, c, D);
+    if (a.dy && a.x) r.x.load((const E*)a.x + row * a.ldx, c, D);
+    if (a.act) r.g.load((const E*)a.gate + row * a.ldg, c, D);
+    if (a.dr) r.dr.load((const E*)a.dr + row * a.lddr, c, D);
+    if (a.dy) r.dy.load((const E*)a.dy + row * a.lddy, c, D);
+    r.st = a.stats ? a.stats[row] : make_float4(0.f, 1.f, 0.f, 1.f);
+    return r;
+  };
+  constexpr bool AHEAD = TPR < 1024;  // 16 waves have 128 registers each
+  Rows next;
+  if constexpr (AHEAD) next = fetch((int64_t)blockIdx.x * ROWS);
   for (int64_t base = (int64_t)blockIdx.x * ROWS; base < a.rows; base += (int64_t)gridDim.x * ROWS) {
-    const int64_t at = base + threadIdx.x / TPR;
-    const bool live = at < a.rows;
-    const int64_t row = live ? at : a.rows - 1;
+    const int64_t row = base + threadIdx.x / TPR;
+    const bool live = row < a.rows;
+    const Rows now = AHEAD ? next : fetch(base);
+    if constexpr (AHEAD) next = fetch(base + (int64_t)gridDim.x * ROWS);
     float n[8], xv[8], gv[8], g[8], dy[8];
-    rn_load<E, VEC>((const E*)a.h + row * a.ldh, c, D, n);
-    if (a.dy && a.x) rn_load<E, VEC>((const E*)a.x + row * a.ldx, c, D, xv);
-    if (a.act) rn_load<E, VEC>((const E*)a.gate + row * a.ldg, c, D, gv);
+    now.h.get(c, D, n);
+    if (a.dy && a.x) now.x.get(c, D, xv);
+    if (a.act) now.g.get(c, D, gv);
     if (a.dr) {
-      rn_load<E, VEC>((const E*)a.dr + row * a.lddr, c, D, g);
+      now.dr.get(c, D, g);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) g[i] = 0.f;
     }
-    if (a.dy) rn_load<E, VEC>((const E*)a.dy + row * a.lddy, c, D, dy);
-    const float4 st = a.stats ? a.stats[row] : make_float4(0.f, 1.f, 0.f, 1.f);
+    if (a.dy) now.dy.get(c, D, dy);
+    const float4 st = now.st;
     // n: the post norm's rows; p = n w + b; f = act(gate), slope = act'(gate); u = p f.
     float p[8], f[8], slope[8], w[8], sc[8];
     rn_vector<P, VEC>(a.scale, a.scale_const, c, D, sc);
@@ -403,7 +448,8 @@ __global__ __launch_bounds__(RN_SUM_WAVES* MG_WAVE) void residual_norm_sums(
 
 // A row's lanes: the fewest that hold it with 8 elements each, so that narrow rows share a wave
 // and a wide one has a workgroup.  (Wider rows at 16 elements a lane had one wave a SIMD in the
-// backward, 256 registers: 65536 rows of 1024 in bf16 took 670 us, at 8 elements a lane 0.)
+// backward, 256 registers: 65536 rows of 1024 in bf16 took 670 us, at 8 elements a lane 397, and
+// with a row's loads a row ahead 258.)
 int rn_tpr(int64_t D) {
   int n = 16;
   while (n * 8 < D) n *= 2;
@@ -412,7 +458,7 @@ int rn_tpr(int64_t D) {
 
 // Workgroups: enough to fill the chip several times over; each has partial sums to write, so
 // the backward takes no more than RN_PARTS.
-constexpr int64_t RN_GRID = 8192, RN_PARTS = 1024;
+constexpr int64_t RN_GRID = 8192, RN_PARTS = 512;
 int64_t rn_grid(int64_t rows, int64_t D, int64_t most) {
   const int tpr = rn_tpr(D), per = tpr > 256 ? 1 : 256 / tpr;
   const int64_t n = (rows + per - 1) / per;
