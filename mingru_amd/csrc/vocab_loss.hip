@@ -24,7 +24,8 @@
 //
 // fp32 inputs are split into three bf16 planes (24 significant bits, exact) and a product takes
 // the six pairs of planes that reach 2^-24: six times the work of bf16, against sixteen times
-// for fp32's own matrix instruction.  bf16 inputs: d is rounded to bf16 once, sums are fp32.
+// for fp32's own matrix instruction.  bf16 inputs: d, without the factor of a mean, is rounded
+// to bf16 once; sums are fp32.
 // With a bias, x has a column of ones behind its own, which makes db one more column of dW.
 #include "mg_common.h"
 
@@ -146,6 +147,7 @@ struct VlArgs {
   int64_t ldo, po;         // elements between rows, between the splits' results
   int m_out, n_out;        // what of it is written
   void* extra;             // column m_out in a vector of its own
+  const float* scale;      // of every element, on the device
   int out_f32;
   int64_t pe;              // extra: elements between the splits'
 };
@@ -437,6 +439,7 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
   }
   if constexpr (EPI == VL_OUT) {
     const bool f32 = a.out_f32;
+    const float scale = *a.scale;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int n = nw + 32 * j;
@@ -449,7 +452,7 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
           const int m = mw + 32 * i + 8 * q;
           float v[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) v[x] = acc[i][j][4 * q + x];
+          for (int x = 0; x < 4; ++x) v[x] = scale * acc[i][j][4 * q + x];
           if (m + 4 <= a.m_out && (a.ldo & 3) == 0) {
             if (f32) *reinterpret_cast<float4*>((float*)a.out + row + m) = make_float4(v[0], v[1], v[2], v[3]);
             else *reinterpret_cast<uint2*>((u16*)a.out + row + m) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
@@ -539,14 +542,17 @@ __global__ __launch_bounds__(256) void vl_left_out(const int* __restrict__ pos, 
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i < N && pos[i] < 0) loss[i] = 0.f;
 }
-// Upstream gradients of the counted rows.  reduction: 0 each row's own, 1 mean, 2 sum.
+// Upstream gradients of the counted rows, and a factor for all of them.  reduction: 0 each row's
+// own, 1 mean, 2 sum.  The factor is kept out of d: one over the count, rounded to bf16 in every
+// row's largest entry (the target's), would put all gradients off by the same 2^-9.
 __global__ __launch_bounds__(256) void vl_upstream(const float* __restrict__ up,
                                                    const int* __restrict__ idx,
                                                    const int* __restrict__ count, int reduction,
-                                                   float* __restrict__ g) {
+                                                   float* __restrict__ g,
+                                                   float* __restrict__ scale) {
   const int j = blockIdx.x * 256 + threadIdx.x, n = *count;
-  if (j >= n) return;
-  g[j] = reduction == 0 ? up[idx[j]] : reduction == 1 ? up[0] / (float)n : up[0];
+  if (j == 0) *scale = reduction == 0 ? 1.f : reduction == 1 ? up[0] / (float)(n > 0 ? n : 1) : up[0];
+  if (j < n) g[j] = reduction == 0 ? up[idx[j]] : 1.f;
 }
 // out[i][c] = sum of the parts' rows, pos[i] if given (0 where that is negative).
 template <typename E>
@@ -634,7 +640,7 @@ constexpr int64_t VL_D_BYTES = 512ll << 20;
 struct Back {
   int64_t vp, pieces;   // columns of a piece
   int dx_splits, dw_splits;
-  float *g, *dx_part, *dw_part, *db_part;
+  float *g, *scale, *dx_part, *dw_part, *db_part;
   u16* d;
   size_t bytes;
 };
@@ -646,7 +652,7 @@ Back vl_back(const Shape& s, void* base) {
   b.pieces = (s.V + b.vp - 1) / b.vp;
   const int64_t steps = s.planes == 1 ? 1 : 6;
   b.dx_splits = vl_splits((s.np + TN - 1) / TN * ((s.D + TM - 1) / TM), b.vp / BK * steps);
-  b.dw_splits = vl_splits(b.vp / TN * ((s.D + TM) / TM), s.np / BK * steps);
+  b.dw_splits = vl_splits(b.vp / TN * ((s.D + TM - 1) / TM), s.np / BK * steps);
   char* p = (char*)base;
   const auto take = [&](int64_t n) {
     char* at = p;
@@ -654,6 +660,7 @@ Back vl_back(const Shape& s, void* base) {
     return at;
   };
   b.g = (float*)take(s.N * 4);
+  b.scale = (float*)take(4);
   b.d = (u16*)take(s.planes * s.np * b.vp * 2);
   b.dx_part = (float*)take(b.pieces * b.dx_splits * s.N * s.D * 4);
   b.dw_part = b.dw_splits > 1 ? (float*)take(b.dw_splits * b.vp * s.D * 4) : nullptr;
@@ -766,7 +773,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
   if (ws_bytes < b.bytes) return MG_ERR_WORKSPACE;
   const int e = dtype ? 2 : 4;
   hipLaunchKernelGGL(vl_upstream, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, stream, dloss,
-                     t.idx, t.count, reduction, b.g);
+                     t.idx, t.count, reduction, b.g, b.scale);
   for (int64_t v0 = 0, piece = 0; v0 < V; v0 += b.vp, ++piece) {
     const int64_t cols = V - v0 < b.vp ? V - v0 : b.vp, kc = up_to(cols, PADK);
     VlArgs a = vl_logits(s, t, w, bias, v0, cols);
@@ -780,7 +787,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
       c.K = (int)kc, c.ka = (int)cols;
       c.mt = (int)((D + TM - 1) / TM), c.nt = (int)((s.np + TN - 1) / TN), c.splits = b.dx_splits;
       c.out = b.dx_part + piece * b.dx_splits * N * D;
-      c.ldo = D, c.po = N * D, c.m_out = (int)D, c.n_out = (int)N, c.out_f32 = 1;
+      c.ldo = D, c.po = N * D, c.m_out = (int)D, c.n_out = (int)N, c.out_f32 = 1, c.scale = b.scale;
       rc = vl_run<VL_OUT, true, false>(dtype, c, stream);
     }
     if (rc == MG_OK && dw) {
@@ -790,7 +797,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
       c.k_count = t.count, c.ka = 1 << 30;
       c.mt = (int)((D + (db ? 1 : 0) + TM - 1) / TM), c.nt = (int)((cols + TN - 1) / TN);
       c.splits = b.dw_splits;
-      c.ldo = D, c.m_out = (int)D, c.n_out = (int)cols;
+      c.ldo = D, c.m_out = (int)D, c.n_out = (int)cols, c.scale = b.scale;
       void* const to = (char*)dw + v0 * D * e;
       void* const to_b = db ? (char*)db + v0 * e : nullptr;
       if (b.dw_splits > 1) {

@@ -59,6 +59,8 @@ def _rows(t, D):
     """``t`` as rows of ``D`` consecutive elements and the elements between them."""
     if t is None:
         return None, 0
+    if t.is_contiguous():
+        return t, D
     if t.stride(-1) != 1 and D > 1:
         t = t.contiguous()
     t = t.reshape(-1, D)
@@ -69,31 +71,41 @@ def _rows(t, D):
     return t, t.stride(0)
 
 
+def _residual_norm_fwd(h, x, gate, vectors, kinds, number, eps, keep):
+    """``r``, ``y`` or ``None``, and for the backward (``keep``) the rows' statistics and the tags."""
+    D = h.shape[-1]
+    h2, ldh = _rows(h, D)
+    x2, ldx = _rows(x, D)
+    g2, ldg = _rows(gate, D)
+    rows = h.numel() // D
+    r = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    y = torch.empty_like(r) if kinds[2] else None
+    stats = None
+    if keep and (kinds[0] or kinds[2]):
+        stats = torch.empty(rows, 4, dtype=torch.float32, device=h.device)
+    first = next((t for t in vectors if t is not None), h)
+    tags = (_DTYPE_TAG[h.dtype], _DTYPE_TAG[first.dtype], *kinds)
+    scale, post_w, post_b, pre_w, pre_b = vectors
+    _call("mg_residual_norm_fwd", *tags, _ptr(h2), ldh, _ptr(x2), ldx, _ptr(g2), ldg,
+          _ptr(scale), number, _ptr(post_w), _ptr(post_b), _ptr(pre_w), _ptr(pre_b), _ptr(r),
+          _ptr(y), _ptr(stats), rows, D, eps, _stream(h))
+    return r, y, stats, tags
+
+
+def _grad_wanted(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
 class _ResidualNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, x, gate, scale, post_w, post_b, pre_w, pre_b, kinds, number, eps):
         ctx.set_materialize_grads(False)
-        D = h.shape[-1]
-        h2, ldh = _rows(h, D)
-        x2, ldx = _rows(x, D)
-        g2, ldg = _rows(gate, D)
         vectors = [t if t is None else t.contiguous()
                    for t in (scale, post_w, post_b, pre_w, pre_b)]
-        first = next((t for t in vectors if t is not None), h2)
-        rows = h2.shape[0]
-        r = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-        y = torch.empty_like(r) if kinds[2] else None
-        stats = None
-        if any(ctx.needs_input_grad) and (kinds[0] or kinds[2]):
-            stats = torch.empty(rows, 4, dtype=torch.float32, device=h.device)
-        tags = (_DTYPE_TAG[h.dtype], _DTYPE_TAG[first.dtype], *kinds)
-        scale, post_w, post_b, pre_w, pre_b = vectors
-        _call("mg_residual_norm_fwd", *tags, _ptr(h2), ldh, _ptr(x2), ldx, _ptr(g2), ldg,
-              _ptr(scale), number, _ptr(post_w), _ptr(post_b), _ptr(pre_w), _ptr(pre_b), _ptr(r),
-              _ptr(y), _ptr(stats), rows, D, eps, _stream(h))
+        r, y, stats, ctx.tags = _residual_norm_fwd(h, x, gate, vectors, kinds, number, eps, True)
         ctx.save_for_backward(h, x, gate, stats, *vectors)
-        ctx.tags, ctx.number, ctx.eps = tags, number, eps
-        return (r, y) if kinds[2] else r
+        ctx.number, ctx.eps = number, eps
+        return r if y is None else (r, y)
 
     @staticmethod
     @once_differentiable
@@ -109,7 +121,7 @@ class _ResidualNormFn(torch.autograd.Function):
         g2, ldg = _rows(gate, D)
         dr2, lddr = _rows(dr, D)
         dy2, lddy = _rows(dy, D)
-        rows = h2.shape[0]
+        rows = h.numel() // D
 
         def like(i):
             return torch.empty(h.shape, dtype=h.dtype, device=dev) if need[i] else None
@@ -146,8 +158,14 @@ def residual_norm_impl(h, x, gate, scale, post_w, post_b, pre_w, pre_b, post, ac
             h.dtype == torch.float32:
         vectors = [t if t is None else t.float() for t in vectors]
     kinds = (_NORM_TAG[post], _GATE_TAG[act], _NORM_TAG[pre])
-    out = _funnel("residual_norm", _ResidualNormFn.apply, h, x, gate, *vectors, kinds, number,
-                  float(eps))
+    if _grad_wanted(h, x, gate, *vectors):
+        out = _funnel("residual_norm", _ResidualNormFn.apply, h, x, gate, *vectors, kinds, number,
+                      float(eps))
+    else:
+        vectors = [t if t is None else t.contiguous() for t in vectors]
+        r, y, *_ = _funnel("residual_norm", _residual_norm_fwd, h, x, gate, vectors, kinds, number,
+                           float(eps), False)
+        out = r if y is None else (r, y)
     if h.dtype == dtype:
         return out
     return tuple(t.to(dtype) for t in out) if kinds[2] else out.to(dtype)
@@ -173,24 +191,29 @@ def _array(values):
     return (ctypes.c_int64 * len(values))(*values)
 
 
+def _linear_attention_fwd(q, k, v, g, h0, lengths, scale):
+    """``o``, the final state, what the backward needs of the pass, sizes and strides."""
+    (B, T, Hk, dk), (H, dv) = q.shape, v.shape[2:]
+    tag, dev = _DTYPE_TAG[q.dtype], q.device
+    size = (tag, B, T, H, Hk, dk, dv)
+    o = torch.empty(B, T, H, dv, dtype=q.dtype, device=dev)
+    h = torch.empty(B, H, dk, dv, dtype=torch.float32, device=dev)
+    state = _workspace(_size("mg_linear_attention_state_bytes", *size), dev)
+    strides = (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_decay_strides(g, 2))
+    _call("mg_linear_attention_fwd", tag, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _array(strides),
+          _ptr(lengths), _ptr(h0), _ptr(o), _ptr(h), _ptr(state), state.numel(), B, T, H, Hk,
+          dk, dv, scale, _stream(q))
+    return o, h, state, size, strides
+
+
 class _LinearAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, h0, lengths, scale):
         ctx.set_materialize_grads(False)
         q, k, v = (_last_dense(t) for t in (q, k, v))
-        (B, T, Hk, dk), (H, dv) = q.shape, v.shape[2:]
-        tag, dev = _DTYPE_TAG[q.dtype], q.device
-        size = (tag, B, T, H, Hk, dk, dv)
-        o = torch.empty(B, T, H, dv, dtype=q.dtype, device=dev)
-        h = torch.empty(B, H, dk, dv, dtype=torch.float32, device=dev)
-        state = _workspace(_size("mg_linear_attention_state_bytes", *size), dev)
-        strides = (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_decay_strides(g, 2))
-        _call("mg_linear_attention_fwd", tag, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _array(strides),
-              _ptr(lengths), _ptr(h0), _ptr(o), _ptr(h), _ptr(state), state.numel(), B, T, H, Hk,
-              dk, dv, scale, _stream(q))
-        if any(ctx.needs_input_grad):
-            ctx.save_for_backward(q, k, v, g, h0, lengths, h, state)
-            ctx.size, ctx.strides, ctx.scale = size, strides, scale
+        o, h, state, ctx.size, ctx.strides = _linear_attention_fwd(q, k, v, g, h0, lengths, scale)
+        ctx.save_for_backward(q, k, v, g, h0, lengths, h, state)
+        ctx.scale = scale
         return o, h
 
     @staticmethod
@@ -230,8 +253,13 @@ def linear_attention_impl(q, k, v, g, h0, lengths, scale):
         h0 = h0.contiguous()
     if lengths is not None:
         lengths = lengths.to(torch.int32).contiguous()
-    o, h = _funnel("linear_attention", _LinearAttentionFn.apply, q, k, v, g, h0, lengths, scale)
-    return o.to(dtype), h
+    if _grad_wanted(q, k, v, g, h0):
+        o, h = _funnel("linear_attention", _LinearAttentionFn.apply, q, k, v, g, h0, lengths, scale)
+    else:
+        q, k, v = (_last_dense(t) for t in (q, k, v))
+        o, h, *_ = _funnel("linear_attention", _linear_attention_fwd, q, k, v, g, h0, lengths,
+                           scale)
+    return o if o.dtype == dtype else o.to(dtype), h
 
 
 def linear_attention_step_impl(q, k, v, g, h, scale):
@@ -257,25 +285,32 @@ def linear_attention_step_impl(q, k, v, g, h, scale):
 _REDUCTION_TAG = {"none": 0, "mean": 1, "sum": 2}
 
 
+def _vocab_loss_fwd(x, w, bias, target, ignore_index, reduction):
+    """The loss, what the backward needs of the pass, and sizes; ``w`` dense and aligned."""
+    x2, ldx = _rows(x, x.shape[-1])
+    N, (V, D) = target.numel(), w.shape
+    tag, dev = _DTYPE_TAG[x.dtype], x.device
+    state = _workspace(_size("mg_vocab_loss_state_bytes", tag, N, V, D), dev)
+    ws = _workspace(_size("mg_vocab_loss_fwd_workspace_bytes", tag, N, V, D), dev)
+    loss = torch.empty(N if reduction == 0 else (), dtype=torch.float32, device=dev)
+    _call("mg_vocab_loss_fwd", tag, _ptr(x2), ldx, _ptr(w), _ptr(bias), _ptr(target),
+          ignore_index, reduction, _ptr(loss), N, V, D, _ptr(state), state.numel(), _ptr(ws),
+          ws.numel(), _stream(x))
+    return loss, state, (tag, N, V, D)
+
+
+def _dense_aligned(w):
+    w = w.contiguous()
+    return w.clone() if w.data_ptr() % 16 else w
+
+
 class _VocabLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, target, ignore_index, reduction):
-        x2, ldx = _rows(x, x.shape[-1])
-        w = w.contiguous()
-        if w.data_ptr() % 16:
-            w = w.clone()
-        N, (V, D) = x2.shape[0], w.shape
-        tag, dev = _DTYPE_TAG[x.dtype], x.device
-        state = _workspace(_size("mg_vocab_loss_state_bytes", tag, N, V, D), dev)
-        ws = _workspace(_size("mg_vocab_loss_fwd_workspace_bytes", tag, N, V, D), dev)
-        loss = torch.empty(N if reduction == 0 else (), dtype=torch.float32, device=dev)
-        bias = bias if bias is None else bias.contiguous()
-        _call("mg_vocab_loss_fwd", tag, _ptr(x2), ldx, _ptr(w), _ptr(bias), _ptr(target),
-              ignore_index, reduction, _ptr(loss), N, V, D, _ptr(state), state.numel(), _ptr(ws),
-              ws.numel(), _stream(x))
-        if any(ctx.needs_input_grad):
-            ctx.save_for_backward(w, bias, state)
-            ctx.size, ctx.shape, ctx.reduction = (tag, N, V, D), x.shape, reduction
+        w, bias = _dense_aligned(w), bias if bias is None else bias.contiguous()
+        loss, state, ctx.size = _vocab_loss_fwd(x, w, bias, target, ignore_index, reduction)
+        ctx.save_for_backward(w, bias, state)
+        ctx.shape, ctx.reduction = x.shape, reduction
         return loss
 
     @staticmethod
@@ -302,6 +337,10 @@ def linear_cross_entropy_impl(x, weight, target, bias, ignore_index, reduction):
         raise ScanFallback(f"linear_cross_entropy kernels take fewer than 2^30 rows and "
                            f"vocabulary entries and rows of at most 2^20 (got {N}, {V}, {D})")
     t = target.reshape(-1).to(torch.int64).contiguous()
-    loss = _funnel("linear_cross_entropy", _VocabLossFn.apply, x, weight, bias, t,
-                   int(ignore_index), _REDUCTION_TAG[reduction])
+    rest = t, int(ignore_index), _REDUCTION_TAG[reduction]
+    if _grad_wanted(x, weight, bias):
+        loss = _funnel("linear_cross_entropy", _VocabLossFn.apply, x, weight, bias, *rest)
+    else:
+        loss = _funnel("linear_cross_entropy", _vocab_loss_fwd, x, _dense_aligned(weight),
+                       bias if bias is None else bias.contiguous(), *rest)[0]
     return loss.view(target.shape) if reduction == "none" else loss

@@ -221,7 +221,11 @@ def _attention_checks(what, q, k, v, log_decay, h, lead):
 
 def _attention_types(q, k, v, log_decay, h):
     """Inputs in one type, decays and state in 32 bits (64 where an input has them)."""
-    dtype = torch.promote_types(torch.promote_types(q.dtype, k.dtype), v.dtype)
+    dtype = q.dtype
+    if k.dtype is dtype and v.dtype is dtype and dtype is not torch.float64 and \
+            log_decay.dtype is torch.float32 and (h is None or h.dtype is torch.float32):
+        return q, k, v, log_decay, h
+    dtype = torch.promote_types(torch.promote_types(dtype, k.dtype), v.dtype)
     wide = torch.float64 if torch.float64 in (dtype, log_decay.dtype) else torch.float32
     if wide == torch.float64:
         dtype = wide
