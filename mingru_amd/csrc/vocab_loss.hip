@@ -22,10 +22,14 @@
 // consecutive (near), or the other way round (far, read with ds_read_b64_tr_b16): x, W and d
 // all lie in memory once, and each is near in one product and far in another.
 //
-// fp32 inputs are split into three bf16 planes (24 significant bits, exact) and a product takes
-// the six pairs of planes that reach 2^-24: six times the work of bf16, against sixteen times
-// for fp32's own matrix instruction.  bf16 inputs: d, without the factor of a mean, is rounded
-// to bf16 once; sums are fp32.
+// fp32 inputs are scaled by a power of two that takes the largest finite one (of x, of W) to
+// 2^14 .. 2^15, and split into two fp16 planes, hi + lo: 22 significant bits down to 2^-28 of
+// the largest, then fewer, to 2^-39 of it: an error of the logits far below what fp32 sums
+// leave.  A product takes the three pairs hi hi, hi lo, lo hi: three times the work of bf16,
+// against sixteen times for fp32's own matrix instruction and six for three bf16 planes (24
+// bits at any size; 2047 x 10007 x 392 took 575 us with them, 365 with these).  d, in -1 .. 1, is
+// scaled by 2^15.
+// bf16 inputs: d, without the factor of a mean, is rounded to bf16 once; sums are fp32.
 // With a bias, x has a column of ones behind its own, which makes db one more column of dW.
 #include "mg_common.h"
 
@@ -53,11 +57,33 @@ __device__ __forceinline__ unsigned pack2(float x, float y) {
 }
 __device__ __forceinline__ float low(unsigned u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float high(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
-// What a plane leaves for the next ones; an infinity or NaN is the first plane's alone.
-__device__ __forceinline__ float rest(float x, u16 plane) {
-  const float r = x - to_f(plane);
+// fp16 planes.  What hi leaves for lo; an infinity or NaN is hi's alone.
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ unsigned pack2h(float x, float y) {
+  const f16x2 h = {(_Float16)x, (_Float16)y};
+  return __builtin_bit_cast(unsigned, h);
+}
+__device__ __forceinline__ float rest(float x, unsigned pair, int i) {
+  const float r = x - (float)__builtin_bit_cast(f16x2, pair)[i];
   return r == r ? r : 0.f;
 }
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int d = 32; d; d /= 2) x = fmaxf(x, __shfl_xor(x, d));
+  return x;
+}
+// The power of two that takes `top` to 2^14 .. 2^15, from 2^-60 to 2^50 (two of them, and a bias
+// times both, stay finite); 1 for 0.
+__device__ __forceinline__ float scale_of(float top) {
+  if (!(top > 0.f)) return 1.f;
+  int e;
+  frexpf(top, &e);  // top = m 2^e, m in 1/2 .. 1
+  e = 15 - e;
+  return ldexpf(1.f, e < -60 ? -60 : e > 50 ? 50 : e);
+}
+constexpr int MAX_PARTS = 256;
+constexpr float ONE_SCALE = 16384.f, D_SCALE = 32768.f;
 
 // ---- packing ----------------------------------------------------------------------------
 // Counted rows in order: idx[j] the j-th one's row, pos[i] a row's place or -1, tgt[j] its
@@ -66,53 +92,115 @@ __global__ __launch_bounds__(1024) void vl_index(const int64_t* __restrict__ tar
                                                  int64_t ignore, int64_t V, int* __restrict__ idx,
                                                  int* __restrict__ pos, int* __restrict__ tgt,
                                                  int* __restrict__ count, int N) {
-  __shared__ int s_n[16];
+  __shared__ int s_n[2][16];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  int base = 0;
-  for (int i0 = 0; i0 < N; i0 += 1024) {
-    const int i = i0 + tid;
-    const int64_t t = i < N ? target[i] : ignore;
-    const bool in = i < N && t != ignore;
-    const unsigned long long m = __ballot(in);
-    __syncthreads();
-    if (lane == 0) s_n[w] = __popcll(m);
-    __syncthreads();
-    int at = base, all = 0;
+  int base = 0, turn = 0;
+  // Four rows in a row a thread; the next ones are loaded before the waves meet.
+  int64_t t[4], u[4];
+  const auto load = [&](int i0, int64_t (&to)[4]) {
 #pragma unroll
-    for (int u = 0; u < 16; ++u) {
-      at += u < w ? s_n[u] : 0;
-      all += s_n[u];
+    for (int x = 0; x < 4; ++x) to[x] = i0 + tid * 4 + x < N ? target[i0 + tid * 4 + x] : ignore;
+  };
+  load(0, t);
+  for (int i0 = 0; i0 < N; i0 += 4096, turn ^= 1) {
+    load(i0 + 4096, u);
+    int mine = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) mine += t[x] != ignore;
+    int sum = mine;  // over the lanes up to this one
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int v = __shfl_up(sum, d);
+      if (lane >= d) sum += v;
     }
-    at += __popcll(m & ((1ull << lane) - 1));
-    if (in) idx[at] = i, tgt[at] = t >= 0 && t < V ? (int)t : -1;
-    if (i < N) pos[i] = in ? at : -1;
-    base += all;
+    if (lane == 63) s_n[turn][w] = sum;
+    __syncthreads();
+    int at = base + sum - mine;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      at += x < w ? s_n[turn][x] : 0;
+      base += s_n[turn][x];
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int i = i0 + tid * 4 + x;
+      const bool in = t[x] != ignore;
+      if (in) idx[at] = i, tgt[at] = t[x] >= 0 && t[x] < V ? (int)t[x] : -1;
+      if (i < N) pos[i] = in ? at : -1;
+      at += in;
+      t[x] = u[x];
+    }
   }
   if (tid == 0) *count = base;
 }
 
-// Rows of `cols` elements in PL planes of bf16, `ld` elements a row, 0 past the columns except
-// a 1 at `ones`.  idx: the counted rows, padded with rows of 0 to a multiple of the contracted step; null: all rows.
+// The largest finite magnitude of the (counted) rows, in MAX_PARTS parts; of src's first `most`
+// elements at most.
+__global__ __launch_bounds__(1024) void vl_absmax(const float* __restrict__ src, int64_t ld,
+                                                 int64_t cols, int64_t most,
+                                                 const int* __restrict__ idx,
+                                                 const int* __restrict__ count, int64_t rows,
+                                                 float* __restrict__ part) {
+  __shared__ float s[16];
+  const int64_t n = count ? *count : rows;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  float top = 0.f;
+  for (int64_t j = blockIdx.x * 16 + w; j < n; j += MAX_PARTS * 16) {
+    const int64_t at = (idx ? (int64_t)idx[j] : j) * ld;
+    const int64_t end = cols < most - at ? cols : most - at;
+#pragma unroll 4
+    for (int64_t c = lane; c < end; c += 64) {
+      const float x = fabsf(src[at + c]);
+      top = x < INFINITY ? fmaxf(top, x) : top;
+    }
+  }
+  top = wave_max(top);
+  if (lane == 0) s[w] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+    part[blockIdx.x] = top;
+  }
+}
+
+// Rows of `cols` elements in PL planes, `ld` elements a row, 0 past the columns except a one at
+// `ones`.  idx: the counted rows, padded with rows of 0 to a multiple of the contracted step;
+// null: all rows.  Two planes are fp16 of the values times the scale that the parts of the
+// largest magnitude give (written to `scale`; the one times ONE_SCALE), one is bf16.
 template <typename E, int PL>
 __global__ __launch_bounds__(256) void vl_pack(const E* __restrict__ src, int64_t lds_, int cols,
                                                u16* __restrict__ dst, int ld, int64_t plane,
                                                const int* __restrict__ idx,
                                                const int* __restrict__ count, int64_t rows,
-                                               int ones) {
+                                               int ones, const float* __restrict__ top,
+                                               float* __restrict__ scale) {
+  float by = 1.f;
+  if constexpr (PL == 2) {
+    __shared__ float s_top[4];
+    const float t = wave_max(top[threadIdx.x]);
+    if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = t;
+    __syncthreads();
+    by = scale_of(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *scale = by;
+  }
   const int64_t j = blockIdx.x;
   const int64_t n = count ? *count : rows;
   if (j >= (n + PADK - 1) / PADK * PADK) return;
   const bool live = j < n;
   const E* s = src + (live ? (idx ? (int64_t)idx[j] : j) * lds_ : 0);
   for (int c = threadIdx.x * 2; c < ld; c += 512) {
-    float x = live && c < cols ? to_f(s[c]) : 0.f, y = live && c + 1 < cols ? to_f(s[c + 1]) : 0.f;
-    if (live && c == ones) x = 1.f;
-    if (live && c + 1 == ones) y = 1.f;
-#pragma unroll
-    for (int p = 0; p < PL; ++p) {
-      const u16 a = to_bf(x), b = to_bf(y);
-      *reinterpret_cast<unsigned*>(dst + p * plane + j * ld + c) = a | ((unsigned)b << 16);
-      x = rest(x, a), y = rest(y, b);
+    float x = live && c < cols ? to_f(s[c]) * by : 0.f;
+    float y = live && c + 1 < cols ? to_f(s[c + 1]) * by : 0.f;
+    if (live && c == ones) x = PL == 2 ? ONE_SCALE : 1.f;
+    if (live && c + 1 == ones) y = PL == 2 ? ONE_SCALE : 1.f;
+    unsigned* const to = reinterpret_cast<unsigned*>(dst + j * ld + c);
+    if constexpr (PL == 1) {
+      *to = pack2(x, y);
+    } else {
+      const unsigned hi = pack2h(x, y);
+      *to = hi;
+      *reinterpret_cast<unsigned*>(dst + plane + j * ld + c) = pack2h(rest(x, hi, 0), rest(y, hi, 1));
     }
   }
 }
@@ -123,6 +211,7 @@ enum { VL_LSE = 0, VL_D = 1, VL_OUT = 2 };
 struct VlArgs {
   const u16 *A, *B;        // M's and N's operands
   int64_t pa, pb;          // elements between their planes
+  const float *sa, *sb;    // fp16 planes: what they were scaled by
   int lda, ldb;            // elements between rows
   int m_rows, n_rows;      // rows (near) or columns (far) that exist; read places are clamped
   const int* m_count;      // on the device, in their place, if not null
@@ -218,15 +307,19 @@ __device__ __forceinline__ void step_put(u16* m, u32x4 x, int i) {
   *reinterpret_cast<u32x4*>(m + (FAR ? far_place<W>(v / (W / 8), v % (W / 8)) : near_place(v >> 2, v & 3))) = x;
 }
 
-// Pairs of planes whose product is not below 2^-24 of the whole, smallest first.
+// Pairs of planes in a product, the smaller ones first: lo hi, hi lo, hi hi.
 template <int PL>
 __device__ __forceinline__ void pair_of(int i, int& a, int& b) {
-  if constexpr (PL == 1) {
-    a = b = 0;
-  } else {
-    a = (0x001102 >> (4 * (5 - i))) & 15;  // 0 2 1 1 0 0 from the last digit on
-    b = (0x010120 >> (4 * (5 - i))) & 15;
-  }
+  a = PL == 2 && i == 0;
+  b = PL == 2 && i == 1;
+}
+template <int PL>
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+  if constexpr (PL == 2)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
 template <int EPI, bool AFAR, bool BFAR, int PL, typename E>
@@ -253,7 +346,7 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
   const int K = a.k_count ? (*a.k_count + PADK - 1) / PADK * PADK : a.K;
   if (m0 >= m_rows || n0 >= n_rows) return;
 
-  constexpr int PAIRS = PL == 1 ? 1 : 6;
+  constexpr int PAIRS = PL == 2 ? 3 : 1;
   const int ksteps = K / BK;
   const int per = (ksteps + a.splits - 1) / a.splits;
   const int s0 = split * per, s1 = s0 + per < ksteps ? s0 + per : ksteps;
@@ -299,9 +392,10 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
   // A row's bias is where its sum starts; past the vocabulary that is -inf, so that such a
   // column's exponentials are 0.
   f32x16 acc[4][2];
+  const float by = PL == 2 ? *a.sa * *a.sb : 1.f;  // a power of two
   if constexpr (EPI != VL_OUT) {
     const int m = m0 + tid;
-    s_bias[tid] = m >= m_rows ? -INFINITY : a.bias ? to_f(((const E*)a.bias)[a.v0 + m]) : 0.f;
+    s_bias[tid] = m >= m_rows ? -INFINITY : a.bias ? to_f(((const E*)a.bias)[a.v0 + m]) * by : 0.f;
     __syncthreads();
     const float* const bw = s_bias + wm * 128 + 4 * (lane >> 5);
 #pragma unroll
@@ -343,7 +437,7 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[from][i], fb[from][j], acc[i][j], 0, 0, 0);
+        acc[i][j] = mma<PL>(fa[from][i], fb[from][j], acc[i][j]);
     __builtin_amdgcn_sched_barrier(0);
   };
   if (steps > 0) {
@@ -369,6 +463,8 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
   // Lane: column n = n0 + 64 wn + 32 j + (lane & 31) of the result; rows m = m0 + 128 wm +
   // 32 i + 8 q + 4 (lane >> 5) + x in acc[i][j][4 q + x].
   const int half = lane >> 5, mw = m0 + wm * 128 + 4 * half, nw = n0 + wn * 64 + (lane & 31);
+  // exp(l) of logits that are still scaled.
+  const float unit = 1.f / by, log2 = 1.4426950408889634f * unit;
   if constexpr (EPI == VL_LSE) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -380,16 +476,17 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
       if (__ballot(t >= 0 && t < 128 && n < n_rows)) {
 #pragma unroll
         for (int c = 0; c < 64; ++c)
-          if (t == 8 * (c >> 2) + (c & 3) && n < n_rows) a.tlogit[n] = acc[c >> 4][j][c & 15];
+          if (t == 8 * (c >> 2) + (c & 3) && n < n_rows)
+            a.tlogit[n] = acc[c >> 4][j][c & 15] * unit;
       }
       top = fmaxf(top, __shfl_xor(top, 32));
       const float ref = top == -INFINITY ? 0.f : top;
       float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < 64; ++c) sum += __expf(acc[c >> 4][j][c & 15] - ref);
+      for (int c = 0; c < 64; ++c) sum += __builtin_amdgcn_exp2f((acc[c >> 4][j][c & 15] - ref) * log2);
       sum += __shfl_xor(sum, 32);
       // fmaxf drops a NaN; the sum keeps it.
-      if (half == 0 && n < n_rows) a.part[(int64_t)(2 * mt + wm) * a.n_ld + n] = make_float2(top, sum);
+      if (half == 0 && n < n_rows) a.part[(int64_t)(2 * mt + wm) * a.n_ld + n] = make_float2(top * unit, sum);
     }
   }
   if constexpr (EPI == VL_D) {
@@ -402,11 +499,11 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
     for (int j = 0; j < 2; ++j) {
       const int n = nw + 32 * j, r = n < n_rows ? n : n_rows - 1;
       const float2 soft = a.soft[r];
-      const float g = n < n_rows ? a.g[r] : 0.f, sg = soft.y * g;
+      const float g = n < n_rows ? a.g[r] : 0.f, sg = soft.y * g, top = soft.x * by;
       const int t = a.tgt[r] - a.v0 - mw;
 #pragma unroll
       for (int c = 0; c < 64; ++c) {
-        acc[c >> 4][j][c & 15] = __expf(acc[c >> 4][j][c & 15] - soft.x) * sg;
+        acc[c >> 4][j][c & 15] = __builtin_amdgcn_exp2f((acc[c >> 4][j][c & 15] - top) * log2) * sg;
       }
       if (__ballot(t >= 0 && t < 128)) {
 #pragma unroll
@@ -419,10 +516,14 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
         for (int c = 0; c < 16; ++c) {
           f32x16& v = acc[c >> 2][j];
           const int e = 4 * (c & 3);
-          const unsigned u0 = pack2(v[e], v[e + 1]), u1 = pack2(v[e + 2], v[e + 3]);
+          const unsigned u0 = PL == 2 ? pack2h(v[e], v[e + 1]) : pack2(v[e], v[e + 1]);
+          const unsigned u1 = PL == 2 ? pack2h(v[e + 2], v[e + 3]) : pack2(v[e + 2], v[e + 3]);
           *reinterpret_cast<uint2*>(stage + sr * TM + (((wm * 16 + c) ^ (sr & 31)) << 3) + 4 * half) =
               make_uint2(u0, u1);
-          if (q + 1 < PL) v[e] -= low(u0), v[e + 1] -= high(u0), v[e + 2] -= low(u1), v[e + 3] -= high(u1);
+          if (q + 1 < PL) {
+            v[e] = rest(v[e], u0, 0), v[e + 1] = rest(v[e + 1], u0, 1);
+            v[e + 2] = rest(v[e + 2], u1, 0), v[e + 3] = rest(v[e + 3], u1, 1);
+          }
         }
         __syncthreads();
 #pragma unroll
@@ -439,7 +540,7 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
   }
   if constexpr (EPI == VL_OUT) {
     const bool f32 = a.out_f32;
-    const float scale = *a.scale;
+    const float scale = *a.scale * unit, scale1 = PL == 2 ? *a.scale / (ONE_SCALE * *a.sb) : *a.scale;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int n = nw + 32 * j;
@@ -463,8 +564,9 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
                 if (f32) ((float*)a.out)[row + m + x] = v[x];
                 else ((u16*)a.out)[row + m + x] = to_bf(v[x]);
               } else if (m + x == a.m_out && a.extra) {
-                if (f32) ((float*)a.extra)[split * a.pe + n] = v[x];
-                else ((u16*)a.extra)[n] = to_bf(v[x]);
+                const float e = scale1 * acc[i][j][4 * q + x];
+                if (f32) ((float*)a.extra)[split * a.pe + n] = e;
+                else ((u16*)a.extra)[n] = to_bf(e);
               }
             }
           }
@@ -545,14 +647,32 @@ __global__ __launch_bounds__(256) void vl_left_out(const int* __restrict__ pos, 
 // Upstream gradients of the counted rows, and a factor for all of them.  reduction: 0 each row's
 // own, 1 mean, 2 sum.  The factor is kept out of d: one over the count, rounded to bf16 in every
 // row's largest entry (the target's), would put all gradients off by the same 2^-9.
+// top (fp16 planes): g gets d's scale; rows' own gradients, whose largest magnitude it has, are
+// brought to 1/2 .. 1 first.  Both together are written to d_scale.
 __global__ __launch_bounds__(256) void vl_upstream(const float* __restrict__ up,
                                                    const int* __restrict__ idx,
                                                    const int* __restrict__ count, int reduction,
+                                                   const float* __restrict__ top,
                                                    float* __restrict__ g,
-                                                   float* __restrict__ scale) {
+                                                   float* __restrict__ scale,
+                                                   float* __restrict__ d_scale) {
   const int j = blockIdx.x * 256 + threadIdx.x, n = *count;
-  if (j == 0) *scale = reduction == 0 ? 1.f : reduction == 1 ? up[0] / (float)(n > 0 ? n : 1) : up[0];
-  if (j < n) g[j] = reduction == 0 ? up[idx[j]] : 1.f;
+  float by = 1.f;
+  if (top) {
+    by = D_SCALE;
+    if (reduction == 0) {
+      __shared__ float s[4];
+      const float t = wave_max(top[threadIdx.x]);
+      if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = t;
+      __syncthreads();
+      by = scale_of(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+    }
+  }
+  if (j == 0) {
+    *scale = reduction == 0 ? 1.f : reduction == 1 ? up[0] / (float)(n > 0 ? n : 1) : up[0];
+    *d_scale = by;
+  }
+  if (j < n) g[j] = (reduction == 0 ? up[idx[j]] : 1.f) * by;
 }
 // out[i][c] = sum of the parts' rows, pos[i] if given (0 where that is negative).
 template <typename E>
@@ -596,13 +716,14 @@ bool vl_shape(int dtype, int64_t N, int64_t V, int64_t D, Shape* s) {
     return false;
   s->N = N, s->V = V, s->D = D;
   s->np = up_to(N, PADK), s->kp = up_to(D, PADK), s->dx = up_to(D + 1, PADK);
-  s->planes = dtype ? 1 : 3;
+  s->planes = dtype ? 1 : 2;
   s->own_w = dtype == 0 || D % PADK != 0;
   return true;
 }
 struct State {
   int *idx, *pos, *tgt, *count;
   float2* soft;
+  float *sx, *sw;  // scales of the packed planes
   u16 *xc, *wc;
   size_t bytes;
 };
@@ -614,7 +735,8 @@ State vl_state(const Shape& s, void* base) {
     return at;
   };
   State t;
-  t.count = (int*)take(256);
+  t.count = (int*)take(4);
+  t.sx = (float*)take(4), t.sw = (float*)take(4);
   t.idx = (int*)take(s.N * 4), t.pos = (int*)take(s.N * 4), t.tgt = (int*)take(s.N * 4);
   t.soft = (float2*)take(s.N * 8);
   t.xc = (u16*)take(s.planes * s.np * s.dx * 2);
@@ -640,7 +762,7 @@ constexpr int64_t VL_D_BYTES = 512ll << 20;
 struct Back {
   int64_t vp, pieces;   // columns of a piece
   int dx_splits, dw_splits;
-  float *g, *scale, *dx_part, *dw_part, *db_part;
+  float *g, *scale, *d_scale, *top, *dx_part, *dw_part, *db_part;
   u16* d;
   size_t bytes;
 };
@@ -650,7 +772,7 @@ Back vl_back(const Shape& s, void* base) {
   b.pieces = (s.V + (most > TM ? most : TM) - 1) / (most > TM ? most : TM);
   b.vp = up_to((s.V + b.pieces - 1) / b.pieces, TM);
   b.pieces = (s.V + b.vp - 1) / b.vp;
-  const int64_t steps = s.planes == 1 ? 1 : 6;
+  const int64_t steps = s.planes == 1 ? 1 : 3;
   b.dx_splits = vl_splits((s.np + TN - 1) / TN * ((s.D + TM - 1) / TM), b.vp / BK * steps);
   b.dw_splits = vl_splits(b.vp / TN * ((s.D + TM - 1) / TM), s.np / BK * steps);
   char* p = (char*)base;
@@ -660,7 +782,8 @@ Back vl_back(const Shape& s, void* base) {
     return at;
   };
   b.g = (float*)take(s.N * 4);
-  b.scale = (float*)take(4);
+  b.scale = (float*)take(4), b.d_scale = (float*)take(4);
+  b.top = (float*)take(MAX_PARTS * 4);
   b.d = (u16*)take(s.planes * s.np * b.vp * 2);
   b.dx_part = (float*)take(b.pieces * b.dx_splits * s.N * s.D * 4);
   b.dw_part = b.dw_splits > 1 ? (float*)take(b.dw_splits * b.vp * s.D * 4) : nullptr;
@@ -675,7 +798,7 @@ int vl_run(int dtype, VlArgs& a, hipStream_t stream) {
   if (work > (1ll << 30)) return MG_ERR_TOO_LARGE;
   const dim3 grid((unsigned)((work + 7) / 8 * 8));
   if (dtype) hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 1, u16>), grid, dim3(NT), 0, stream, a);
-  else hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 3, float>), grid, dim3(NT), 0, stream, a);
+  else hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 2, float>), grid, dim3(NT), 0, stream, a);
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
 
@@ -686,6 +809,7 @@ VlArgs vl_logits(const Shape& s, const State& t, const void* w, const void* bias
   a.A = (s.own_w ? t.wc : (const u16*)w) + v0 * s.kp;
   a.lda = (int)s.kp, a.pa = s.V * s.kp;
   a.B = t.xc, a.ldb = (int)s.dx, a.pb = s.np * s.dx;
+  a.sa = t.sw, a.sb = t.sx;
   a.m_rows = (int)cols, a.n_count = t.count;
   a.K = (int)s.kp, a.ka = 1 << 30;
   a.mt = (int)((cols + TM - 1) / TM), a.nt = (int)((s.np + TN - 1) / TN), a.splits = 1;
@@ -695,12 +819,20 @@ VlArgs vl_logits(const Shape& s, const State& t, const void* w, const void* bias
 
 int64_t vl_part_rows(const Shape& s) { return 2 * ((s.V + TM - 1) / TM); }
 
-template <typename E, int PL>
-void vl_pack_run(const void* src, int64_t ld, int64_t cols, u16* dst, int64_t dld, int64_t plane,
-                 const int* idx, const int* count, int64_t rows, int64_t grid, int ones,
-                 hipStream_t stream) {
-  hipLaunchKernelGGL((vl_pack<E, PL>), dim3((unsigned)grid), dim3(256), 0, stream, (const E*)src, ld,
-                     (int)cols, dst, (int)dld, plane, idx, count, rows, ones);
+void vl_pack_run(int dtype, const void* src, int64_t ld, int64_t cols, u16* dst, int64_t dld,
+                 int64_t plane, const int* idx, const int* count, int64_t rows, int64_t grid,
+                 int ones, float* top, float* scale, hipStream_t stream) {
+  if (dtype) {
+    hipLaunchKernelGGL((vl_pack<u16, 1>), dim3((unsigned)grid), dim3(256), 0, stream,
+                       (const u16*)src, ld, (int)cols, dst, (int)dld, plane, idx, count, rows, ones,
+                       (const float*)nullptr, (float*)nullptr);
+    return;
+  }
+  hipLaunchKernelGGL(vl_absmax, dim3(MAX_PARTS), dim3(1024), 0, stream, (const float*)src, ld, cols,
+                     (int64_t)1 << 62, idx, count, rows, top);
+  hipLaunchKernelGGL((vl_pack<float, 2>), dim3((unsigned)grid), dim3(256), 0, stream,
+                     (const float*)src, ld, (int)cols, dst, (int)dld, plane, idx, count, rows, ones,
+                     top, scale);
 }
 
 }  // namespace
@@ -715,7 +847,7 @@ size_t mg_vocab_loss_state_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
 size_t mg_vocab_loss_fwd_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
   Shape s;
   if (!vl_shape(dtype, N, V, D, &s)) return 0;
-  return vl_part_rows(s) * s.np * sizeof(float2) + s.np * sizeof(float) + s.N * sizeof(float);
+  return vl_part_rows(s) * s.np * sizeof(float2) + (s.np + s.N + 2 * MAX_PARTS) * sizeof(float);
 }
 
 size_t mg_vocab_loss_bwd_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
@@ -736,16 +868,15 @@ int mg_vocab_loss_fwd(int dtype, const void* x, int64_t ldx, const void* w, cons
     return MG_ERR_WORKSPACE;
   float2* const part = (float2*)ws;
   float* const tlogit = (float*)(part + vl_part_rows(s) * s.np);
-  float* const rows = reduction ? tlogit + s.np : loss;
+  float* const rows = reduction ? tlogit + s.np + 2 * MAX_PARTS : loss;
   hipLaunchKernelGGL(vl_index, dim3(1), dim3(1024), 0, stream, target, ignore_index, V, t.idx,
                      t.pos, t.tgt, t.count, (int)N);
-  if (dtype) {
-    vl_pack_run<u16, 1>(x, ldx, D, t.xc, s.dx, 0, t.idx, t.count, N, s.np, (int)D, stream);
-    if (s.own_w) vl_pack_run<u16, 1>(w, D, D, t.wc, s.kp, 0, nullptr, nullptr, V, V, -1, stream);
-  } else {
-    vl_pack_run<float, 3>(x, ldx, D, t.xc, s.dx, s.np * s.dx, t.idx, t.count, N, s.np, (int)D, stream);
-    vl_pack_run<float, 3>(w, D, D, t.wc, s.kp, s.V * s.kp, nullptr, nullptr, V, V, -1, stream);
-  }
+  float* const top = tlogit + s.np;  // both packings' parts, one after the other
+  vl_pack_run(dtype, x, ldx, D, t.xc, s.dx, s.np * s.dx, t.idx, t.count, N, s.np, (int)D, top, t.sx,
+              stream);
+  if (s.own_w)
+    vl_pack_run(dtype, w, D, D, t.wc, s.kp, V * s.kp, nullptr, nullptr, V, V, -1, top + MAX_PARTS,
+                t.sw, stream);
   VlArgs a = vl_logits(s, t, w, bias, 0, V);
   a.part = part, a.tlogit = tlogit;
   const int rc = vl_run<VL_LSE, false, false>(dtype, a, stream);
@@ -772,8 +903,13 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
   const Back b = vl_back(s, ws);
   if (ws_bytes < b.bytes) return MG_ERR_WORKSPACE;
   const int e = dtype ? 2 : 4;
+  float* const top = dtype ? nullptr : b.top;
+  if (top && reduction == 0)
+    hipLaunchKernelGGL(vl_absmax, dim3(MAX_PARTS), dim3(1024), 0, stream, dloss, (int64_t)256,
+                       (int64_t)256, N, (const int*)nullptr, (const int*)nullptr, (N + 255) / 256,
+                       top);
   hipLaunchKernelGGL(vl_upstream, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, stream, dloss,
-                     t.idx, t.count, reduction, b.g, b.scale);
+                     t.idx, t.count, reduction, top, b.g, b.scale, b.d_scale);
   for (int64_t v0 = 0, piece = 0; v0 < V; v0 += b.vp, ++piece) {
     const int64_t cols = V - v0 < b.vp ? V - v0 : b.vp, kc = up_to(cols, PADK);
     VlArgs a = vl_logits(s, t, w, bias, v0, cols);
@@ -783,6 +919,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
     if (rc == MG_OK && dx) {
       VlArgs c = {};
       c.A = a.A, c.lda = a.lda, c.pa = a.pa, c.m_rows = (int)s.kp;
+      c.sa = t.sw, c.sb = b.d_scale;
       c.B = b.d, c.ldb = (int)kc, c.pb = a.pd, c.n_count = t.count;
       c.K = (int)kc, c.ka = (int)cols;
       c.mt = (int)((D + TM - 1) / TM), c.nt = (int)((s.np + TN - 1) / TN), c.splits = b.dx_splits;
@@ -793,6 +930,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
     if (rc == MG_OK && dw) {
       VlArgs c = {};
       c.A = t.xc, c.lda = (int)s.dx, c.pa = s.np * s.dx, c.m_rows = (int)s.dx;
+      c.sa = t.sx, c.sb = b.d_scale;
       c.B = b.d, c.ldb = (int)kc, c.pb = a.pd, c.n_rows = (int)kc;
       c.k_count = t.count, c.ka = 1 << 30;
       c.mt = (int)((D + (db ? 1 : 0) + TM - 1) / TM), c.nt = (int)((cols + TN - 1) / TN);
