@@ -55,8 +55,6 @@ __device__ __forceinline__ unsigned pack2(float x, float y) {
   asm("" : "+v"(u));
   return u;
 }
-__device__ __forceinline__ float low(unsigned u) { return __uint_as_float(u << 16); }
-__device__ __forceinline__ float high(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
 // fp16 planes.  What hi leaves for lo; an infinity or NaN is hi's alone.
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -289,12 +287,20 @@ __device__ __forceinline__ void step_places(int (&at)[W / 64], int r0, int rows,
     }
   }
 }
-// Vector i of a step.  CLAMP: a far operand's rows past the `left` ones from p on (none or fewer
+// Vector i of a step.  TAIL: a near operand's columns past the `left` ones from p on are 0 (what
+// lies there is the next row's).  CLAMP: a far operand's rows past the `left` ones from p on (none or fewer
 // in a step that is padding alone) are the last one again: the other operand is 0 there.
-template <bool CLAMP, int W>
+template <bool CLAMP, bool TAIL, int W>
 __device__ __forceinline__ u32x4 step_load(const u16* p, const int (&at)[W / 64], int i,
                                            int left, int ld) {
   int o = at[i];
+  if constexpr (TAIL) {
+    // The thread's column is the same in all of its vectors; column 0 of the row stands in.
+    const int c = (threadIdx.x & 3) * 8;
+    const bool in = c < left;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(p + (in ? o : o - c));
+    return in ? x : u32x4{0, 0, 0, 0};
+  }
   if constexpr (CLAMP) {
     const int over = (int)(threadIdx.x + i * NT) / (W / 8) - (left - 1);
     o -= (over > 0 ? over : 0) * ld;
@@ -322,7 +328,7 @@ __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-template <int EPI, bool AFAR, bool BFAR, int PL, typename E>
+template <int EPI, bool AFAR, bool BFAR, int PL, bool TAIL, typename E>
 __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
   __shared__ __align__(16) u16 lds[2][(TM + TN) * BK];  // the buffers: A, then B
   __shared__ __align__(16) float s_bias[TM];
@@ -377,10 +383,10 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
   const auto load = [&](int half) {
 #pragma unroll
     for (int v = half * VA / 2; v < (half + 1) * VA / 2; ++v)
-      xa[v] = step_load<AFAR && !BFAR, TM>(fA, oa, v, a.ka - f_k * BK, a.lda);
+      xa[v] = step_load<AFAR && !BFAR, TAIL, TM>(fA, oa, v, a.ka - f_k * BK, a.lda);
 #pragma unroll
     for (int v = half * VB / 2; v < (half + 1) * VB / 2; ++v)
-      xb[v] = step_load<false, TN>(fB, ob, v, 0, a.ldb);
+      xb[v] = step_load<false, false, TN>(fB, ob, v, 0, a.ldb);
   };
   const auto put = [&](int s, int half) {
 #pragma unroll
@@ -685,6 +691,7 @@ __global__ __launch_bounds__(256) void vl_sum(const float* __restrict__ part, in
     const int64_t i = x / cols, j = pos ? pos[i] : i;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (j >= 0)
+#pragma unroll 8
       for (int p = 0; p < parts; ++p) {
         const float4 v = *reinterpret_cast<const float4*>(part + p * po + j * cols + x % cols);
         s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
@@ -708,6 +715,7 @@ constexpr int64_t up_to(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
 struct Shape {
   int64_t N, V, D, np, kp, dx;  // padded rows, contracted columns, columns of packed x
+  int64_t lw;                    // elements between W's rows, as the products read them
   int planes;
   bool own_w;                    // W is packed too
 };
@@ -717,7 +725,8 @@ bool vl_shape(int dtype, int64_t N, int64_t V, int64_t D, Shape* s) {
   s->N = N, s->V = V, s->D = D;
   s->np = up_to(N, PADK), s->kp = up_to(D, PADK), s->dx = up_to(D + 1, PADK);
   s->planes = dtype ? 1 : 2;
-  s->own_w = dtype == 0 || D % PADK != 0;
+  s->own_w = dtype == 0 || D % 8 != 0;
+  s->lw = s->own_w ? s->kp : D;
   return true;
 }
 struct State {
@@ -746,12 +755,14 @@ State vl_state(const Shape& s, void* base) {
 }
 
 // Parts of the contracted axis for `tiles` result tiles on 256 CUs of two workgroups: the fewest
-// steps in a row.
-int vl_splits(int64_t tiles, int64_t steps) {
+// steps (about 0.8 us each) in a row, beside what the parts of `size` elements cost to write and
+// to add (16 bytes an element, 4 TB/s, and a load after another in a thread: 0.2 us a part).
+int vl_splits(int64_t tiles, int64_t steps, int64_t size) {
   int best = 1;
   double least = 1e300;
-  for (int s = 1; s <= 16 && (s == 1 || steps / s >= 16); ++s) {
-    const double cost = (double)((tiles * s + 511) / 512) * ((steps + s - 1) / s + 8) + 4.0 * (s - 1);
+  for (int s = 1; s <= 128 && (s == 1 || steps / s >= 16); ++s) {
+    const double cost = (double)((tiles * s + 511) / 512) * ((steps + s - 1) / s + 8) +
+                        (s - 1) * (0.25 + 5e-6 * (double)size);
     if (cost < least) least = cost, best = s;
   }
   return best;
@@ -773,8 +784,8 @@ Back vl_back(const Shape& s, void* base) {
   b.vp = up_to((s.V + b.pieces - 1) / b.pieces, TM);
   b.pieces = (s.V + b.vp - 1) / b.vp;
   const int64_t steps = s.planes == 1 ? 1 : 3;
-  b.dx_splits = vl_splits((s.np + TN - 1) / TN * ((s.D + TM - 1) / TM), b.vp / BK * steps);
-  b.dw_splits = vl_splits(b.vp / TN * ((s.D + TM - 1) / TM), s.np / BK * steps);
+  b.dx_splits = vl_splits((s.np + TN - 1) / TN * ((s.D + TM - 1) / TM), b.vp / BK * steps, s.N * s.D);
+  b.dw_splits = vl_splits(b.vp / TN * ((s.D + TM - 1) / TM), s.np / BK * steps, b.vp * s.D);
   char* p = (char*)base;
   const auto take = [&](int64_t n) {
     char* at = p;
@@ -797,8 +808,16 @@ int vl_run(int dtype, VlArgs& a, hipStream_t stream) {
   const int64_t work = (int64_t)a.mt * a.nt * a.splits;
   if (work > (1ll << 30)) return MG_ERR_TOO_LARGE;
   const dim3 grid((unsigned)((work + 7) / 8 * 8));
-  if (dtype) hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 1, u16>), grid, dim3(NT), 0, stream, a);
-  else hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 2, float>), grid, dim3(NT), 0, stream, a);
+  // W is read where it lies if its rows are whole vectors; the zeros behind rows that are not
+  // whole steps cost selections, so rows that are do without them.
+  if constexpr (EPI != VL_OUT) {
+    if (dtype && a.lda % BK) {
+      hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 1, true, u16>), grid, dim3(NT), 0, stream, a);
+      return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
+    }
+  }
+  if (dtype) hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 1, false, u16>), grid, dim3(NT), 0, stream, a);
+  else hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 2, false, float>), grid, dim3(NT), 0, stream, a);
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
 
@@ -806,12 +825,12 @@ int vl_run(int dtype, VlArgs& a, hipStream_t stream) {
 VlArgs vl_logits(const Shape& s, const State& t, const void* w, const void* bias, int64_t v0,
                  int64_t cols) {
   VlArgs a = {};
-  a.A = (s.own_w ? t.wc : (const u16*)w) + v0 * s.kp;
-  a.lda = (int)s.kp, a.pa = s.V * s.kp;
+  a.A = (s.own_w ? t.wc : (const u16*)w) + v0 * s.lw;
+  a.lda = (int)s.lw, a.pa = s.V * s.lw;
   a.B = t.xc, a.ldb = (int)s.dx, a.pb = s.np * s.dx;
   a.sa = t.sw, a.sb = t.sx;
   a.m_rows = (int)cols, a.n_count = t.count;
-  a.K = (int)s.kp, a.ka = 1 << 30;
+  a.K = (int)up_to(s.lw, BK), a.ka = (int)s.lw;
   a.mt = (int)((cols + TM - 1) / TM), a.nt = (int)((s.np + TN - 1) / TN), a.splits = 1;
   a.v0 = (int)v0, a.V = (int)s.V, a.bias = bias, a.tgt = t.tgt, a.n_ld = (int)s.np;
   return a;
@@ -918,7 +937,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
     int rc = vl_run<VL_D, false, false>(dtype, a, stream);
     if (rc == MG_OK && dx) {
       VlArgs c = {};
-      c.A = a.A, c.lda = a.lda, c.pa = a.pa, c.m_rows = (int)s.kp;
+      c.A = a.A, c.lda = a.lda, c.pa = a.pa, c.m_rows = (int)s.lw;
       c.sa = t.sw, c.sb = b.d_scale;
       c.B = b.d, c.ldb = (int)kc, c.pb = a.pd, c.n_count = t.count;
       c.K = (int)kc, c.ka = (int)cols;
