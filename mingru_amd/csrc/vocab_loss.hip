@@ -710,6 +710,8 @@ __global__ __launch_bounds__(256) void vl_sum(const float* __restrict__ part, in
   }
 }
 
+#include "vocab_few.h"
+
 // ---- host ------------------------------------------------------------------------------------
 constexpr int64_t up_to(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
@@ -718,7 +720,13 @@ struct Shape {
   int64_t lw;                    // elements between W's rows, as the products read them
   int planes;
   bool own_w;                    // W is packed too
+  int few;                       // blocks of 32 rows (1, 2, 4) on vocab_few.h's kernels, or 0
+  int64_t ldd;                   // their d's row
 };
+
+// Pieces of the vocabulary: as few as keep d in half a gigabyte.
+constexpr int64_t VL_D_BYTES = 512ll << 20;
+
 bool vl_shape(int dtype, int64_t N, int64_t V, int64_t D, Shape* s) {
   if ((dtype & ~1) || N < 1 || V < 1 || D < 1 || N > (1 << 30) || V > (1 << 30) || D > (1 << 20))
     return false;
@@ -727,6 +735,9 @@ bool vl_shape(int dtype, int64_t N, int64_t V, int64_t D, Shape* s) {
   s->planes = dtype ? 1 : 2;
   s->own_w = dtype == 0 || D % 8 != 0;
   s->lw = s->own_w ? s->kp : D;
+  s->ldd = up_to(V, 128);
+  s->few = dtype == 0 && N <= FEW && D >= 4 && FEW * s->ldd * 4 <= VL_D_BYTES
+               ? (N <= 32 ? 1 : N <= 64 ? 2 : 4) : 0;
   return true;
 }
 struct State {
@@ -748,10 +759,48 @@ State vl_state(const Shape& s, void* base) {
   t.sx = (float*)take(4), t.sw = (float*)take(4);
   t.idx = (int*)take(s.N * 4), t.pos = (int*)take(s.N * 4), t.tgt = (int*)take(s.N * 4);
   t.soft = (float2*)take(s.N * 8);
-  t.xc = (u16*)take(s.planes * s.np * s.dx * 2);
-  t.wc = s.own_w ? (u16*)take(s.planes * s.V * s.kp * 2) : nullptr;
+  t.xc = (u16*)take(s.few ? 32 * s.few * s.dx * 4 : s.planes * s.np * s.dx * 2);
+  t.wc = s.own_w && !s.few ? (u16*)take(s.planes * s.V * s.kp * 2) : nullptr;
   t.bytes = p - (char*)base;
   return t;
+}
+
+// ---- few rows --------------------------------------------------------------------------------
+int few_tiles(const Shape& s) { return s.few == 1 ? 1 : 2; }  // blocks of 32 columns a workgroup
+int64_t few_parts(const Shape& s) { return (s.V + 32 * few_tiles(s) - 1) / (32 * few_tiles(s)); }
+// dx's parts: columns of the vocabulary in each, for about two workgroups a CU.
+int64_t few_per(const Shape& s) {
+  const int64_t tiles = (s.D + 127) / 128, want = (512 + tiles - 1) / tiles;
+  return up_to((s.V + want - 1) / want, 32);
+}
+FewArgs few_args(const Shape& s, const State& t, const void* w, const void* bias) {
+  FewArgs a = {};
+  a.x = (const float*)t.xc, a.w = (const float*)w, a.bias = (const float*)bias;
+  a.ldx = (int)s.dx, a.D = (int)s.D, a.V = (int)s.V, a.ldd = (int)s.ldd, a.parts = (int)few_parts(s);
+  a.idx = t.idx, a.tgt = t.tgt, a.count = t.count;
+  return a;
+}
+template <int EPI>
+void few_logits(const Shape& s, const FewArgs& a, hipStream_t stream) {
+  const dim3 grid((unsigned)few_parts(s));
+  if (s.few == 1) hipLaunchKernelGGL((vl_few_logits<EPI, 1, 1>), grid, dim3(256), 0, stream, a);
+  else if (s.few == 2) hipLaunchKernelGGL((vl_few_logits<EPI, 2, 2>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((vl_few_logits<EPI, 4, 2>), grid, dim3(256), 0, stream, a);
+}
+template <int NB>
+void few_products(const Shape& s, const State& t, const FewArgs& a, float* dx_part, void* dw, void* db,
+                  hipStream_t stream) {
+  if (dx_part) {
+    const int64_t per = few_per(s);
+    hipLaunchKernelGGL(vl_few_dx<NB>, dim3((unsigned)((s.D + 127) / 128), (unsigned)((s.V + per - 1) / per)),
+                       dim3(256), 0, stream, a.d, a.ldd, a.w, a.V, a.D, (int)s.N, a.count, (int)per, dx_part);
+  }
+  if (dw) {
+    const int64_t tiles = (s.D + 127) / 128, wgs = (s.V + 127) / 128, split = (1024 + wgs - 1) / wgs;
+    hipLaunchKernelGGL(vl_few_dw<NB>, dim3((unsigned)wgs, (unsigned)(split < tiles ? split : tiles)),
+                       dim3(256), 0, stream, a.d, a.ldd, a.x, a.ldx, a.V, a.D, a.count, (float*)dw,
+                       (float*)db);
+  }
 }
 
 // Parts of the contracted axis for `tiles` result tiles on 256 CUs of two workgroups: the fewest
@@ -768,8 +817,6 @@ int vl_splits(int64_t tiles, int64_t steps, int64_t size) {
   return best;
 }
 
-// Pieces of the vocabulary: as few as keep d in half a gigabyte.
-constexpr int64_t VL_D_BYTES = 512ll << 20;
 struct Back {
   int64_t vp, pieces;   // columns of a piece
   int dx_splits, dw_splits;
@@ -778,7 +825,13 @@ struct Back {
   size_t bytes;
 };
 Back vl_back(const Shape& s, void* base) {
-  Back b;
+  Back b = {};
+  if (s.few) {
+    const int64_t d = up_to(32 * s.few * s.ldd * 4, 256), per = few_per(s);
+    b.d = (u16*)base, b.dx_part = (float*)((char*)base + d);
+    b.bytes = d + (s.V + per - 1) / per * s.N * s.D * 4;
+    return b;
+  }
   const int64_t most = VL_D_BYTES / (s.np * 2 * s.planes);
   b.pieces = (s.V + (most > TM ? most : TM) - 1) / (most > TM ? most : TM);
   b.vp = up_to((s.V + b.pieces - 1) / b.pieces, TM);
@@ -866,6 +919,7 @@ size_t mg_vocab_loss_state_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
 size_t mg_vocab_loss_fwd_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
   Shape s;
   if (!vl_shape(dtype, N, V, D, &s)) return 0;
+  if (s.few) return s.N * (few_parts(s) * sizeof(float2) + 2 * sizeof(float));
   return vl_part_rows(s) * s.np * sizeof(float2) + (s.np + s.N + 2 * MAX_PARTS) * sizeof(float);
 }
 
@@ -886,8 +940,28 @@ int mg_vocab_loss_fwd(int dtype, const void* x, int64_t ldx, const void* w, cons
   if (state_bytes < t.bytes || ws_bytes < mg_vocab_loss_fwd_workspace_bytes(dtype, N, V, D))
     return MG_ERR_WORKSPACE;
   float2* const part = (float2*)ws;
-  float* const tlogit = (float*)(part + vl_part_rows(s) * s.np);
-  float* const rows = reduction ? tlogit + s.np + 2 * MAX_PARTS : loss;
+  float* const tlogit = (float*)(part + (s.few ? N * few_parts(s) : vl_part_rows(s) * s.np));
+  float* const rows = !reduction ? loss : s.few ? tlogit + N : tlogit + s.np + 2 * MAX_PARTS;
+  const auto finish = [&]() {
+    if (reduction)
+      hipLaunchKernelGGL(vl_total, dim3(1), dim3(1024), 0, stream, rows, t.pos, t.count, (int)N,
+                         (int)(reduction == 1), loss);
+    else
+      hipLaunchKernelGGL(vl_left_out, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, stream, t.pos,
+                         (int)N, loss);
+    return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
+  };
+  if (s.few) {
+    hipLaunchKernelGGL(vl_few_index, dim3(32 * s.few), dim3(256), 0, stream, target, ignore_index,
+                       (int)V, (int)N, (const float*)x, ldx, (int)D, t.idx, t.pos, t.tgt, t.count,
+                       (float*)t.xc, (int)s.dx);
+    FewArgs a = few_args(s, t, w, bias);
+    a.part = part, a.tlogit = tlogit;
+    few_logits<VL_LSE>(s, a, stream);
+    hipLaunchKernelGGL(vl_few_join, dim3((unsigned)N), dim3(256), 0, stream, part, a.parts, tlogit,
+                       t.tgt, t.idx, t.count, t.soft, rows);
+    return finish();
+  }
   hipLaunchKernelGGL(vl_index, dim3(1), dim3(1024), 0, stream, target, ignore_index, V, t.idx,
                      t.pos, t.tgt, t.count, (int)N);
   float* const top = tlogit + s.np;  // both packings' parts, one after the other
@@ -902,13 +976,7 @@ int mg_vocab_loss_fwd(int dtype, const void* x, int64_t ldx, const void* w, cons
   if (rc != MG_OK) return rc;
   hipLaunchKernelGGL(vl_join, dim3((unsigned)((N + 63) / 64)), dim3(1024), 0, stream, part, tlogit,
                      t.tgt, t.idx, t.count, (int)vl_part_rows(s), (int)s.np, t.soft, rows);
-  if (reduction)
-    hipLaunchKernelGGL(vl_total, dim3(1), dim3(1024), 0, stream, rows, t.pos, t.count, (int)N,
-                       (int)(reduction == 1), loss);
-  else
-    hipLaunchKernelGGL(vl_left_out, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, stream, t.pos,
-                       (int)N, loss);
-  return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
+  return finish();
 }
 
 int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* dloss,
@@ -921,6 +989,18 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
   const State t = vl_state(s, const_cast<void*>(state));
   const Back b = vl_back(s, ws);
   if (ws_bytes < b.bytes) return MG_ERR_WORKSPACE;
+  if (s.few) {
+    FewArgs a = few_args(s, t, w, bias);
+    a.soft = t.soft, a.up = dloss, a.reduction = reduction, a.d = (float*)b.d;
+    few_logits<VL_D>(s, a, stream);
+    (s.few == 1 ? few_products<1> : s.few == 2 ? few_products<2> : few_products<4>)(
+        s, t, a, dx ? b.dx_part : nullptr, dw, db, stream);
+    if (dx)
+      hipLaunchKernelGGL(vl_sum<float>, dim3((unsigned)((N * D / 4 + 256) / 256)), dim3(256), 0, stream,
+                         b.dx_part, N * D, (int)((V + few_per(s) - 1) / few_per(s)), t.pos, N * D,
+                         (int)D, (float*)dx);
+    return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
+  }
   const int e = dtype ? 2 : 4;
   float* const top = dtype ? nullptr : b.top;
   if (top && reduction == 0)

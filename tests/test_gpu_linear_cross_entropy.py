@@ -61,6 +61,22 @@ def test_sizes(cuda, N, V, D, dtype):
     check(cuda, N, V, D, dtype, seed=N, ignored=0.0 if N < 4 else 0.3)
 
 
+@pytest.mark.parametrize("N, V, D", [(1, 1, 4), (2, 31, 7), (31, 33, 5), (32, 129, 36), (33, 640, 31),
+                                     (64, 1000, 129), (90, 100, 1001), (128, 5003, 66),
+                                     (129, 130, 33), (8, 4099, 1000)])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_few_rows(cuda, N, V, D, reduction):
+    """Up to 128 fp32 rows have kernels of their own; whole vectors of bf16 weights lie in place."""
+    check(cuda, N, V, D, torch.float32, reduction, bias=V % 2 == 0, seed=N, ignored=0.2 if N > 8 else 0)
+    check(cuda, N, V, D - D % 8 + 8, torch.bfloat16, reduction, seed=N)
+
+
+def test_few_rows_left_out(cuda):
+    for N in (20, 60, 120):
+        check(cuda, N, 300, 64, torch.float32, "none", ignored=0.9)
+        check(cuda, N, 300, 64, torch.float32, "none", ignored=1.0)
+
+
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 @pytest.mark.parametrize("bias", [True, False])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
