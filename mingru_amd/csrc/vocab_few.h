@@ -1,15 +1,17 @@
 // The vocabulary loss of a few fp32 rows (vocab_loss.hip's formulas): 1 to 128 of them, where
 // reading W bounds the work.  W is read where it lies, in fp32, and nothing is split into planes:
 // packing it costs a pass to find its scale and three times its size beside.  The matrix
-// instruction is fp32's own, 32 x 32 x 2; at 64 rows its time is what reading W takes.
+// instructions are fp32's own, whose time at 64 rows is what reading W takes.
 //
-// Every product takes its operands from memory straight to registers, without LDS: a lane's 16
-// bytes are four elements of four instructions, whose contracted elements (or columns) are
-// numbered as the lanes hold them.  Four waves a workgroup: NB blocks of 32 rows, times 4 / NB
-// parts of the contracted axis, joined through LDS in a fixed order.
+// Four waves a workgroup: NB blocks of 32 rows, times 4 / NB parts of the contracted axis, joined
+// through LDS in a fixed order.  dx's and dW's products have W's and x's columns across the lanes
+// and take their operands from memory straight to registers: a lane's 16 bytes are four columns
+// of four instructions, or four contracted elements, numbered as the lanes hold them.
 //
-// 8 x 33304 x 1000, forward: 26 us for reading W; 89 x 18250 x 768 with gradients: 65 us of
-// matrix instructions.  FIGURES
+// Kernel times: 8 x 33304 x 1000 forward 41 us (W's 133 MB in 28.5, 4.7 TB/s; on planes 163);
+// with gradients, 4 x 50557 x 512 126 us (four times 103 MB at the rate of a copy: 80; on planes
+// 250), 64 x 18250 x 768 144, 128 of them 253 (90 at fp32's matrix rate).  On planes 129 rows
+// take 268, so 128 is where this ends.
 #pragma once
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -57,78 +59,105 @@ __global__ __launch_bounds__(256) void vl_few_index(const int64_t* __restrict__ 
   for (int c = tid; c < ld; c += 256) to[(int64_t)j * ld + c] = row >= 0 && c < D ? x[row * ldx + c] : 0.f;
 }
 
-// LSE and D.  A workgroup: 32 MI columns of the vocabulary (the instruction's rows), all rows.
-template <int EPI, int NB, int MI>
+// LSE and D.  A workgroup: 16 MI columns of the vocabulary (the instruction's rows), NB blocks of
+// 16 NJ rows.  Both operands have the contracted elements in a row, so a lane's fragments are 16
+// bytes of 64 rows' places: read from memory like that, each was an access of its own, and the
+// caches gave a quarter of their rate (N = 8: 47 us in place of 28.5).  So steps of 32 KP columns go
+// through LDS, from registers that hold the next step's; vector c of row r lies at few_slot.
+template <int KP>
+__device__ __forceinline__ int few_slot(int r, int c) {
+  return r * 8 * KP + (KP == 1 ? c ^ (r & 7) : c ^ (r & 7) ^ ((c & 1) << 3));
+}
+template <int EPI, int NB, int MI, int NJ>
 __global__ __launch_bounds__(256) void vl_few_logits(FewArgs a) {
-  constexpr int KP = 4 / NB;
-  __shared__ float s_acc[KP > 1 ? KP - 1 : 1][NB][MI][KP > 1 ? 16 : 1][64];
-  const int lane = threadIdx.x & 63, wave = mg_uniform(threadIdx.x >> 6);
-  const int nb = wave % NB, kp = wave / NB, l = lane & 31, h = lane >> 5;
-  const int v0 = blockIdx.x * 32 * MI, rows = *a.count, n = nb * 32 + l;
-  const int chunks = (a.D + 31) / 32, per = (chunks + KP - 1) / KP;
-  const int c0 = kp * per, c1 = nb * 32 < rows ? (c0 + per < chunks ? c0 + per : chunks) : 0;
-  const float* wr[MI];
+  constexpr int KP = 4 / NB, W = 32 * KP, RW = 16 * MI, RX = 16 * NJ * NB;
+  constexpr int VW = RW * 8 * KP / 256, VX = RX * 8 * KP / 256;  // vectors of a thread
+  static_assert((KP - 1) * NB * MI * NJ * 64 <= (RW + RX) * 8 * KP, "the join's room");
+  __shared__ f32x4 lds[(RW + RX) * 8 * KP];
+  f32x4* const lx = lds + RW * 8 * KP;
+  const int tid = threadIdx.x, lane = tid & 63, wave = mg_uniform(tid >> 6);
+  const int nb = wave % NB, kp = wave / NB, l = lane & 15, h = lane >> 4;
+  const int v0 = blockIdx.x * RW, rows = *a.count, n0 = nb * 16 * NJ;
+  const float *pw[VW], *px[VX];
+  int sw[VW], sx[VX];
+  const int c4 = tid % (8 * KP) * 4;  // the column of a thread's vectors
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const int v = v0 + 32 * i + l;
-    wr[i] = a.w + (int64_t)(v < a.V ? v : a.V - 1) * a.D;
+  for (int i = 0; i < VW; ++i) {
+    const int r = (tid + 256 * i) / (8 * KP), v = v0 + r;
+    pw[i] = a.w + (int64_t)(v < a.V ? v : a.V - 1) * a.D + c4;
+    sw[i] = few_slot<KP>(r, c4 / 4);
   }
-  const float* const xr = a.x + (int64_t)n * a.ldx + 4 * h;
-  // 32 contracted elements, 8 g + 4 h + e in element e of vector g.  W's past its columns are 0.
-  const auto load = [&](f32x4 (&w)[MI][4], f32x4 (&x)[4], int c) {
-    if (c * 32 + 32 <= a.D) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) w[i][g] = *reinterpret_cast<const f32x4u*>(wr[i] + c * 32 + g * 8 + 4 * h);
-    } else {
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k = c * 32 + g * 8 + 4 * h + e;
-            const float y = wr[i][k < a.D ? k : a.D - 1];
-            w[i][g][e] = k < a.D ? y : 0.f;
-          }
-    }
-#pragma unroll
-    for (int g = 0; g < 4; ++g) x[g] = *reinterpret_cast<const f32x4*>(xr + c * 32 + g * 8);
-  };
-  f32x16 acc[MI];
+  for (int i = 0; i < VX; ++i) {
+    const int r = (tid + 256 * i) / (8 * KP);
+    px[i] = a.x + (int64_t)r * a.ldx + c4;
+    sx[i] = few_slot<KP>(r, c4 / 4);
+  }
+  f32x4 acc[MI][NJ], yw[VW], yx[VX];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
-  f32x4 w[2][MI][4], x[2][4];
-  const auto mul = [&](const f32x4 (&w)[MI][4], const f32x4 (&x)[4]) {
+    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const auto load = [&](int k) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
+    for (int i = 0; i < VW; ++i) yw[i] = *reinterpret_cast<const f32x4u*>(pw[i] + k);
+#pragma unroll
+    for (int i = 0; i < VX; ++i) yx[i] = *reinterpret_cast<const f32x4*>(px[i] + k);
+  };
+  const auto put = [&]() {
+#pragma unroll
+    for (int i = 0; i < VW; ++i) lds[sw[i]] = yw[i];
+#pragma unroll
+    for (int i = 0; i < VX; ++i) lx[sx[i]] = yx[i];
+  };
+  const auto mul = [&]() {
+    if (n0 >= rows) return;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      f32x4 fw[MI], fx[NJ];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) fw[i] = lds[few_slot<KP>(16 * i + l, 8 * kp + 4 * g + h)];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) fx[j] = lx[few_slot<KP>(n0 + 16 * j + l, 8 * kp + 4 * g + h)];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int i = 0; i < MI; ++i)
-          acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(w[i][g][e], x[g][e], acc[i], 0, 0, 0);
-  };
-  // The next chunk's loads are under way during a chunk's products (the last one's again at the
-  // end).
-  if (c0 < c1) {
-    load(w[0], x[0], c0);
-    for (int c = c0; c < c1; c += 2) {
-      load(w[1], x[1], c + 1 < c1 ? c + 1 : c);
-      mul(w[0], x[0]);
-      if (c + 1 >= c1) break;
-      load(w[0], x[0], c + 2 < c1 ? c + 2 : c + 1);
-      mul(w[1], x[1]);
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fw[i][e], fx[j][e], acc[i][j], 0, 0, 0);
     }
+  };
+  const int whole = a.D / W;
+  if (whole) load(0);
+  for (int c = 0; c < whole; ++c) {
+    put();
+    __syncthreads();
+    load((c + 1 < whole ? c + 1 : c) * W);
+    mul();
+    __syncthreads();
+  }
+  if (a.D % W) {  // 0 past the last column
+    const int k = whole * W;
+#pragma unroll
+    for (int i = 0; i < VW; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) yw[i][e] = k + c4 + e < a.D ? pw[i][k + e] : 0.f;
+#pragma unroll
+    for (int i = 0; i < VX; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) yx[i][e] = k + c4 + e < a.D ? px[i][k + e] : 0.f;
+    put();
+    __syncthreads();
+    mul();
+    __syncthreads();
   }
   if constexpr (KP > 1) {
     if (kp > 0) {
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s_acc[kp - 1][nb][i][e][lane] = acc[i][e];
+        for (int j = 0; j < NJ; ++j) lds[(((kp - 1) * NB + nb) * MI * NJ + i * NJ + j) * 64 + lane] = acc[i][j];
     }
     __syncthreads();
     if (kp > 0) return;
@@ -137,55 +166,62 @@ __global__ __launch_bounds__(256) void vl_few_logits(FewArgs a) {
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][e] += s_acc[p - 1][nb][i][e][lane];
+        for (int j = 0; j < NJ; ++j) {
+          const f32x4 y = lds[(((p - 1) * NB + nb) * MI * NJ + i * NJ + j) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] += y[e];
+        }
   }
-  // Row n, columns v0 + 32 i + 8 q + 4 h + x in acc[i][4 q + x].  Past the vocabulary -inf.
+  // Row n0 + 16 j + l, columns v0 + 16 i + 4 h + e in acc[i][j][e].  Past the vocabulary -inf.
   const float log2 = 1.4426950408889634f;
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int v = v0 + 32 * i + 8 * (e >> 2) + 4 * h + (e & 3);
-      if (v >= a.V) acc[i][e] = -INFINITY;
-      else if (a.bias) acc[i][e] += a.bias[v];
+    for (int e = 0; e < 4; ++e) {
+      const int v = v0 + 16 * i + 4 * h + e;
+      const float b = a.bias && v < a.V ? a.bias[v] : 0.f;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j][e] = v < a.V ? acc[i][j][e] + b : -INFINITY;
     }
-  const int r = n < rows ? n : 0, t = a.tgt[r] - v0 - 4 * h;
-  if constexpr (EPI == VL_LSE) {
-    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+  for (int j = 0; j < NJ; ++j) {
+    const int n = n0 + 16 * j + l, r = n < rows ? n : 0, t = a.tgt[r] - v0 - 4 * h;
+    if constexpr (EPI == VL_LSE) {
+      float top = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        top = fmaxf(top, acc[i][e]);
-        if (t == 32 * i + 8 * (e >> 2) + (e & 3) && n < rows) a.tlogit[n] = acc[i][e];
-      }
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
+      for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+        for (int e = 0; e < 4; ++e) {
+          top = fmaxf(top, acc[i][j][e]);
+          if (t == 16 * i + e && n < rows) a.tlogit[n] = acc[i][j][e];
+        }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float ref = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f((acc[i][e] - ref) * log2);
-    sum += __shfl_xor(sum, 32);
-    if (h == 0 && n < rows) a.part[(int64_t)n * a.parts + blockIdx.x] = make_float2(top, sum);
-  } else {
-    const float2 soft = a.soft[r];
-    float g = a.reduction ? a.up[0] : rows > 0 ? a.up[a.idx[r]] : 0.f;
-    if (a.reduction == 1) g /= (float)(rows > 0 ? rows : 1);
-    const float sg = soft.y * g;
+      for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+        for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f((acc[i][j][e] - ref) * log2);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      if (h == 0 && n < rows) a.part[(int64_t)n * a.parts + blockIdx.x] = make_float2(top, sum);
+    } else {
+      const float2 soft = a.soft[r];
+      float g = a.reduction ? a.up[0] : rows > 0 ? a.up[a.idx[r]] : 0.f;
+      if (a.reduction == 1) g /= (float)(rows > 0 ? rows : 1);
+      const float sg = soft.y * g;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int i = 0; i < MI; ++i) {
         f32x4 y;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          y[x] = __builtin_amdgcn_exp2f((acc[i][4 * q + x] - soft.x) * log2) * sg -
-                 (t == 32 * i + 8 * q + x ? g : 0.f);
-          y[x] = n < rows ? y[x] : 0.f;
+        for (int e = 0; e < 4; ++e) {
+          y[e] = __builtin_amdgcn_exp2f((acc[i][j][e] - soft.x) * log2) * sg - (t == 16 * i + e ? g : 0.f);
+          y[e] = n < rows ? y[e] : 0.f;
         }
-        *reinterpret_cast<f32x4*>(a.d + (int64_t)n * a.ldd + v0 + 32 * i + 8 * q + 4 * h) = y;
+        *reinterpret_cast<f32x4*>(a.d + (int64_t)n * a.ldd + v0 + 16 * i + 4 * h) = y;
       }
+    }
   }
 }
 

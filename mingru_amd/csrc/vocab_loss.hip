@@ -30,6 +30,7 @@
 // bits at any size; 2047 x 10007 x 392 took 575 us with them, 365 with these).  d, in -1 .. 1, is
 // scaled by 2^15.
 // bf16 inputs: d, without the factor of a mean, is rounded to bf16 once; sums are fp32.
+// Up to 128 fp32 rows take vocab_few.h's kernels.
 // With a bias, x has a column of ones behind its own, which makes db one more column of dW.
 #include "mg_common.h"
 
@@ -783,9 +784,11 @@ FewArgs few_args(const Shape& s, const State& t, const void* w, const void* bias
 template <int EPI>
 void few_logits(const Shape& s, const FewArgs& a, hipStream_t stream) {
   const dim3 grid((unsigned)few_parts(s));
-  if (s.few == 1) hipLaunchKernelGGL((vl_few_logits<EPI, 1, 1>), grid, dim3(256), 0, stream, a);
-  else if (s.few == 2) hipLaunchKernelGGL((vl_few_logits<EPI, 2, 2>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((vl_few_logits<EPI, 4, 2>), grid, dim3(256), 0, stream, a);
+  if (s.few == 2) hipLaunchKernelGGL((vl_few_logits<EPI, 2, 4, 2>), grid, dim3(256), 0, stream, a);
+  else if (s.few == 4) hipLaunchKernelGGL((vl_few_logits<EPI, 4, 4, 2>), grid, dim3(256), 0, stream, a);
+  else if (EPI == VL_LSE && s.N <= 16)  // d's 32 rows are all written
+    hipLaunchKernelGGL((vl_few_logits<VL_LSE, 1, 2, 1>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((vl_few_logits<EPI, 1, 2, 2>), grid, dim3(256), 0, stream, a);
 }
 template <int NB>
 void few_products(const Shape& s, const State& t, const FewArgs& a, float* dx_part, void* dw, void* db,
