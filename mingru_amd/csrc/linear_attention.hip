@@ -40,7 +40,12 @@
 // into the gradient of g) is split into three bf16 planes, 24 significant bits, at three times
 // the products: with two planes the states were 2.4e-6 off and the gradient of g 7e-6.
 //
-// Bound: LDS reads of operand fragments, then memory.
+// Bound: a wave's own chain of a chunk -- barriers, LDS reads of operand fragments and the vector
+// instructions that decay and split them -- with one workgroup a CU past heads 64 wide; memory
+// would be a quarter of it.  16 x 2048 tokens of 8 heads of 128, bf16, with gradients: 443 us
+// (sweeps: states 36, o 88, adjoint states 36, dq 138, dk and dv 150; joins 14, dg 11).
+// One sequence of 65536 tokens, forward: 239 us.  One token of 256 sequences of 16 heads: 112 us,
+// 4.8 TB/s of states read and written.
 #include "mg_common.h"
 
 namespace {

@@ -22,6 +22,9 @@
 // second launch adds the partials in order.  No atomics: results are the same on every run.
 //
 // Everything between loads and stores is fp32; variances are of the centred values.
+//
+// 65536 rows of 1024, bf16, RMS norm, sigmoid gate, stream and LayerNorm: forward 142 us (4.7
+// TB/s), backward 252 (4.3 TB/s); a large copy reaches 5.15.
 #include "mg_common.h"
 
 namespace {
