@@ -38,6 +38,7 @@ __global__ __launch_bounds__(256) void vl_few_index(const int64_t* __restrict__ 
                                                     const float* __restrict__ x, int64_t ldx, int D,
                                                     int* __restrict__ idx, int* __restrict__ pos,
                                                     int* __restrict__ tgt, int* __restrict__ count,
+                                                    float* __restrict__ loss,
                                                     float* __restrict__ to, int ld) {
   __shared__ int s_n[2], s_row;
   const int tid = threadIdx.x, j = blockIdx.x;
@@ -51,6 +52,7 @@ __global__ __launch_bounds__(256) void vl_few_index(const int64_t* __restrict__ 
   if (in && at == j) s_row = tid;
   if (j == 0 && tid < N) {
     pos[tid] = in ? at : -1;
+    if (!in && loss) loss[tid] = 0.f;
     if (in) idx[at] = tid, tgt[at] = t >= 0 && t < V ? (int)t : -1;
     if (tid == 0) *count = s_n[0] + s_n[1];
   }

@@ -86,11 +86,13 @@ constexpr float ONE_SCALE = 16384.f, D_SCALE = 32768.f;
 
 // ---- packing ----------------------------------------------------------------------------
 // Counted rows in order: idx[j] the j-th one's row, pos[i] a row's place or -1, tgt[j] its
-// target, -1 where that lies outside the vocabulary.  One workgroup.
+// target, -1 where that lies outside the vocabulary; and the left-out rows' losses, 0, if those
+// are wanted.  One workgroup.
 __global__ __launch_bounds__(1024) void vl_index(const int64_t* __restrict__ target,
                                                  int64_t ignore, int64_t V, int* __restrict__ idx,
                                                  int* __restrict__ pos, int* __restrict__ tgt,
-                                                 int* __restrict__ count, int N) {
+                                                 int* __restrict__ count, float* __restrict__ loss,
+                                                 int N) {
   __shared__ int s_n[2][16];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   int base = 0, turn = 0;
@@ -126,6 +128,7 @@ __global__ __launch_bounds__(1024) void vl_index(const int64_t* __restrict__ tar
       const bool in = t[x] != ignore;
       if (in) idx[at] = i, tgt[at] = t[x] >= 0 && t[x] < V ? (int)t[x] : -1;
       if (i < N) pos[i] = in ? at : -1;
+      if (i < N && !in && loss) loss[i] = 0.f;
       at += in;
       t[x] = u[x];
     }
@@ -620,8 +623,7 @@ __global__ __launch_bounds__(1024) void vl_join(const float2* __restrict__ part,
   loss[idx[n]] = in ? (top - tlogit[n]) + logf(sum) : __builtin_nanf("");
 }
 
-// The rows' losses, 0 where they are left out; or their sum, over the count if `mean`, in a
-// fixed order.  One workgroup.
+// The counted rows' losses' sum, over the count if `mean`, in a fixed order.  One workgroup.
 __global__ __launch_bounds__(1024) void vl_total(const float* __restrict__ loss,
                                                  const int* __restrict__ pos,
                                                  const int* __restrict__ count, int N, int mean,
@@ -645,11 +647,6 @@ __global__ __launch_bounds__(1024) void vl_total(const float* __restrict__ loss,
     for (int i = 0; i < 16; ++i) t += s[i];
     *out = (float)(mean ? t / (*count > 0 ? *count : 1) : t);
   }
-}
-__global__ __launch_bounds__(256) void vl_left_out(const int* __restrict__ pos, int N,
-                                                   float* __restrict__ loss) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i < N && pos[i] < 0) loss[i] = 0.f;
 }
 // Upstream gradients of the counted rows, and a factor for all of them.  reduction: 0 each row's
 // own, 1 mean, 2 sum.  The factor is kept out of d: one over the count, rounded to bf16 in every
@@ -945,19 +942,17 @@ int mg_vocab_loss_fwd(int dtype, const void* x, int64_t ldx, const void* w, cons
   float2* const part = (float2*)ws;
   float* const tlogit = (float*)(part + (s.few ? N * few_parts(s) : vl_part_rows(s) * s.np));
   float* const rows = !reduction ? loss : s.few ? tlogit + N : tlogit + s.np + 2 * MAX_PARTS;
+  float* const zero = reduction ? nullptr : loss;
   const auto finish = [&]() {
     if (reduction)
       hipLaunchKernelGGL(vl_total, dim3(1), dim3(1024), 0, stream, rows, t.pos, t.count, (int)N,
                          (int)(reduction == 1), loss);
-    else
-      hipLaunchKernelGGL(vl_left_out, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, stream, t.pos,
-                         (int)N, loss);
     return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
   };
   if (s.few) {
     hipLaunchKernelGGL(vl_few_index, dim3(32 * s.few), dim3(256), 0, stream, target, ignore_index,
                        (int)V, (int)N, (const float*)x, ldx, (int)D, t.idx, t.pos, t.tgt, t.count,
-                       (float*)t.xc, (int)s.dx);
+                       zero, (float*)t.xc, (int)s.dx);
     FewArgs a = few_args(s, t, w, bias);
     a.part = part, a.tlogit = tlogit;
     few_logits<VL_LSE>(s, a, stream);
@@ -966,7 +961,7 @@ int mg_vocab_loss_fwd(int dtype, const void* x, int64_t ldx, const void* w, cons
     return finish();
   }
   hipLaunchKernelGGL(vl_index, dim3(1), dim3(1024), 0, stream, target, ignore_index, V, t.idx,
-                     t.pos, t.tgt, t.count, (int)N);
+                     t.pos, t.tgt, t.count, zero, (int)N);
   float* const top = tlogit + s.np;  // both packings' parts, one after the other
   vl_pack_run(dtype, x, ldx, D, t.xc, s.dx, s.np * s.dx, t.idx, t.count, N, s.np, (int)D, top, t.sx,
               stream);
