@@ -175,7 +175,8 @@ __global__ __launch_bounds__(256) void vl_pack(const E* __restrict__ src, int64_
                                                u16* __restrict__ dst, int ld, int64_t plane,
                                                const int* __restrict__ idx,
                                                const int* __restrict__ count, int64_t rows,
-                                               int ones, const float* __restrict__ top,
+                                               int64_t out_rows, int ones,
+                                               const float* __restrict__ top,
                                                float* __restrict__ scale) {
   float by = 1.f;
   if constexpr (PL == 2) {
@@ -186,23 +187,34 @@ __global__ __launch_bounds__(256) void vl_pack(const E* __restrict__ src, int64_
     by = scale_of(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])));
     if (blockIdx.x == 0 && threadIdx.x == 0) *scale = by;
   }
-  const int64_t j = blockIdx.x;
+  // A wave a row, four elements a lane.
+  typedef E E4 __attribute__((ext_vector_type(4), aligned(sizeof(E))));
+  const int64_t j = blockIdx.x * 4ll + (threadIdx.x >> 6);
   const int64_t n = count ? *count : rows;
-  if (j >= (n + PADK - 1) / PADK * PADK) return;
+  if (j >= (n + PADK - 1) / PADK * PADK || j >= out_rows) return;
   const bool live = j < n;
   const E* s = src + (live ? (idx ? (int64_t)idx[j] : j) * lds_ : 0);
-  for (int c = threadIdx.x * 2; c < ld; c += 512) {
-    float x = live && c < cols ? to_f(s[c]) * by : 0.f;
-    float y = live && c + 1 < cols ? to_f(s[c + 1]) * by : 0.f;
-    if (live && c == ones) x = PL == 2 ? ONE_SCALE : 1.f;
-    if (live && c + 1 == ones) y = PL == 2 ? ONE_SCALE : 1.f;
-    unsigned* const to = reinterpret_cast<unsigned*>(dst + j * ld + c);
+  for (int c = (threadIdx.x & 63) * 4; c < ld; c += 256) {
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (live && c + 4 <= cols) {
+      const E4 y = *reinterpret_cast<const E4*>(s + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = to_f(y[e]) * by;
+    } else if (live) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (c + e < cols) x[e] = to_f(s[c + e]) * by;
+        if (c + e == ones) x[e] = PL == 2 ? ONE_SCALE : 1.f;
+      }
+    }
+    u16* const to = dst + j * ld + c;
     if constexpr (PL == 1) {
-      *to = pack2(x, y);
+      *reinterpret_cast<uint2*>(to) = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
     } else {
-      const unsigned hi = pack2h(x, y);
-      *to = hi;
-      *reinterpret_cast<unsigned*>(dst + plane + j * ld + c) = pack2h(rest(x, hi, 0), rest(y, hi, 1));
+      const unsigned a = pack2h(x[0], x[1]), b = pack2h(x[2], x[3]);
+      *reinterpret_cast<uint2*>(to) = make_uint2(a, b);
+      *reinterpret_cast<uint2*>(to + plane) = make_uint2(pack2h(rest(x[0], a, 0), rest(x[1], a, 1)),
+                                                         pack2h(rest(x[2], b, 0), rest(x[3], b, 1)));
     }
   }
 }
@@ -892,19 +904,19 @@ VlArgs vl_logits(const Shape& s, const State& t, const void* w, const void* bias
 int64_t vl_part_rows(const Shape& s) { return 2 * ((s.V + TM - 1) / TM); }
 
 void vl_pack_run(int dtype, const void* src, int64_t ld, int64_t cols, u16* dst, int64_t dld,
-                 int64_t plane, const int* idx, const int* count, int64_t rows, int64_t grid,
-                 int ones, float* top, float* scale, hipStream_t stream) {
+                 int64_t plane, const int* idx, const int* count, int64_t rows,
+                 int64_t out_rows, int ones, float* top, float* scale, hipStream_t stream) {
+  const dim3 grid((unsigned)((out_rows + 3) / 4));
   if (dtype) {
-    hipLaunchKernelGGL((vl_pack<u16, 1>), dim3((unsigned)grid), dim3(256), 0, stream,
-                       (const u16*)src, ld, (int)cols, dst, (int)dld, plane, idx, count, rows, ones,
+    hipLaunchKernelGGL((vl_pack<u16, 1>), grid, dim3(256), 0, stream, (const u16*)src, ld,
+                       (int)cols, dst, (int)dld, plane, idx, count, rows, out_rows, ones,
                        (const float*)nullptr, (float*)nullptr);
     return;
   }
   hipLaunchKernelGGL(vl_absmax, dim3(MAX_PARTS), dim3(1024), 0, stream, (const float*)src, ld, cols,
                      (int64_t)1 << 62, idx, count, rows, top);
-  hipLaunchKernelGGL((vl_pack<float, 2>), dim3((unsigned)grid), dim3(256), 0, stream,
-                     (const float*)src, ld, (int)cols, dst, (int)dld, plane, idx, count, rows, ones,
-                     top, scale);
+  hipLaunchKernelGGL((vl_pack<float, 2>), grid, dim3(256), 0, stream, (const float*)src, ld,
+                     (int)cols, dst, (int)dld, plane, idx, count, rows, out_rows, ones, top, scale);
 }
 
 }  // namespace
