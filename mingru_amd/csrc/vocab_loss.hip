@@ -642,12 +642,17 @@ __global__ __launch_bounds__(1024) void vl_total(const float* __restrict__ loss,
                                                  float* __restrict__ out) {
   __shared__ double s[16];
   double a[4] = {0.0, 0.0, 0.0, 0.0};
+  // Both loads of all four rows go out before a sum; a left-out row's loss is whatever lies there.
   for (int i = threadIdx.x; i < N; i += 4096) {
+    float v[4];
+    int p[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int x = i + u * 1024;
-      if (x < N && pos[x] >= 0) a[u] += (double)loss[x];
+      const int x = i + u * 1024 < N ? i + u * 1024 : i;
+      v[u] = loss[x], p[u] = i + u * 1024 < N ? pos[x] : -1;
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) a[u] += p[u] >= 0 ? (double)v[u] : 0.0;
   }
   double t = (a[0] + a[1]) + (a[2] + a[3]);
 #pragma unroll
