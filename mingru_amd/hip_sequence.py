@@ -3,7 +3,7 @@
 Same manners as :mod:`mingru_amd.hip_scans`: ``*_impl`` functions take the public
 function's checked arguments, run on torch's current stream with outputs and workspaces
 from torch's caching allocator, differentiate through ``torch.autograd.Function`` wrappers
-(no double backward), and raise ``ScanFallback`` for a call they decline.
+(no double backward, no forward mode), and raise ``ScanFallback`` for a call they decline.
 """
 
 from __future__ import annotations
@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .hip_scans import (
@@ -44,6 +45,15 @@ def _half_to_float(*ts):
             t = t.float()
         out.append(t)
     return out
+
+
+def _no_tangents(what, *ts):
+    """Declines inputs with a forward-mode tangent: the native calls read the primals alone, and
+    an output without a tangent counts as a constant."""
+    # Outside of every dual level (-1), where nothing has a tangent, nothing is looked at.
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise ScanFallback(f"{what} kernels have no forward-mode derivatives")
 
 
 # ---------------------------------------------------------------------------
@@ -147,6 +157,7 @@ class _ResidualNormFn(torch.autograd.Function):
 def residual_norm_impl(h, x, gate, scale, post_w, post_b, pre_w, pre_b, post, act, pre, number,
                        eps):
     """``residual_norm`` on checked arguments (``number``: the scale where ``scale`` is None)."""
+    _no_tangents("residual_norm", h, x, gate, scale, post_w, post_b, pre_w, pre_b)
     if h.shape[-1] > _NORM_MAX_D:
         raise ScanFallback(f"residual_norm kernels hold rows of at most {_NORM_MAX_D} elements "
                            f"(got {h.shape[-1]})")
@@ -244,6 +255,7 @@ class _LinearAttentionFn(torch.autograd.Function):
 
 def linear_attention_impl(q, k, v, g, h0, lengths, scale):
     """``linear_attention`` on checked arguments of one type."""
+    _no_tangents("linear_attention", q, k, v, g, h0)
     if max(q.shape[-1], v.shape[-1]) > _ATTENTION_MAX_D:
         raise ScanFallback(f"linear_attention kernels take head sizes up to {_ATTENTION_MAX_D} "
                            f"(got {q.shape[-1]} and {v.shape[-1]})")
@@ -264,6 +276,7 @@ def linear_attention_impl(q, k, v, g, h0, lengths, scale):
 
 def linear_attention_step_impl(q, k, v, g, h, scale):
     """``linear_attention_step`` on checked arguments of one type."""
+    _no_tangents("linear_attention_step", q, k, v, g, h)
     dtype = q.dtype
     q, k, v, g, h = _half_to_float(q, k, v, g, h)
     q, k, v = (_last_dense(t) for t in (q, k, v))
@@ -331,6 +344,7 @@ class _VocabLossFn(torch.autograd.Function):
 
 def linear_cross_entropy_impl(x, weight, target, bias, ignore_index, reduction):
     """``linear_cross_entropy`` on checked arguments of one type."""
+    _no_tangents("linear_cross_entropy", x, weight, bias)
     x, weight, bias = _half_to_float(x, weight, bias)
     N, (V, D) = target.numel(), weight.shape
     if not _size("mg_vocab_loss_state_bytes", _DTYPE_TAG[x.dtype], N, V, D):
