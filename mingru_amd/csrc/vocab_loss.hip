@@ -10,7 +10,9 @@
 // Forward: one product whose epilogue keeps, for each row and 128 columns of the vocabulary,
 // the largest logit and the sum of exponentials against it, and the target's logit; a second
 // launch joins them.  Backward, in pieces of the vocabulary: the product again, whose epilogue
-// turns the logits into d; then dx's share and dW's piece as products over d.  So 8 N V D
+// turns the logits into d; then dW's piece and dx's share as products over d, the latter added
+// to what the pieces before left, in order, so that memory holds a piece of d and one dx (or a
+// few, where the contracted axis is split) however many pieces there are.  So 8 N V D
 // operations in place of 6 with kept logits: at D = 1024 a logit's recomputation costs less
 // than writing and reading it in fp32.
 //
@@ -252,6 +254,7 @@ struct VlArgs {
   void* extra;             // column m_out in a vector of its own
   const float* scale;      // of every element, on the device
   int out_f32;
+  int add;                 // fp32: out += the product
   int64_t pe;              // extra: elements between the splits'
 };
 
@@ -577,13 +580,19 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) v[x] = scale * acc[i][j][4 * q + x];
           if (m + 4 <= a.m_out && (a.ldo & 3) == 0) {
-            if (f32) *reinterpret_cast<float4*>((float*)a.out + row + m) = make_float4(v[0], v[1], v[2], v[3]);
-            else *reinterpret_cast<uint2*>((u16*)a.out + row + m) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+            if (f32) {
+              float4* const to = reinterpret_cast<float4*>((float*)a.out + row + m);
+              if (a.add) {
+                const float4 y = *to;
+                v[0] += y.x, v[1] += y.y, v[2] += y.z, v[3] += y.w;
+              }
+              *to = make_float4(v[0], v[1], v[2], v[3]);
+            } else *reinterpret_cast<uint2*>((u16*)a.out + row + m) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
           } else {
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               if (m + x < a.m_out) {
-                if (f32) ((float*)a.out)[row + m + x] = v[x];
+                if (f32) ((float*)a.out)[row + m + x] = a.add ? ((float*)a.out)[row + m + x] + v[x] : v[x];
                 else ((u16*)a.out)[row + m + x] = to_bf(v[x]);
               } else if (m + x == a.m_out && a.extra) {
                 const float e = scale1 * acc[i][j][4 * q + x];
@@ -866,7 +875,7 @@ Back vl_back(const Shape& s, void* base) {
   b.scale = (float*)take(4), b.d_scale = (float*)take(4);
   b.top = (float*)take(MAX_PARTS * 4);
   b.d = (u16*)take(s.planes * s.np * b.vp * 2);
-  b.dx_part = (float*)take(b.pieces * b.dx_splits * s.N * s.D * 4);
+  b.dx_part = (float*)take(b.dx_splits * s.N * s.D * 4);  // pieces add to it one after another
   b.dw_part = b.dw_splits > 1 ? (float*)take(b.dw_splits * b.vp * s.D * 4) : nullptr;
   b.db_part = b.dw_splits > 1 ? (float*)take(b.dw_splits * b.vp * 4) : nullptr;
   b.bytes = p - (char*)base;
@@ -1024,7 +1033,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
                        top);
   hipLaunchKernelGGL(vl_upstream, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, stream, dloss,
                      t.idx, t.count, reduction, top, b.g, b.scale, b.d_scale);
-  for (int64_t v0 = 0, piece = 0; v0 < V; v0 += b.vp, ++piece) {
+  for (int64_t v0 = 0; v0 < V; v0 += b.vp) {
     const int64_t cols = V - v0 < b.vp ? V - v0 : b.vp, kc = up_to(cols, PADK);
     VlArgs a = vl_logits(s, t, w, bias, v0, cols);
     a.soft = t.soft, a.g = b.g;
@@ -1037,7 +1046,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
       c.B = b.d, c.ldb = (int)kc, c.pb = a.pd, c.n_count = t.count;
       c.K = (int)kc, c.ka = (int)cols;
       c.mt = (int)((D + TM - 1) / TM), c.nt = (int)((s.np + TN - 1) / TN), c.splits = b.dx_splits;
-      c.out = b.dx_part + piece * b.dx_splits * N * D;
+      c.out = b.dx_part, c.add = v0 > 0;
       c.ldo = D, c.po = N * D, c.m_out = (int)D, c.n_out = (int)N, c.out_f32 = 1, c.scale = b.scale;
       rc = vl_run<VL_OUT, true, false>(dtype, c, stream);
     }
@@ -1078,13 +1087,12 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
   }
   if (dx) {
     const int64_t n = N * D;
-    const int parts = (int)(b.pieces * b.dx_splits);
     const dim3 grid((unsigned)((n / 4 + 256) / 256));
     if (dtype)
-      hipLaunchKernelGGL(vl_sum<u16>, grid, dim3(256), 0, stream, b.dx_part, n, parts, t.pos, n,
+      hipLaunchKernelGGL(vl_sum<u16>, grid, dim3(256), 0, stream, b.dx_part, n, b.dx_splits, t.pos, n,
                          (int)D, (u16*)dx);
     else
-      hipLaunchKernelGGL(vl_sum<float>, grid, dim3(256), 0, stream, b.dx_part, n, parts, t.pos, n,
+      hipLaunchKernelGGL(vl_sum<float>, grid, dim3(256), 0, stream, b.dx_part, n, b.dx_splits, t.pos, n,
                          (int)D, (float*)dx);
   }
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
