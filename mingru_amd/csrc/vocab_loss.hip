@@ -29,8 +29,8 @@
 // the largest, then fewer, to 2^-39 of it: an error of the logits far below what fp32 sums
 // leave.  A product takes the three pairs hi hi, hi lo, lo hi: three times the work of bf16,
 // against sixteen times for fp32's own matrix instruction and six for three bf16 planes (24
-// bits at any size; 2047 x 10007 x 392 took 575 us with them, 365 with these).  d, in -1 .. 1, is
-// scaled by 2^15.
+// bits at any size; 2047 x 10007 x 392 took 575 us with them, 365 with these).  d, in -1 .. 1
+// without its upstream gradient, is scaled by 2^15.
 // bf16 inputs: d, without the factor of a mean, is rounded to bf16 once; sums are fp32.
 // Up to 128 fp32 rows take vocab_few.h's kernels.
 // With a bias, x has a column of ones behind its own, which makes db one more column of dW.
@@ -138,11 +138,9 @@ __global__ __launch_bounds__(1024) void vl_index(const int64_t* __restrict__ tar
   if (tid == 0) *count = base;
 }
 
-// The largest finite magnitude of the (counted) rows, in MAX_PARTS parts; of src's first `most`
-// elements at most.
+// The largest finite magnitude of the (counted) rows, in MAX_PARTS parts.
 __global__ __launch_bounds__(1024) void vl_absmax(const float* __restrict__ src, int64_t ld,
-                                                 int64_t cols, int64_t most,
-                                                 const int* __restrict__ idx,
+                                                 int64_t cols, const int* __restrict__ idx,
                                                  const int* __restrict__ count, int64_t rows,
                                                  float* __restrict__ part) {
   __shared__ float s[16];
@@ -151,9 +149,8 @@ __global__ __launch_bounds__(1024) void vl_absmax(const float* __restrict__ src,
   float top = 0.f;
   for (int64_t j = blockIdx.x * 16 + w; j < n; j += MAX_PARTS * 16) {
     const int64_t at = (idx ? (int64_t)idx[j] : j) * ld;
-    const int64_t end = cols < most - at ? cols : most - at;
 #pragma unroll 4
-    for (int64_t c = lane; c < end; c += 64) {
+    for (int64_t c = lane; c < cols; c += 64) {
       const float x = fabsf(src[at + c]);
       top = x < INFINITY ? fmaxf(top, x) : top;
     }
@@ -565,7 +562,8 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
   }
   if constexpr (EPI == VL_OUT) {
     const bool f32 = a.out_f32;
-    const float scale = *a.scale * unit, scale1 = PL == 2 ? *a.scale / (ONE_SCALE * *a.sb) : *a.scale;
+    // Apart from `unit`, which brings the sums to their size: their product may be below what fp32 holds.
+    const float scale = *a.scale, unit1 = PL == 2 ? 1.f / (ONE_SCALE * *a.sb) : 1.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int n = nw + 32 * j;
@@ -578,7 +576,7 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
           const int m = mw + 32 * i + 8 * q;
           float v[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) v[x] = scale * acc[i][j][4 * q + x];
+          for (int x = 0; x < 4; ++x) v[x] = scale * (unit * acc[i][j][4 * q + x]);
           if (m + 4 <= a.m_out && (a.ldo & 3) == 0) {
             if (f32) {
               float4* const to = reinterpret_cast<float4*>((float*)a.out + row + m);
@@ -595,7 +593,7 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
                 if (f32) ((float*)a.out)[row + m + x] = a.add ? ((float*)a.out)[row + m + x] + v[x] : v[x];
                 else ((u16*)a.out)[row + m + x] = to_bf(v[x]);
               } else if (m + x == a.m_out && a.extra) {
-                const float e = scale1 * acc[i][j][4 * q + x];
+                const float e = scale * (unit1 * acc[i][j][4 * q + x]);
                 if (f32) ((float*)a.extra)[split * a.pe + n] = e;
                 else ((u16*)a.extra)[n] = to_bf(e);
               }
@@ -674,41 +672,118 @@ __global__ __launch_bounds__(1024) void vl_total(const float* __restrict__ loss,
     *out = (float)(mean ? t / (*count > 0 ? *count : 1) : t);
   }
 }
-// Upstream gradients of the counted rows, and a factor for all of them.  reduction: 0 each row's
-// own, 1 mean, 2 sum.  The factor is kept out of d: one over the count, rounded to bf16 in every
-// row's largest entry (the target's), would put all gradients off by the same 2^-9.
-// top (fp16 planes): g gets d's scale; rows' own gradients, whose largest magnitude it has, are
-// brought to 1/2 .. 1 first.  Both together are written to d_scale.
+// What d is multiplied by in its epilogue (g), and factors for all of it.  reduction: 0 each row's
+// own, 1 mean, 2 sum.  A factor for all is kept out of d: one over the count, rounded to bf16 in
+// every row's largest entry (the target's), would put all gradients off by the same 2^-9.
+// fp16 planes (d_scale not null) hold d without any upstream gradient, times D_SCALE: a row of
+// small weight would lose its bits beside one of large weight.  dx's rows are multiplied by their
+// own where they are summed, and dW's product takes x's rows times `weight`, the upstream gradients
+// over the power of two w_scale, whose largest (top: of the counted rows) is 1/2 .. 1 (.. 2 at the
+// type's end).
 __global__ __launch_bounds__(256) void vl_upstream(const float* __restrict__ up,
                                                    const int* __restrict__ idx,
                                                    const int* __restrict__ count, int reduction,
                                                    const float* __restrict__ top,
-                                                   float* __restrict__ g,
+                                                   float* __restrict__ g, float* __restrict__ weight,
                                                    float* __restrict__ scale,
+                                                   float* __restrict__ w_scale,
                                                    float* __restrict__ d_scale) {
   const int j = blockIdx.x * 256 + threadIdx.x, n = *count;
-  float by = 1.f;
+  int e = 0;
   if (top) {
-    by = D_SCALE;
-    if (reduction == 0) {
-      __shared__ float s[4];
-      const float t = wave_max(top[threadIdx.x]);
-      if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = t;
-      __syncthreads();
-      by = scale_of(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
-    }
+    __shared__ float s[4];
+    const float t = wave_max(top[threadIdx.x]);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = t;
+    __syncthreads();
+    frexpf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), &e);
+    if (e > 127) e = 127;
   }
   if (j == 0) {
     *scale = reduction == 0 ? 1.f : reduction == 1 ? up[0] / (float)(n > 0 ? n : 1) : up[0];
-    *d_scale = by;
+    *w_scale = top ? ldexpf(1.f, e) : *scale;
+    if (d_scale) *d_scale = D_SCALE;
   }
-  if (j < n) g[j] = (reduction == 0 ? up[idx[j]] : 1.f) * by;
+  if (j >= n) return;
+  g[j] = d_scale ? D_SCALE : reduction == 0 ? up[idx[j]] : 1.f;
+  if (top) weight[j] = ldexpf(up[idx[j]], -e);
 }
-// out[i][c] = sum of the parts' rows, pos[i] if given (0 where that is negative).
+
+// Packed rows in two planes, scaled by *sx, times their weights: the largest finite magnitude in
+// MAX_PARTS parts (of the high plane: 2^-11 of it off at most, and a plane holds twice what its
+// scale makes of it), then in two planes with a scale of their own.  The column of ones becomes the
+// weights, times ONE_SCALE.
+__device__ __forceinline__ void vl_halves(uint2 u, float (&x)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = (float)__builtin_bit_cast(f16x2, e < 2 ? u.x : u.y)[e & 1];
+}
+__global__ __launch_bounds__(1024) void vl_weigh_top(const u16* __restrict__ x, int ld, int cols,
+                                                    const float* __restrict__ weight,
+                                                    const float* __restrict__ sx,
+                                                    const int* __restrict__ count,
+                                                    float* __restrict__ part) {
+  __shared__ float s[16];
+  const int n = *count, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  float top = 0.f;
+  for (int j = blockIdx.x * 16 + w; j < n; j += MAX_PARTS * 16) {
+    const float by = weight[j] / *sx;
+#pragma unroll 4
+    for (int c = lane * 4; c < cols; c += 256) {
+      float v[4];
+      vl_halves(*reinterpret_cast<const uint2*>(x + (int64_t)j * ld + c), v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float y = fabsf(v[e] * by);
+        top = c + e < cols && y < INFINITY ? fmaxf(top, y) : top;
+      }
+    }
+  }
+  top = wave_max(top);
+  if (lane == 0) s[w] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+    part[blockIdx.x] = top;
+  }
+}
+__global__ __launch_bounds__(256) void vl_weigh(const u16* __restrict__ x, u16* __restrict__ to,
+                                                int ld, int64_t plane, int cols,
+                                                const float* __restrict__ weight,
+                                                const float* __restrict__ sx,
+                                                const int* __restrict__ count,
+                                                const float* __restrict__ top,
+                                                float* __restrict__ scale) {
+  __shared__ float s_top[4];
+  const float t = wave_max(top[threadIdx.x]);
+  if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = t;
+  __syncthreads();
+  const float by = scale_of(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])));
+  if (blockIdx.x == 0 && threadIdx.x == 0) *scale = by;
+  const int64_t j = blockIdx.x * 4ll + (threadIdx.x >> 6);
+  const int n = *count;
+  if (j >= (n + PADK - 1) / PADK * PADK) return;
+  const float g = j < n ? weight[j] : 0.f, f = j < n ? g / *sx : 0.f;
+  for (int c = (threadIdx.x & 63) * 4; c < ld; c += 256) {
+    const u16* const p = x + j * ld + c;
+    float hi[4], lo[4], y[4];
+    vl_halves(*reinterpret_cast<const uint2*>(p), hi);
+    vl_halves(*reinterpret_cast<const uint2*>(p + plane), lo);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      y[e] = c + e < cols ? (hi[e] + lo[e]) * f * by : c + e == cols ? g * ONE_SCALE : 0.f;
+    const unsigned a = pack2h(y[0], y[1]), b = pack2h(y[2], y[3]);
+    u16* const q = to + j * ld + c;
+    *reinterpret_cast<uint2*>(q) = make_uint2(a, b);
+    *reinterpret_cast<uint2*>(q + plane) = make_uint2(pack2h(rest(y[0], a, 0), rest(y[1], a, 1)),
+                                                      pack2h(rest(y[2], b, 0), rest(y[3], b, 1)));
+  }
+}
+// out[i][c] = sum of the parts' rows, pos[i] if given (0 where that is negative), times by[i] if given.
 template <typename E>
 __global__ __launch_bounds__(256) void vl_sum(const float* __restrict__ part, int64_t po,
                                               int parts, const int* __restrict__ pos, int64_t n,
-                                              int cols, E* __restrict__ out) {
+                                              int cols, const float* __restrict__ by,
+                                              E* __restrict__ out) {
   const int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (x >= n) return;
   if ((cols & 3) == 0) {
@@ -720,6 +795,7 @@ __global__ __launch_bounds__(256) void vl_sum(const float* __restrict__ part, in
         const float4 v = *reinterpret_cast<const float4*>(part + p * po + j * cols + x % cols);
         s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
       }
+    if (by && j >= 0) s.x *= by[i], s.y *= by[i], s.z *= by[i], s.w *= by[i];
     if constexpr (sizeof(E) == 4) *reinterpret_cast<float4*>(out + x) = s;
     else *reinterpret_cast<uint2*>(out + x) = make_uint2(pack2(s.x, s.y), pack2(s.z, s.w));
     return;
@@ -729,6 +805,7 @@ __global__ __launch_bounds__(256) void vl_sum(const float* __restrict__ part, in
     float s = 0.f;
     if (j >= 0)
       for (int p = 0; p < parts; ++p) s += part[p * po + j * cols + y % cols];
+    if (by && j >= 0) s *= by[i];
     if constexpr (sizeof(E) == 4) out[y] = s;
     else out[y] = to_bf(s);
   }
@@ -846,8 +923,8 @@ int vl_splits(int64_t tiles, int64_t steps, int64_t size) {
 struct Back {
   int64_t vp, pieces;   // columns of a piece
   int dx_splits, dw_splits;
-  float *g, *scale, *d_scale, *top, *dx_part, *dw_part, *db_part;
-  u16* d;
+  float *g, *scale, *w_scale, *d_scale, *top, *weight, *sxw, *dx_part, *dw_part, *db_part;
+  u16 *d, *xw;  // xw: x's packed rows times their weights
   size_t bytes;
 };
 Back vl_back(const Shape& s, void* base) {
@@ -872,9 +949,13 @@ Back vl_back(const Shape& s, void* base) {
     return at;
   };
   b.g = (float*)take(s.N * 4);
-  b.scale = (float*)take(4), b.d_scale = (float*)take(4);
+  b.scale = (float*)take(4), b.w_scale = (float*)take(4), b.d_scale = (float*)take(4);
   b.top = (float*)take(MAX_PARTS * 4);
   b.d = (u16*)take(s.planes * s.np * b.vp * 2);
+  if (s.planes == 2) {
+    b.weight = (float*)take(s.N * 4), b.sxw = (float*)take(4);
+    b.xw = (u16*)take(s.planes * s.np * s.dx * 2);
+  }
   b.dx_part = (float*)take(b.dx_splits * s.N * s.D * 4);  // pieces add to it one after another
   b.dw_part = b.dw_splits > 1 ? (float*)take(b.dw_splits * b.vp * s.D * 4) : nullptr;
   b.db_part = b.dw_splits > 1 ? (float*)take(b.dw_splits * b.vp * 4) : nullptr;
@@ -928,7 +1009,7 @@ void vl_pack_run(int dtype, const void* src, int64_t ld, int64_t cols, u16* dst,
     return;
   }
   hipLaunchKernelGGL(vl_absmax, dim3(MAX_PARTS), dim3(1024), 0, stream, (const float*)src, ld, cols,
-                     (int64_t)1 << 62, idx, count, rows, top);
+                     idx, count, rows, top);
   hipLaunchKernelGGL((vl_pack<float, 2>), grid, dim3(256), 0, stream, (const float*)src, ld,
                      (int)cols, dst, (int)dld, plane, idx, count, rows, out_rows, ones, top, scale);
 }
@@ -1022,17 +1103,24 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
     if (dx)
       hipLaunchKernelGGL(vl_sum<float>, dim3((unsigned)((N * D / 4 + 256) / 256)), dim3(256), 0, stream,
                          b.dx_part, N * D, (int)((V + few_per(s) - 1) / few_per(s)), t.pos, N * D,
-                         (int)D, (float*)dx);
+                         (int)D, (const float*)nullptr, (float*)dx);
     return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
   }
   const int e = dtype ? 2 : 4;
-  float* const top = dtype ? nullptr : b.top;
-  if (top && reduction == 0)
-    hipLaunchKernelGGL(vl_absmax, dim3(MAX_PARTS), dim3(1024), 0, stream, dloss, (int64_t)256,
-                       (int64_t)256, N, (const int*)nullptr, (const int*)nullptr, (N + 255) / 256,
-                       top);
+  const bool weighted = !dtype && reduction == 0;
+  float* const top = weighted ? b.top : nullptr;
+  if (weighted)
+    hipLaunchKernelGGL(vl_absmax, dim3(MAX_PARTS), dim3(1024), 0, stream, dloss, (int64_t)1,
+                       (int64_t)1, t.idx, t.count, N, top);
   hipLaunchKernelGGL(vl_upstream, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, stream, dloss,
-                     t.idx, t.count, reduction, top, b.g, b.scale, b.d_scale);
+                     t.idx, t.count, reduction, top, b.g, b.weight, b.scale, b.w_scale,
+                     dtype ? nullptr : b.d_scale);
+  if (weighted && dw) {
+    hipLaunchKernelGGL(vl_weigh_top, dim3(MAX_PARTS), dim3(1024), 0, stream, t.xc, (int)s.dx, (int)D,
+                       b.weight, t.sx, t.count, top);
+    hipLaunchKernelGGL(vl_weigh, dim3((unsigned)((s.np + 3) / 4)), dim3(256), 0, stream, t.xc, b.xw,
+                       (int)s.dx, s.np * s.dx, (int)D, b.weight, t.sx, t.count, top, b.sxw);
+  }
   for (int64_t v0 = 0; v0 < V; v0 += b.vp) {
     const int64_t cols = V - v0 < b.vp ? V - v0 : b.vp, kc = up_to(cols, PADK);
     VlArgs a = vl_logits(s, t, w, bias, v0, cols);
@@ -1052,13 +1140,13 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
     }
     if (rc == MG_OK && dw) {
       VlArgs c = {};
-      c.A = t.xc, c.lda = (int)s.dx, c.pa = s.np * s.dx, c.m_rows = (int)s.dx;
-      c.sa = t.sx, c.sb = b.d_scale;
+      c.A = weighted ? b.xw : t.xc, c.lda = (int)s.dx, c.pa = s.np * s.dx, c.m_rows = (int)s.dx;
+      c.sa = weighted ? b.sxw : t.sx, c.sb = b.d_scale;
       c.B = b.d, c.ldb = (int)kc, c.pb = a.pd, c.n_rows = (int)kc;
       c.k_count = t.count, c.ka = 1 << 30;
       c.mt = (int)((D + (db ? 1 : 0) + TM - 1) / TM), c.nt = (int)((cols + TN - 1) / TN);
       c.splits = b.dw_splits;
-      c.ldo = D, c.m_out = (int)D, c.n_out = (int)cols, c.scale = b.scale;
+      c.ldo = D, c.m_out = (int)D, c.n_out = (int)cols, c.scale = b.w_scale;
       void* const to = (char*)dw + v0 * D * e;
       void* const to_b = db ? (char*)db + v0 * e : nullptr;
       if (b.dw_splits > 1) {
@@ -1076,10 +1164,11 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
           const dim3 grid((unsigned)((n / 4 + 256) / 256));
           if (dtype)
             hipLaunchKernelGGL(vl_sum<u16>, grid, dim3(256), 0, stream, from, n, b.dw_splits,
-                               (const int*)nullptr, n, wide, (u16*)(k ? to_b : to));
+                               (const int*)nullptr, n, wide, (const float*)nullptr, (u16*)(k ? to_b : to));
           else
             hipLaunchKernelGGL(vl_sum<float>, grid, dim3(256), 0, stream, from, n, b.dw_splits,
-                               (const int*)nullptr, n, wide, (float*)(k ? to_b : to));
+                               (const int*)nullptr, n, wide, (const float*)nullptr,
+                               (float*)(k ? to_b : to));
         }
       }
     }
@@ -1090,10 +1179,10 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
     const dim3 grid((unsigned)((n / 4 + 256) / 256));
     if (dtype)
       hipLaunchKernelGGL(vl_sum<u16>, grid, dim3(256), 0, stream, b.dx_part, n, b.dx_splits, t.pos, n,
-                         (int)D, (u16*)dx);
+                         (int)D, (const float*)nullptr, (u16*)dx);
     else
       hipLaunchKernelGGL(vl_sum<float>, grid, dim3(256), 0, stream, b.dx_part, n, b.dx_splits, t.pos, n,
-                         (int)D, (float*)dx);
+                         (int)D, weighted ? dloss : nullptr, (float*)dx);
   }
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
