@@ -23,7 +23,9 @@
 //   e_i = sum_{j<i} X_ij - sum_{j>i} X_ji + q_i.dq_i^inter - k_i.dk_i^inter,
 //   X_ij = scale D_ij (q_i.k_j)(do_i.v_j),
 // the diagonal cancelling exactly, and dg_t = sum_{i>=t} e_i + <R_end, S_end> over a segment,
-// so that what cancels in the sum is never longer than a segment.
+// so that what cancels in the sum is never longer than a segment.  Past the next step that starts
+// over all of it cancels but for rounding, so there the sum ends, without <R_end, S_end>: a
+// document's gradient holds nothing of the ones behind it.
 //
 // Split.  A workgroup of 8 waves walks over the chunks of one (batch, head, segment) with the
 // state in its registers (32 a lane at dk = dv = 128): the state never goes through memory
@@ -864,8 +866,8 @@ __global__ __launch_bounds__(256) void la_join(const float* __restrict__ first,
   }
 }
 
-// e: the queries' side less the keys'.  dg_t = sum of e from t to its segment's end + <R, S> there; 0 past a sequence's length and
-// at steps that start over.
+// e: the queries' side less the keys'.  dg_t = sum of e from t up to the next step that starts over,
+// or to its segment's end + <R, S> there; 0 past a sequence's length and at steps that start over.
 // A workgroup of 16 waves takes a segment: at fewer the product's loads wait for one another
 // (4 waves: 35 us at 128 heads of 2048 tokens, 16: 9).
 constexpr int DG_NT = 1024, DG_W = DG_NT / MG_WAVE;
@@ -875,6 +877,7 @@ __global__ __launch_bounds__(DG_NT) void la_decay_grad(LaArgs a, const float* st
                                                        float* __restrict__ dg, int C) {
   __shared__ double s_e[DG_W];
   __shared__ float s_t[DG_W];
+  __shared__ int s_over[DG_W];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, seg = blockIdx.y;
   const int64_t bh = blockIdx.x;
   const int ss = a.dk * a.dv;
@@ -908,19 +911,25 @@ __global__ __launch_bounds__(DG_NT) void la_decay_grad(LaArgs a, const float* st
     const int64_t t = hi - DG_NT + tid;
     const float e = t >= t0 ? a.e[bh * a.T + t] - keys[bh * a.T + t] : 0.f;
     const float gt = t >= t0 ? g[t * a.gs[1]] : 0.f;
-    const float s = mg_wave_suffix_sum(e);
-    if (lane == 0) s_t[w] = s;
-    __syncthreads();
-    double later = E;
+    const bool over = t >= t0 && t < len && (double)gt * 1.4426950408889634 < -126.0;
+    const uint64_t starts = __ballot(over), after = lane < 63 ? starts >> (lane + 1) : 0;
+    const int end = after ? lane + __ffsll((unsigned long long)after) : 64;  // the next start's lane
+    float s = e;  // over the lanes from this one on, up to `end`
 #pragma unroll
-    for (int i = 0; i < DG_W; ++i) {
-      if (i > w) later += (double)s_t[i];
-      E += (double)s_t[i];
+    for (int d = 1; d < 64; d *= 2) {
+      const float y = __shfl_down(s, d);
+      if (lane + d < end) s += y;
     }
-    if (t >= t0) {
-      const bool off = t >= len || (double)gt * 1.4426950408889634 < -126.0;
-      dg[(b * a.T + t) * a.H + h] = off ? 0.f : (float)(later + (double)s);
+    // What a wave adds to the ones before it, and whether anything behind it does.
+    if (lane == 0) s_t[w] = over ? 0.f : s, s_over[w] = starts != 0;
+    __syncthreads();
+    double later = 0.0;
+#pragma unroll
+    for (int i = DG_W - 1; i >= 0; --i) {
+      if (i == w && end == 64) later = E;
+      E = (double)s_t[i] + (s_over[i] ? 0.0 : E);
     }
+    if (t >= t0) dg[(b * a.T + t) * a.H + h] = over || t >= len ? 0.f : (float)(later + (double)s);
     __syncthreads();
   }
 }
