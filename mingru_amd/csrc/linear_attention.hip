@@ -950,7 +950,8 @@ __global__ __launch_bounds__(256) void la_heads_sum(const float* __restrict__ pa
 
 // ---- one token -------------------------------------------------------------------------------
 // A workgroup takes 32 columns of a head's state: 8 lanes of 4 columns, 32 groups of rows.
-// Bound by the read and write of the state.
+// Bound by the read and write of the state.  A step that starts over, by the sweeps' rule, takes
+// nothing from the old state, and does not multiply it by 0: that would keep a NaN or an infinity.
 struct LaStep {
   const void *q, *k, *v;
   const float *g, *h;
@@ -970,7 +971,8 @@ __global__ __launch_bounds__(256) void la_step(LaStep a) {
   const T* q = (const T*)a.q + b * a.qs[0] + kh * a.qs[1];
   const T* k = (const T*)a.k + b * a.ks[0] + kh * a.ks[1];
   const T* v = (const T*)a.v + b * a.vs[0] + h * a.vs[1];
-  const float decay = expf(a.g[b * a.gs[0] + h * a.gs[1]]);
+  const float g = a.g[b * a.gs[0] + h * a.gs[1]], decay = expf(g);
+  const bool over = (double)g * 1.4426950408889634 < -126.0;
   const float* S = a.h + bh * (int64_t)a.dk * dv;
   float* So = a.h_out + bh * (int64_t)a.dk * dv;
   float vv[4], o[4] = {0.f, 0.f, 0.f, 0.f};
@@ -994,7 +996,7 @@ __global__ __launch_bounds__(256) void la_step(LaStep a) {
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      x[i] = decay * x[i] + kr * vv[i];
+      x[i] = (over ? 0.f : decay * x[i]) + kr * vv[i];
       o[i] += qr * x[i];
     }
     if (wide) {

@@ -307,8 +307,10 @@ def linear_attention_step(q_t, k_t, v_t, log_decay_t, h_prev=None, scale=None):
             return out
     rep = H // Hk
     kw, qw = (t.to(g.dtype).repeat_interleave(rep, 1) for t in (k, q))
-    a = torch.where(_over(g), torch.zeros_like(g), g.exp()).expand(B, H)
-    h = a[..., None, None] * h + kw[..., None] * v.to(g.dtype)[..., None, :]
+    # Selected, not multiplied by 0, which would keep what is not finite.
+    kept = torch.where(_over(g).expand(B, H)[..., None, None], torch.zeros_like(h),
+                       g.exp().expand(B, H)[..., None, None] * h)
+    h = kept + kw[..., None] * v.to(g.dtype)[..., None, :]
     return (scale * (qw[..., None, :] @ h)[..., 0, :]).to(q.dtype), h
 
 
