@@ -17,7 +17,9 @@
 // nothing is divided.  The sums G are formed in fp64 and kept as two floats: near pairs deep
 // in a chunk are differences of large sums.  A step whose factor is below the smallest normal
 // float (-inf among them) starts over: steps before and after it are told apart by a count,
-// which keeps the sums finite.
+// which keeps the sums finite.  What comes through the state is left out there, by a product in
+// which 0 times a NaN or an infinity, that a caller's old state may hold, is 0.  (Tokens that are not
+// finite do reach the others of their chunk, through the products' zeros.)
 //
 // Gradient of g.  G_i enters o_i with do_i.o_i and every later use of k_j v_j^T with -k_j.dk_j:
 //   e_i = sum_{j<i} X_ij - sum_{j>i} X_ji + q_i.dq_i^inter - k_i.dk_i^inter,
@@ -342,6 +344,15 @@ __device__ __forceinline__ void store4(float* p, int c, int d, f32x4 x) {
   }
 }
 
+// f x, and 0 where f is 0 whatever x is: v_mul_legacy_f32's own rule, an instruction in place of
+// the two of a selection.
+__device__ float mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
+__device__ __forceinline__ f32x4 times(float f, f32x4 x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = mul_legacy(f, x[i]);
+  return x;
+}
+
 // A chunk's (C, D) block on its way from memory to LDS, 16 bytes a vector; 0 outside the
 // sequence and the d columns.  WIDE: vectors are aligned and lie inside a row or outside it;
 // they are loaded from a place inside the block in any case and cleared when they are used,
@@ -642,7 +653,7 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
 #pragma unroll
       for (int i = 0; i < TS::TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TS::TN; ++j) S[i][j] *= keep;
+        for (int j = 0; j < TS::TN; ++j) S[i][j] = times(keep, S[i][j]);
       take_up<T, TS, C, DV, DK>(S, rows_v, rows_k, weights[n & 1]);
       fall *= keep;
     };
@@ -746,7 +757,7 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
             T* const p = base + (unsigned)i * (unsigned)(a.H * dv);
 #pragma unroll
             for (int m = 0; m < TV::TM; ++m)
-              store4<WIDE>(p, TV::m0(m) + 4 * lg, dv, in[m][j] + f * acv[m][j]);
+              store4<WIDE>(p, TV::m0(m) + 4 * lg, dv, in[m][j] + times(f, acv[m][j]));
           }
         }
       }
@@ -783,7 +794,7 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
 #pragma unroll
           for (int m = 0; m < TK::TM; ++m) {
             const int c = TK::m0(m) + 4 * lg;
-            const f32x4 y = f * ack[m][j], x = get4((REV ? sK : sQ) + place<T, DK>(i, c));
+            const f32x4 y = times(f, ack[m][j]), x = get4((REV ? sK : sQ) + place<T, DK>(i, c));
 #pragma unroll
             for (int u = 0; u < 4; ++u) dot += y[u] * x[u];
             if (i < rows) {
@@ -860,7 +871,7 @@ __global__ __launch_bounds__(256) void la_join(const float* __restrict__ first,
     for (int u = 0; u < 8; ++u) {
       if (i0 + u >= n) break;
       const int64_t seg = bh * n + (rev ? n - 1 - i0 - u : i0 + u);
-      s = f[u] * s + y[u];
+      s = f[u] == 0.f ? y[u] : f[u] * s + y[u];  // a start in between: as the sweeps
       bound[seg * ss + at] = s;
     }
   }

@@ -192,9 +192,14 @@ def _eager_linear_attention(q, k, v, g, h, lengths, scale):
         lower = torch.ones(gc.shape[-1], gc.shape[-1], dtype=torch.bool, device=q.device).tril()
         D = _spans(total, count, lower).to(q.dtype)
         carried = torch.where(count == 0, total.exp(), torch.zeros_like(total)).to(q.dtype)
-        o = carried[..., None] * (qc @ h) + ((qc @ kc.transpose(-1, -2)) * D) @ vc
+        # Past a start the state before is left out, in the gradients too, rather than multiplied
+        # by 0, which would keep what is not finite.
+        over = (count > 0)[..., None]
+        through = (qc.masked_fill(over, 0) @ h).masked_fill(over, 0)
+        o = carried[..., None] * through + ((qc @ kc.transpose(-1, -2)) * D) @ vc
         out.append(scale * o)
-        h = carried[..., -1, None, None] * h + (kc * D[..., -1, :, None]).transpose(-1, -2) @ vc
+        h = (carried[..., -1, None, None] * h.masked_fill(over[..., -1, :, None], 0)
+             + (kc * D[..., -1, :, None]).transpose(-1, -2) @ vc)
     return torch.cat(out, 2).transpose(1, 2), h
 
 
@@ -246,7 +251,7 @@ def linear_attention(q, k, v, log_decay, h_0=None, lengths=None, scale=None):
         ``Hk`` divides ``H``; each query and key head serves ``H / Hk`` heads in a row.
     log_decay : (B, T, H), or (H) for one decay a head
         At most 0.  ``-inf``, and any value whose factor is below the smallest normal float,
-        starts a new document: nothing of the state before is seen after it.
+        starts a new document: nothing of the state before is seen after it, whatever it holds.
     h_0 : (B, H, dk, dv), optional
         The state to start from, 0 by default.
     lengths : (B) integers, optional
