@@ -264,6 +264,12 @@ def linear_attention_impl(q, k, v, g, h0, lengths, scale):
     if h0 is not None:
         h0 = h0.contiguous()
     if lengths is not None:
+        if q.shape[1] >= 2**31:
+            raise ScanFallback(f"linear_attention kernels take lengths below 2^31 (got {q.shape[1]} "
+                               "tokens)")
+        if lengths.dtype.itemsize > 4 or lengths.dtype == torch.uint32:
+            # The type to come holds what matters of them only.
+            lengths = lengths.to(torch.int64).clamp(0, q.shape[1])
         lengths = lengths.to(torch.int32).contiguous()
     if _grad_wanted(q, k, v, g, h0):
         o, h = _funnel("linear_attention", _LinearAttentionFn.apply, q, k, v, g, h0, lengths, scale)
