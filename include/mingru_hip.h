@@ -468,10 +468,10 @@ int mg_residual_norm_bwd(int dtype, int pdtype, int post, int act, int pre, cons
  * No reference kernels (the reference's matrix-state mixer is the delta rule).
  *   S_t = exp(g_t) S_{t-1} + k_t v_t^T;  o_t = scale S_t^T q_t
  * q, k (B, T, Hk, dk), v and o (B, T, H, dv) in dtype (0 fp32, 1 bf16), Hk dividing H; g (log
- * decay, (B, T, H)) and the states (B, H, dk, dv) fp32; 1 <= dk, dv <= 128.  A g whose factor
- * is below the smallest normal float starts the state over.  strides: a host array of element
- * strides (batch, token, head) of q, k, v, g and, for the backward, the output's gradient;
- * their last dimension is dense.  lengths (B) or NULL: tokens of right-padded sequences.  h0
+ * decay, (B, T, H)) and the states (B, H, dk, dv) fp32; 1 <= dk, dv <= 128; fewer than 2^23
+ * pairs B H (2^24 for one token).  A g whose factor is below the smallest normal float starts
+ * the state over.  strides: a host array of element strides (batch, token, head) of q, k, v, g
+ * and, for the backward, the output's gradient; their last dimension is dense.  lengths (B) or NULL: tokens of right-padded sequences.  h0
  * NULL for 0.
  * state: what the forward leaves for the backward (states between the segments of a
  * sequence); needed by the forward in any case.  Backward: dhT NULL for 0, dh0 may be NULL;

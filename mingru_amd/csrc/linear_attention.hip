@@ -882,15 +882,14 @@ __global__ __launch_bounds__(256) void la_join(const float* __restrict__ first,
 // A workgroup of 16 waves takes a segment: at fewer the product's loads wait for one another
 // (4 waves: 35 us at 128 heads of 2048 tokens, 16: 9).
 constexpr int DG_NT = 1024, DG_W = DG_NT / MG_WAVE;
-__global__ __launch_bounds__(DG_NT) void la_decay_grad(LaArgs a, const float* states,
-                                                       const float* adjoints, const float* last_r,
-                                                       const float* __restrict__ keys,
-                                                       float* __restrict__ dg, int C) {
+__device__ __forceinline__ void la_decay_grad_of(const LaArgs& a, const float* states,
+                                                 const float* adjoints, const float* last_r,
+                                                 const float* __restrict__ keys,
+                                                 float* __restrict__ dg, int C, int64_t bh) {
   __shared__ double s_e[DG_W];
   __shared__ float s_t[DG_W];
   __shared__ int s_over[DG_W];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, seg = blockIdx.y;
-  const int64_t bh = blockIdx.x;
   const int ss = a.dk * a.dv;
   const int64_t b = bh / a.H;
   const int h = (int)(bh % a.H);
@@ -945,18 +944,30 @@ __global__ __launch_bounds__(DG_NT) void la_decay_grad(LaArgs a, const float* st
   }
 }
 
+// Pairs past the grid's are taken in turn: a launch has fewer than 2^32 threads.  (The barrier
+// that ends the loop over a segment's tokens, of which each has some, frees the LDS for the next.)
+constexpr int64_t DG_GRID = 1 << 21;
+__global__ __launch_bounds__(DG_NT) void la_decay_grad(LaArgs a, const float* states,
+                                                       const float* adjoints, const float* last_r,
+                                                       const float* __restrict__ keys,
+                                                       float* __restrict__ dg, int C, int64_t BH) {
+  for (int64_t bh = blockIdx.x; bh < BH; bh += gridDim.x)
+    la_decay_grad_of(a, states, adjoints, last_r, keys, dg, C, bh);
+}
+
 // A key head's gradient: the sum over the heads that share it, in order.
+constexpr int64_t SUM_GRID = 1 << 23;  // 2^31 threads of the fewer than 2^32 that a launch can have
 template <typename T>
 __global__ __launch_bounds__(256) void la_heads_sum(const float* __restrict__ part,
                                                     T* __restrict__ out, int64_t n, int group,
                                                     int d) {
-  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (x >= n) return;
-  const float* p = part + x / d * group * d + x % d;
-  float s = 0.f;
-  for (int i = 0; i < group; ++i) s += p[(int64_t)i * d];
-  if constexpr (sizeof(T) == 2) out[x] = __builtin_bit_cast(u16, (__bf16)s);
-  else out[x] = s;
+  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < n; x += SUM_GRID * 256) {
+    const float* p = part + x / d * group * d + x % d;
+    float s = 0.f;
+    for (int i = 0; i < group; ++i) s += p[(int64_t)i * d];
+    if constexpr (sizeof(T) == 2) out[x] = __builtin_bit_cast(u16, (__bf16)s);
+    else out[x] = s;
+  }
 }
 
 // ---- one token -------------------------------------------------------------------------------
@@ -1033,11 +1044,13 @@ __global__ __launch_bounds__(256) void la_step(LaStep a) {
 
 // ---- host ------------------------------------------------------------------------------------
 constexpr int LA_MAXD = 128;
+// Pairs of a sequence and a head, each a workgroup of the sweeps: a launch has fewer than 2^32 threads.
+constexpr int64_t LA_PAIRS = (1ll << 32) / NT;
 
 bool la_ok(int dtype, int64_t B, int64_t T, int H, int Hk, int dk, int dv) {
   return !(dtype & ~1) && B >= 1 && T >= 1 && H >= 1 && Hk >= 1 && H % Hk == 0 && dk >= 1 &&
          dv >= 1 && dk <= LA_MAXD && dv <= LA_MAXD && H <= (1 << 16) &&
-         B * H <= (1ll << 24) && T <= (1ll << 32);
+         B < LA_PAIRS && B * H < LA_PAIRS && T <= (1ll << 32);
 }
 
 struct Plan {
@@ -1129,7 +1142,8 @@ int la_join_run(const float* first, float* bound, const float* decay, int64_t BH
 
 int la_sum_run(int dtype, const float* part, void* out, int64_t n, int group, int d,
                hipStream_t stream) {
-  const dim3 grid((unsigned)((n + 255) / 256));
+  const int64_t blocks = (n + 255) / 256;
+  const dim3 grid((unsigned)(blocks < SUM_GRID ? blocks : SUM_GRID));
   if (dtype)
     hipLaunchKernelGGL(la_heads_sum<u16>, grid, dim3(256), 0, stream, part, (u16*)out, n, group, d);
   else
@@ -1234,8 +1248,9 @@ int mg_linear_attention_bwd(int dtype, const void* q, const void* k, const void*
   if (rc == MG_OK && part) rc = la_sum_run(dtype, part, dk_, B * T * Hk * dk, a.group, dk, stream);
   if (rc != MG_OK) return rc;
   a.first = hT, a.e = queries;
-  hipLaunchKernelGGL(la_decay_grad, dim3((unsigned)BH, (unsigned)p.segs), dim3(DG_NT), 0, stream, a,
-                     (const float*)state, (const float*)adjoints, dhT, keys, dg, p.C);
+  hipLaunchKernelGGL(la_decay_grad, dim3((unsigned)(BH < DG_GRID ? BH : DG_GRID), (unsigned)p.segs),
+                     dim3(DG_NT), 0, stream, a, (const float*)state, (const float*)adjoints, dhT, keys,
+                     dg, p.C, BH);
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
 
@@ -1245,7 +1260,7 @@ int mg_linear_attention_step(int dtype, const void* q, const void* k, const void
                              hipStream_t stream) {
   if (!q || !k || !v || !g || !strides || !h || !o || !h_out || (dtype & ~1) || B < 1 || H < 1 ||
       Hk < 1 || H % Hk || dk < 1 || dv < 1 || dk > (1 << 16) || dv > (1 << 16) || H > (1 << 20) ||
-      B * H > (1ll << 24))
+      B >= (1ll << 24) || B * H >= (1ll << 24))  // 256 threads a pair: fewer than 2^32
     return MG_ERR_ARG;
   LaStep a = {};
   a.q = q, a.k = k, a.v = v, a.g = g, a.h = h, a.o = o, a.h_out = h_out;

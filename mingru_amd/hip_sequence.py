@@ -187,6 +187,7 @@ def residual_norm_impl(h, x, gate, scale, post_w, post_b, pre_w, pre_b, post, ac
 # ---------------------------------------------------------------------------
 
 _ATTENTION_MAX_D = 128
+_STEP_PAIRS = 2**24  # of a sequence and a head; the pass has its limits from the C entry
 
 
 def _last_dense(t):
@@ -261,15 +262,18 @@ def linear_attention_impl(q, k, v, g, h0, lengths, scale):
                            f"(got {q.shape[-1]} and {v.shape[-1]})")
     dtype = q.dtype
     q, k, v, g, h0 = _half_to_float(q, k, v, g, h0)
+    (B, T, Hk, dk), (H, dv) = q.shape, v.shape[2:]
+    if not _size("mg_linear_attention_state_bytes", _DTYPE_TAG[q.dtype], B, T, H, Hk, dk, dv):
+        raise ScanFallback(f"linear_attention kernels take fewer than 2^23 pairs of a sequence and a "
+                           f"head, up to 2^16 heads and 2^32 tokens (got {B} x {H} and {T})")
     if h0 is not None:
         h0 = h0.contiguous()
     if lengths is not None:
-        if q.shape[1] >= 2**31:
-            raise ScanFallback(f"linear_attention kernels take lengths below 2^31 (got {q.shape[1]} "
-                               "tokens)")
+        if T >= 2**31:
+            raise ScanFallback(f"linear_attention kernels take lengths below 2^31 (got {T} tokens)")
         if lengths.dtype.itemsize > 4 or lengths.dtype == torch.uint32:
             # The type to come holds what matters of them only.
-            lengths = lengths.to(torch.int64).clamp(0, q.shape[1])
+            lengths = lengths.to(torch.int64).clamp(0, T)
         lengths = lengths.to(torch.int32).contiguous()
     if _grad_wanted(q, k, v, g, h0):
         o, h = _funnel("linear_attention", _LinearAttentionFn.apply, q, k, v, g, h0, lengths, scale)
@@ -283,11 +287,14 @@ def linear_attention_impl(q, k, v, g, h0, lengths, scale):
 def linear_attention_step_impl(q, k, v, g, h, scale):
     """``linear_attention_step`` on checked arguments of one type."""
     _no_tangents("linear_attention_step", q, k, v, g, h)
+    (B, Hk, dk), (H, dv) = q.shape, v.shape[1:]
+    if B * H >= _STEP_PAIRS:
+        raise ScanFallback(f"linear_attention_step kernels take fewer than 2^24 pairs of a sequence "
+                           f"and a head (got {B} x {H})")
     dtype = q.dtype
     q, k, v, g, h = _half_to_float(q, k, v, g, h)
     q, k, v = (_last_dense(t) for t in (q, k, v))
     h = h.contiguous()
-    (B, Hk, dk), (H, dv) = q.shape, v.shape[1:]
     o = torch.empty(B, H, dv, dtype=q.dtype, device=q.device)
     h_out = torch.empty_like(h)
     strides = (*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *_decay_strides(g, 1))
