@@ -84,6 +84,16 @@ __device__ __forceinline__ float scale_of(float top) {
   return ldexpf(1.f, e < -60 ? -60 : e > 50 ? 50 : e);
 }
 constexpr int MAX_PARTS = 256;
+// A launch has fewer than 2^32 threads, so a kernel that takes a thread, wave or workgroup for each
+// of what a call has many of takes its first workgroup's place among all as well, and more launches
+// follow where one is not enough.
+constexpr int64_t MAX_THREADS = 1ll << 31;
+template <typename F>
+void vl_launches(int64_t blocks, int threads, F&& launch) {
+  const int64_t most = MAX_THREADS / threads;
+  for (int64_t first = 0; first < blocks; first += most)
+    launch(dim3((unsigned)(blocks - first < most ? blocks - first : most)), dim3(threads), first);
+}
 constexpr float ONE_SCALE = 16384.f, D_SCALE = 32768.f;
 
 // ---- packing ----------------------------------------------------------------------------
@@ -176,7 +186,7 @@ __global__ __launch_bounds__(256) void vl_pack(const E* __restrict__ src, int64_
                                                const int* __restrict__ count, int64_t rows,
                                                int64_t out_rows, int ones,
                                                const float* __restrict__ top,
-                                               float* __restrict__ scale) {
+                                               float* __restrict__ scale, int64_t first) {
   float by = 1.f;
   if constexpr (PL == 2) {
     __shared__ float s_top[4];
@@ -184,11 +194,11 @@ __global__ __launch_bounds__(256) void vl_pack(const E* __restrict__ src, int64_
     if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = t;
     __syncthreads();
     by = scale_of(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])));
-    if (blockIdx.x == 0 && threadIdx.x == 0) *scale = by;
+    if (first + blockIdx.x == 0 && threadIdx.x == 0) *scale = by;
   }
   // A wave a row, four elements a lane.
   typedef E E4 __attribute__((ext_vector_type(4), aligned(sizeof(E))));
-  const int64_t j = blockIdx.x * 4ll + (threadIdx.x >> 6);
+  const int64_t j = (first + blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int64_t n = count ? *count : rows;
   if (j >= (n + PADK - 1) / PADK * PADK || j >= out_rows) return;
   const bool live = j < n;
@@ -233,6 +243,7 @@ struct VlArgs {
   int K;                   // a multiple of the step
   int ka;                  // of them that a far A has rows for, beside a near B
   int mt, nt, splits;      // tiles, and parts of the contracted axis
+  int first, work;         // of all their products, a launch's
   // LSE and D: M the vocabulary from column v0 on, N the packed rows
   int v0, V;               // piece's first column; vocabulary
   const void* bias;
@@ -351,12 +362,13 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = mg_uniform(tid >> 6);
   const int wm = wave & 1, wn = wave >> 1;
   // Tiles in bands of 8 along N, so that neighbours share operands; each XCD takes a run.
-  const int tiles = a.mt * a.nt, work = tiles * a.splits;
+  const int tiles = a.mt * a.nt;
   int id = blockIdx.x;
   {
-    const int per = (work + 7) / 8, x = id & 7, y = id >> 3;
+    const int per = (a.work + 7) / 8, x = id & 7, y = id >> 3;
     id = x * per + y;
-    if (y >= per || id >= work) return;
+    if (y >= per || id >= a.work) return;
+    id += a.first;
   }
   const int split = id / tiles;
   id -= split * tiles;
@@ -612,11 +624,11 @@ __global__ __launch_bounds__(1024) void vl_join(const float2* __restrict__ part,
                                                 const int* __restrict__ idx,
                                                 const int* __restrict__ count, int parts, int ld,
                                                 float2* __restrict__ soft,
-                                                float* __restrict__ loss) {
+                                                float* __restrict__ loss, int first) {
   __shared__ float2 s[16][64];
   const int r = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int n = blockIdx.x * 64 + r, rows = *count;
-  if (blockIdx.x * 64 >= rows) return;
+  const int n = (first + blockIdx.x) * 64 + r, rows = *count;
+  if (n - r >= rows) return;
   const float2* p = part + (n < rows ? n : rows - 1);
   float top = -INFINITY, sum = 0.f;
 #pragma unroll 4
@@ -752,14 +764,14 @@ __global__ __launch_bounds__(256) void vl_weigh(const u16* __restrict__ x, u16* 
                                                 const float* __restrict__ sx,
                                                 const int* __restrict__ count,
                                                 const float* __restrict__ top,
-                                                float* __restrict__ scale) {
+                                                float* __restrict__ scale, int64_t first) {
   __shared__ float s_top[4];
   const float t = wave_max(top[threadIdx.x]);
   if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = t;
   __syncthreads();
   const float by = scale_of(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])));
-  if (blockIdx.x == 0 && threadIdx.x == 0) *scale = by;
-  const int64_t j = blockIdx.x * 4ll + (threadIdx.x >> 6);
+  if (first + blockIdx.x == 0 && threadIdx.x == 0) *scale = by;
+  const int64_t j = (first + blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int n = *count;
   if (j >= (n + PADK - 1) / PADK * PADK) return;
   const float g = j < n ? weight[j] : 0.f, f = j < n ? g / *sx : 0.f;
@@ -783,8 +795,8 @@ template <typename E>
 __global__ __launch_bounds__(256) void vl_sum(const float* __restrict__ part, int64_t po,
                                               int parts, const int* __restrict__ pos, int64_t n,
                                               int cols, const float* __restrict__ by,
-                                              E* __restrict__ out) {
-  const int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+                                              E* __restrict__ out, int64_t first) {
+  const int64_t x = ((first + blockIdx.x) * 256 + threadIdx.x) * 4;
   if (x >= n) return;
   if ((cols & 3) == 0) {
     const int64_t i = x / cols, j = pos ? pos[i] : i;
@@ -840,6 +852,14 @@ bool vl_shape(int dtype, int64_t N, int64_t V, int64_t D, Shape* s) {
   s->few = dtype == 0 && N <= FEW && D >= 4 && FEW * s->ldd * 4 <= VL_D_BYTES
                ? (N <= 32 ? 1 : N <= 64 ? 2 : 4) : 0;
   return true;
+}
+template <typename E>
+void vl_sum_run(const float* part, int64_t po, int parts, const int* pos, int64_t n, int64_t cols,
+                const float* by, void* out, hipStream_t stream) {
+  vl_launches((n / 4 + 256) / 256, 256, [&](dim3 grid, dim3 nt, int64_t first) {
+    hipLaunchKernelGGL(vl_sum<E>, grid, nt, 0, stream, part, po, parts, pos, n, (int)cols, by, (E*)out,
+                       first);
+  });
 }
 struct State {
   int *idx, *pos, *tgt, *count;
@@ -967,17 +987,20 @@ template <int EPI, bool AFAR, bool BFAR>
 int vl_run(int dtype, VlArgs& a, hipStream_t stream) {
   const int64_t work = (int64_t)a.mt * a.nt * a.splits;
   if (work > (1ll << 30)) return MG_ERR_TOO_LARGE;
-  const dim3 grid((unsigned)((work + 7) / 8 * 8));
-  // W is read where it lies if its rows are whole vectors; the zeros behind rows that are not
-  // whole steps cost selections, so rows that are do without them.
-  if constexpr (EPI != VL_OUT) {
-    if (dtype && a.lda % BK) {
-      hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 1, true, u16>), grid, dim3(NT), 0, stream, a);
-      return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
+  vl_launches(work, NT, [&](dim3 n, dim3 nt, int64_t first) {
+    a.first = (int)first, a.work = (int)n.x;
+    const dim3 grid((n.x + 7) / 8 * 8);
+    // W is read where it lies if its rows are whole vectors; the zeros behind rows that are not
+    // whole steps cost selections, so rows that are do without them.
+    if (EPI != VL_OUT && dtype && a.lda % BK) {
+      if constexpr (EPI != VL_OUT)
+        hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 1, true, u16>), grid, nt, 0, stream, a);
+    } else if (dtype) {
+      hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 1, false, u16>), grid, nt, 0, stream, a);
+    } else {
+      hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 2, false, float>), grid, nt, 0, stream, a);
     }
-  }
-  if (dtype) hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 1, false, u16>), grid, dim3(NT), 0, stream, a);
-  else hipLaunchKernelGGL((vl_gemm<EPI, AFAR, BFAR, 2, false, float>), grid, dim3(NT), 0, stream, a);
+  });
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
 
@@ -1001,17 +1024,18 @@ int64_t vl_part_rows(const Shape& s) { return 2 * ((s.V + TM - 1) / TM); }
 void vl_pack_run(int dtype, const void* src, int64_t ld, int64_t cols, u16* dst, int64_t dld,
                  int64_t plane, const int* idx, const int* count, int64_t rows,
                  int64_t out_rows, int ones, float* top, float* scale, hipStream_t stream) {
-  const dim3 grid((unsigned)((out_rows + 3) / 4));
-  if (dtype) {
-    hipLaunchKernelGGL((vl_pack<u16, 1>), grid, dim3(256), 0, stream, (const u16*)src, ld,
-                       (int)cols, dst, (int)dld, plane, idx, count, rows, out_rows, ones,
-                       (const float*)nullptr, (float*)nullptr);
-    return;
-  }
-  hipLaunchKernelGGL(vl_absmax, dim3(MAX_PARTS), dim3(1024), 0, stream, (const float*)src, ld, cols,
-                     idx, count, rows, top);
-  hipLaunchKernelGGL((vl_pack<float, 2>), grid, dim3(256), 0, stream, (const float*)src, ld,
-                     (int)cols, dst, (int)dld, plane, idx, count, rows, out_rows, ones, top, scale);
+  if (!dtype)
+    hipLaunchKernelGGL(vl_absmax, dim3(MAX_PARTS), dim3(1024), 0, stream, (const float*)src, ld, cols,
+                       idx, count, rows, top);
+  vl_launches((out_rows + 3) / 4, 256, [&](dim3 grid, dim3 nt, int64_t first) {
+    if (dtype)
+      hipLaunchKernelGGL((vl_pack<u16, 1>), grid, nt, 0, stream, (const u16*)src, ld, (int)cols, dst,
+                         (int)dld, plane, idx, count, rows, out_rows, ones, (const float*)nullptr,
+                         (float*)nullptr, first);
+    else
+      hipLaunchKernelGGL((vl_pack<float, 2>), grid, nt, 0, stream, (const float*)src, ld, (int)cols, dst,
+                         (int)dld, plane, idx, count, rows, out_rows, ones, top, scale, first);
+  });
 }
 
 }  // namespace
@@ -1079,8 +1103,10 @@ int mg_vocab_loss_fwd(int dtype, const void* x, int64_t ldx, const void* w, cons
   a.part = part, a.tlogit = tlogit;
   const int rc = vl_run<VL_LSE, false, false>(dtype, a, stream);
   if (rc != MG_OK) return rc;
-  hipLaunchKernelGGL(vl_join, dim3((unsigned)((N + 63) / 64)), dim3(1024), 0, stream, part, tlogit,
-                     t.tgt, t.idx, t.count, (int)vl_part_rows(s), (int)s.np, t.soft, rows);
+  vl_launches((N + 63) / 64, 1024, [&](dim3 grid, dim3 nt, int64_t first) {
+    hipLaunchKernelGGL(vl_join, grid, nt, 0, stream, part, tlogit, t.tgt, t.idx, t.count,
+                       (int)vl_part_rows(s), (int)s.np, t.soft, rows, (int)first);
+  });
   return finish();
 }
 
@@ -1101,9 +1127,8 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
     (s.few == 1 ? few_products<1> : s.few == 2 ? few_products<2> : few_products<4>)(
         s, t, a, dx ? b.dx_part : nullptr, dw, db, stream);
     if (dx)
-      hipLaunchKernelGGL(vl_sum<float>, dim3((unsigned)((N * D / 4 + 256) / 256)), dim3(256), 0, stream,
-                         b.dx_part, N * D, (int)((V + few_per(s) - 1) / few_per(s)), t.pos, N * D,
-                         (int)D, (const float*)nullptr, (float*)dx);
+      vl_sum_run<float>(b.dx_part, N * D, (int)((V + few_per(s) - 1) / few_per(s)), t.pos, N * D, D,
+                        nullptr, dx, stream);
     return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
   }
   const int e = dtype ? 2 : 4;
@@ -1118,8 +1143,10 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
   if (weighted && dw) {
     hipLaunchKernelGGL(vl_weigh_top, dim3(MAX_PARTS), dim3(1024), 0, stream, t.xc, (int)s.dx, (int)D,
                        b.weight, t.sx, t.count, top);
-    hipLaunchKernelGGL(vl_weigh, dim3((unsigned)((s.np + 3) / 4)), dim3(256), 0, stream, t.xc, b.xw,
-                       (int)s.dx, s.np * s.dx, (int)D, b.weight, t.sx, t.count, top, b.sxw);
+    vl_launches(s.np / 4, 256, [&](dim3 grid, dim3 nt, int64_t first) {
+      hipLaunchKernelGGL(vl_weigh, grid, nt, 0, stream, t.xc, b.xw, (int)s.dx, s.np * s.dx, (int)D,
+                         b.weight, t.sx, t.count, top, b.sxw, first);
+    });
   }
   for (int64_t v0 = 0; v0 < V; v0 += b.vp) {
     const int64_t cols = V - v0 < b.vp ? V - v0 : b.vp, kc = up_to(cols, PADK);
@@ -1160,30 +1187,16 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
         for (int k = 0; k < (db ? 2 : 1); ++k) {
           const int64_t n = k ? cols : cols * D;
           const float* const from = k ? b.db_part : b.dw_part;
-          const int wide = k ? 1 : (int)D;
-          const dim3 grid((unsigned)((n / 4 + 256) / 256));
-          if (dtype)
-            hipLaunchKernelGGL(vl_sum<u16>, grid, dim3(256), 0, stream, from, n, b.dw_splits,
-                               (const int*)nullptr, n, wide, (const float*)nullptr, (u16*)(k ? to_b : to));
-          else
-            hipLaunchKernelGGL(vl_sum<float>, grid, dim3(256), 0, stream, from, n, b.dw_splits,
-                               (const int*)nullptr, n, wide, (const float*)nullptr,
-                               (float*)(k ? to_b : to));
+          (dtype ? vl_sum_run<u16> : vl_sum_run<float>)(from, n, b.dw_splits, nullptr, n, k ? 1 : D, nullptr,
+                                                        k ? to_b : to, stream);
         }
       }
     }
     if (rc != MG_OK) return rc;
   }
-  if (dx) {
-    const int64_t n = N * D;
-    const dim3 grid((unsigned)((n / 4 + 256) / 256));
-    if (dtype)
-      hipLaunchKernelGGL(vl_sum<u16>, grid, dim3(256), 0, stream, b.dx_part, n, b.dx_splits, t.pos, n,
-                         (int)D, (const float*)nullptr, (u16*)dx);
-    else
-      hipLaunchKernelGGL(vl_sum<float>, grid, dim3(256), 0, stream, b.dx_part, n, b.dx_splits, t.pos, n,
-                         (int)D, weighted ? dloss : nullptr, (float*)dx);
-  }
+  if (dx)
+    (dtype ? vl_sum_run<u16> : vl_sum_run<float>)(b.dx_part, N * D, b.dx_splits, t.pos, N * D, D,
+                                                  weighted ? dloss : nullptr, dx, stream);
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
 
