@@ -11,7 +11,8 @@ import pytest
 import torch
 
 from mingru_amd import linear_attention
-from tests.test_linear_attention import inputs, recurrence
+from tests.test_gpu_attention_planes import on_device
+from tests.test_linear_attention import inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -66,8 +67,9 @@ def test_gradients_of_many_sizes(cuda, dtype, B, T, H, Hk, dk, dv, starts):
         do[:, lo:hi] *= (1.0, 1e5, 1e-5, 1e2)[n % 4]
     do = do.to(dtype)
     dh = torch.randn(B, H, dk, dv, generator=r)
-    ref = [t.double().requires_grad_() for t in vals]
-    want = torch.autograd.grad(recurrence(*ref), ref, (do.double(), dh.double()))[3]
+    ref = [t.to(cuda).double().requires_grad_() for t in vals]
+    up = (do.to(cuda).double(), dh.to(cuda).double())
+    want = torch.autograd.grad(on_device(*ref), ref, up)[3].cpu()
     dev = [t.to(cuda).requires_grad_() for t in vals]
     got = torch.autograd.grad(linear_attention(*dev), dev, (do.to(cuda), dh.to(cuda)))[3]
     got = got.double().cpu()
