@@ -24,13 +24,16 @@
 // consecutive (near), or the other way round (far, read with ds_read_b64_tr_b16): x, W and d
 // all lie in memory once, and each is near in one product and far in another.
 //
-// fp32 inputs are scaled by a power of two that takes the largest finite one (of x, of W) to
-// 2^14 .. 2^15, and split into two fp16 planes, hi + lo: 22 significant bits down to 2^-28 of
-// the largest, then fewer, to 2^-39 of it: an error of the logits far below what fp32 sums
-// leave.  A product takes the three pairs hi hi, hi lo, lo hi: three times the work of bf16,
-// against sixteen times for fp32's own matrix instruction and six for three bf16 planes (24
-// bits at any size; 2047 x 10007 x 392 took 575 us with them, 365 with these).  d, in -1 .. 1
-// without its upstream gradient, is scaled by 2^15.
+// fp32 inputs are scaled by a power of two that takes the largest finite one (of each row of x, of
+// all of W) to 2^14 .. 2^15, and split into two fp16 planes, hi + lo: 22 significant bits down to
+// 2^-17 of the largest, then fewer, to 2^-39 of it: an error of the logits far below what fp32
+// sums leave.  A product takes the three pairs hi hi, hi lo, lo hi: three times the work of bf16,
+// against sixteen times for fp32's own matrix instruction and six for three bf16 planes (24 bits
+// at any size; 2047 x 10007 x 392 took 575 us with them, 365 with these).  d's rows, without their
+// upstream gradients, are brought to 2^14 .. 2^15 by powers of two from the forward's losses: the
+// largest entry is 1 - p of the target.  dW's product sums over rows, so it takes x's rows times
+// their upstream gradients over these powers, split again with one scale: what a row adds is held
+// to 2^-39 of the largest that a row of the call adds.
 // bf16 inputs: d, without the factor of a mean, is rounded to bf16 once; sums are fp32.
 // Up to 128 fp32 rows take vocab_few.h's kernels.
 // With a bias, x has a column of ones behind its own, which makes db one more column of dW.
@@ -74,14 +77,14 @@ __device__ __forceinline__ float wave_max(float x) {
   for (int d = 32; d; d /= 2) x = fmaxf(x, __shfl_xor(x, d));
   return x;
 }
-// The power of two that takes `top` to 2^14 .. 2^15, from 2^-60 to 2^50 (two of them, and a bias
-// times both, stay finite); 1 for 0.
-__device__ __forceinline__ float scale_of(float top) {
+// The power of two that takes `top` to 2^14 .. 2^15, from 2^least to 2^50 (two of them, and a bias
+// times both, stay finite); 1 for 0.  Rows of x go down to 2^-100, all of W to 2^-60.
+__device__ __forceinline__ float scale_of(float top, int least) {
   if (!(top > 0.f)) return 1.f;
   int e;
   frexpf(top, &e);  // top = m 2^e, m in 1/2 .. 1
   e = 15 - e;
-  return ldexpf(1.f, e < -60 ? -60 : e > 50 ? 50 : e);
+  return ldexpf(1.f, e < least ? least : e > 50 ? 50 : e);
 }
 constexpr int MAX_PARTS = 256;
 // A launch has fewer than 2^32 threads, so a kernel that takes a thread, wave or workgroup for each
@@ -95,6 +98,7 @@ void vl_launches(int64_t blocks, int threads, F&& launch) {
     launch(dim3((unsigned)(blocks - first < most ? blocks - first : most)), dim3(threads), first);
 }
 constexpr float ONE_SCALE = 16384.f, D_SCALE = 32768.f;
+constexpr int D_LEAST = -16;  // exponent of d's largest entry, below which its own rounding error counts
 
 // ---- packing ----------------------------------------------------------------------------
 // Counted rows in order: idx[j] the j-th one's row, pos[i] a row's place or -1, tgt[j] its
@@ -178,7 +182,8 @@ __global__ __launch_bounds__(1024) void vl_absmax(const float* __restrict__ src,
 // Rows of `cols` elements in PL planes, `ld` elements a row, 0 past the columns except a one at
 // `ones`.  idx: the counted rows, padded with rows of 0 to a multiple of the contracted step;
 // null: all rows.  Two planes are fp16 of the values times the scale that the parts of the
-// largest magnitude give (written to `scale`; the one times ONE_SCALE), one is bf16.
+// largest magnitude give or, without them, times a scale of each row's own (written to `scale`; no
+// one there), one is bf16.
 template <typename E, int PL>
 __global__ __launch_bounds__(256) void vl_pack(const E* __restrict__ src, int64_t lds_, int cols,
                                                u16* __restrict__ dst, int ld, int64_t plane,
@@ -188,12 +193,12 @@ __global__ __launch_bounds__(256) void vl_pack(const E* __restrict__ src, int64_
                                                const float* __restrict__ top,
                                                float* __restrict__ scale, int64_t first) {
   float by = 1.f;
-  if constexpr (PL == 2) {
+  if (PL == 2 && top) {
     __shared__ float s_top[4];
     const float t = wave_max(top[threadIdx.x]);
     if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = t;
     __syncthreads();
-    by = scale_of(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])));
+    by = scale_of(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])), -60);
     if (first + blockIdx.x == 0 && threadIdx.x == 0) *scale = by;
   }
   // A wave a row, four elements a lane.
@@ -203,6 +208,25 @@ __global__ __launch_bounds__(256) void vl_pack(const E* __restrict__ src, int64_
   if (j >= (n + PADK - 1) / PADK * PADK || j >= out_rows) return;
   const bool live = j < n;
   const E* s = src + (live ? (idx ? (int64_t)idx[j] : j) * lds_ : 0);
+  if (PL == 2 && !top && live) {
+    float most = 0.f;
+    for (int c = (threadIdx.x & 63) * 4; c < cols; c += 256) {
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+      if (c + 4 <= cols) {
+        const E4 y = *reinterpret_cast<const E4*>(s + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = fabsf(to_f(y[e]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < cols) x[e] = fabsf(to_f(s[c + e]));
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = x[e] < INFINITY ? fmaxf(most, x[e]) : most;
+    }
+    by = scale_of(wave_max(most), -100);
+    if ((threadIdx.x & 63) == 0) scale[j] = by;
+  }
   for (int c = (threadIdx.x & 63) * 4; c < ld; c += 256) {
     float x[4] = {0.f, 0.f, 0.f, 0.f};
     if (live && c + 4 <= cols) {
@@ -213,7 +237,7 @@ __global__ __launch_bounds__(256) void vl_pack(const E* __restrict__ src, int64_
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (c + e < cols) x[e] = to_f(s[c + e]) * by;
-        if (c + e == ones) x[e] = PL == 2 ? ONE_SCALE : 1.f;
+        if (PL == 1 && c + e == ones) x[e] = 1.f;
       }
     }
     u16* const to = dst + j * ld + c;
@@ -234,7 +258,7 @@ enum { VL_LSE = 0, VL_D = 1, VL_OUT = 2 };
 struct VlArgs {
   const u16 *A, *B;        // M's and N's operands
   int64_t pa, pb;          // elements between their planes
-  const float *sa, *sb;    // fp16 planes: what they were scaled by
+  const float *sa, *sb;    // fp16 planes: what they were scaled by; LSE and D: sb of each row
   int lda, ldb;            // elements between rows
   int m_rows, n_rows;      // rows (near) or columns (far) that exist; read places are clamped
   const int* m_count;      // on the device, in their place, if not null
@@ -426,10 +450,17 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
   // A row's bias is where its sum starts; past the vocabulary that is -inf, so that such a
   // column's exponentials are 0.
   f32x16 acc[4][2];
-  const float by = PL == 2 ? *a.sa * *a.sb : 1.f;  // a power of two
+  float by[2] = {1.f, 1.f};  // powers of two: what the lane's two rows' sums are scaled by
   if constexpr (EPI != VL_OUT) {
     const int m = m0 + tid;
-    s_bias[tid] = m >= m_rows ? -INFINITY : a.bias ? to_f(((const E*)a.bias)[a.v0 + m]) * by : 0.f;
+    s_bias[tid] = m >= m_rows ? -INFINITY : a.bias ? to_f(((const E*)a.bias)[a.v0 + m]) : 0.f;
+    if constexpr (PL == 2) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int n = n0 + wn * 64 + 32 * j + (lane & 31);
+        by[j] = *a.sa * a.sb[n < n_rows ? n : n_rows - 1];
+      }
+    }
     __syncthreads();
     const float* const bw = s_bias + wm * 128 + 4 * (lane >> 5);
 #pragma unroll
@@ -437,8 +468,8 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
       const float4 b = *reinterpret_cast<const float4*>(bw + 8 * c);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        acc[c >> 2][j][4 * (c & 3)] = b.x, acc[c >> 2][j][4 * (c & 3) + 1] = b.y;
-        acc[c >> 2][j][4 * (c & 3) + 2] = b.z, acc[c >> 2][j][4 * (c & 3) + 3] = b.w;
+        acc[c >> 2][j][4 * (c & 3)] = b.x * by[j], acc[c >> 2][j][4 * (c & 3) + 1] = b.y * by[j];
+        acc[c >> 2][j][4 * (c & 3) + 2] = b.z * by[j], acc[c >> 2][j][4 * (c & 3) + 3] = b.w * by[j];
       }
     }
   } else {
@@ -498,7 +529,8 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
   // 32 i + 8 q + 4 (lane >> 5) + x in acc[i][j][4 q + x].
   const int half = lane >> 5, mw = m0 + wm * 128 + 4 * half, nw = n0 + wn * 64 + (lane & 31);
   // exp(l) of logits that are still scaled.
-  const float unit = 1.f / by, log2 = 1.4426950408889634f * unit;
+  const float unit[2] = {1.f / by[0], 1.f / by[1]};
+  const float log2[2] = {1.4426950408889634f * unit[0], 1.4426950408889634f * unit[1]};
   if constexpr (EPI == VL_LSE) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -511,16 +543,16 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
 #pragma unroll
         for (int c = 0; c < 64; ++c)
           if (t == 8 * (c >> 2) + (c & 3) && n < n_rows)
-            a.tlogit[n] = acc[c >> 4][j][c & 15] * unit;
+            a.tlogit[n] = acc[c >> 4][j][c & 15] * unit[j];
       }
       top = fmaxf(top, __shfl_xor(top, 32));
       const float ref = top == -INFINITY ? 0.f : top;
       float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < 64; ++c) sum += __builtin_amdgcn_exp2f((acc[c >> 4][j][c & 15] - ref) * log2);
+      for (int c = 0; c < 64; ++c) sum += __builtin_amdgcn_exp2f((acc[c >> 4][j][c & 15] - ref) * log2[j]);
       sum += __shfl_xor(sum, 32);
       // fmaxf drops a NaN; the sum keeps it.
-      if (half == 0 && n < n_rows) a.part[(int64_t)(2 * mt + wm) * a.n_ld + n] = make_float2(top * unit, sum);
+      if (half == 0 && n < n_rows) a.part[(int64_t)(2 * mt + wm) * a.n_ld + n] = make_float2(top * unit[j], sum);
     }
   }
   if constexpr (EPI == VL_D) {
@@ -533,11 +565,11 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
     for (int j = 0; j < 2; ++j) {
       const int n = nw + 32 * j, r = n < n_rows ? n : n_rows - 1;
       const float2 soft = a.soft[r];
-      const float g = n < n_rows ? a.g[r] : 0.f, sg = soft.y * g, top = soft.x * by;
+      const float g = n < n_rows ? a.g[r] : 0.f, sg = soft.y * g, top = soft.x * by[j];
       const int t = a.tgt[r] - a.v0 - mw;
 #pragma unroll
       for (int c = 0; c < 64; ++c) {
-        acc[c >> 4][j][c & 15] = __builtin_amdgcn_exp2f((acc[c >> 4][j][c & 15] - top) * log2) * sg;
+        acc[c >> 4][j][c & 15] = __builtin_amdgcn_exp2f((acc[c >> 4][j][c & 15] - top) * log2[j]) * sg;
       }
       if (__ballot(t >= 0 && t < 128)) {
 #pragma unroll
@@ -574,8 +606,8 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
   }
   if constexpr (EPI == VL_OUT) {
     const bool f32 = a.out_f32;
-    // Apart from `unit`, which brings the sums to their size: their product may be below what fp32 holds.
-    const float scale = *a.scale, unit1 = PL == 2 ? 1.f / (ONE_SCALE * *a.sb) : 1.f;
+    // Apart from `size`, which brings the sums to theirs: the product of both may be below what fp32 holds.
+    const float scale = *a.scale, size = PL == 2 ? 1.f / (*a.sa * *a.sb) : 1.f, unit1 = PL == 2 ? 1.f / (ONE_SCALE * *a.sb) : 1.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int n = nw + 32 * j;
@@ -588,7 +620,7 @@ __global__ __launch_bounds__(NT, 2) void vl_gemm(VlArgs a) {
           const int m = mw + 32 * i + 8 * q;
           float v[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) v[x] = scale * (unit * acc[i][j][4 * q + x]);
+          for (int x = 0; x < 4; ++x) v[x] = scale * (size * acc[i][j][4 * q + x]);
           if (m + 4 <= a.m_out && (a.ldo & 3) == 0) {
             if (f32) {
               float4* const to = reinterpret_cast<float4*>((float*)a.out + row + m);
@@ -624,7 +656,8 @@ __global__ __launch_bounds__(1024) void vl_join(const float2* __restrict__ part,
                                                 const int* __restrict__ idx,
                                                 const int* __restrict__ count, int parts, int ld,
                                                 float2* __restrict__ soft,
-                                                float* __restrict__ loss, int first) {
+                                                float* __restrict__ loss,
+                                                float* __restrict__ most, int first) {
   __shared__ float2 s[16][64];
   const int r = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int n = (first + blockIdx.x) * 64 + r, rows = *count;
@@ -651,7 +684,9 @@ __global__ __launch_bounds__(1024) void vl_join(const float2* __restrict__ part,
   // The largest logit and the sum stay apart: their log sum would round at the logits' size.
   const bool in = tgt[n] >= 0;
   soft[n] = make_float2(in ? top : __builtin_nanf(""), 1.f / sum);
-  loss[idx[n]] = in ? (top - tlogit[n]) + logf(sum) : __builtin_nanf("");
+  const float l = in ? (top - tlogit[n]) + logf(sum) : __builtin_nanf("");
+  loss[idx[n]] = l;
+  if (most) most[n] = -expm1f(-l);  // 1 - p of the target: d's largest entry
 }
 
 // The counted rows' losses' sum, over the count if `mean`, in a fixed order.  One workgroup.
@@ -687,16 +722,19 @@ __global__ __launch_bounds__(1024) void vl_total(const float* __restrict__ loss,
 // What d is multiplied by in its epilogue (g), and factors for all of it.  reduction: 0 each row's
 // own, 1 mean, 2 sum.  A factor for all is kept out of d: one over the count, rounded to bf16 in
 // every row's largest entry (the target's), would put all gradients off by the same 2^-9.
-// fp16 planes (d_scale not null) hold d without any upstream gradient, times D_SCALE: a row of
-// small weight would lose its bits beside one of large weight.  dx's rows are multiplied by their
-// own where they are summed, and dW's product takes x's rows times `weight`, the upstream gradients
-// over the power of two w_scale, whose largest (top: of the counted rows) is 1/2 .. 1 (.. 2 at the
-// type's end).
+// fp16 planes (most not null, the rows' largest entries of d without its upstream gradient) hold d
+// over a power of two of each row's own, times D_SCALE, without upstream gradients: rows whose own
+// are small would lose their bits beside large ones.  What d lacks, `back`, multiplies dx's rows
+// where they are summed; dW's product takes x's rows times `weight`, the same over the power of two
+// w_scale, which brings the largest upstream gradient of the counted rows (top, for reduction 0) to
+// 1/2 .. 1 (.. 2 at the type's end).
 __global__ __launch_bounds__(256) void vl_upstream(const float* __restrict__ up,
                                                    const int* __restrict__ idx,
                                                    const int* __restrict__ count, int reduction,
+                                                   const float* __restrict__ most,
                                                    const float* __restrict__ top,
-                                                   float* __restrict__ g, float* __restrict__ weight,
+                                                   float* __restrict__ g, float* __restrict__ back,
+                                                   float* __restrict__ weight,
                                                    float* __restrict__ scale,
                                                    float* __restrict__ w_scale,
                                                    float* __restrict__ d_scale) {
@@ -713,14 +751,25 @@ __global__ __launch_bounds__(256) void vl_upstream(const float* __restrict__ up,
   if (j == 0) {
     *scale = reduction == 0 ? 1.f : reduction == 1 ? up[0] / (float)(n > 0 ? n : 1) : up[0];
     *w_scale = top ? ldexpf(1.f, e) : *scale;
-    if (d_scale) *d_scale = D_SCALE;
+    *d_scale = D_SCALE;
   }
   if (j >= n) return;
-  g[j] = d_scale ? D_SCALE : reduction == 0 ? up[idx[j]] : 1.f;
-  if (top) weight[j] = ldexpf(up[idx[j]], -e);
+  const float own = reduction == 0 ? up[idx[j]] : 1.f;
+  if (!most) {
+    g[j] = own;
+    return;
+  }
+  int k = D_LEAST;
+  if (most[j] > 0.f) {
+    frexpf(most[j], &k);
+    k = k > 0 ? 0 : k < D_LEAST ? D_LEAST : k;
+  }
+  g[j] = ldexpf(D_SCALE, -k);
+  back[j] = ldexpf(own, k);
+  weight[j] = ldexpf(own, k - e);
 }
 
-// Packed rows in two planes, scaled by *sx, times their weights: the largest finite magnitude in
+// Packed rows in two planes, scaled by sx, times their weights: the largest finite magnitude in
 // MAX_PARTS parts (of the high plane: 2^-11 of it off at most, and a plane holds twice what its
 // scale makes of it), then in two planes with a scale of their own.  The column of ones becomes the
 // weights, times ONE_SCALE.
@@ -737,7 +786,7 @@ __global__ __launch_bounds__(1024) void vl_weigh_top(const u16* __restrict__ x, 
   const int n = *count, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   float top = 0.f;
   for (int j = blockIdx.x * 16 + w; j < n; j += MAX_PARTS * 16) {
-    const float by = weight[j] / *sx;
+    const float by = weight[j] / sx[j];
 #pragma unroll 4
     for (int c = lane * 4; c < cols; c += 256) {
       float v[4];
@@ -769,12 +818,12 @@ __global__ __launch_bounds__(256) void vl_weigh(const u16* __restrict__ x, u16* 
   const float t = wave_max(top[threadIdx.x]);
   if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = t;
   __syncthreads();
-  const float by = scale_of(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])));
+  const float by = scale_of(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])), -100);
   if (first + blockIdx.x == 0 && threadIdx.x == 0) *scale = by;
   const int64_t j = (first + blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int n = *count;
   if (j >= (n + PADK - 1) / PADK * PADK) return;
-  const float g = j < n ? weight[j] : 0.f, f = j < n ? g / *sx : 0.f;
+  const float g = j < n ? weight[j] : 0.f, f = j < n ? g / sx[j] : 0.f;
   for (int c = (threadIdx.x & 63) * 4; c < ld; c += 256) {
     const u16* const p = x + j * ld + c;
     float hi[4], lo[4], y[4];
@@ -790,7 +839,8 @@ __global__ __launch_bounds__(256) void vl_weigh(const u16* __restrict__ x, u16* 
                                                       pack2h(rest(y[2], b, 0), rest(y[3], b, 1)));
   }
 }
-// out[i][c] = sum of the parts' rows, pos[i] if given (0 where that is negative), times by[i] if given.
+// out[i][c] = sum of the parts' rows, pos[i] if given (0 where that is negative), times by of the same
+// row if given.
 template <typename E>
 __global__ __launch_bounds__(256) void vl_sum(const float* __restrict__ part, int64_t po,
                                               int parts, const int* __restrict__ pos, int64_t n,
@@ -807,7 +857,7 @@ __global__ __launch_bounds__(256) void vl_sum(const float* __restrict__ part, in
         const float4 v = *reinterpret_cast<const float4*>(part + p * po + j * cols + x % cols);
         s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
       }
-    if (by && j >= 0) s.x *= by[i], s.y *= by[i], s.z *= by[i], s.w *= by[i];
+    if (by && j >= 0) s.x *= by[j], s.y *= by[j], s.z *= by[j], s.w *= by[j];
     if constexpr (sizeof(E) == 4) *reinterpret_cast<float4*>(out + x) = s;
     else *reinterpret_cast<uint2*>(out + x) = make_uint2(pack2(s.x, s.y), pack2(s.z, s.w));
     return;
@@ -817,7 +867,7 @@ __global__ __launch_bounds__(256) void vl_sum(const float* __restrict__ part, in
     float s = 0.f;
     if (j >= 0)
       for (int p = 0; p < parts; ++p) s += part[p * po + j * cols + y % cols];
-    if (by && j >= 0) s *= by[i];
+    if (by && j >= 0) s *= by[j];
     if constexpr (sizeof(E) == 4) out[y] = s;
     else out[y] = to_bf(s);
   }
@@ -864,7 +914,8 @@ void vl_sum_run(const float* part, int64_t po, int parts, const int* pos, int64_
 struct State {
   int *idx, *pos, *tgt, *count;
   float2* soft;
-  float *sx, *sw;  // scales of the packed planes
+  float *sx, *sw;  // scales of the packed planes: of each row of x, of W
+  float* most;     // with them: rows' largest entries of d
   u16 *xc, *wc;
   size_t bytes;
 };
@@ -877,7 +928,9 @@ State vl_state(const Shape& s, void* base) {
   };
   State t;
   t.count = (int*)take(4);
-  t.sx = (float*)take(4), t.sw = (float*)take(4);
+  const bool own = s.planes == 2 && !s.few;
+  t.sx = own ? (float*)take(s.N * 4) : nullptr, t.most = own ? (float*)take(s.N * 4) : nullptr;
+  t.sw = (float*)take(4);
   t.idx = (int*)take(s.N * 4), t.pos = (int*)take(s.N * 4), t.tgt = (int*)take(s.N * 4);
   t.soft = (float2*)take(s.N * 8);
   t.xc = (u16*)take(s.few ? 32 * s.few * s.dx * 4 : s.planes * s.np * s.dx * 2);
@@ -943,7 +996,7 @@ int vl_splits(int64_t tiles, int64_t steps, int64_t size) {
 struct Back {
   int64_t vp, pieces;   // columns of a piece
   int dx_splits, dw_splits;
-  float *g, *scale, *w_scale, *d_scale, *top, *weight, *sxw, *dx_part, *dw_part, *db_part;
+  float *g, *scale, *w_scale, *d_scale, *top, *back, *weight, *sxw, *dx_part, *dw_part, *db_part;
   u16 *d, *xw;  // xw: x's packed rows times their weights
   size_t bytes;
 };
@@ -973,7 +1026,7 @@ Back vl_back(const Shape& s, void* base) {
   b.top = (float*)take(MAX_PARTS * 4);
   b.d = (u16*)take(s.planes * s.np * b.vp * 2);
   if (s.planes == 2) {
-    b.weight = (float*)take(s.N * 4), b.sxw = (float*)take(4);
+    b.back = (float*)take(s.N * 4), b.weight = (float*)take(s.N * 4), b.sxw = (float*)take(4);
     b.xw = (u16*)take(s.planes * s.np * s.dx * 2);
   }
   b.dx_part = (float*)take(b.dx_splits * s.N * s.D * 4);  // pieces add to it one after another
@@ -1024,7 +1077,7 @@ int64_t vl_part_rows(const Shape& s) { return 2 * ((s.V + TM - 1) / TM); }
 void vl_pack_run(int dtype, const void* src, int64_t ld, int64_t cols, u16* dst, int64_t dld,
                  int64_t plane, const int* idx, const int* count, int64_t rows,
                  int64_t out_rows, int ones, float* top, float* scale, hipStream_t stream) {
-  if (!dtype)
+  if (top)
     hipLaunchKernelGGL(vl_absmax, dim3(MAX_PARTS), dim3(1024), 0, stream, (const float*)src, ld, cols,
                        idx, count, rows, top);
   vl_launches((out_rows + 3) / 4, 256, [&](dim3 grid, dim3 nt, int64_t first) {
@@ -1051,7 +1104,7 @@ size_t mg_vocab_loss_fwd_workspace_bytes(int dtype, int64_t N, int64_t V, int64_
   Shape s;
   if (!vl_shape(dtype, N, V, D, &s)) return 0;
   if (s.few) return s.N * (few_parts(s) * sizeof(float2) + 2 * sizeof(float));
-  return vl_part_rows(s) * s.np * sizeof(float2) + (s.np + s.N + 2 * MAX_PARTS) * sizeof(float);
+  return vl_part_rows(s) * s.np * sizeof(float2) + (s.np + s.N + MAX_PARTS) * sizeof(float);
 }
 
 size_t mg_vocab_loss_bwd_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
@@ -1072,7 +1125,7 @@ int mg_vocab_loss_fwd(int dtype, const void* x, int64_t ldx, const void* w, cons
     return MG_ERR_WORKSPACE;
   float2* const part = (float2*)ws;
   float* const tlogit = (float*)(part + (s.few ? N * few_parts(s) : vl_part_rows(s) * s.np));
-  float* const rows = !reduction ? loss : s.few ? tlogit + N : tlogit + s.np + 2 * MAX_PARTS;
+  float* const rows = !reduction ? loss : s.few ? tlogit + N : tlogit + s.np + MAX_PARTS;
   float* const zero = reduction ? nullptr : loss;
   const auto finish = [&]() {
     if (reduction)
@@ -1093,19 +1146,18 @@ int mg_vocab_loss_fwd(int dtype, const void* x, int64_t ldx, const void* w, cons
   }
   hipLaunchKernelGGL(vl_index, dim3(1), dim3(1024), 0, stream, target, ignore_index, V, t.idx,
                      t.pos, t.tgt, t.count, zero, (int)N);
-  float* const top = tlogit + s.np;  // both packings' parts, one after the other
-  vl_pack_run(dtype, x, ldx, D, t.xc, s.dx, s.np * s.dx, t.idx, t.count, N, s.np, (int)D, top, t.sx,
+  vl_pack_run(dtype, x, ldx, D, t.xc, s.dx, s.np * s.dx, t.idx, t.count, N, s.np, (int)D, nullptr, t.sx,
               stream);
   if (s.own_w)
-    vl_pack_run(dtype, w, D, D, t.wc, s.kp, V * s.kp, nullptr, nullptr, V, V, -1, top + MAX_PARTS,
-                t.sw, stream);
+    vl_pack_run(dtype, w, D, D, t.wc, s.kp, V * s.kp, nullptr, nullptr, V, V, -1,
+                dtype ? nullptr : tlogit + s.np, t.sw, stream);
   VlArgs a = vl_logits(s, t, w, bias, 0, V);
   a.part = part, a.tlogit = tlogit;
   const int rc = vl_run<VL_LSE, false, false>(dtype, a, stream);
   if (rc != MG_OK) return rc;
   vl_launches((N + 63) / 64, 1024, [&](dim3 grid, dim3 nt, int64_t first) {
     hipLaunchKernelGGL(vl_join, grid, nt, 0, stream, part, tlogit, t.tgt, t.idx, t.count,
-                       (int)vl_part_rows(s), (int)s.np, t.soft, rows, (int)first);
+                       (int)vl_part_rows(s), (int)s.np, t.soft, rows, t.most, (int)first);
   });
   return finish();
 }
@@ -1132,20 +1184,19 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
     return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
   }
   const int e = dtype ? 2 : 4;
-  const bool weighted = !dtype && reduction == 0;
-  float* const top = weighted ? b.top : nullptr;
-  if (weighted)
+  float* const top = !dtype && reduction == 0 ? b.top : nullptr;
+  if (top)
     hipLaunchKernelGGL(vl_absmax, dim3(MAX_PARTS), dim3(1024), 0, stream, dloss, (int64_t)1,
                        (int64_t)1, t.idx, t.count, N, top);
   hipLaunchKernelGGL(vl_upstream, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, stream, dloss,
-                     t.idx, t.count, reduction, top, b.g, b.weight, b.scale, b.w_scale,
-                     dtype ? nullptr : b.d_scale);
-  if (weighted && dw) {
+                     t.idx, t.count, reduction, t.most, top, b.g, b.back, b.weight, b.scale, b.w_scale,
+                     b.d_scale);
+  if (!dtype && dw) {
     hipLaunchKernelGGL(vl_weigh_top, dim3(MAX_PARTS), dim3(1024), 0, stream, t.xc, (int)s.dx, (int)D,
-                       b.weight, t.sx, t.count, top);
+                       b.weight, t.sx, t.count, b.top);
     vl_launches(s.np / 4, 256, [&](dim3 grid, dim3 nt, int64_t first) {
       hipLaunchKernelGGL(vl_weigh, grid, nt, 0, stream, t.xc, b.xw, (int)s.dx, s.np * s.dx, (int)D,
-                         b.weight, t.sx, t.count, top, b.sxw, first);
+                         b.weight, t.sx, t.count, b.top, b.sxw, first);
     });
   }
   for (int64_t v0 = 0; v0 < V; v0 += b.vp) {
@@ -1167,8 +1218,8 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
     }
     if (rc == MG_OK && dw) {
       VlArgs c = {};
-      c.A = weighted ? b.xw : t.xc, c.lda = (int)s.dx, c.pa = s.np * s.dx, c.m_rows = (int)s.dx;
-      c.sa = weighted ? b.sxw : t.sx, c.sb = b.d_scale;
+      c.A = dtype ? t.xc : b.xw, c.lda = (int)s.dx, c.pa = s.np * s.dx, c.m_rows = (int)s.dx;
+      c.sa = b.sxw, c.sb = b.d_scale;
       c.B = b.d, c.ldb = (int)kc, c.pb = a.pd, c.n_rows = (int)kc;
       c.k_count = t.count, c.ka = 1 << 30;
       c.mt = (int)((D + (db ? 1 : 0) + TM - 1) / TM), c.nt = (int)((cols + TN - 1) / TN);
@@ -1196,7 +1247,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
   }
   if (dx)
     (dtype ? vl_sum_run<u16> : vl_sum_run<float>)(b.dx_part, N * D, b.dx_splits, t.pos, N * D, D,
-                                                  weighted ? dloss : nullptr, dx, stream);
+                                                  b.back, dx, stream);
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
 
