@@ -32,6 +32,8 @@ def _dispatch(what: str, is_cuda: bool, call):
         status = scans.available()
         if status is not True:
             raise scans.ScanFallback(str(status))
+        if not is_cuda:
+            raise scans.ScanFallback("HIP kernels need GPU tensors")
         from mingru_amd import hip_sequence
 
         return call(hip_sequence)

@@ -56,7 +56,9 @@ def test_tangents_are_not_dropped(monkeypatch, name, which):
     f, inputs = CASES[name]
     want = _tangents(f, inputs, which)
     calls = []
-    monkeypatch.setattr(sequence_ops, "_resolve_scan_mode", lambda is_cuda: "auto")  # as on the GPU
+    dispatch = sequence_ops._dispatch  # as on the GPU
+    monkeypatch.setattr(sequence_ops, "_dispatch", lambda what, is_cuda, call: dispatch(what, True, call))
+    monkeypatch.setenv("MINGRU_SCAN", "auto")
     monkeypatch.setattr(sequence_ops, "_warned", set())
     monkeypatch.setattr(hip_scans, "available", lambda: True)
     monkeypatch.setattr(hip_sequence, "_stream", lambda t: 0)
