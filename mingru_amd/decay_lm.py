@@ -111,7 +111,12 @@ class DecayLM(nn.Module):
     @torch.no_grad()
     def generate(self, prompt, n: int, lengths=None):
         """The ``n`` likeliest next tokens, one after another, after each prompt (B, T), whose
-        ``lengths`` (B) leave off padding at the end."""
+        ``lengths`` (B), of 1 to T tokens, leave off padding at the end."""
+        T = prompt.shape[1]
+        if T == 0:
+            raise ValueError("the prompt has no token to go on from")
+        if lengths is not None and bool(((lengths < 1) | (lengths > T)).any()):
+            raise ValueError(f"lengths are from 1 to the prompt's {T} tokens (got {lengths.tolist()})")
         y, state = self(prompt, lengths=lengths)
         rows = torch.arange(len(prompt), device=prompt.device)
         y = y[:, -1] if lengths is None else y[rows, lengths.long() - 1]
