@@ -39,16 +39,19 @@
 // v_mfma_f32_16x16x32_bf16, fp32 inputs with v_mfma_f32_16x16x4_f32 (C = 32).  Operands lie
 // in LDS as they lie in memory, (token, feature) and (dk, dv); where the contracted index is
 // the slow one a bf16 fragment comes from two ds_read_b64_tr_b16.  Rounding, bf16: inputs are
-// exact.  What only feeds bf16 outputs (the C x C matrices, the state in o and dv) is rounded
-// to bf16 once; what feeds fp32 outputs (decayed keys and queries into the states, the states
-// into the gradient of g) is split into three bf16 planes, 24 significant bits, at three times
-// the products: with two planes the states were 2.4e-6 off and the gradient of g 7e-6.
+// exact.  Operands that are not inputs are split into bf16 planes, with a product for each.  What
+// only feeds bf16 outputs (the C x C matrices, the state in o and dv) into two, 16 significant
+// bits, so that the outputs' own rounding is the only one that counts: with one plane they were
+// 2.35e-3 off in place of 1.66e-3, prompts of 65536 tokens took 250 us in place of 268 and the
+// training pass below 450 in place of 470.  What feeds fp32 outputs (decayed keys and queries into
+// the states, the states into the gradient of g) into three, 24 bits: with two the states were
+// 2.4e-6 off and the gradient of g 7e-6.
 //
 // Bound: a wave's own chain of a chunk -- barriers, LDS reads of operand fragments and the vector
 // instructions that decay and split them -- with one workgroup a CU past heads 64 wide; memory
-// would be a quarter of it.  16 x 2048 tokens of 8 heads of 128, bf16, with gradients: 443 us
-// (sweeps: states 36, o 88, adjoint states 36, dq 138, dk and dv 150; joins 14, dg 11).
-// One sequence of 65536 tokens, forward: 239 us.  One token of 256 sequences of 16 heads: 112 us,
+// would be a quarter of it.  16 x 2048 tokens of 8 heads of 128, bf16, with gradients: 470 us
+// (under a profiler: states 36, o 97, adjoint states 36, dq 143, dk and dv 164; joins 10 each, dg 15).
+// One sequence of 65536 tokens, forward: 268 us.  One token of 256 sequences of 16 heads: 112 us,
 // 4.8 TB/s of states read and written.
 #include "mg_common.h"
 
@@ -315,6 +318,13 @@ __device__ __forceinline__ uint2 put4_split(u16* p0, u16* p1, f32x4 x) {
   }
   return u;
 }
+// In two planes, the second returned.
+__device__ __forceinline__ uint2 put4_rest(u16* p0, f32x4 x) {
+  const uint2 u = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
+  *reinterpret_cast<uint2*>(p0) = u;
+  return make_uint2(pack2(x[0] - low(u.x), x[1] - high(u.x)), pack2(x[2] - low(u.y), x[3] - high(u.y)));
+}
+__device__ __forceinline__ uint2 put4_rest(float*, f32x4) { return make_uint2(0u, 0u); }
 __device__ __forceinline__ f32x4 get4(const u16* p) {
   const uint2 u = *reinterpret_cast<const uint2*>(p);
   return f32x4{low(u.x), high(u.x), low(u.y), high(u.y)};
@@ -454,30 +464,40 @@ __device__ __forceinline__ void make_gates(Gate* out, float* w, float g, float s
 }
 
 // ---- the sweep -------------------------------------------------------------------------------
-// LDS, in elements.  The plain sweeps have two sets of a chunk's operands where they fit, one
-// being filled while the other is used (TWO).  The gradients' have one; the state's two leading planes lie in S
-// and S1, and once they are read the third lies in S.
+// LDS, in elements.  The plain sweeps fill the next chunk's place while this one's is used (TWO): the
+// state passes have two sets of operands; LA_OUT two of the values alone, since its queries, keys
+// and state are read by the time that the chunk matrices are there.  (Two whole sets would leave no
+// room for the states' second plane: with one, prompt-long took 270 us.)  The gradients' have one
+// set; the state's two leading planes lie in S and S1, and once they are read the third lies in S,
+// and the second planes of LA_DKV's matrices in S1.
 template <typename T, int C, int DK, int DV, int MODE>
 struct Lds {
   static constexpr int HV = Op<T>::HALVES;
   static constexpr bool GRAD = MODE == LA_DQ || MODE == LA_DKV;
   static constexpr bool BARE = MODE == LA_STATE || MODE == LA_RSTATE;
   static constexpr int K = 0;  // keys (LA_RSTATE: queries)
-  static constexpr int V = K + C * DK;  // values (LA_RSTATE: output gradients)
-  static constexpr int Q = V + C * DV;
+  static constexpr int Q = K + C * DK;
   static constexpr int O = Q + (BARE ? 0 : C * DK);
-  static constexpr int SET = O + (GRAD ? C * DV : 0);
-  static constexpr int REST = (BARE ? 0 : C * C + DK * DV);
-  static constexpr bool TWO = !GRAD && (2 * SET + REST) * (int)sizeof(T) <= 156 * 1024;
-  static constexpr int P = SET * (TWO ? 2 : 1);
-  static constexpr int P2 = P + (BARE ? 0 : C * C);
-  static constexpr int S = P2 + (MODE == LA_DKV ? C * C : 0);  // state
+  static constexpr int V = O + (GRAD ? C * DV : 0);  // values (LA_RSTATE: output gradients)
+  static constexpr int SET = V + C * DV;
+  static constexpr bool TWO = !GRAD;
+  static constexpr int NEXT_K = BARE ? SET : 0, NEXT_V = BARE ? SET : TWO ? SET - V : 0;  // to the other place
+  // Chunk matrices and states, in two planes each.
+  static constexpr int MATS = BARE ? 0 : MODE == LA_DKV ? 2 : HV, STATES = BARE ? 0 : HV;
+  static constexpr int P = BARE ? 2 * SET : SET + (TWO ? C * DV : 0);
+  static constexpr int P2 = P + (BARE ? 0 : C * C);  // LA_DKV: the second matrix, else P's second plane
+  static constexpr int S = P + MATS * C * C;
   static constexpr int S1 = S + (BARE ? 0 : DK * DV);
-  static constexpr int BYTES = (S1 + (GRAD ? DK * DV * (HV - 1) : 0)) * (int)sizeof(T);
+  static constexpr int SECOND = MODE == LA_DKV && HV > 1 ? 2 * C * C : 0;
+  static constexpr int LAST = SECOND > DK * DV ? SECOND : DK * DV;
+  static constexpr int BYTES = (S + (STATES > 0 ? DK * DV : 0) + (STATES > 1 ? LAST : 0)) * (int)sizeof(T);
 };
 
+// Waves a SIMD: registers for two workgroups a CU where the LDS has room for two.
+constexpr int la_waves(int DK, int DV, bool WIDE) { return WIDE && DK <= 64 && DV <= 64 ? 4 : 2; }
+
 template <typename T, int C, int DK, int DV, int MODE, bool WIDE>
-__global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
+__global__ __launch_bounds__(NT, la_waves(DK, DV, WIDE)) void la_sweep(LaArgs a) {
   typedef Lds<T, C, DK, DV, MODE> L;
   constexpr int PL = Op<T>::PLANES;
   constexpr bool REV = MODE == LA_RSTATE || MODE == LA_DKV, BARE = L::BARE, GRAD = L::GRAD, TWO = L::TWO;
@@ -584,26 +604,26 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
   }
   // A fetched chunk, and the state in its leading planes, into LDS.
   const auto put_chunk = [&](int n) {
-    T* const set = lds + (TWO ? (n & 1) * L::SET : 0);
+    T *const to_k = lds + L::K + (n & 1) * L::NEXT_K, *const to_v = lds + L::V + (n & 1) * L::NEXT_V;
     const int rows = rows_at(at(n));
     if constexpr (MODE != LA_RSTATE) {
       bk.mask(rows, dk), bv.mask(rows, dv);
-      bk.put(set + L::K), bv.put(set + L::V);
+      bk.put(to_k), bv.put(to_v);
     }
     if constexpr (MODE != LA_STATE) {
       bq.mask(rows, dk);
-      bq.put(set + (MODE == LA_RSTATE ? L::K : L::Q));
+      bq.put(MODE == LA_RSTATE ? to_k : lds + L::Q);
     }
     if constexpr (GRAD || MODE == LA_RSTATE) {
       bo.mask(rows, dv);
-      bo.put(set + (MODE == LA_RSTATE ? L::V : L::O));
+      bo.put(MODE == LA_RSTATE ? to_v : lds + L::O);
     }
   };
   uint2 third[TS::TM][TS::TN];  // the third plane, until there is room for it
   const auto put_state = [&]() {
     each_tile([&](int i, int j, int r, int c) {
       const int p = place<T, DV>(r, c);
-      if constexpr (GRAD && PL > 1) third[i][j] = put4_split(sS + p, sS1 + p, S[i][j]);
+      if constexpr (PL > 1) third[i][j] = put4_split(sS + p, sS1 + p, S[i][j]);
       else put4(sS + p, S[i][j]);
     });
   };
@@ -644,9 +664,8 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
       __syncthreads();
       if (n + 1 < chunks) fetch(at(n + 1));
     }
-    const T* const set = lds + (TWO ? (n & 1) * L::SET : 0);
-    const T *const sK = set + L::K, *const sV = set + L::V, *const sQ = set + L::Q,
-            *const sO = set + L::O;
+    const T *const sK = lds + L::K + (n & 1) * L::NEXT_K, *const sV = lds + L::V + (n & 1) * L::NEXT_V;
+    const T *const sQ = lds + L::Q, *const sO = lds + L::O;
     const Gate end = ga[C - 1];
     const float keep = span0(end);
     const auto update = [&](const T* rows_v, const T* rows_k) {
@@ -662,6 +681,7 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
       if (n + 2 < chunks) g_next = decays(n + 2);
     }
     f32x4 ack[TK::TM][TK::TN], acv[TV::TM][TV::TN];
+    uint2 lo[TC::TM][TC::TN], lo2[TC::TM][TC::TN];  // LA_DKV: the matrices' second planes
     if constexpr (!BARE) {
       // Chunk matrices, M the token that is contracted next, N the other: (j, i) towards the
       // queries' side, (i, j) towards the keys'.
@@ -706,8 +726,15 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
                 col[im][x] += xs;
               }
             }
-            put4(sP + place<T, C>(nn, mm), p);
-            if constexpr (MODE == LA_DKV) put4(sP2 + place<T, C>(nn, mm), p2);
+            const int at_p = place<T, C>(nn, mm);
+            if constexpr (PL == 1) {
+              put4(sP + at_p, p);
+              if constexpr (MODE == LA_DKV) put4(sP2 + at_p, p2);
+            } else if constexpr (MODE == LA_DKV) {
+              lo[im][jn] = put4_rest(sP + at_p, p), lo2[im][jn] = put4_rest(sP2 + at_p, p2);
+            } else {
+              *reinterpret_cast<uint2*>(sP2 + at_p) = put4_rest(sP + at_p, p);
+            }
           }
           if constexpr (MODE == LA_DQ) {
             row = mg_pair_sum<32>(mg_pair_sum<16>(row));
@@ -725,61 +752,117 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
         }
       }
       // What comes through the state: o's, dq's or dk's and dv's.
+      const T* const two[2] = {sS, sS1};
       if constexpr (MODE != LA_DQ) {
         clear<TV>(acv);
-        product<T, TV, DK, true, false, DV, DK, 1, 1>(acv, ps, REV ? pk : pq);
+        if constexpr (PL > 1) product<T, TV, DK, true, false, DV, DK, 2, 1>(acv, two, REV ? pk : pq);
+        else product<T, TV, DK, true, false, DV, DK, 1, 1>(acv, ps, REV ? pk : pq);
       }
       if constexpr (GRAD) {
         clear<TK>(ack);
-        if constexpr (PL > 1) {
-          const T* const two[2] = {sS, sS1};
-          product<T, TK, DV, false, false, DV, DV, 2, 1>(ack, two, REV ? pv : po);
-        } else {
-          product<T, TK, DV, false, false, DV, DV, 1, 1>(ack, ps, REV ? pv : po);
-        }
+        if constexpr (PL > 1) product<T, TK, DV, false, false, DV, DV, 2, 1>(ack, two, REV ? pv : po);
+        else product<T, TK, DV, false, false, DV, DV, 1, 1>(ack, ps, REV ? pv : po);
       }
     }
     if constexpr (!GRAD) update(sV, sK);
     if constexpr (!BARE) __syncthreads();  // the chunk matrices are there, the state is read
 
-    const auto out_v = [&](T* to, const T* far, auto&& factor) {
-      f32x4 in[TV::TM][TV::TN];
-      clear<TV>(in);
-      const T *const af[1] = {far}, *const pp[1] = {sP};
+    // Through the plane p of a chunk matrix, added to what is there.
+    const auto sum_v = [&](f32x4 (&in)[TV::TM][TV::TN], const T* far, const T* p) {
+      const T *const af[1] = {far}, *const pp[1] = {p};
       product<T, TV, C, true, false, DV, C, 1, 1>(in, af, pp);
+    };
+    const auto sum_k = [&](f32x4 (&in)[TK::TM][TK::TN], const T* p) {
+      const T *const af[1] = {REV ? sQ : sK}, *const pp[1] = {p};
+      product<T, TK, C, true, false, DK, C, 1, 1>(in, af, pp);
+    };
+    const auto scale_v = [&](auto&& factor) {
+#pragma unroll
+      for (int j = 0; j < TV::TN; ++j) {
+        const float f = factor(TV::n0(j) + lr);
+#pragma unroll
+        for (int m = 0; m < TV::TM; ++m) acv[m][j] = times(f, acv[m][j]);
+      }
+    };
+    const auto out_v = [&](T* to) {
       if (TV::live()) {
         T* const base = to + ((b * T_ + t) * a.H + h) * dv;
 #pragma unroll
         for (int j = 0; j < TV::TN; ++j) {
           const int i = TV::n0(j) + lr;
-          const float f = factor(i);
           if (i < rows) {
             T* const p = base + (unsigned)i * (unsigned)(a.H * dv);
 #pragma unroll
-            for (int m = 0; m < TV::TM; ++m)
-              store4<WIDE>(p, TV::m0(m) + 4 * lg, dv, in[m][j] + times(f, acv[m][j]));
+            for (int m = 0; m < TV::TM; ++m) store4<WIDE>(p, TV::m0(m) + 4 * lg, dv, acv[m][j]);
           }
         }
       }
     };
-    if constexpr (MODE == LA_OUT)
-      out_v((T*)a.out, sV, [&](int i) { return a.scale * span0(ga[i]); });
-    if constexpr (MODE == LA_DKV)
-      out_v((T*)a.out2, sO, [&](int i) { return span(end, ga[i]); });
+    if constexpr (MODE == LA_OUT) {
+      scale_v([&](int i) { return a.scale * span0(ga[i]); });
+      sum_v(acv, sV, sP);
+      if constexpr (PL > 1) sum_v(acv, sV, sP2);
+      out_v((T*)a.out);
+    }
+    if constexpr (MODE == LA_DKV) {
+      scale_v([&](int i) { return span(end, ga[i]); });
+      sum_v(acv, sO, sP);
+      if constexpr (PL == 1) out_v((T*)a.out2);
+    }
     if constexpr (GRAD) {
-      // dq or dk of the chunk itself, then the state's third plane.
-      f32x4 in[TK::TM][TK::TN];
-      clear<TK>(in);
-      const T *const rk[1] = {REV ? sQ : sK}, *const pp[1] = {REV ? sP2 : sP};
-      product<T, TK, C, true, false, DK, C, 1, 1>(in, rk, pp);
-      if constexpr (PL > 1)
+      // The planes that had no room before: the state's third one, and dk's and dv's matrices' second
+      // ones; dq of the chunk itself.
+      if constexpr (PL > 1) {
         each_tile([&](int i, int j, int r, int c) {
           *reinterpret_cast<uint2*>(sS + place<T, DV>(r, c)) = third[i][j];
         });
-      __syncthreads();  // the chunk's rows are read, the third plane is there
+        if constexpr (MODE == LA_DKV)
+          if (TC::live())
+#pragma unroll
+            for (int jn = 0; jn < TC::TN; ++jn)
+#pragma unroll
+              for (int im = 0; im < TC::TM; ++im) {
+                const int at_p = place<T, C>(TC::n0(jn) + lr, TC::m0(im) + 4 * lg);
+                *reinterpret_cast<uint2*>(sS1 + at_p) = lo[im][jn];
+                *reinterpret_cast<uint2*>(sS1 + C * C + at_p) = lo2[im][jn];
+              }
+      }
+      f32x4 in[TK::TM][TK::TN];
+      if constexpr (MODE == LA_DQ) {
+        clear<TK>(in);
+        sum_k(in, sP);
+        if constexpr (PL > 1) sum_k(in, sP2);
+      }
+      __syncthreads();  // those planes are there
       if constexpr (PL > 1) {
+        if constexpr (MODE == LA_DKV) {
+          sum_v(acv, sO, sS1);
+          out_v((T*)a.out2);
+        }
         const T *const third[1] = {sS}, *const rv[1] = {REV ? sV : sO};
         product<T, TK, DV, false, false, DV, DV, 1, 1>(ack, third, rv);
+      }
+      if (TK::live()) {
+#pragma unroll
+        for (int j = 0; j < TK::TN; ++j) {
+          const int i = TK::n0(j) + lr;
+          const float f = REV ? span(end, ga[i]) : a.scale * span0(ga[i]);
+          float dot = 0.f;
+#pragma unroll
+          for (int m = 0; m < TK::TM; ++m) {
+            ack[m][j] = times(f, ack[m][j]);
+            const f32x4 x = get4((REV ? sK : sQ) + place<T, DK>(i, TK::m0(m) + 4 * lg));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) dot += ack[m][j][u] * x[u];
+            if constexpr (MODE == LA_DQ) ack[m][j] += in[m][j];
+          }
+          dot = mg_pair_sum<32>(mg_pair_sum<16>(dot));
+          if (lane < 16) s_dot[TK::wm()][i] = dot;
+        }
+      }
+      if constexpr (MODE == LA_DKV) {
+        sum_k(ack, sP2);
+        if constexpr (PL > 1) sum_k(ack, sS1 + C * C);
       }
       if (TK::live()) {
         const int64_t base = ((b * T_ + t) * a.H + h) * dk;
@@ -788,22 +871,15 @@ __global__ __launch_bounds__(NT, 2) void la_sweep(LaArgs a) {
 #pragma unroll
         for (int j = 0; j < TK::TN; ++j) {
           const int i = TK::n0(j) + lr;
-          const float f = REV ? span(end, ga[i]) : a.scale * span0(ga[i]);
           const unsigned row = (unsigned)i * (unsigned)(a.H * dk);
-          float dot = 0.f;
+          if (i < rows) {
 #pragma unroll
-          for (int m = 0; m < TK::TM; ++m) {
-            const int c = TK::m0(m) + 4 * lg;
-            const f32x4 y = times(f, ack[m][j]), x = get4((REV ? sK : sQ) + place<T, DK>(i, c));
-#pragma unroll
-            for (int u = 0; u < 4; ++u) dot += y[u] * x[u];
-            if (i < rows) {
-              if (a.part) store4<WIDE>(part + row, c, dk, y + in[m][j]);
-              else store4<WIDE>(out + row, c, dk, y + in[m][j]);
+            for (int m = 0; m < TK::TM; ++m) {
+              const int c = TK::m0(m) + 4 * lg;
+              if (a.part) store4<WIDE>(part + row, c, dk, ack[m][j]);
+              else store4<WIDE>(out + row, c, dk, ack[m][j]);
             }
           }
-          dot = mg_pair_sum<32>(mg_pair_sum<16>(dot));
-          if (lane < 16) s_dot[TK::wm()][i] = dot;
         }
       }
       update(REV ? sO : sV, REV ? sQ : sK);
