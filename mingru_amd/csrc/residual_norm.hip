@@ -211,10 +211,19 @@ __device__ __forceinline__ float2 rn_stats(const float (&v)[8], int kind, int c,
   return make_float2(mean, 1.f / sqrtf(q[0] * inv + eps));
 }
 
-// 1 / (1 + e^-x) from the hardware's exponential and reciprocal, each 1 ulp off at most but for
-// the rounding of x log2 e: 1e-7 of the result for |x| < 1, 5e-7 at |x| = 10.
+// 1 / (1 + e^-x) from the hardware's exponential and reciprocal, each 1 ulp off at most.  For fp32
+// rows, what the product x log2 e rounds off is put back: 2e-7 of the result at any x, where it would
+// be up to 6e-8 |x| (4e-6 at -87).  An infinite x leaves a NaN in the factor, which fmaxf drops.
+// For bf16 rows, rounded to 2^-9, it stays off (norm-train 389 us, with it 397).
+template <typename E>
 __device__ __forceinline__ float rn_sigmoid(float x) {
-  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+  const float t = -1.44269502f * x;  // log2 e = 1.44269502 + 1.92596e-8
+  float e = __builtin_amdgcn_exp2f(t);
+  if constexpr (sizeof(E) == 4) {
+    const float rest = fmaf(-1.92596299e-8f, x, fmaf(-1.44269502f, x, -t));
+    e *= fmaxf(fmaf(0.693147181f, rest, 1.f), 0.5f);
+  }
+  return __builtin_amdgcn_rcpf(1.f + e);
 }
 
 template <typename E, typename P, int TPR, bool VEC>
@@ -243,7 +252,7 @@ __global__ __launch_bounds__(rn_threads(TPR)) void residual_norm_fwd(RnArgs a) {
     if (a.act) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float s = rn_sigmoid(gv[i]);
+        const float s = rn_sigmoid<E>(gv[i]);
         u[i] *= a.act == RN_SILU ? s * gv[i] : s;
       }
     }
@@ -340,7 +349,7 @@ __global__ __launch_bounds__(rn_threads(TPR)) void residual_norm_bwd(RnArgs a) {
     for (int i = 0; i < 8; ++i) {
       f[i] = 1.f, slope[i] = 0.f;
       if (a.act) {
-        const float s = rn_sigmoid(gv[i]), ds = s * (1.f - s);
+        const float s = rn_sigmoid<E>(gv[i]), ds = s * (1.f - s);
         f[i] = a.act == RN_SILU ? s * gv[i] : s;
         slope[i] = a.act == RN_SILU ? s + gv[i] * ds : ds;
       }
