@@ -244,7 +244,8 @@ def linear_attention(q, k, v, log_decay, h_0=None, lengths=None, scale=None):
     """Attention through a state that decays: a prompt's or a training batch's whole pass.
 
     ``S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T`` and ``o_t = scale * S_t^T q_t`` for each
-    sequence and head.
+    sequence and head.  On the GPU the kernels take head sizes up to 128; larger ones run the
+    eager body, with the warning of a decline.
 
     Parameters
     ----------
@@ -331,7 +332,8 @@ _REDUCTIONS = ("none", "mean", "sum")
 def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index=-100, reduction="mean"):
     """Softmax cross entropy of ``x @ weight.T + bias`` against ``target``, without keeping the
     logits: on the GPU they are formed tile by tile, and again in the backward pass in pieces of
-    the vocabulary.
+    the vocabulary.  There, with more than 128 rows, float32 weights are held to 2**-39 of their
+    largest magnitude.
 
     Parameters
     ----------
