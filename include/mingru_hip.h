@@ -504,11 +504,12 @@ int mg_linear_attention_step(int dtype, const void* q, const void* k, const void
  * ignore_index are left out; another target outside the vocabulary gives a NaN.  reduction: 0
  * none (loss (N)), 1 mean over the counted rows (0 if there are none), 2 sum.
  * state: what the forward leaves for the backward.  Backward: dloss is (N) or a scalar; dx
- * (N, D) and dw (V, D) with db (V) may be NULL, db only together with dw.  Sizes up to 2^30
- * rows and entries and D up to 2^20. */
+ * (N, D) and dw (V, D) with db (V) may be NULL, db only together with dw; without dx the
+ * workspace may lack dx_bytes of its size.  Sizes up to 2^30 rows and entries and D up to 2^20. */
 size_t mg_vocab_loss_state_bytes(int dtype, int64_t N, int64_t V, int64_t D);
 size_t mg_vocab_loss_fwd_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D);
 size_t mg_vocab_loss_bwd_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t D);
+size_t mg_vocab_loss_bwd_dx_bytes(int dtype, int64_t N, int64_t V, int64_t D);
 int mg_vocab_loss_fwd(int dtype, const void* x, int64_t ldx, const void* w, const void* bias,
                       const int64_t* target, int64_t ignore_index, int reduction, float* loss,
                       int64_t N, int64_t V, int64_t D, void* state, size_t state_bytes, void* ws,

@@ -146,6 +146,7 @@ _SIGNATURES = {
     "mg_vocab_loss_state_bytes": (_SZ, [_I32, _I64, _I64, _I64]),
     "mg_vocab_loss_fwd_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64]),
     "mg_vocab_loss_bwd_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64]),
+    "mg_vocab_loss_bwd_dx_bytes": (_SZ, [_I32, _I64, _I64, _I64]),
     "mg_vocab_loss_fwd": (
         _I32,
         [_I32, _P, _I64, _P, _P, _P, _I64, _I32, _P, _I64, _I64, _I64, _P, _SZ, _P, _SZ, _P],

@@ -998,14 +998,15 @@ struct Back {
   int dx_splits, dw_splits;
   float *g, *scale, *w_scale, *d_scale, *top, *back, *weight, *sxw, *dx_part, *dw_part, *db_part;
   u16 *d, *xw;  // xw: x's packed rows times their weights
-  size_t bytes;
+  size_t bytes, dx_bytes;  // dx_part is last, and not needed without dx
 };
 Back vl_back(const Shape& s, void* base) {
   Back b = {};
   if (s.few) {
     const int64_t d = up_to(32 * s.few * s.ldd * 4, 256), per = few_per(s);
     b.d = (u16*)base, b.dx_part = (float*)((char*)base + d);
-    b.bytes = d + (s.V + per - 1) / per * s.N * s.D * 4;
+    b.dx_bytes = (s.V + per - 1) / per * s.N * s.D * 4;
+    b.bytes = d + b.dx_bytes;
     return b;
   }
   const int64_t most = VL_D_BYTES / (s.np * 2 * s.planes);
@@ -1029,9 +1030,10 @@ Back vl_back(const Shape& s, void* base) {
     b.back = (float*)take(s.N * 4), b.weight = (float*)take(s.N * 4), b.sxw = (float*)take(4);
     b.xw = (u16*)take(s.planes * s.np * s.dx * 2);
   }
-  b.dx_part = (float*)take(b.dx_splits * s.N * s.D * 4);  // pieces add to it one after another
   b.dw_part = b.dw_splits > 1 ? (float*)take(b.dw_splits * b.vp * s.D * 4) : nullptr;
   b.db_part = b.dw_splits > 1 ? (float*)take(b.dw_splits * b.vp * 4) : nullptr;
+  b.dx_bytes = b.dx_splits * s.N * s.D * 4;
+  b.dx_part = (float*)take(b.dx_bytes);  // pieces add to it one after another
   b.bytes = p - (char*)base;
   return b;
 }
@@ -1112,6 +1114,11 @@ size_t mg_vocab_loss_bwd_workspace_bytes(int dtype, int64_t N, int64_t V, int64_
   return vl_shape(dtype, N, V, D, &s) ? vl_back(s, nullptr).bytes : 0;
 }
 
+size_t mg_vocab_loss_bwd_dx_bytes(int dtype, int64_t N, int64_t V, int64_t D) {
+  Shape s;
+  return vl_shape(dtype, N, V, D, &s) ? vl_back(s, nullptr).dx_bytes : 0;
+}
+
 int mg_vocab_loss_fwd(int dtype, const void* x, int64_t ldx, const void* w, const void* bias,
                       const int64_t* target, int64_t ignore_index, int reduction, float* loss,
                       int64_t N, int64_t V, int64_t D, void* state, size_t state_bytes, void* ws,
@@ -1171,7 +1178,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
     return MG_ERR_ARG;
   const State t = vl_state(s, const_cast<void*>(state));
   const Back b = vl_back(s, ws);
-  if (ws_bytes < b.bytes) return MG_ERR_WORKSPACE;
+  if (ws_bytes < b.bytes - (dx ? 0 : b.dx_bytes)) return MG_ERR_WORKSPACE;
   if (s.few) {
     FewArgs a = few_args(s, t, w, bias);
     a.soft = t.soft, a.up = dloss, a.reduction = reduction, a.d = (float*)b.d;

@@ -347,7 +347,10 @@ class _VocabLossFn(torch.autograd.Function):
         dx = torch.empty(ctx.shape, dtype=w.dtype, device=w.device) if need[0] else None
         db = torch.empty_like(bias) if need[2] else None
         dw = torch.empty_like(w) if need[1] or db is not None else None
-        ws = _workspace(_size("mg_vocab_loss_bwd_workspace_bytes", *ctx.size), w.device)
+        nbytes = _size("mg_vocab_loss_bwd_workspace_bytes", *ctx.size)
+        if dx is None:
+            nbytes -= _size("mg_vocab_loss_bwd_dx_bytes", *ctx.size)
+        ws = _workspace(nbytes, w.device)
         tag, N, V, D = ctx.size
         _call("mg_vocab_loss_bwd", tag, _ptr(w), _ptr(bias), _ptr(dloss.contiguous()),
               ctx.reduction, _ptr(dx), _ptr(dw), _ptr(db), N, V, D, _ptr(state), _ptr(ws),

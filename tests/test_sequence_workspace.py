@@ -29,3 +29,16 @@ def test_loss_backward_does_not_grow_with_the_vocabulary(lib, dtype, N, V, D):
     assert ws <= d + 4 * (4 * N * D) + (1 << 29), (ws, d)
     if N * V >= 1 << 32:  # what it is there for: the logits' own bytes are far more
         assert ws <= N * V * 4 / 2 + 4 * (4 * N * D), ws
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("N, V, D", [(64, 50257, 768), (4096, 32768, 1024), (262144, 128256, 4096)])
+def test_loss_backward_without_dx_lacks_its_part(lib, dtype, N, V, D):
+    whole = lib.mg_vocab_loss_bwd_workspace_bytes(dtype, N, V, D)
+    dx = lib.mg_vocab_loss_bwd_dx_bytes(dtype, N, V, D)
+    assert 4 * N * D <= dx < whole
+    P = 4096  # never followed by the refused calls
+    call = lambda to, nbytes: lib.mg_vocab_loss_bwd(  # noqa: E731
+        dtype, P, None, P, 1, to, P, None, N, V, D, P, P, nbytes, None)
+    assert call(P, whole - 1) == 3
+    assert call(None, whole - dx - 1) == 3
