@@ -518,6 +518,61 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
                       int reduction, void* dx, void* dw, void* db, int64_t N, int64_t V, int64_t D,
                       const void* state, void* ws, size_t ws_bytes, mg_stream_t stream);
 
+/* ---- a paged cache of keys and values, and the attention that reads it ---------------
+ * No reference kernels.  dtype: 0 fp32, 1 bf16, 2 fp16, of all tensors.  A cache is k_cache (N,
+ * Hk, P, dk) and v_cache (N, Hk, P, dv), N pages of P tokens; token p of sequence b lies in page
+ * pages[b, p / P] at p % P.  Last dimensions are dense, other strides are given in elements.
+ * ints: which integer arrays are int64 rather than int32, a bit each.
+ *
+ * mg_paged_append: new tokens k (B, T, Hk, dk), v (B, T, Hk, dv), token t of sequence b at
+ * position start[b] + t, go into the caches; q (B, T, H, dk) or NULL goes to q_out, dense.  With
+ * n > 0 frequencies (fp32, or fp64 for freq_dtype 1), 2 n <= dk, n <= 2048, elements i and i + n
+ * (2 i and 2 i + 1 if interleaved) of q and k turn by position times freq[i] radians.  lengths
+ * (B) or NULL: tokens of right-padded sequences; the rest has no effect but queries of 0.  A
+ * token of a negative page is not kept; one outside of its row of M pages, or of a page from N
+ * on, is not kept and its queries are NaN.  strides: q, k, v (sequence, token, head), k_cache,
+ * v_cache (page, head, slot), pages (sequence).  ints: bit 0 pages, 1 start, 2 lengths.
+ *
+ * mg_paged_attention_step: o (B, H, dv) = softmax(scale q K^T) V of q (B, H, dk) over the last
+ * `window` (0: all) of lengths[b] tokens, for dk, dv <= 256, B H < 2^24, M P < 2^31 - 1024.  A
+ * length of 0 gives 0; one above M P, or a page that is needed and not in the cache, NaN.
+ * strides: q (sequence, head), k_cache, v_cache (page, head, slot), pages (sequence).  ints: bit
+ * 0 pages, 1 lengths. */
+int mg_paged_append(int dtype, const void* q, const void* k, const void* v, void* k_cache,
+                    void* v_cache, void* q_out, const int64_t* strides, int ints,
+                    const void* pages, const void* start, const void* lengths, int freq_dtype,
+                    const void* freq, int n, int interleaved, int64_t B, int64_t T, int H, int Hk,
+                    int dk, int dv, int64_t N, int64_t M, int64_t P, mg_stream_t stream);
+size_t mg_paged_attention_workspace_bytes(int dtype, int64_t B, int H, int Hk, int dk, int dv,
+                                          int64_t M, int64_t P);
+int mg_paged_attention_step(int dtype, const void* q, const void* k_cache, const void* v_cache,
+                            const int64_t* strides, int ints, const void* pages,
+                            const void* lengths, void* o, int64_t B, int H, int Hk, int dk, int dv,
+                            int64_t N, int64_t M, int64_t P, int64_t window, float scale, void* ws,
+                            size_t ws_bytes, mg_stream_t stream);
+
+/* ---- a beam search's selection, and the reordering of states --------------------------
+ * No reference kernels.  mg_beam_select: the W <= 64 best of the candidates scores[b, k] +
+ * logits[b, k, v] - log(sum(exp(logits[b, k]))) of K <= 256 beams and V tokens, B K < 2^22, K V <
+ * 2^31; equal ones by the lower k, then the lower v.  logits (B, K, V) in dtype (0 fp32, 1 bf16,
+ * 2 fp16), its last dimension dense; scores fp32; finished (B, K) bytes or NULL: beams whose one
+ * candidate is the token `end` (-1: none) at the beam's score.  Beams whose score or sum is not
+ * finite have candidates of -inf.  out, parents, tokens, done (bytes; NULL without end) are (B, W),
+ * dense.  strides in elements: logits (b, k), scores (b, k), finished (b, k).
+ *
+ * mg_reorder_rows: row b W + w of each of `count` tensors dst becomes row b K + parents[b, w] of
+ * its src, 0 where that is not one of K.  strides: bytes between rows of src; bytes: of a row
+ * (those of dst follow one another); src, dst, strides, bytes are host arrays.  parents (B, W) is
+ * int32, or int64 if wide, with pb and pw elements between its rows and columns. */
+size_t mg_beam_select_workspace_bytes(int dtype, int64_t B, int64_t K, int64_t V, int W);
+int mg_beam_select(int dtype, const void* logits, const float* scores, const void* finished,
+                   const int64_t* strides, int64_t end, float* out, int64_t* parents,
+                   int64_t* tokens, void* done, int64_t B, int64_t K, int64_t V, int W, void* ws,
+                   size_t ws_bytes, mg_stream_t stream);
+int mg_reorder_rows(int count, const void* const* src, void* const* dst, const int64_t* strides,
+                    const int64_t* bytes, int wide, const void* parents, int64_t pb, int64_t pw,
+                    int64_t B, int64_t K, int64_t W, mg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,8 +5,8 @@ Public surface (same names and signatures as chris-santiago/minGRU,
 ``MinGRUStack`` and the scan primitives ``parallel_scan_log``, ``linear_scan``,
 ``matrix_scan``, ``matrix_affine_scan``.
 
-Beside them stand the operators of :mod:`mingru_amd.sequence_ops`, which the reference
-does not have.
+Beside them stand the operators of :mod:`mingru_amd.sequence_ops` and
+:mod:`mingru_amd.decode_ops`, which the reference does not have.
 
 The GPU backend, :mod:`mingru_amd.hip_scans`, is never imported by
 ``import mingru_amd``: its public names resolve lazily (PEP 562) on first
@@ -15,6 +15,8 @@ access, and the ``MINGRU_SCAN`` seam imports it only for GPU tensors.
 
 from .min_gru import *  # noqa: F401,F403
 from .min_gru import __all__ as _min_gru_all
+from .decode_ops import *  # noqa: F401,F403
+from .decode_ops import __all__ as _decode_all
 from .sequence_ops import *  # noqa: F401,F403
 from .sequence_ops import __all__ as _sequence_all
 
@@ -28,7 +30,7 @@ _BACKEND_EXPORTS = (
     "delta_scan_impl",
 )
 
-__all__ = [*_min_gru_all, *_sequence_all, "__version__"]
+__all__ = [*_min_gru_all, *_sequence_all, *_decode_all, "__version__"]
 
 
 def __getattr__(name: str) -> object:

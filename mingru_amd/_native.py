@@ -30,6 +30,7 @@ _I32 = ctypes.c_int
 _F32 = ctypes.c_float
 _SZ = ctypes.c_size_t
 _PI64 = ctypes.POINTER(ctypes.c_int64)
+_PP = ctypes.POINTER(ctypes.c_void_p)
 
 _SIGNATURES = {
     "mg_linear_scan_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
@@ -162,6 +163,25 @@ _SIGNATURES = {
         _I32,
         [_I32] * 5 + [_P, _I64] * 3 + [_P, _F32] + [_P] * 4 + [_P, _I64] * 2 + [_P] * 8
         + [_I64, _I64, _F32, _P, _SZ, _P],
+    ),
+    "mg_paged_append": (
+        _I32,
+        [_I32] + [_P] * 6 + [_PI64, _I32] + [_P] * 3 + [_I32, _P, _I32, _I32, _I64, _I64]
+        + [_I32] * 4 + [_I64] * 3 + [_P],
+    ),
+    "mg_paged_attention_workspace_bytes": (_SZ, [_I32, _I64] + [_I32] * 4 + [_I64] * 2),
+    "mg_paged_attention_step": (
+        _I32,
+        [_I32] + [_P] * 3 + [_PI64, _I32] + [_P] * 3 + [_I64] + [_I32] * 4 + [_I64] * 4
+        + [_F32, _P, _SZ, _P],
+    ),
+    "mg_beam_select_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64, _I32]),
+    "mg_beam_select": (
+        _I32,
+        [_I32] + [_P] * 3 + [_PI64, _I64] + [_P] * 4 + [_I64] * 3 + [_I32, _P, _SZ, _P],
+    ),
+    "mg_reorder_rows": (
+        _I32, [_I32, _PP, _PP, _PI64, _PI64, _I32, _P] + [_I64] * 5 + [_P],
     ),
 }
 

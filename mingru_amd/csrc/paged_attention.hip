@@ -1,0 +1,676 @@
+// Attention of each sequence's newest token over a paged cache (gfx950).
+//
+//   s_j = scale q . k_j;  o = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s)
+// over a sequence's last tokens, for each head; the heads of a group share a key head.
+//
+// Bound by memory: every key and value is read once.  The unit of work is a tile of 32 tokens
+// (16 in fp32) of one key head, held by one wave, for 16 query heads of the group on the matrix
+// cores: rows beyond the group are idle there, but at 16 rows a bf16 tile of 16 KB costs about
+// 260 cycles of matrix instructions, where its share of the memory's rate is 2000.
+//
+// Sums as the matrix cores take them (lane = 16 g + c, g < 4):
+// * A lane loads its tile's tokens 4 g + j (and 16 + 4 g + j), 1/16 of a row (chunk c) of each, so
+//   that a wave's load covers whole rows of four tokens.
+// * S^T = K Q^T.  The keys go through LDS, rows padded by 16 bytes, private to the wave: no
+//   barrier.  The result has query c in lane's column c, tokens 4 g + i in its registers.
+// * O^T = V^T P^T.  The tokens that a lane's probabilities belong to are the tokens whose values
+//   it loaded, so neither moves between lanes: the product's rows are the elements E c + e of
+//   all chunks c at one e (E elements a chunk), a fragment of them is a lane's element e of
+//   each of its tokens.
+// * Half types' probabilities are two summands of their type, so that their rounding is 2^-16
+//   (bf16) of them: one of 2^-9 is as large as the result's own.
+// Maxima, sums and O are fp32, with O scaled again only where a maximum rises.
+//
+// Work is divided on the device, where the lengths are: the steps (four tiles, one for each wave
+// of a workgroup) of all sequences and key heads form one row, cut into equal shares for as
+// many workgroups as the chip holds at once.  So ragged batches, one long sequence and many short
+// ones all keep every CU busy, and the host looks at no length.  A share that holds all steps of
+// a head writes its output; others leave (max, sum, O) to a second launch, in a fixed order.
+#include "mg_paged.h"
+
+namespace {
+
+constexpr int PA_NW = 4, PA_NT = PA_NW * MG_WAVE, PA_ROWS = 16;
+
+struct PaArgs {
+  const void *q, *k, *v;
+  void* o;
+  Ints pages, lengths;
+  int64_t qs[2];          // strides in elements: sequence, head
+  int64_t ks[3], vs[3];   // page, head, slot
+  int64_t page_stride;
+  int64_t B, N;
+  int64_t room;           // tokens that a row of pages holds
+  int64_t window;         // 0: all tokens
+  Divisor P;
+  int H, Hk, group, tiles_q, dk, dv;
+  float scale;            // times log2 e
+  int shares;
+  float* part;            // (2 shares, rows, dv) sums, then (2 shares, rows, 2) maxima and sums
+  int rows;
+};
+
+// ---- element types ---------------------------------------------------------------------
+template <typename T>
+struct Elem;
+template <>
+struct Elem<Bf16> {
+  static constexpr int KEYS = 32, PAD = 8;
+  typedef bf16x8 Frag;
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ unsigned pack(float x, float y) {
+    const bf16x2 h = {(__bf16)x, (__bf16)y};
+    unsigned u = __builtin_bit_cast(unsigned, h);
+    asm("" : "+v"(u));  // keeps the pair one packed conversion
+    return u;
+  }
+  static __device__ __forceinline__ float low(unsigned u) { return __uint_as_float(u << 16); }
+  static __device__ __forceinline__ float high(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+};
+template <>
+struct Elem<Fp16> {
+  static constexpr int KEYS = 32, PAD = 8;
+  typedef f16x8 Frag;
+  static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ unsigned pack(float x, float y) {
+    const f16x2 h = {(_Float16)x, (_Float16)y};
+    return __builtin_bit_cast(unsigned, h);
+  }
+  static __device__ __forceinline__ float low(unsigned u) {
+    return (float)__builtin_bit_cast(f16x2, u)[0];
+  }
+  static __device__ __forceinline__ float high(unsigned u) {
+    return (float)__builtin_bit_cast(f16x2, u)[1];
+  }
+};
+template <>
+struct Elem<float> {
+  static constexpr int KEYS = 16, PAD = 4;
+};
+
+// A lane's chunk of a row: E elements in registers of 32 bits.
+template <typename T, int E>
+struct Chunk {
+  static constexpr int W = E * sizeof(T) / 4;
+  unsigned w[W];
+};
+
+// Chunk c of a row of d elements.  VEC: d, strides and pointers are multiples of 16 bytes (8
+// where a chunk is 8), so that a vector lies in the row or behind it as a whole.  What lies
+// behind is read from the row's start and set to 0 later (pa_clear).
+template <typename T, int E, bool VEC>
+__device__ __forceinline__ void pa_load(const T* row, int c, int d, Chunk<T, E>& x) {
+  constexpr int W = Chunk<T, E>::W;
+  if constexpr (VEC) {
+    constexpr int L = W < 4 ? W : 4, VE = L * 4 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < W / L; ++i) {
+      const int at = c * E + i * VE;
+      const T* p = row + (at < d ? at : 0);
+      if constexpr (L == 2) {
+        const u32x2 v = *(const u32x2*)p;
+        x.w[0] = v[0], x.w[1] = v[1];
+      } else {
+        const u32x4 v = *(const u32x4*)p;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x.w[4 * i + j] = v[j];
+      }
+    }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int at = c * E + i;
+      x.w[i] = ((const unsigned*)row)[at < d ? at : 0];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int at = c * E + 2 * i;
+      const unsigned lo = ((const u16*)row)[at < d ? at : 0];
+      const unsigned hi = ((const u16*)row)[at + 1 < d ? at + 1 : 0];
+      x.w[i] = lo | hi << 16;
+    }
+  }
+}
+// Elements from d on become 0.
+template <typename T, int E>
+__device__ __forceinline__ void pa_clear(int c, int d, Chunk<T, E>& x) {
+#pragma unroll
+  for (int i = 0; i < Chunk<T, E>::W; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      x.w[i] = c * E + i < d ? x.w[i] : 0u;
+    } else {
+      const int at = c * E + 2 * i;
+      x.w[i] = at + 1 < d ? x.w[i] : (at < d ? x.w[i] & 0xffffu : 0u);
+    }
+  }
+}
+
+__device__ __forceinline__ float pa_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// Maximum and sum over the lanes of one column (g of lane = 16 g + c), in all of them.
+__device__ __forceinline__ float pa_max(float x) {
+  unsigned u = __float_as_uint(x);
+  auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  u = __float_as_uint(x);
+  r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pa_sum(float x) { return mg_pair_sum<32>(mg_pair_sum<16>(x)); }
+
+// ---- the division of work --------------------------------------------------------------
+// A sequence's tokens that count, [first, end), and the steps of SPAN tokens that hold them.
+struct PaSeq {
+  int64_t first, end;
+  int64_t step0, steps;  // of one key head
+  bool bad;              // longer than its pages
+};
+template <int SPAN>
+__device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, int64_t b) {
+  PaSeq s;
+  int64_t n = a.lengths[b];
+  s.bad = n > a.room;
+  n = n < 0 ? 0 : (s.bad ? a.room : n);
+  s.end = n;
+  s.first = a.window && n > a.window ? n - a.window : 0;
+  s.step0 = s.first / SPAN;
+  s.steps = n > 0 ? (n + SPAN - 1) / SPAN - s.step0 : 0;
+  return s;
+}
+
+// The sum of all steps, and of those before sequence `upto` (a sequence's pairs of a key head and
+// 16 of its queries come one after another).  The whole workgroup calls it.
+struct PaSums {
+  int64_t all, before;
+};
+template <int SPAN>
+__device__ __forceinline__ PaSums pa_sums(const PaArgs& a, int64_t upto, int64_t* lds) {
+  int64_t all = 0, before = 0;
+  for (int64_t b = threadIdx.x; b < a.B; b += PA_NT) {
+    const int64_t n = pa_seq<SPAN>(a, b).steps;
+    all += n;
+    before += b < upto ? n : 0;
+  }
+#pragma unroll
+  for (int d = 1; d < MG_WAVE; d *= 2) {
+    all += __shfl_xor(all, d);
+    before += __shfl_xor(before, d);
+  }
+  if ((threadIdx.x & (MG_WAVE - 1)) == 0) {
+    lds[2 * (threadIdx.x / MG_WAVE)] = all;
+    lds[2 * (threadIdx.x / MG_WAVE) + 1] = before;
+  }
+  __syncthreads();
+  PaSums s = {0, 0};
+  for (int w = 0; w < PA_NW; ++w) s.all += lds[2 * w], s.before += lds[2 * w + 1];
+  __syncthreads();
+  const int64_t pairs = (int64_t)a.Hk * a.tiles_q;
+  s.all *= pairs, s.before *= pairs;
+  return s;
+}
+// Share w of `shares` holds the steps [w all / shares, (w + 1) all / shares).
+__device__ __forceinline__ int64_t pa_share(int64_t w, int64_t all, int shares) {
+  return w * all / shares;
+}
+__device__ __forceinline__ int64_t pa_holder(int64_t step, int64_t all, int shares) {
+  return ((step + 1) * shares - 1) / all;
+}
+
+// ---- the main kernel -------------------------------------------------------------------
+template <typename T, int D>
+struct PaShape {
+  static constexpr int KEYS = Elem<T>::KEYS;    // tokens of a tile
+  static constexpr int SPAN = KEYS * PA_NW;     // of a step
+  static constexpr int E = D / 16;              // elements of a chunk
+  static constexpr int NK = KEYS / 4;           // tokens of a lane
+  static constexpr int LD = D + Elem<T>::PAD;   // elements of a key's row in LDS
+  static constexpr int OLD = D + 4;             // floats of an output row in LDS
+  static constexpr int BYTES = KEYS * LD * sizeof(T);  // of a wave
+  // Workgroups of a CU: at D = 256 a tile, its successor, queries and outputs need 300 registers.
+  static constexpr int GROUPS = D == 256 ? 1 : 2;
+  static_assert(PA_ROWS * OLD * 4 <= BYTES, "the outputs lie where the keys were");
+};
+
+// FOURS: pages hold a multiple of 4 tokens, so that a lane's tokens 4 g + j share one.
+template <typename T, int D, bool VEC, bool FOURS>
+__global__ __launch_bounds__(PA_NT, (PaShape<T, D>::GROUPS)) void paged_attention(PaArgs a) {
+  typedef PaShape<T, D> S;
+  constexpr int KEYS = S::KEYS, E = S::E, NK = S::NK, LD = S::LD, OLD = S::OLD, SPAN = S::SPAN;
+  constexpr int NG = NK / 4;  // groups of four tokens of a lane
+  typedef Chunk<T, E> C;
+  __shared__ alignas(16) unsigned char s_tile[PA_NW][S::BYTES];
+  __shared__ float s_max[PA_NW][PA_ROWS], s_sum[PA_NW][PA_ROWS];
+  __shared__ int64_t s_find[2 * PA_NW];
+
+  const int lane = threadIdx.x & (MG_WAVE - 1), wave = (int)mg_uniform(threadIdx.x / MG_WAVE);
+  const int c = lane & 15, g = lane >> 4;
+  T* const tile = (T*)s_tile[wave];
+  float* const sums = (float*)s_tile[wave];
+
+  // This share's first step, and the sequence that it lies in.
+  const int64_t all = pa_sums<SPAN>(a, 0, s_find).all;
+  int64_t at = pa_share(blockIdx.x, all, a.shares);
+  const int64_t stop = pa_share(blockIdx.x + 1, all, a.shares);
+  if (at >= stop) return;
+  const int64_t pairs = (int64_t)a.Hk * a.tiles_q;
+  int64_t b = 0, before = 0;
+  {
+    // Each thread sums a run of sequences; the one whose run holds the step looks it up there.
+    const int64_t run = (a.B + PA_NT - 1) / PA_NT, b0 = run * threadIdx.x;
+    int64_t n = 0;
+    for (int64_t i = b0; i < b0 + run && i < a.B; ++i) n += pa_seq<SPAN>(a, i).steps;
+    n *= pairs;
+    int64_t sum = n;
+#pragma unroll
+    for (int d = 1; d < MG_WAVE; d *= 2) {
+      const int64_t up = __shfl_up(sum, d);
+      sum += lane >= d ? up : 0;
+    }
+    if (lane == MG_WAVE - 1) s_find[wave] = sum;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) sum += s_find[w];
+    __syncthreads();
+    int64_t start = sum - n;
+    if (at >= start && at < sum) {
+      int64_t i = b0;
+      for (;; ++i) {
+        const int64_t m = pa_seq<SPAN>(a, i).steps * pairs;
+        if (at < start + m) break;
+        start += m;
+      }
+      s_find[0] = i, s_find[1] = start;
+    }
+    __syncthreads();
+    b = s_find[0], before = s_find[1];
+  }
+  const bool short_k = D != a.dk;
+  bool head = true;  // of this share
+  while (at < stop) {
+    PaSeq seq = pa_seq<SPAN>(a, b);
+    while (at >= before + seq.steps * pairs) {
+      before += seq.steps * pairs;
+      seq = pa_seq<SPAN>(a, ++b);
+    }
+    const int64_t pair = (at - before) / seq.steps, in = at - before - pair * seq.steps;
+    const int64_t here = seq.steps - in < stop - at ? seq.steps - in : stop - at;
+    const int hk = (int)(pair / a.tiles_q), q0 = (int)(pair - (int64_t)hk * a.tiles_q) * PA_ROWS;
+    const int rows = a.group - q0 < PA_ROWS ? a.group - q0 : PA_ROWS;
+    const T* const kc = (const T*)a.k + hk * a.ks[1];
+    const T* const vc = (const T*)a.v + hk * a.vs[1];
+    const int64_t table = b * a.page_stride;
+    const int first = (int)seq.first, end = (int)seq.end;
+
+    // Queries: column c, the elements that a key's fragment holds, 0 behind the head's.
+    constexpr int QW = D * sizeof(T) / 16 / 4;  // vectors of 16 bytes
+    u32x4 qf[QW];
+    {
+      const T* row = (const T*)a.q + b * a.qs[0] + (int64_t)(hk * a.group + q0 + (c < rows ? c : 0)) * a.qs[1];
+      constexpr int VE = 16 / sizeof(T);
+#pragma unroll
+      for (int s = 0; s < QW; ++s) {
+        Chunk<T, VE> x;
+        pa_load<T, VE, false>(row, 4 * s + g, a.dk, x);
+        pa_clear<T, VE>(4 * s + g, a.dk, x);
+        qf[s] = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
+      }
+    }
+
+    f32x4 o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float top = -__builtin_inff(), sum = 0.f;
+
+    // The first token of this wave's tile in step i of this piece.
+    const int base0 = (int)((seq.step0 + in) * SPAN) + wave * KEYS;
+    C kr[NK], vr[NK];
+    int page[FOURS ? NG : NK];  // -1: not in the cache
+    // The pages of a tile's tokens; tokens behind the last take its page.
+    auto look = [&](int base) {
+#pragma unroll
+      for (int i = 0; i < (FOURS ? NG : NK); ++i) {
+        int key = base + (FOURS ? 16 * i + 4 * g : 16 * (i / 4) + 4 * g + i % 4);
+        key = key < end ? key : end - 1;
+        const int64_t p = a.pages[table + pg_div((unsigned)key, a.P)];
+        page[i] = p >= 0 && p < a.N ? (int)p : -1;
+      }
+    };
+    unsigned bad = 0, bad_next = 0;  // tokens of this lane whose page is not in the cache
+    int64_t vo[FOURS ? NG : NK];
+    // Loads of the keys, from the pages that were looked up; the values' places are kept.
+    auto keys = [&](int base) {
+      bad_next = 0;
+#pragma unroll
+      for (int i = 0; i < (FOURS ? NG : NK); ++i) {
+        int key = base + (FOURS ? 16 * i + 4 * g : 16 * (i / 4) + 4 * g + i % 4);
+        const int last = FOURS ? (end - 1) & ~3 : end - 1;
+        key = key < end ? key : last;
+        const int slot = key - (int)(pg_div((unsigned)key, a.P) * a.P.d);
+        bad_next |= page[i] < 0 ? 1u << i : 0u;
+        const int64_t p = page[i] < 0 ? 0 : page[i];
+        vo[i] = p * a.vs[0] + slot * a.vs[2];
+        const T* row = kc + p * a.ks[0] + slot * a.ks[2];
+        if constexpr (FOURS) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            pa_load<T, E, VEC>(row + j * a.ks[2], c, a.dk, kr[4 * i + j]);
+        } else {
+          pa_load<T, E, VEC>(row, c, a.dk, kr[i]);
+        }
+      }
+    };
+    auto values = [&] {
+#pragma unroll
+      for (int i = 0; i < (FOURS ? NG : NK); ++i) {
+        const T* row = vc + vo[i];
+        if constexpr (FOURS) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            pa_load<T, E, VEC>(row + j * a.vs[2], c, a.dv, vr[4 * i + j]);
+        } else {
+          pa_load<T, E, VEC>(row, c, a.dv, vr[i]);
+        }
+      }
+    };
+    look(base0);
+    keys(base0);
+    values();
+    look(here > 1 ? base0 + SPAN : end);
+    for (int64_t i = 0; i < here; ++i) {
+      const int base = base0 + (int)i * SPAN;
+      // Keys into LDS, and the next tile's on their way.
+#pragma unroll
+      for (int j = 0; j < NK; ++j) {
+        if (short_k) pa_clear<T, E>(c, a.dk, kr[j]);
+        T* dst = tile + (16 * (j / 4) + 4 * g + j % 4) * LD + c * E;
+        if constexpr (C::W == 2) {
+          *(u32x2*)dst = u32x2{kr[j].w[0], kr[j].w[1]};
+        } else {
+#pragma unroll
+          for (int w = 0; w < C::W; w += 4)
+            *(u32x4*)((unsigned*)dst + w) =
+                u32x4{kr[j].w[w], kr[j].w[w + 1], kr[j].w[w + 2], kr[j].w[w + 3]};
+        }
+      }
+      bad = bad_next;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      // Under no condition: loads under one would be waited for where the branches meet.  Behind
+      // the piece every lane asks for the last token, one row.
+      const int next = i + 1 < here ? base + SPAN : end;
+      keys(next);
+      look(i + 2 < here ? next + SPAN : end);
+      // A wave without a token here (the ends of the row of tokens) has nothing to add.
+      if (base < end && base + KEYS > first) {
+        f32x4 s[NG];
+#pragma unroll
+        for (int t = 0; t < NG; ++t) {
+          s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int x = 0; x < QW; ++x) {
+            const u32x4 kf = *(const u32x4*)((const unsigned char*)(tile + (16 * t + c) * LD) + 64 * x + 16 * g);
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                    __uint_as_float(kf[e]), __uint_as_float(qf[x][e]), s[t], 0, 0, 0);
+            } else {
+              s[t] = Elem<T>::mma(kf, qf[x], s[t]);
+            }
+          }
+        }
+        float p[NK], peak = -__builtin_inff();
+        const bool whole = base >= first && base + KEYS <= end && __ballot(bad != 0) == 0;
+#pragma unroll
+        for (int j = 0; j < NK; ++j) p[j] = s[j / 4][j % 4] * a.scale;
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < NK; ++j) {
+            const int key = base + 16 * (j / 4) + 4 * g + j % 4;
+            const bool live = key >= first && key < end;
+            const bool lost = bad >> (FOURS ? j / 4 : j) & 1;
+            p[j] = live ? (lost ? __builtin_nanf("") : p[j]) : -__builtin_inff();
+            // 0 times a value that is not finite would be a NaN.
+#pragma unroll
+            for (int w = 0; w < C::W; ++w) vr[j].w[w] = live ? vr[j].w[w] : 0u;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NK; ++j) peak = fmaxf(peak, p[j]);
+        peak = fmaxf(pa_max(peak), top);
+        const float from = peak == -__builtin_inff() ? 0.f : peak;
+        if (__ballot(peak > top) != 0) {
+          const float down = pa_exp2(top - from);
+          sum *= down;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] *= down;
+          top = peak;
+        }
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+          p[j] = pa_exp2(p[j] - from);
+          sum += p[j];
+        }
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int j = 0; j < NK; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[j].w[e]), p[j], o[e],
+                                                          0, 0, 0);
+        } else {
+          u32x4 hi, lo;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            hi[j] = Elem<T>::pack(p[2 * j], p[2 * j + 1]);
+            lo[j] = Elem<T>::pack(p[2 * j] - Elem<T>::low(hi[j]), p[2 * j + 1] - Elem<T>::high(hi[j]));
+          }
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            u32x4 vf;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)  // element e of tokens 2 j and 2 j + 1
+              vf[j] = __builtin_amdgcn_perm(vr[2 * j + 1].w[e / 2], vr[2 * j].w[e / 2],
+                                            e & 1 ? 0x07060302u : 0x05040100u);
+            o[e] = Elem<T>::mma(vf, hi, o[e]);
+            o[e] = Elem<T>::mma(vf, lo, o[e]);
+          }
+        }
+      }
+      values();
+      __builtin_amdgcn_wave_barrier();
+    }
+
+    // The waves' sums, in LDS where the keys were.
+    sum = pa_sum(sum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *(f32x4*)(sums + c * OLD + E * (4 * g + i) + e) =
+            f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
+    }
+    if (lane < PA_ROWS) s_max[wave][lane] = top, s_sum[wave][lane] = sum;
+    __syncthreads();
+    const bool done = here == seq.steps;
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (head ? 0 : 1);
+    for (int n = threadIdx.x; n < rows * (D / 4); n += PA_NT) {
+      const int r = n / (D / 4), x = 4 * (n - r * (D / 4));
+      if (x >= a.dv) continue;
+      float m = s_max[0][r];
+      for (int w = 1; w < PA_NW; ++w) m = fmaxf(m, s_max[w][r]);
+      const float from = m == -__builtin_inff() ? 0.f : m;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      float l = 0.f;
+      for (int w = 0; w < PA_NW; ++w) {
+        const float down = pa_exp2(s_max[w][r] - from);
+        l += down * s_sum[w][r];
+        v += down * *(const f32x4*)((const float*)s_tile[w] + r * OLD + x);
+      }
+      if (done) {
+        T* dst = (T*)a.o + (b * a.H + hk * a.group + q0 + r) * (int64_t)a.dv;
+        const float inv = seq.bad ? __builtin_nanf("") : 1.f / l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (x + e < a.dv) dst[x + e] = pg_round<T>(v[e] * inv);
+      } else {
+        float* dst = a.part + (slot * a.rows + r) * a.dv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (x + e < a.dv) dst[x + e] = v[e];
+        if (x == 0) {
+          float* stat = a.part + 2 * (int64_t)a.shares * a.rows * a.dv + (slot * a.rows + r) * 2;
+          stat[0] = m, stat[1] = l;
+        }
+      }
+    }
+    __syncthreads();
+    at += here;
+    head = false;
+  }
+}
+
+// Joins the pieces of one query head: a workgroup each.
+template <typename T, int SPAN>
+__global__ __launch_bounds__(PA_NT) void paged_attention_join(PaArgs a) {
+  __shared__ int64_t s_find[2 * PA_NW];
+  __shared__ float s_part[PA_NT];
+  const int64_t b = blockIdx.x / a.H;
+  const int h = (int)(blockIdx.x - b * a.H), hk = h / a.group, in = h - hk * a.group;
+  const int r = in % PA_ROWS;
+  const PaSeq seq = pa_seq<SPAN>(a, b);
+  T* const dst = (T*)a.o + (b * a.H + h) * (int64_t)a.dv;
+  if (seq.steps == 0) {
+    for (int x = threadIdx.x; x < a.dv; x += PA_NT)
+      dst[x] = pg_round<T>(seq.bad ? __builtin_nanf("") : 0.f);
+    return;
+  }
+  const PaSums s = pa_sums<SPAN>(a, b, s_find);
+  const int64_t from = s.before + ((int64_t)hk * a.tiles_q + in / PA_ROWS) * seq.steps;
+  const int64_t w0 = pa_holder(from, s.all, a.shares);
+  const int64_t w1 = pa_holder(from + seq.steps - 1, s.all, a.shares);
+  if (w0 == w1) return;  // one share held it and has written it
+  const int64_t slot0 = 2 * w0 + (pa_share(w0, s.all, a.shares) == from ? 0 : 1);
+  // The pieces are slot0, then the first ones of w0 + 1 .. w1 (shares without a step have none).
+  const float* const stat = a.part + 2 * (int64_t)a.shares * a.rows * a.dv;
+  auto slot = [&](int64_t w) { return (w == w0 ? slot0 : 2 * w) * a.rows + r; };
+  float top = -__builtin_inff();
+  for (int64_t w = w0; w <= w1; ++w)
+    if (pa_share(w, s.all, a.shares) < pa_share(w + 1, s.all, a.shares))
+      top = fmaxf(top, stat[2 * slot(w)]);
+  const float base = top == -__builtin_inff() ? 0.f : top;
+  // Threads side by side take elements, groups of them every n-th piece.
+  int wide = 1;
+  while (wide < a.dv) wide *= 2;
+  if (wide > PA_NT) wide = PA_NT;
+  const int groups = PA_NT / wide, mine = threadIdx.x / wide, x = threadIdx.x - mine * wide;
+  float v = 0.f, l = 0.f;
+  for (int64_t w = w0 + mine; w <= w1; w += groups) {
+    if (pa_share(w, s.all, a.shares) == pa_share(w + 1, s.all, a.shares)) continue;
+    const int64_t at = slot(w);
+    const float down = pa_exp2(stat[2 * at] - base);
+    l += down * stat[2 * at + 1];
+    if (x < a.dv) v += down * a.part[at * a.dv + x];
+  }
+  s_part[threadIdx.x] = v;
+  __syncthreads();
+  float total = 0.f;
+  if (mine == 0)
+    for (int i = 0; i < groups; ++i) total += s_part[i * wide + x];
+  __syncthreads();
+  s_part[threadIdx.x] = l;
+  __syncthreads();
+  if (mine == 0 && x < a.dv) {
+    float sum = 0.f;
+    for (int i = 0; i < groups; ++i) sum += s_part[i * wide + x];
+    dst[x] = pg_round<T>(seq.bad ? __builtin_nanf("") : total / sum);
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------
+// Shares: as many as the chip's 256 CUs hold workgroups at once.
+int pa_most(int dk, int dv) { return 256 * (dk > 128 || dv > 128 ? 1 : 2); }
+
+bool pa_ok(int dtype, int64_t B, int H, int Hk, int dk, int dv, int64_t M, int64_t P) {
+  return dtype >= 0 && dtype <= 2 && B >= 1 && H >= 1 && Hk >= 1 && H % Hk == 0 && dk >= 1 &&
+         dv >= 1 && dk <= 256 && dv <= 256 && M >= 1 && P >= 1 && P < 1ll << 31 &&
+         M < 1ll << 31 && M * P < (1ll << 31) - 1024 && B < 1ll << 24 && H < 1 << 24 &&
+         B * H < 1ll << 24;
+}
+int pa_span(int dtype) { return dtype == 0 ? PaShape<float, 64>::SPAN : PaShape<Bf16, 64>::SPAN; }
+// Workgroups: no more than there can be steps.
+int pa_shares(int dtype, int64_t B, int H, int Hk, int dk, int dv, int64_t M, int64_t P) {
+  const int64_t span = pa_span(dtype), tiles = (H / Hk + PA_ROWS - 1) / PA_ROWS;
+  const int64_t per = (M * P + span - 1) / span * Hk * tiles;
+  const int64_t most = pa_most(dk, dv);
+  return (int)(per >= most || B >= most || per * B >= most ? most : per * B);
+}
+int pa_rows(int H, int Hk) { return H / Hk < PA_ROWS ? H / Hk : PA_ROWS; }
+
+template <typename T, int D>
+void pa_launch(const PaArgs& a, bool vec, bool fours, hipStream_t stream) {
+  const dim3 grid(a.shares), nt(PA_NT);
+  if (vec && fours) hipLaunchKernelGGL((paged_attention<T, D, true, true>), grid, nt, 0, stream, a);
+  else if (vec) hipLaunchKernelGGL((paged_attention<T, D, true, false>), grid, nt, 0, stream, a);
+  else hipLaunchKernelGGL((paged_attention<T, D, false, false>), grid, nt, 0, stream, a);
+}
+template <typename T>
+int pa_run(const PaArgs& a, hipStream_t stream) {
+  const int d = a.dk > a.dv ? a.dk : a.dv, D = d <= 64 ? 64 : (d <= 128 ? 128 : 256);
+  // Vectors of a chunk: 16 bytes, 8 where a chunk is no more.
+  const int bytes = D * (int)sizeof(T) / 16 < 16 ? 8 : 16, e = sizeof(T);
+  bool vec = a.dk * e % bytes == 0 && a.dv * e % bytes == 0 &&
+             (((uintptr_t)a.k | (uintptr_t)a.v) & (bytes - 1)) == 0;
+  for (int i = 0; i < 3; ++i)
+    vec = vec && (a.ks[i] * e) % bytes == 0 && (a.vs[i] * e) % bytes == 0;
+  const bool fours = a.P.d % 4 == 0;
+  if (D == 64) pa_launch<T, 64>(a, vec, fours, stream);
+  else if (D == 128) pa_launch<T, 128>(a, vec, fours, stream);
+  else pa_launch<T, 256>(a, vec, fours, stream);
+  if (hipGetLastError() != hipSuccess) return MG_ERR_LAUNCH;
+  hipLaunchKernelGGL((paged_attention_join<T, PaShape<T, 64>::SPAN>), dim3((unsigned)(a.B * a.H)),
+                     dim3(PA_NT), 0, stream, a);
+  return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mg_paged_attention_workspace_bytes(int dtype, int64_t B, int H, int Hk, int dk, int dv,
+                                          int64_t M, int64_t P) {
+  if (!pa_ok(dtype, B, H, Hk, dk, dv, M, P)) return 0;
+  return (size_t)2 * pa_shares(dtype, B, H, Hk, dk, dv, M, P) * pa_rows(H, Hk) * (dv + 2) * sizeof(float);
+}
+
+int mg_paged_attention_step(int dtype, const void* q, const void* k_cache, const void* v_cache,
+                            const int64_t* strides, int ints, const void* pages,
+                            const void* lengths, void* o, int64_t B, int H, int Hk, int dk, int dv,
+                            int64_t N, int64_t M, int64_t P, int64_t window, float scale, void* ws,
+                            size_t ws_bytes, hipStream_t stream) {
+  if (!q || !k_cache || !v_cache || !strides || !pages || !lengths || !o || !ws || ints < 0 ||
+      ints > 3 || N < 1 || N >= 1ll << 31 || window < 0 || !pa_ok(dtype, B, H, Hk, dk, dv, M, P))
+    return MG_ERR_ARG;
+  if (ws_bytes < mg_paged_attention_workspace_bytes(dtype, B, H, Hk, dk, dv, M, P))
+    return MG_ERR_WORKSPACE;
+  PaArgs a = {};
+  a.q = q, a.k = k_cache, a.v = v_cache, a.o = o;
+  a.pages = Ints{pages, ints & 1}, a.lengths = Ints{lengths, ints >> 1};
+  a.qs[0] = strides[0], a.qs[1] = strides[1];
+  for (int i = 0; i < 3; ++i) a.ks[i] = strides[2 + i], a.vs[i] = strides[5 + i];
+  a.page_stride = strides[8];
+  a.B = B, a.N = N, a.room = M * P, a.window = window, a.P = pg_divisor(P);
+  a.H = H, a.Hk = Hk, a.group = H / Hk, a.tiles_q = (a.group + PA_ROWS - 1) / PA_ROWS;
+  a.dk = dk, a.dv = dv;
+  a.scale = scale * 1.4426950408889634f;
+  a.shares = pa_shares(dtype, B, H, Hk, dk, dv, M, P), a.part = (float*)ws, a.rows = pa_rows(H, Hk);
+  if (dtype == 0) return pa_run<float>(a, stream);
+  return dtype == 1 ? pa_run<Bf16>(a, stream) : pa_run<Fp16>(a, stream);
+}
+
+}  // extern "C"

@@ -11,6 +11,7 @@ run the eager body, which defines the results.
 
 from __future__ import annotations
 
+import importlib
 import warnings
 
 import torch
@@ -22,8 +23,9 @@ __all__ = ["linear_attention", "linear_attention_step", "linear_cross_entropy", 
 _warned: set = set()
 
 
-def _dispatch(what: str, is_cuda: bool, call):
-    """``call(hip_sequence)``, or ``None`` for the eager body; the modes' rules as for the scans."""
+def _dispatch(what: str, is_cuda: bool, call, module: str = "hip_sequence"):
+    """``call(mingru_amd.<module>)``, or ``None`` for the eager body; the modes' rules as for the
+    scans."""
     mode = _resolve_scan_mode(is_cuda)
     if mode is None:
         return None
@@ -34,9 +36,7 @@ def _dispatch(what: str, is_cuda: bool, call):
             raise scans.ScanFallback(str(status))
         if not is_cuda:
             raise scans.ScanFallback("HIP kernels need GPU tensors")
-        from mingru_amd import hip_sequence
-
-        return call(hip_sequence)
+        return call(importlib.import_module(f"mingru_amd.{module}"))
 
     result, reason = _resolve_native_dispatch(mode, what, _call)
     if reason is None:
