@@ -8,10 +8,11 @@
 // joins a row's sums and ranks the parts' candidates by their scores in fp64.
 //
 // The W largest (W <= 64) of a stream of keys, in one wave: the best 64 so far lie sorted over
-// the lanes.  A key that beats the W-th of them goes to a buffer in LDS; 64 of them are
-// sorted and merged (bitonic, over the lanes).  A long row has few such keys: after n of them
-// a new one comes with W / n, so that most tiles cost a comparison.  Before the first tile
-// nothing is known; the W-th largest of its lanes' maxima is a bound that W keys reach.
+// the lanes.  Of the keys that a lane each offers, those that beat the W-th of them are put in
+// one by one where they are few, or sorted and merged (bitonic, over the lanes).  A long row has
+// few such keys: after n of them a new one comes with W / n, so that most elements cost a
+// comparison.  The lanes' largest elements of the first tile, sorted, are the first best.
+// Lanes exchange keys by row operations and swaps of half rows, without LDS.
 // Keys are whole numbers that order as (value, lower index first), no two alike: the result
 // does not depend on the order of arrival, and ties fall as they are defined.
 //
@@ -22,24 +23,75 @@
 namespace {
 
 // ---- sorted lists over a wave -----------------------------------------------------------
-// Orders as (value, lower index first); 0 is below every key.
-struct Key32 {
-  unsigned long long k;
-  __device__ __forceinline__ bool above(const Key32& o) const { return k > o.k; }
-  __device__ __forceinline__ Key32 from(int lane) const {
-    return Key32{(unsigned long long)__shfl((long long)k, lane)};
+__device__ __forceinline__ int bs_lane() { return threadIdx.x & (MG_WAVE - 1); }
+
+// x of lane ^ D.
+template <int CTRL>
+__device__ __forceinline__ unsigned bs_dpp(unsigned x) {
+  return (unsigned)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xf, 0xf, false);
+}
+template <int D>
+__device__ __forceinline__ unsigned bs_xor(unsigned x) {
+  if constexpr (D == 1) {
+    return bs_dpp<0xB1>(x);  // quad_perm 1, 0, 3, 2
+  } else if constexpr (D == 2) {
+    return bs_dpp<0x4E>(x);  // quad_perm 2, 3, 0, 1
+  } else if constexpr (D == 4) {
+    return bs_dpp<0x1B>(bs_dpp<0x141>(x));  // lane ^ 7 (row_half_mirror), then ^ 3
+  } else if constexpr (D == 8) {
+    return bs_dpp<0x128>(x);  // row_ror:8
+  } else if constexpr (D == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return bs_lane() & 16 ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return bs_lane() & 32 ? r[0] : r[1];
   }
+}
+// x of lane ^ 63.
+__device__ __forceinline__ unsigned bs_mirror(unsigned x) {
+  return bs_xor<32>(bs_xor<16>(bs_dpp<0x140>(x)));  // row_mirror: lane ^ 15
+}
+__device__ __forceinline__ unsigned bs_read(unsigned x, int lane) {
+  return (unsigned)__builtin_amdgcn_readlane((int)x, lane);
+}
+__device__ __forceinline__ unsigned bs_prev(unsigned x) {  // of the lane before; 0 in lane 0
+  return __float_as_uint(mg_wave_prev(__uint_as_float(x)));
+}
+
+// A key orders as (value, lower index first); 0 is below every key.  Key32's value is of 32
+// bits, above its inverted index; Key64's of 64.
+struct Key32 {
+  unsigned w[2];
+  __device__ __forceinline__ unsigned long long all() const {
+    return (unsigned long long)w[1] << 32 | w[0];
+  }
+  __device__ __forceinline__ bool above(const Key32& o) const { return all() > o.all(); }
 };
 struct Key64 {
-  unsigned long long k;
-  unsigned i;  // ~index
-  __device__ __forceinline__ bool above(const Key64& o) const {
-    return k > o.k || (k == o.k && i > o.i);
+  unsigned w[3];
+  __device__ __forceinline__ unsigned long long value() const {
+    return (unsigned long long)w[2] << 32 | w[1];
   }
-  __device__ __forceinline__ Key64 from(int lane) const {
-    return Key64{(unsigned long long)__shfl((long long)k, lane), (unsigned)__shfl((int)i, lane)};
+  __device__ __forceinline__ bool above(const Key64& o) const {
+    return value() > o.value() || (value() == o.value() && w[0] > o.w[0]);
   }
 };
+template <typename K, typename F>
+__device__ __forceinline__ K bs_map(const K& x, F&& f) {
+  K y;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(K) / 4); ++i) y.w[i] = f(x.w[i], i);
+  return y;
+}
+template <typename K>
+__device__ __forceinline__ K bs_pick(bool first, const K& x, const K& y) {
+  return bs_map(x, [&](unsigned w, int i) { return first ? w : y.w[i]; });
+}
+template <typename K>
+__device__ __forceinline__ K bs_from(const K& x, int lane) {  // the same lane for all
+  return bs_map(x, [&](unsigned w, int) { return bs_read(w, lane); });
+}
 
 __device__ __forceinline__ unsigned bs_order(float x) {
   const unsigned u = __float_as_uint(x + 0.f);  // -0 becomes 0
@@ -56,70 +108,67 @@ __device__ __forceinline__ double bs_value(unsigned long long o) {
   return __longlong_as_double((long long)(o >> 63 ? o & ~(1ull << 63) : ~o));
 }
 
-__device__ __forceinline__ int bs_lane() { return threadIdx.x & (MG_WAVE - 1); }
-
-// One exchange with lane ^ d: the larger key stays where `up` holds.
-template <typename K>
-__device__ __forceinline__ void bs_swap(K& x, int d, bool up) {
-  const K o = x.from(bs_lane() ^ d);
-  x = x.above(o) == up ? x : o;
+// One exchange with lane ^ D: the larger key stays where `up` holds.
+template <int D, typename K>
+__device__ __forceinline__ void bs_swap(K& x, bool up) {
+  const K o = bs_map(x, [](unsigned w, int) { return bs_xor<D>(w); });
+  x = bs_pick(x.above(o) == up, x, o);
+}
+// A bitonic row of 2 D lanes becomes falling (up) or rising.
+template <int D, typename K>
+__device__ __forceinline__ void bs_settle(K& x, bool up) {
+  bs_swap<D>(x, ((bs_lane() & D) == 0) == up);
+  if constexpr (D > 1) bs_settle<D / 2>(x, up);
 }
 // Falling over the lanes.
 template <typename K>
 __device__ __forceinline__ void bs_sort(K& x) {
   const int lane = bs_lane();
-  for (int n = 2; n <= MG_WAVE; n *= 2)
-    for (int d = n / 2; d > 0; d /= 2) bs_swap(x, d, ((lane & d) == 0) == ((lane & n) == 0));
+  bs_settle<1>(x, (lane & 2) == 0);
+  bs_settle<2>(x, (lane & 4) == 0);
+  bs_settle<4>(x, (lane & 8) == 0);
+  bs_settle<8>(x, (lane & 16) == 0);
+  bs_settle<16>(x, (lane & 32) == 0);
+  bs_settle<32>(x, true);
 }
 // The 64 largest of two falling lists.
 template <typename K>
 __device__ __forceinline__ void bs_merge(K& best, const K& more) {
-  const K o = more.from(MG_WAVE - 1 - bs_lane());
-  if (o.above(best)) best = o;
-  for (int d = MG_WAVE / 2; d > 0; d /= 2) bs_swap(best, d, (bs_lane() & d) == 0);
+  const K o = bs_map(more, [](unsigned w, int) { return bs_mirror(w); });
+  best = bs_pick(o.above(best), o, best);
+  bs_settle<32>(best, true);
 }
 
-// The W largest of what is offered.  buffer: 2 * 64 keys of LDS, the wave's own.
+// The W largest of what is offered.
 template <typename K>
 struct Best {
-  K best, bar;  // bar: the W-th largest so far, or a bound that W keys reach
-  K* buffer;
-  int count, W;
-  bool bound;  // bar is such a bound: a key like it counts
-  __device__ __forceinline__ void init(K* lds, int width) {
-    best = K{}, bar = K{}, buffer = lds, count = 0, W = width, bound = false;
+  K best, bar;  // falling over the lanes, and the W-th of them
+  int last;     // W - 1
+  __device__ __forceinline__ void start(const K& x, int W) {
+    best = x, last = W - 1;
+    bs_sort(best);
+    bar = bs_from(best, last);
   }
-  __device__ __forceinline__ void flush() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const int lane = bs_lane(), n = count < MG_WAVE ? count : MG_WAVE;
-    K x = lane < n ? buffer[lane] : K{};
-    bs_sort(x);
-    bs_merge(best, x);
-    const K last = best.from(W - 1);
-    if (last.above(bar) || !bar.above(last)) bar = last, bound = false;
-    const K rest = lane < count - n ? buffer[n + lane] : K{};
-    __builtin_amdgcn_wave_barrier();
-    if (lane < count - n) buffer[lane] = rest;
-    count -= n;
-  }
-  // One key of each lane, K{} for none.
-  __device__ __forceinline__ void offer(const K& x) {
-    const bool in = x.above(K{}) && (x.above(bar) || (bound && !bar.above(x)));
-    const unsigned long long who = __ballot(in);
+  // One key of each lane, 0 for none.
+  __device__ __forceinline__ void offer(K x) {
+    const bool in = x.above(bar);
+    unsigned long long who = __ballot(in);
     if (who == 0) return;
-    if (in) buffer[count + __popcll(who & ((1ull << bs_lane()) - 1))] = x;
-    count += __popcll(who);
-    if (count >= MG_WAVE) flush();
-  }
-  // A bound from the lanes' largest keys, before anything is offered.
-  __device__ __forceinline__ void hint(K x) {
-    bs_sort(x);
-    bar = x.from(W - 1);
-    bound = true;
-  }
-  __device__ __forceinline__ void finish() {
-    while (count) flush();
+    // Where a sort's 27 exchanges cost less.
+    if (__popcll(who) > 8) {
+      x = bs_pick(in, x, K{});
+      bs_sort(x);
+      bs_merge(best, x);
+    } else {
+      do {
+        const K one = bs_from(x, __ffsll(who) - 1);
+        who &= who - 1;
+        const int at = __popcll(__ballot(best.above(one)));
+        const K up = bs_map(best, [](unsigned w, int) { return bs_prev(w); });
+        best = bs_pick(bs_lane() < at, best, bs_pick(bs_lane() == at, one, up));
+      } while (who);
+    }
+    bar = bs_from(best, last);
   }
 };
 
@@ -156,7 +205,6 @@ struct BsVec {
 template <typename T>
 __global__ __launch_bounds__(BS_NT) void beam_rows(BsArgs a) {
   constexpr int N = BsVec<T>::N, ALL = N * BS_VECTORS, TILE = ALL * MG_WAVE;
-  __shared__ Key32 s_buffer[BS_NW][2 * MG_WAVE];
   const int lane = bs_lane(), wave = (int)mg_uniform(threadIdx.x / MG_WAVE);
   const int64_t id = (int64_t)blockIdx.x * BS_NW + wave;
   const int64_t row = id / a.parts;
@@ -174,17 +222,19 @@ __global__ __launch_bounds__(BS_NT) void beam_rows(BsArgs a) {
   const int begin = part * a.per, stop = all - begin < a.per ? all : begin + a.per;
 
   Best<Key32> list;
-  list.init(s_buffer[wave], a.W);
   // No maximum is below the lowest number, so that a lane of -inf alone, or without an element,
   // has a sum of 0.
   float top = -3.402823466e38f, sum = 0.f;
-  for (int at = begin; at < stop; at += TILE) {
-    uint4 raw[BS_VECTORS];
+  uint4 raw[BS_VECTORS];
+  auto load = [&](int at) {
 #pragma unroll
     for (int i = 0; i < BS_VECTORS; ++i) {
       const int e = at + (i * MG_WAVE + lane) * N;
       raw[i] = lines[(e < stop ? e : begin) / N];
     }
+  };
+  if (begin < stop) load(begin);
+  for (int at = begin; at < stop; at += TILE) {
     float v[ALL];
     float peak = -__builtin_inff();
     const bool whole = at >= skew && at + TILE <= stop;
@@ -194,6 +244,7 @@ __global__ __launch_bounds__(BS_NT) void beam_rows(BsArgs a) {
 #pragma unroll
       for (int j = 0; j < N; ++j) v[i * N + j] = pg_float(p[j]);
     }
+    load(at + TILE < stop ? at + TILE : begin);
     if (!whole) {  // what is not in the row adds nothing
 #pragma unroll
       for (int i = 0; i < ALL; ++i) {
@@ -213,57 +264,83 @@ __global__ __launch_bounds__(BS_NT) void beam_rows(BsArgs a) {
     auto key = [&](int i) {
       const int e = at + ((i / N) * MG_WAVE + lane) * N + i % N;
       const bool in = e >= skew && e < stop;
-      return Key32{in ? (unsigned long long)bs_order(v[i]) << 32 | ~(unsigned)(e - skew) : 0ull};
+      return Key32{{in ? ~(unsigned)(e - skew) : 0u, in ? bs_order(v[i]) : 0u}};
     };
+    int own = -1;  // this lane's element among the first best
     if (at == begin) {
-      Key32 most = {0};
+      Key32 most = {};
 #pragma unroll
       for (int i = 0; i < ALL; ++i) {
         const Key32 x = key(i);
-        most = x.above(most) ? x : most;
+        const bool more = x.above(most);
+        most = bs_pick(more, x, most);
+        own = more ? i : own;
       }
-      list.hint(most);
-    } else if (__ballot(bs_order(peak) >= (unsigned)(list.bar.k >> 32)) == 0) {
-      continue;
+      list.start(most, a.W);
     }
+    // By values first: most elements are below the W-th best.
+    float bar = bs_value(list.bar.w[1]);
+    if (list.bar.all() == 0) bar = -__builtin_inff();
+    if (__ballot(peak >= bar) == 0) continue;
 #pragma unroll
-    for (int i = 0; i < ALL; ++i) list.offer(key(i));
+    for (int i = 0; i < ALL; ++i) {
+      if (__ballot(v[i] >= bar) == 0) continue;
+      list.offer(bs_pick(i == own, Key32{}, key(i)));
+      bar = list.bar.all() == 0 ? -__builtin_inff() : bs_value(list.bar.w[1]);
+    }
   }
-  list.finish();
   float m = top;
 #pragma unroll
   for (int d = 1; d < MG_WAVE; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
   const float total = mg_group_sum<64>(sum * __expf(top - m));
   if (lane == 0) a.stats[id] = make_float2(m, total);
-  if (lane < a.W) a.keys[id * a.W + lane] = list.best.k;
+  if (lane < a.W) a.keys[id * a.W + lane] = begin < stop ? list.best.all() : 0ull;
 }
 
 // ---- the selection -----------------------------------------------------------------------
 constexpr int BS_MAX_K = 256;
 
+__device__ __forceinline__ double bs_row_sum(double x) {  // over 16 lanes
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned long long u = (unsigned long long)__double_as_longlong(x);
+    unsigned lo = (unsigned)u, hi = (unsigned)(u >> 32);
+    if (i == 0) lo = bs_xor<1>(lo), hi = bs_xor<1>(hi);
+    else if (i == 1) lo = bs_xor<2>(lo), hi = bs_xor<2>(hi);
+    else if (i == 2) lo = bs_xor<4>(lo), hi = bs_xor<4>(hi);
+    else lo = bs_xor<8>(lo), hi = bs_xor<8>(hi);
+    x += __longlong_as_double((long long)((unsigned long long)hi << 32 | lo));
+  }
+  return x;
+}
+
 template <int NW>
 __global__ __launch_bounds__(NW* MG_WAVE) void beam_pick(BsArgs a) {
-  __shared__ Key64 s_buffer[NW][2 * MG_WAVE];
+  __shared__ Key64 s_list[NW / 2][MG_WAVE];
   __shared__ double s_norm[BS_MAX_K], s_score[BS_MAX_K];
   __shared__ unsigned char s_kind[BS_MAX_K];
   enum { LIVE = 0, FINISHED = 1, DEAD = 2 };
   const int lane = bs_lane(), wave = (int)mg_uniform(threadIdx.x / MG_WAVE);
   const int64_t b = blockIdx.x;
-  for (int k = wave; k < a.K; k += NW) {
-    const float score = a.scores[b * a.ss[0] + k * a.ss[1]];
-    const bool finite = bs_finite(score), over = bs_finished(a, b, k);
+  // Sixteen lanes a row.
+  for (int k0 = 0; k0 < a.K; k0 += NW * 4) {
+    const int k = k0 + (int)threadIdx.x / 16, in = threadIdx.x & 15;
+    const int at = k < a.K ? k : a.K - 1;
+    const float score = a.scores[b * a.ss[0] + at * a.ss[1]];
+    const bool finite = bs_finite(score), over = bs_finished(a, b, at);
+    const float2* st = a.stats + (b * a.K + at) * a.parts;
     float m = -__builtin_inff();
     double sum = 0.0;
-    if (finite && !over) {
-      const float2* st = a.stats + (b * a.K + k) * a.parts;
-      for (int i = lane; i < a.parts; i += MG_WAVE) m = fmaxf(m, st[i].x);
-#pragma unroll
-      for (int d = 1; d < MG_WAVE; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-      for (int i = lane; i < a.parts; i += MG_WAVE) sum += (double)st[i].y * (double)__expf(st[i].x - m);
-#pragma unroll
-      for (int d = 1; d < MG_WAVE; d *= 2) sum += __shfl_xor(sum, d);
+    if (finite && !over) {  // written by the first launch
+      for (int i = in; i < a.parts; i += 16) m = fmaxf(m, st[i].x);
+      m = fmaxf(m, mg_row_ror<8>(m));
+      m = fmaxf(m, mg_row_ror<4>(m));
+      m = fmaxf(m, mg_row_ror<2>(m));
+      m = fmaxf(m, mg_row_ror<1>(m));
+      for (int i = in; i < a.parts; i += 16) sum += (double)st[i].y * (double)__expf(st[i].x - m);
+      sum = bs_row_sum(sum);
     }
-    if (lane == 0) {
+    if (in == 0 && k < a.K) {
       const double norm = (double)m + log(sum);
       s_score[k] = score, s_norm[k] = over ? 0.0 : norm;
       s_kind[k] = !finite ? DEAD : (over ? FINISHED : (fabs(norm) < __builtin_inf() ? LIVE : DEAD));
@@ -272,53 +349,53 @@ __global__ __launch_bounds__(NW* MG_WAVE) void beam_pick(BsArgs a) {
   __syncthreads();
 
   Best<Key64> list;
-  list.init(s_buffer[wave], a.W);
   const int each = a.parts * a.W, all = a.K * each;
-  for (int at = wave * MG_WAVE; at < all; at += NW * MG_WAVE) {
-    const int n = at + lane;
-    Key64 x = {0, 0};
+  auto key = [&](double score, unsigned index) {
+    const unsigned long long o = bs_order(score);
+    return Key64{{~index, (unsigned)o, (unsigned)(o >> 32)}};
+  };
+  auto candidate = [&](int n) {
+    Key64 x = {};
     if (n < all) {
       const int k = n / each, r = n - k * each;
       if (s_kind[k] == LIVE) {
-        const unsigned long long key = a.keys[(b * a.K + k) * each + r];
-        if (key) {
-          const unsigned token = ~(unsigned)key;
-          x.k = bs_order(s_score[k] + ((double)bs_value((unsigned)(key >> 32)) - s_norm[k]));
-          x.i = ~((unsigned)k * (unsigned)a.V + token);
-        }
-      } else if (r < a.W) {  // without a part of the row: its end, and the first tokens at -inf
+        const unsigned long long from = a.keys[(b * a.K + k) * each + r];
+        if (from)
+          x = key(s_score[k] + ((double)bs_value((unsigned)(from >> 32)) - s_norm[k]),
+                  (unsigned)k * (unsigned)a.V + ~(unsigned)from);
+      } else if (r < a.W) {  // no part of the row: its end, and the first tokens at -inf
         const bool over = s_kind[k] == FINISHED, first = over && r == 0;
         int token = first ? a.end : r - (over ? 1 : 0);
         if (over && !first && token >= a.end) ++token;
-        if (token < a.V) {
-          x.k = bs_order(first ? s_score[k] : -__builtin_inf());
-          x.i = ~((unsigned)k * (unsigned)a.V + (unsigned)token);
-        }
+        if (token < a.V)
+          x = key(first ? s_score[k] : -__builtin_inf(), (unsigned)k * (unsigned)a.V + (unsigned)token);
       }
     }
-    if (at == wave * MG_WAVE) list.hint(x);
-    list.offer(x);
+    return x;
+  };
+  list.start(candidate(wave * MG_WAVE + lane), a.W);
+  for (int at = (wave + NW) * MG_WAVE; at < all; at += NW * MG_WAVE) list.offer(candidate(at + lane));
+  // The waves' lists, by halves.
+#pragma unroll
+  for (int half = NW / 2; half > 0; half /= 2) {
+    if (wave >= half && wave < 2 * half) s_list[wave - half][lane] = list.best;
+    __syncthreads();
+    if (wave < half) bs_merge(list.best, s_list[wave][lane]);
+    __syncthreads();
   }
-  list.finish();
-  // The waves' lists, joined by the first.
-  __syncthreads();
-  if (lane < a.W) s_buffer[wave][lane] = list.best;
-  __syncthreads();
-  if (wave != 0) return;
-  for (int w = 1; w < NW; ++w) bs_merge(list.best, lane < a.W ? s_buffer[w][lane] : Key64{0, 0});
-  if (lane < a.W) {
-    const unsigned flat = ~list.best.i;
+  if (wave == 0 && lane < a.W) {
+    const unsigned flat = ~list.best.w[0];
     const int k = (int)(flat / (unsigned)a.V), token = (int)(flat - (unsigned)k * (unsigned)a.V);
     const int64_t n = b * a.W + lane;
-    a.out[n] = (float)bs_value(list.best.k);
+    a.out[n] = (float)bs_value(list.best.value());
     a.parents[n] = k, a.tokens[n] = token;
     if (a.done) a.done[n] = token == a.end || bs_finished(a, b, k);
   }
 }
 
-// Waves of a row: enough to fill the chip's 256 CUs with 8 waves each, no less than a tile each.
+// Waves of a row: enough to fill the chip's 256 CUs with 16 waves each, no less than a tile each.
 int bs_parts(int64_t rows, int V, int tile) {
-  int64_t want = (2048 + rows - 1) / rows;
+  int64_t want = (4096 + rows - 1) / rows;
   const int64_t most = ((int64_t)V + 8 + tile - 1) / tile;
   return (int)(want < most ? want : most);
 }
@@ -433,7 +510,11 @@ int mg_beam_select(int dtype, const void* logits, const float* scores, const voi
   else if (dtype == 1) hipLaunchKernelGGL(beam_rows<Bf16>, grid, nt, 0, stream, a);
   else hipLaunchKernelGGL(beam_rows<Fp16>, grid, nt, 0, stream, a);
   if (hipGetLastError() != hipSuccess) return MG_ERR_LAUNCH;
-  hipLaunchKernelGGL(beam_pick<4>, dim3((unsigned)B), dim3(4 * MG_WAVE), 0, stream, a);
+  // Sixteen waves where four would have more than eight rounds of candidates.
+  if (K * a.parts * W <= 8 * 4 * MG_WAVE)
+    hipLaunchKernelGGL(beam_pick<4>, dim3((unsigned)B), dim3(4 * MG_WAVE), 0, stream, a);
+  else
+    hipLaunchKernelGGL(beam_pick<16>, dim3((unsigned)B), dim3(16 * MG_WAVE), 0, stream, a);
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
 

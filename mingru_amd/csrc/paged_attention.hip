@@ -184,42 +184,49 @@ __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, int64_t b) {
   return s;
 }
 
-// The sum of all steps, and of those before sequence `upto` (a sequence's pairs of a key head and
-// 16 of its queries come one after another).  The whole workgroup calls it.
-struct PaSums {
-  int64_t all, before;
+// The steps of all sequences one after another, a sequence's pairs of a key head and 16 of its
+// queries in a row.  Each thread sums a run of sequences; the whole workgroup calls it.
+struct PaRow {
+  int64_t all;         // steps in all
+  int64_t from, sum;   // before this thread's run, and behind it
+  int64_t first, run;  // its sequences
 };
 template <int SPAN>
-__device__ __forceinline__ PaSums pa_sums(const PaArgs& a, int64_t upto, int64_t* lds) {
-  int64_t all = 0, before = 0;
-  for (int64_t b = threadIdx.x; b < a.B; b += PA_NT) {
-    const int64_t n = pa_seq<SPAN>(a, b).steps;
-    all += n;
-    before += b < upto ? n : 0;
-  }
+__device__ __forceinline__ PaRow pa_row(const PaArgs& a, int64_t* lds) {
+  const int lane = threadIdx.x & (MG_WAVE - 1), wave = threadIdx.x / MG_WAVE;
+  PaRow r;
+  r.run = (a.B + PA_NT - 1) / PA_NT, r.first = r.run * threadIdx.x;
+  int64_t n = 0;
+  for (int64_t i = r.first; i < r.first + r.run && i < a.B; ++i) n += pa_seq<SPAN>(a, i).steps;
+  n *= (int64_t)a.Hk * a.tiles_q;
+  r.sum = n;
+  // Where one sequence is all, one thread knows.
+  if (a.B > 1) {
 #pragma unroll
-  for (int d = 1; d < MG_WAVE; d *= 2) {
-    all += __shfl_xor(all, d);
-    before += __shfl_xor(before, d);
+    for (int d = 1; d < MG_WAVE; d *= 2) {
+      const int64_t up = __shfl_up(r.sum, d);
+      r.sum += lane >= d ? up : 0;
+    }
   }
-  if ((threadIdx.x & (MG_WAVE - 1)) == 0) {
-    lds[2 * (threadIdx.x / MG_WAVE)] = all;
-    lds[2 * (threadIdx.x / MG_WAVE) + 1] = before;
+  if (lane == (a.B > 1 ? MG_WAVE - 1 : 0)) lds[wave] = r.sum;
+  __syncthreads();
+  r.all = 0;
+#pragma unroll
+  for (int w = 0; w < PA_NW; ++w) {
+    r.sum += w < wave ? lds[w] : 0;
+    r.all += lds[w];
   }
+  r.from = r.sum - n;
   __syncthreads();
-  PaSums s = {0, 0};
-  for (int w = 0; w < PA_NW; ++w) s.all += lds[2 * w], s.before += lds[2 * w + 1];
-  __syncthreads();
-  const int64_t pairs = (int64_t)a.Hk * a.tiles_q;
-  s.all *= pairs, s.before *= pairs;
-  return s;
+  return r;
 }
-// Share w of `shares` holds the steps [w all / shares, (w + 1) all / shares).
-__device__ __forceinline__ int64_t pa_share(int64_t w, int64_t all, int shares) {
-  return w * all / shares;
+// Share w of n holds the steps [w all / n, (w + 1) all / n); no share is empty, as n <= all.
+__device__ __forceinline__ int pa_shares_used(const PaArgs& a, int64_t all) {
+  return all < a.shares ? (int)all : a.shares;
 }
-__device__ __forceinline__ int64_t pa_holder(int64_t step, int64_t all, int shares) {
-  return ((step + 1) * shares - 1) / all;
+__device__ __forceinline__ int64_t pa_share(int64_t w, int64_t all, int n) { return w * all / n; }
+__device__ __forceinline__ int64_t pa_holder(int64_t step, int64_t all, int n) {
+  return ((step + 1) * n - 1) / all;
 }
 
 // ---- the main kernel -------------------------------------------------------------------
@@ -246,7 +253,7 @@ __global__ __launch_bounds__(PA_NT, (PaShape<T, D>::GROUPS)) void paged_attentio
   typedef Chunk<T, E> C;
   __shared__ alignas(16) unsigned char s_tile[PA_NW][S::BYTES];
   __shared__ float s_max[PA_NW][PA_ROWS], s_sum[PA_NW][PA_ROWS];
-  __shared__ int64_t s_find[2 * PA_NW];
+  __shared__ int64_t s_find[PA_NW];
 
   const int lane = threadIdx.x & (MG_WAVE - 1), wave = (int)mg_uniform(threadIdx.x / MG_WAVE);
   const int c = lane & 15, g = lane >> 4;
@@ -254,37 +261,22 @@ __global__ __launch_bounds__(PA_NT, (PaShape<T, D>::GROUPS)) void paged_attentio
   float* const sums = (float*)s_tile[wave];
 
   // This share's first step, and the sequence that it lies in.
-  const int64_t all = pa_sums<SPAN>(a, 0, s_find).all;
-  int64_t at = pa_share(blockIdx.x, all, a.shares);
-  const int64_t stop = pa_share(blockIdx.x + 1, all, a.shares);
-  if (at >= stop) return;
+  const PaRow row = pa_row<SPAN>(a, s_find);
+  const int shares = pa_shares_used(a, row.all);
+  if ((int)blockIdx.x >= shares) return;
+  int64_t at = pa_share(blockIdx.x, row.all, shares);
+  const int64_t stop = pa_share(blockIdx.x + 1, row.all, shares);
   const int64_t pairs = (int64_t)a.Hk * a.tiles_q;
   int64_t b = 0, before = 0;
-  {
-    // Each thread sums a run of sequences; the one whose run holds the step looks it up there.
-    const int64_t run = (a.B + PA_NT - 1) / PA_NT, b0 = run * threadIdx.x;
-    int64_t n = 0;
-    for (int64_t i = b0; i < b0 + run && i < a.B; ++i) n += pa_seq<SPAN>(a, i).steps;
-    n *= pairs;
-    int64_t sum = n;
-#pragma unroll
-    for (int d = 1; d < MG_WAVE; d *= 2) {
-      const int64_t up = __shfl_up(sum, d);
-      sum += lane >= d ? up : 0;
-    }
-    if (lane == MG_WAVE - 1) s_find[wave] = sum;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) sum += s_find[w];
-    __syncthreads();
-    int64_t start = sum - n;
-    if (at >= start && at < sum) {
-      int64_t i = b0;
-      for (;; ++i) {
-        const int64_t m = pa_seq<SPAN>(a, i).steps * pairs;
-        if (at < start + m) break;
-        start += m;
+  if (a.B > 1) {
+    if (at >= row.from && at < row.sum) {  // one thread's run holds it
+      b = row.first, before = row.from;
+      for (;; ++b) {
+        const int64_t m = pa_seq<SPAN>(a, b).steps * pairs;
+        if (at < before + m) break;
+        before += m;
       }
-      s_find[0] = i, s_find[1] = start;
+      s_find[0] = b, s_find[1] = before;
     }
     __syncthreads();
     b = s_find[0], before = s_find[1];
@@ -536,10 +528,13 @@ __global__ __launch_bounds__(PA_NT, (PaShape<T, D>::GROUPS)) void paged_attentio
 }
 
 // Joins the pieces of one query head: a workgroup each.
+constexpr int PA_MOST = 512;  // shares
 template <typename T, int SPAN>
 __global__ __launch_bounds__(PA_NT) void paged_attention_join(PaArgs a) {
-  __shared__ int64_t s_find[2 * PA_NW];
-  __shared__ float s_part[PA_NT];
+  __shared__ int64_t s_find[PA_NW + 1];
+  __shared__ float s_weight[PA_MOST], s_red[2 * PA_NW];
+  __shared__ f32x4 s_part[PA_NT];
+  const int lane = threadIdx.x & (MG_WAVE - 1), wave = threadIdx.x / MG_WAVE;
   const int64_t b = blockIdx.x / a.H;
   const int h = (int)(blockIdx.x - b * a.H), hk = h / a.group, in = h - hk * a.group;
   const int r = in % PA_ROWS;
@@ -550,45 +545,80 @@ __global__ __launch_bounds__(PA_NT) void paged_attention_join(PaArgs a) {
       dst[x] = pg_round<T>(seq.bad ? __builtin_nanf("") : 0.f);
     return;
   }
-  const PaSums s = pa_sums<SPAN>(a, b, s_find);
-  const int64_t from = s.before + ((int64_t)hk * a.tiles_q + in / PA_ROWS) * seq.steps;
-  const int64_t w0 = pa_holder(from, s.all, a.shares);
-  const int64_t w1 = pa_holder(from + seq.steps - 1, s.all, a.shares);
-  if (w0 == w1) return;  // one share held it and has written it
-  const int64_t slot0 = 2 * w0 + (pa_share(w0, s.all, a.shares) == from ? 0 : 1);
-  // The pieces are slot0, then the first ones of w0 + 1 .. w1 (shares without a step have none).
-  const float* const stat = a.part + 2 * (int64_t)a.shares * a.rows * a.dv;
-  auto slot = [&](int64_t w) { return (w == w0 ? slot0 : 2 * w) * a.rows + r; };
-  float top = -__builtin_inff();
-  for (int64_t w = w0; w <= w1; ++w)
-    if (pa_share(w, s.all, a.shares) < pa_share(w + 1, s.all, a.shares))
-      top = fmaxf(top, stat[2 * slot(w)]);
-  const float base = top == -__builtin_inff() ? 0.f : top;
-  // Threads side by side take elements, groups of them every n-th piece.
-  int wide = 1;
-  while (wide < a.dv) wide *= 2;
-  if (wide > PA_NT) wide = PA_NT;
-  const int groups = PA_NT / wide, mine = threadIdx.x / wide, x = threadIdx.x - mine * wide;
-  float v = 0.f, l = 0.f;
-  for (int64_t w = w0 + mine; w <= w1; w += groups) {
-    if (pa_share(w, s.all, a.shares) == pa_share(w + 1, s.all, a.shares)) continue;
-    const int64_t at = slot(w);
-    const float down = pa_exp2(stat[2 * at] - base);
-    l += down * stat[2 * at + 1];
-    if (x < a.dv) v += down * a.part[at * a.dv + x];
+  const PaRow row = pa_row<SPAN>(a, s_find);
+  int64_t before = 0;
+  if (a.B > 1) {
+    if (b >= row.first && b < row.first + row.run) {
+      before = row.from;
+      for (int64_t i = row.first; i < b; ++i)
+        before += pa_seq<SPAN>(a, i).steps * (int64_t)a.Hk * a.tiles_q;
+      s_find[PA_NW] = before;
+    }
+    __syncthreads();
+    before = s_find[PA_NW];
   }
+  const int shares = pa_shares_used(a, row.all);
+  const int64_t from = before + ((int64_t)hk * a.tiles_q + in / PA_ROWS) * seq.steps;
+  const int w0 = (int)pa_holder(from, row.all, shares);
+  const int n = (int)pa_holder(from + seq.steps - 1, row.all, shares) - w0 + 1;
+  if (n == 1) return;  // one share held it and has written it
+  // The pieces are the first or second one of w0, then the first ones of w0 + 1 .. w0 + n - 1.
+  const int second = pa_share(w0, row.all, shares) == from ? 0 : 1;
+  const float* const stat = a.part + 2 * (int64_t)a.shares * a.rows * a.dv;
+  auto place = [&](int i) { return ((int64_t)2 * (w0 + i) + (i ? 0 : second)) * a.rows + r; };
+  float m[PA_MOST / PA_NT], l[PA_MOST / PA_NT], top = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < PA_MOST / PA_NT; ++j) {
+    const int i = threadIdx.x + j * PA_NT;
+    const float2 st = *(const float2*)(stat + 2 * place(i < n ? i : 0));
+    m[j] = i < n ? st.x : -__builtin_inff(), l[j] = i < n ? st.y : 0.f;
+    top = fmaxf(top, m[j]);
+  }
+#pragma unroll
+  for (int d = 1; d < MG_WAVE; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  if (lane == 0) s_red[wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < PA_NW; ++w) top = fmaxf(top, s_red[w]);
+  const float base = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+  for (int j = 0; j < PA_MOST / PA_NT; ++j) {
+    const int i = threadIdx.x + j * PA_NT;
+    const float down = pa_exp2(m[j] - base);
+    if (i < n) s_weight[i] = down;
+    sum += i < n ? down * l[j] : 0.f;
+  }
+  sum = mg_group_sum<64>(sum);
+  if (lane == 0) s_red[PA_NW + wave] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < PA_NW; ++w) sum += s_red[PA_NW + w];
+  // Threads side by side take four elements each, groups of them every n-th piece.
+  int wide = 1;
+  while (4 * wide < a.dv) wide *= 2;
+  const int groups = PA_NT / wide, mine = threadIdx.x / wide, x = 4 * (threadIdx.x - mine * wide);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](int i) {
+    const float* p = a.part + place(i) * a.dv;
+    const float down = s_weight[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += down * p[x + e < a.dv ? x + e : 0];
+  };
+  int i = mine;
+  for (; i + 3 * groups < n; i += 4 * groups) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) add(i + j * groups);
+  }
+  for (; i < n; i += groups) add(i);
   s_part[threadIdx.x] = v;
   __syncthreads();
-  float total = 0.f;
-  if (mine == 0)
-    for (int i = 0; i < groups; ++i) total += s_part[i * wide + x];
-  __syncthreads();
-  s_part[threadIdx.x] = l;
-  __syncthreads();
-  if (mine == 0 && x < a.dv) {
-    float sum = 0.f;
-    for (int i = 0; i < groups; ++i) sum += s_part[i * wide + x];
-    dst[x] = pg_round<T>(seq.bad ? __builtin_nanf("") : total / sum);
+  if (mine == 0) {
+    for (int j = 1; j < groups; ++j) v += s_part[j * wide + threadIdx.x];
+    const float inv = seq.bad ? __builtin_nanf("") : 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (x + e < a.dv) dst[x + e] = pg_round<T>(v[e] * inv);
   }
 }
 

@@ -73,7 +73,6 @@ def _turned(x, position, frequencies, interleaved):
     return torch.cat((part, rest), -1)
 
 
-@torch.no_grad()
 def paged_cache_append(k, v, k_cache, v_cache, pages, start, *, q=None, lengths=None,
                        frequencies=None, interleaved=False):
     """Puts new tokens' keys and values into a paged cache, in place, with keys and queries
@@ -139,6 +138,13 @@ def paged_cache_append(k, v, k_cache, v_cache, pages, start, *, q=None, lengths=
             "hip_decode")
         if done is not None:
             return done[0]
+    return _eager_append(k, v, k_cache, v_cache, pages, start, q, lengths, frequencies, interleaved)
+
+
+@torch.no_grad()
+def _eager_append(k, v, k_cache, v_cache, pages, start, q, lengths, frequencies, interleaved):
+    what = "paged_cache_append"
+    (B, T), (N, _, P, _) = k.shape[:2], k_cache.shape
     t = torch.arange(T, device=k.device)
     position = start.long()[:, None] + t
     live = (t < lengths.long()[:, None]) if lengths is not None else torch.ones_like(position) > 0
@@ -165,7 +171,6 @@ def paged_cache_append(k, v, k_cache, v_cache, pages, start, *, q=None, lengths=
 # ---------------------------------------------------------------------------
 
 
-@torch.no_grad()
 def paged_attention_step(q, k_cache, v_cache, pages, lengths, *, scale=None, window=None):
     """Attention of each sequence's newest token over its paged cache.
 
@@ -219,6 +224,13 @@ def paged_attention_step(q, k_cache, v_cache, pages, lengths, *, scale=None, win
             q, k_cache, v_cache, pages, lengths, scale, window), "hip_decode")
         if out is not None:
             return out
+    return _eager_attention(q, k_cache, v_cache, pages, lengths, scale, window)
+
+
+@torch.no_grad()
+def _eager_attention(q, k_cache, v_cache, pages, lengths, scale, window):
+    what = "paged_attention_step"
+    (B, H, dk), (N, Hk, P, dv) = q.shape, v_cache.shape
     if B == 0:
         return q.new_zeros(B, H, dv)
     lengths = lengths.long().clamp(min=0)
@@ -252,7 +264,6 @@ def paged_attention_step(q, k_cache, v_cache, pages, lengths, *, scale=None, win
 # ---------------------------------------------------------------------------
 
 
-@torch.no_grad()
 def beam_select(logits, scores, width=None, *, end=None, finished=None):
     """A beam search's choice of the best continuations over beams and vocabulary.
 
@@ -307,6 +318,12 @@ def beam_select(logits, scores, width=None, *, end=None, finished=None):
             logits, scores, width, end, finished), "hip_decode")
         if out is not None:
             return out
+    return _eager_select(logits, scores, width, end, finished)
+
+
+@torch.no_grad()
+def _eager_select(logits, scores, width, end, finished):
+    V = logits.shape[2]
     wide = torch.promote_types(torch.promote_types(logits.dtype, scores.dtype), torch.float32)
     x, s = logits.double(), scores.double()
     total = torch.logsumexp(x, -1)
@@ -336,12 +353,12 @@ def _leaves(states, out: list):
     """The tensors of nested lists, tuples and dicts, in order."""
     if torch.is_tensor(states):
         out.append(states)
-    elif isinstance(states, dict):
-        for s in states.values():
-            _leaves(s, out)
-    elif isinstance(states, (list, tuple)):
-        for s in states:
-            _leaves(s, out)
+    elif isinstance(states, (dict, list, tuple)):
+        for s in states.values() if isinstance(states, dict) else states:
+            if isinstance(s, torch.Tensor):
+                out.append(s)
+            else:
+                _leaves(s, out)
     elif states is not None:
         raise TypeError("reorder_states: states are tensors, None, and lists, tuples and dicts of "
                         f"them (got {type(states).__name__})")
@@ -354,14 +371,13 @@ def _rebuilt(states, new):
     if isinstance(states, dict):
         return {k: _rebuilt(s, new) for k, s in states.items()}
     if isinstance(states, (list, tuple)):
-        each = [_rebuilt(s, new) for s in states]
+        each = [next(new) if isinstance(s, torch.Tensor) else _rebuilt(s, new) for s in states]
         if hasattr(states, "_fields"):
             return type(states)(*each)
         return each if isinstance(states, list) else tuple(each)
     return None
 
 
-@torch.no_grad()
 def reorder_states(states, parents):
     """Every state's rows in the order of the chosen beams.
 
@@ -386,23 +402,29 @@ def reorder_states(states, parents):
         raise ValueError(f"{what}: parents is (B, W) (got {tuple(parents.shape)})")
     B, W = parents.shape
     tensors = _leaves(states, [])
-    for t in tensors:
-        if t.device != parents.device:
-            raise ValueError(f"{what}: a state is on {t.device}, parents on {parents.device}")
-        if t.dim() < 1 or t.shape[0] != tensors[0].shape[0] or (t.shape[0] % B if B else t.shape[0]):
-            raise ValueError(f"{what}: each state has B K rows, the same for all, with B = {B} (got "
-                             f"{tuple(t.shape)})")
     if not tensors:
         return _rebuilt(states, iter(()))
-    K = tensors[0].shape[0] // B if B else 0
+    rows, device = len(tensors[0]) if tensors[0].dim() else -1, parents.device
+    for t in tensors:
+        if t.device != device:
+            raise ValueError(f"{what}: a state is on {t.device}, parents on {device}")
+        if t.dim() < 1 or len(t) != rows or (rows % B if B else rows):
+            raise ValueError(f"{what}: each state has B K rows, the same for all, with B = {B} (got "
+                             f"{tuple(t.shape)})")
+    K = rows // B if B else 0
     if B * W and K:
         out = _dispatch(what, parents.is_cuda, lambda backend: backend.reorder_states_impl(
             tensors, parents, K), "hip_decode")
         if out is not None:
             return _rebuilt(states, iter(out))
+    return _rebuilt(states, iter(_eager_reorder(tensors, parents, K)))
+
+
+@torch.no_grad()
+def _eager_reorder(tensors, parents, K):
     parents = parents.long()
     outside = (parents < 0) | (parents >= K)
     if bool(outside.any()):
-        raise IndexError(f"{what}: parent {int(parents[outside][0])} is not one of {K} beams")
-    rows = (parents + K * torch.arange(B, device=parents.device)[:, None]).flatten()
-    return _rebuilt(states, iter([t[rows] for t in tensors]))
+        raise IndexError(f"reorder_states: parent {int(parents[outside][0])} is not one of {K} beams")
+    rows = (parents + K * torch.arange(len(parents), device=parents.device)[:, None]).flatten()
+    return [t[rows] for t in tensors]

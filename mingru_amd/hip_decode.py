@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from .hip_scans import ScanFallback, _call, _funnel, _ptr, _size, _stream, _workspace
 from .hip_sequence import _array, _last_dense, _no_tangents
@@ -150,25 +151,35 @@ def _pointers(ts):
 def reorder_states_impl(tensors, parents, K):
     """``reorder_states`` on checked arguments: a list of tensors, of ``K`` rows a search."""
     what = "reorder_states"
-    _no_tangents(what, *[t for t in tensors if t.dtype.is_floating_point])
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _no_tangents(what, *[t for t in tensors if t.dtype.is_floating_point])
     B, W = parents.shape
     if B * W >= 2**31 or K >= 2**31:
         raise ScanFallback(f"{what} kernels write fewer than 2^31 rows (got {B} x {W})")
     if parents.dtype not in (torch.int32, torch.int64):
         parents = parents.to(torch.int64)
     out, src, dst, strides, sizes = [], [], [], [], []
+    rows = B * K
     for t in tensors:
-        new = torch.empty((B * W, *t.shape[1:]), dtype=t.dtype, device=t.device)
+        dense = t.is_contiguous()
+        if dense and W == K:
+            new = torch.empty_like(t)
+        else:
+            new = torch.empty((B * W, *t.shape[1:]), dtype=t.dtype, device=t.device)
         out.append(new)
-        if new.numel() == 0:
+        size = t.nbytes // rows
+        if size == 0:
             continue
-        if not t.is_contiguous() and not t[0].is_contiguous():
+        if dense:
+            strides.append(size)
+        elif t[0].is_contiguous():
+            strides.append(t.stride(0) * t.element_size())
+        else:
             t = t.contiguous()
+            strides.append(size)
         src.append(t)
         dst.append(new)
-        size = t.element_size()
-        sizes.append(new.numel() // (B * W) * size)
-        strides.append(t.stride(0) * size)
+        sizes.append(size)
     if src:
         _funnel(what, _call, "mg_reorder_rows", len(src), _pointers(src), _pointers(dst),
                 _array(strides), _array(sizes), int(parents.dtype == torch.int64), _ptr(parents),

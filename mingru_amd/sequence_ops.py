@@ -12,6 +12,7 @@ run the eager body, which defines the results.
 from __future__ import annotations
 
 import importlib
+import sys
 import warnings
 
 import torch
@@ -36,7 +37,8 @@ def _dispatch(what: str, is_cuda: bool, call, module: str = "hip_sequence"):
             raise scans.ScanFallback(str(status))
         if not is_cuda:
             raise scans.ScanFallback("HIP kernels need GPU tensors")
-        return call(importlib.import_module(f"mingru_amd.{module}"))
+        name = f"mingru_amd.{module}"
+        return call(sys.modules.get(name) or importlib.import_module(name))
 
     result, reason = _resolve_native_dispatch(mode, what, _call)
     if reason is None:
