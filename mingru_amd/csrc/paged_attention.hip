@@ -165,373 +165,439 @@ __device__ __forceinline__ float pa_max(float x) {
 __device__ __forceinline__ float pa_sum(float x) { return mg_pair_sum<32>(mg_pair_sum<16>(x)); }
 
 // ---- the division of work --------------------------------------------------------------
+// Values that every lane holds, in scalar registers.
+__device__ __forceinline__ int64_t pa_uniform(int64_t x) {
+  return (int64_t)((uint64_t)mg_uniform((unsigned)((uint64_t)x >> 32)) << 32 | mg_uniform((unsigned)x));
+}
+
 // A sequence's tokens that count, [first, end), and the steps of SPAN tokens that hold them.
 struct PaSeq {
-  int64_t first, end;
-  int64_t step0, steps;  // of one key head
-  bool bad;              // longer than its pages
+  int first, end;
+  int step0, steps;  // of one key head
+  int bad;           // longer than its pages
 };
 template <int SPAN>
 __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, int64_t b) {
   PaSeq s;
-  int64_t n = a.lengths[b];
+  const int64_t n = a.lengths[b];
   s.bad = n > a.room;
-  n = n < 0 ? 0 : (s.bad ? a.room : n);
-  s.end = n;
-  s.first = a.window && n > a.window ? n - a.window : 0;
-  s.step0 = s.first / SPAN;
-  s.steps = n > 0 ? (n + SPAN - 1) / SPAN - s.step0 : 0;
+  s.end = (int)(n < 0 ? 0 : (n > a.room ? a.room : n));
+  s.first = a.window && s.end > a.window ? s.end - (int)a.window : 0;
+  s.step0 = (unsigned)s.first / SPAN;
+  s.steps = s.end > 0 ? (int)((unsigned)(s.end + SPAN - 1) / SPAN) - s.step0 : 0;
   return s;
 }
+template <int SPAN>
+__device__ __forceinline__ PaSeq pa_seq_uniform(const PaArgs& a, int64_t b) {
+  const PaSeq s = pa_seq<SPAN>(a, b);
+  return PaSeq{(int)mg_uniform(s.first), (int)mg_uniform(s.end), (int)mg_uniform(s.step0),
+               (int)mg_uniform(s.steps), (int)mg_uniform(s.bad)};
+}
 
-// The steps of all sequences one after another, a sequence's pairs of a key head and 16 of its
-// queries in a row.  Each thread sums a run of sequences; the whole workgroup calls it.
-struct PaRow {
-  int64_t all;         // steps in all
-  int64_t from, sum;   // before this thread's run, and behind it
-  int64_t first, run;  // its sequences
+// The steps of sequences [b0, b0 + n), the lanes taking runs of `run` of them, summed over the
+// lanes up to each, itself included.  (No LDS, no barrier: each wave looks for itself.)
+template <int SPAN>
+__device__ __forceinline__ int64_t pa_steps(const PaArgs& a, int64_t b0, int64_t n, int64_t run) {
+  const int lane = threadIdx.x & (MG_WAVE - 1);
+  int64_t sum = 0;
+  for (int64_t i = lane * run; i < (lane + 1) * run && i < n; ++i) sum += pa_seq<SPAN>(a, b0 + i).steps;
+#pragma unroll
+  for (int d = 1; d < MG_WAVE; d *= 2) {
+    const int64_t up = __shfl_up(sum, d);
+    sum += lane >= d ? up : 0;
+  }
+  return sum;
+}
+__device__ __forceinline__ int64_t pa_lane(int64_t x, int lane) {  // the same lane for all
+  return (int64_t)((uint64_t)(unsigned)__builtin_amdgcn_readlane((int)((uint64_t)x >> 32), lane) << 32 |
+                   (unsigned)__builtin_amdgcn_readlane((int)x, lane));
+}
+// All sequences' steps as one row, a sequence's pairs of a key head and 16 of its queries one
+// after another.  Sequence b's first step, or (by_step) the sequence that holds step `at`.
+struct PaPlace {
+  int64_t b, before;
 };
 template <int SPAN>
-__device__ __forceinline__ PaRow pa_row(const PaArgs& a, int64_t* lds) {
-  const int lane = threadIdx.x & (MG_WAVE - 1), wave = threadIdx.x / MG_WAVE;
-  PaRow r;
-  r.run = (a.B + PA_NT - 1) / PA_NT, r.first = r.run * threadIdx.x;
-  int64_t n = 0;
-  for (int64_t i = r.first; i < r.first + r.run && i < a.B; ++i) n += pa_seq<SPAN>(a, i).steps;
-  n *= (int64_t)a.Hk * a.tiles_q;
-  r.sum = n;
-  // Where one sequence is all, one thread knows.
-  if (a.B > 1) {
-#pragma unroll
-    for (int d = 1; d < MG_WAVE; d *= 2) {
-      const int64_t up = __shfl_up(r.sum, d);
-      r.sum += lane >= d ? up : 0;
-    }
-  }
-  if (lane == (a.B > 1 ? MG_WAVE - 1 : 0)) lds[wave] = r.sum;
-  __syncthreads();
-  r.all = 0;
-#pragma unroll
-  for (int w = 0; w < PA_NW; ++w) {
-    r.sum += w < wave ? lds[w] : 0;
-    r.all += lds[w];
-  }
-  r.from = r.sum - n;
-  __syncthreads();
-  return r;
+__device__ __forceinline__ int64_t pa_all(const PaArgs& a, int64_t pairs, int64_t& sums, int64_t& run) {
+  run = (a.B + MG_WAVE - 1) / MG_WAVE;
+  sums = pa_steps<SPAN>(a, 0, a.B, run);
+  return pa_lane(sums, MG_WAVE - 1) * pairs;
 }
+template <int SPAN, bool BY_STEP>
+__device__ __forceinline__ PaPlace pa_find(const PaArgs& a, int64_t pairs, int64_t sums, int64_t run,
+                                           int64_t b, int64_t at) {
+  PaPlace p = {0, 0};
+  int64_t n = a.B;
+  for (;;) {
+    // The run that holds it: the lanes before have all theirs before it.
+    const int lane = BY_STEP ? __popcll(__ballot(p.before + sums * pairs <= at)) : (int)((b - p.b) / run);
+    if (lane > 0) p.before += pa_lane(sums, lane - 1) * pairs;
+    p.b += lane * run;
+    if (run == 1) return p;
+    n = n - lane * run < run ? n - lane * run : run;
+    run = (run + MG_WAVE - 1) / MG_WAVE;
+    sums = pa_steps<SPAN>(a, p.b, n, run);
+  }
+}
+
 // Share w of n holds the steps [w all / n, (w + 1) all / n); no share is empty, as n <= all.
 __device__ __forceinline__ int pa_shares_used(const PaArgs& a, int64_t all) {
   return all < a.shares ? (int)all : a.shares;
 }
-__device__ __forceinline__ int64_t pa_share(int64_t w, int64_t all, int n) { return w * all / n; }
-__device__ __forceinline__ int64_t pa_holder(int64_t step, int64_t all, int n) {
-  return ((step + 1) * n - 1) / all;
+// Quotients of 32 bits where they suffice: those of 64 take some 100 instructions.
+__device__ __forceinline__ int64_t pa_share(int64_t w, int64_t all, int n) {
+  const uint64_t x = (uint64_t)w * (uint64_t)all;
+  return x >> 32 ? (int64_t)(x / (unsigned)n) : (int64_t)((unsigned)x / (unsigned)n);
+}
+__device__ __forceinline__ int pa_holder(int64_t step, int64_t all, int n) {
+  const uint64_t x = (uint64_t)(step + 1) * (unsigned)n - 1;
+  return (x | (uint64_t)all) >> 32 ? (int)(x / (uint64_t)all) : (int)((unsigned)x / (unsigned)all);
 }
 
 // ---- the main kernel -------------------------------------------------------------------
-template <typename T, int D>
+#ifndef G128
+#define G128 2
+#define G64 3
+#endif
+// Workgroups that a CU holds: at 256 a tile, its successor, queries and outputs take 300 registers.
+constexpr int pa_groups(int dk) { return dk > 128 ? 1 : (dk > 64 ? G128 : G64); }
+template <typename T, int DK, int DV>
 struct PaShape {
-  static constexpr int KEYS = Elem<T>::KEYS;    // tokens of a tile
-  static constexpr int SPAN = KEYS * PA_NW;     // of a step
-  static constexpr int E = D / 16;              // elements of a chunk
-  static constexpr int NK = KEYS / 4;           // tokens of a lane
-  static constexpr int LD = D + Elem<T>::PAD;   // elements of a key's row in LDS
-  static constexpr int OLD = D + 4;             // floats of an output row in LDS
+  static constexpr int KEYS = Elem<T>::KEYS;      // tokens of a tile
+  static constexpr int SPAN = KEYS * PA_NW;       // of a step
+  static constexpr int EK = DK / 16, EV = DV / 16;  // elements of a chunk
+  static constexpr int NK = KEYS / 4;             // tokens of a lane
+  static constexpr int LD = DK + Elem<T>::PAD;    // elements of a key's row in LDS
+  static constexpr int OLD = DV + 4;              // floats of an output row in LDS
   static constexpr int BYTES = KEYS * LD * sizeof(T);  // of a wave
-  // Workgroups of a CU: at D = 256 a tile, its successor, queries and outputs need 300 registers.
-  static constexpr int GROUPS = D == 256 ? 1 : 2;
-  static_assert(PA_ROWS * OLD * 4 <= BYTES, "the outputs lie where the keys were");
+  // Workgroups of a CU.
+  static constexpr int GROUPS = pa_groups(DK);
+  static_assert(DV <= DK && PA_ROWS * OLD * 4 <= BYTES, "the outputs lie where the keys were");
+};
+
+// One step of a share, of a piece of one pair's steps: uniform values.
+struct PaStep {
+  PaSeq seq;
+  int64_t b, left;       // sequence; steps of the share behind this piece
+  int hk, tile_q;        // the pair
+  int here, todo;        // steps of the piece, and those from this one on
+  int base;              // this wave's first token
+  bool valid;
 };
 
 // FOURS: pages hold a multiple of 4 tokens, so that a lane's tokens 4 g + j share one.
-template <typename T, int D, bool VEC, bool FOURS>
-__global__ __launch_bounds__(PA_NT, (PaShape<T, D>::GROUPS)) void paged_attention(PaArgs a) {
-  typedef PaShape<T, D> S;
-  constexpr int KEYS = S::KEYS, E = S::E, NK = S::NK, LD = S::LD, OLD = S::OLD, SPAN = S::SPAN;
-  constexpr int NG = NK / 4;  // groups of four tokens of a lane
-  typedef Chunk<T, E> C;
+template <typename T, int DK, int DV, bool VEC, bool FOURS>
+__global__ __launch_bounds__(PA_NT, (PaShape<T, DK, DV>::GROUPS)) void paged_attention(PaArgs a) {
+  typedef PaShape<T, DK, DV> S;
+  constexpr int KEYS = S::KEYS, EK = S::EK, EV = S::EV, NK = S::NK, LD = S::LD, OLD = S::OLD;
+  constexpr int SPAN = S::SPAN;
+  constexpr int NG = NK / 4;               // groups of four tokens of a lane
+  constexpr int NP = FOURS ? NG : NK;      // pages of a lane
+  constexpr int QW = DK * sizeof(T) / 64;  // vectors of 16 bytes of a query's fragment
+  typedef Chunk<T, EK> CK;
+  typedef Chunk<T, EV> CV;
   __shared__ alignas(16) unsigned char s_tile[PA_NW][S::BYTES];
   __shared__ float s_max[PA_NW][PA_ROWS], s_sum[PA_NW][PA_ROWS];
-  __shared__ int64_t s_find[PA_NW];
 
   const int lane = threadIdx.x & (MG_WAVE - 1), wave = (int)mg_uniform(threadIdx.x / MG_WAVE);
   const int c = lane & 15, g = lane >> 4;
   T* const tile = (T*)s_tile[wave];
   float* const sums = (float*)s_tile[wave];
+  const bool short_k = DK != a.dk;
 
-  // This share's first step, and the sequence that it lies in.
-  const PaRow row = pa_row<SPAN>(a, s_find);
-  const int shares = pa_shares_used(a, row.all);
-  if ((int)blockIdx.x >= shares) return;
-  int64_t at = pa_share(blockIdx.x, row.all, shares);
-  const int64_t stop = pa_share(blockIdx.x + 1, row.all, shares);
-  const int64_t pairs = (int64_t)a.Hk * a.tiles_q;
-  int64_t b = 0, before = 0;
-  if (a.B > 1) {
-    if (at >= row.from && at < row.sum) {  // one thread's run holds it
-      b = row.first, before = row.from;
-      for (;; ++b) {
-        const int64_t m = pa_seq<SPAN>(a, b).steps * pairs;
-        if (at < before + m) break;
-        before += m;
-      }
-      s_find[0] = b, s_find[1] = before;
-    }
-    __syncthreads();
-    b = s_find[0], before = s_find[1];
+  // This share's first step.
+  PaStep now;
+  {
+    const int64_t pairs = (int64_t)a.Hk * a.tiles_q;
+    int64_t steps, run;
+    const int64_t all = pa_all<SPAN>(a, pairs, steps, run);
+    const int shares = pa_shares_used(a, all);
+    if ((int)blockIdx.x >= shares) return;
+    const int64_t at = pa_share(blockIdx.x, all, shares);
+    now.left = pa_share(blockIdx.x + 1, all, shares) - at;
+    const PaPlace p = pa_find<SPAN, true>(a, pairs, steps, run, 0, at);
+    now.b = pa_uniform(p.b);
+    now.seq = pa_seq_uniform<SPAN>(a, now.b);
+    const int64_t in = pa_uniform(at - p.before);
+    const int pair = in >> 32 ? (int)(in / now.seq.steps) : (int)((unsigned)in / (unsigned)now.seq.steps);
+    now.hk = pair / a.tiles_q, now.tile_q = pair - now.hk * a.tiles_q;
+    now.todo = (int)(in - (int64_t)pair * now.seq.steps);  // the step, for now
+    now.valid = true;
   }
-  const bool short_k = D != a.dk;
-  bool head = true;  // of this share
-  while (at < stop) {
-    PaSeq seq = pa_seq<SPAN>(a, b);
-    while (at >= before + seq.steps * pairs) {
-      before += seq.steps * pairs;
-      seq = pa_seq<SPAN>(a, ++b);
+  auto open = [&](PaStep& s, int step) {  // a piece from that step of its pair on
+    const int n = s.seq.steps - step;
+    s.here = s.left < n ? (int)s.left : n, s.todo = s.here, s.left -= s.here;
+    s.base = (s.seq.step0 + step) * SPAN + wave * KEYS;
+  };
+  auto advance = [&](PaStep& s) {
+    if (--s.todo > 0) {
+      s.base += SPAN;
+    } else if (s.left > 0) {
+      if (++s.tile_q == a.tiles_q) s.tile_q = 0, ++s.hk;
+      if (s.hk == a.Hk) {
+        s.hk = 0;
+        do s.seq = pa_seq_uniform<SPAN>(a, ++s.b);
+        while (s.seq.steps == 0);
+      }
+      open(s, 0);
+    } else {
+      s.valid = false, s.todo = 1, s.base = s.seq.end;  // every lane asks for the last token
     }
-    const int64_t pair = (at - before) / seq.steps, in = at - before - pair * seq.steps;
-    const int64_t here = seq.steps - in < stop - at ? seq.steps - in : stop - at;
-    const int hk = (int)(pair / a.tiles_q), q0 = (int)(pair - (int64_t)hk * a.tiles_q) * PA_ROWS;
-    const int rows = a.group - q0 < PA_ROWS ? a.group - q0 : PA_ROWS;
-    const T* const kc = (const T*)a.k + hk * a.ks[1];
-    const T* const vc = (const T*)a.v + hk * a.vs[1];
-    const int64_t table = b * a.page_stride;
-    const int first = (int)seq.first, end = (int)seq.end;
+  };
+  open(now, now.todo);
+  PaStep next = now;
+  advance(next);
+  PaStep far = next;
+  advance(far);
 
-    // Queries: column c, the elements that a key's fragment holds, 0 behind the head's.
-    constexpr int QW = D * sizeof(T) / 16 / 4;  // vectors of 16 bytes
-    u32x4 qf[QW];
-    {
-      const T* row = (const T*)a.q + b * a.qs[0] + (int64_t)(hk * a.group + q0 + (c < rows ? c : 0)) * a.qs[1];
-      constexpr int VE = 16 / sizeof(T);
+  CK kr[NK];
+  CV vr[NK];
+  unsigned page[NP], upper[NP];
+  int64_t vo[NP];
+  unsigned bad = 0, bad_next = 0;  // tokens of this lane whose page is not in the cache
+  u32x4 qf[QW];
+  auto token = [&](const PaStep& s, int i) {  // behind the last token, one of its page
+    const int key = s.base + (FOURS ? 16 * i + 4 * g : 16 * (i / 4) + 4 * g + i % 4);
+    return key < s.seq.end ? key : (FOURS ? (s.seq.end - 1) & ~3 : s.seq.end - 1);
+  };
+  // The pages of a step's tokens: both words without a branch, where the loads would be waited
+  // for.  The upper one of an int64 that is a page is 0, as N < 2^31; of an int32 the same word
+  // stands for it.
+  auto look = [&](const PaStep& s) {
+    const unsigned* const row = (const unsigned*)a.pages.p + ((s.b * a.page_stride) << a.pages.wide);
 #pragma unroll
-      for (int s = 0; s < QW; ++s) {
-        Chunk<T, VE> x;
-        pa_load<T, VE, false>(row, 4 * s + g, a.dk, x);
-        pa_clear<T, VE>(4 * s + g, a.dk, x);
-        qf[s] = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
+    for (int i = 0; i < NP; ++i) {
+      const unsigned* const p = row + ((size_t)pg_div((unsigned)token(s, i), a.P) << a.pages.wide);
+      page[i] = p[0], upper[i] = p[a.pages.wide];
+    }
+  };
+  // Loads of the keys, from the pages that were looked up; the values' places are kept.
+  auto keys = [&](const PaStep& s) {
+    const T* const kc = (const T*)a.k + s.hk * a.ks[1];
+    bad_next = 0;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int key = token(s, i);
+      const int slot = key - (int)(pg_div((unsigned)key, a.P) * a.P.d);
+      const bool in = page[i] < (unsigned)a.N && (!a.pages.wide || upper[i] == 0);
+      bad_next |= in ? 0u : 1u << i;
+      const int64_t p = in ? page[i] : 0;
+      vo[i] = s.hk * a.vs[1] + p * a.vs[0] + slot * a.vs[2];
+      const T* row = kc + p * a.ks[0] + slot * a.ks[2];
+      if constexpr (FOURS) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pa_load<T, EK, VEC>(row + j * a.ks[2], c, a.dk, kr[4 * i + j]);
+      } else {
+        pa_load<T, EK, VEC>(row, c, a.dk, kr[i]);
       }
     }
+  };
+  auto values = [&] {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const T* row = (const T*)a.v + vo[i];
+      if constexpr (FOURS) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pa_load<T, EV, VEC>(row + j * a.vs[2], c, a.dv, vr[4 * i + j]);
+      } else {
+        pa_load<T, EV, VEC>(row, c, a.dv, vr[i]);
+      }
+    }
+  };
+  // Queries: column c, the elements that a key's fragment holds, 0 behind the head's.
+  auto queries = [&](const PaStep& s) {
+    const int q0 = s.hk * a.group + s.tile_q * PA_ROWS, rows = a.group - s.tile_q * PA_ROWS;
+    const T* row = (const T*)a.q + s.b * a.qs[0] + (int64_t)(q0 + (c < rows ? c : 0)) * a.qs[1];
+    constexpr int VE = 16 / sizeof(T);
+    // Places in a row are formed anew for each piece: kept, they take a register an element.
+    int chunk = g;
+    asm volatile("" : "+v"(chunk));
+#pragma unroll
+    for (int s = 0; s < QW; ++s) {
+      Chunk<T, VE> x;
+      pa_load<T, VE, false>(row, 4 * s + chunk, a.dk, x);
+      pa_clear<T, VE>(4 * s + chunk, a.dk, x);
+      qf[s] = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
+    }
+  };
 
-    f32x4 o[E];
+  look(now);
+  queries(now);
+  keys(now);
+  values();
+  look(next);
+  f32x4 o[EV];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float top = -__builtin_inff(), sum = 0.f;
-
-    // The first token of this wave's tile in step i of this piece.
-    const int base0 = (int)((seq.step0 + in) * SPAN) + wave * KEYS;
-    C kr[NK], vr[NK];
-    int page[FOURS ? NG : NK];  // -1: not in the cache
-    // The pages of a tile's tokens; tokens behind the last take its page.
-    auto look = [&](int base) {
+  for (int e = 0; e < EV; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float top = -__builtin_inff(), sum = 0.f;
+  bool head = true;  // the share's first piece
+  for (;;) {
+    const int base = now.base, first = now.seq.first, end = now.seq.end;
+    // Keys into LDS, and the next step's on their way, whichever piece it is of.
 #pragma unroll
-      for (int i = 0; i < (FOURS ? NG : NK); ++i) {
-        int key = base + (FOURS ? 16 * i + 4 * g : 16 * (i / 4) + 4 * g + i % 4);
-        key = key < end ? key : end - 1;
-        const int64_t p = a.pages[table + pg_div((unsigned)key, a.P)];
-        page[i] = p >= 0 && p < a.N ? (int)p : -1;
+    for (int j = 0; j < NK; ++j) {
+      if (short_k) pa_clear<T, EK>(c, a.dk, kr[j]);
+      T* dst = tile + (16 * (j / 4) + 4 * g + j % 4) * LD + c * EK;
+      if constexpr (CK::W == 2) {
+        *(u32x2*)dst = u32x2{kr[j].w[0], kr[j].w[1]};
+      } else {
+#pragma unroll
+        for (int w = 0; w < CK::W; w += 4)
+          *(u32x4*)((unsigned*)dst + w) =
+              u32x4{kr[j].w[w], kr[j].w[w + 1], kr[j].w[w + 2], kr[j].w[w + 3]};
       }
-    };
-    unsigned bad = 0, bad_next = 0;  // tokens of this lane whose page is not in the cache
-    int64_t vo[FOURS ? NG : NK];
-    // Loads of the keys, from the pages that were looked up; the values' places are kept.
-    auto keys = [&](int base) {
-      bad_next = 0;
+    }
+    bad = bad_next;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    // Under no condition: loads under one would be waited for where the branches meet.
+    keys(next);
+    look(far);
+    // A wave without a token here (the ends of the row of tokens) has nothing to add.
+    if (base < end && base + KEYS > first) {
+      f32x4 s[NG];
 #pragma unroll
-      for (int i = 0; i < (FOURS ? NG : NK); ++i) {
-        int key = base + (FOURS ? 16 * i + 4 * g : 16 * (i / 4) + 4 * g + i % 4);
-        const int last = FOURS ? (end - 1) & ~3 : end - 1;
-        key = key < end ? key : last;
-        const int slot = key - (int)(pg_div((unsigned)key, a.P) * a.P.d);
-        bad_next |= page[i] < 0 ? 1u << i : 0u;
-        const int64_t p = page[i] < 0 ? 0 : page[i];
-        vo[i] = p * a.vs[0] + slot * a.vs[2];
-        const T* row = kc + p * a.ks[0] + slot * a.ks[2];
-        if constexpr (FOURS) {
+      for (int t = 0; t < NG; ++t) {
+        s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            pa_load<T, E, VEC>(row + j * a.ks[2], c, a.dk, kr[4 * i + j]);
-        } else {
-          pa_load<T, E, VEC>(row, c, a.dk, kr[i]);
-        }
-      }
-    };
-    auto values = [&] {
+        for (int x = 0; x < QW; ++x) {
+          const u32x4 kf = *(const u32x4*)((const unsigned char*)(tile + (16 * t + c) * LD) + 64 * x + 16 * g);
+          if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < (FOURS ? NG : NK); ++i) {
-        const T* row = vc + vo[i];
-        if constexpr (FOURS) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            pa_load<T, E, VEC>(row + j * a.vs[2], c, a.dv, vr[4 * i + j]);
-        } else {
-          pa_load<T, E, VEC>(row, c, a.dv, vr[i]);
-        }
-      }
-    };
-    look(base0);
-    keys(base0);
-    values();
-    look(here > 1 ? base0 + SPAN : end);
-    for (int64_t i = 0; i < here; ++i) {
-      const int base = base0 + (int)i * SPAN;
-      // Keys into LDS, and the next tile's on their way.
-#pragma unroll
-      for (int j = 0; j < NK; ++j) {
-        if (short_k) pa_clear<T, E>(c, a.dk, kr[j]);
-        T* dst = tile + (16 * (j / 4) + 4 * g + j % 4) * LD + c * E;
-        if constexpr (C::W == 2) {
-          *(u32x2*)dst = u32x2{kr[j].w[0], kr[j].w[1]};
-        } else {
-#pragma unroll
-          for (int w = 0; w < C::W; w += 4)
-            *(u32x4*)((unsigned*)dst + w) =
-                u32x4{kr[j].w[w], kr[j].w[w + 1], kr[j].w[w + 2], kr[j].w[w + 3]};
-        }
-      }
-      bad = bad_next;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      // Under no condition: loads under one would be waited for where the branches meet.  Behind
-      // the piece every lane asks for the last token, one row.
-      const int next = i + 1 < here ? base + SPAN : end;
-      keys(next);
-      look(i + 2 < here ? next + SPAN : end);
-      // A wave without a token here (the ends of the row of tokens) has nothing to add.
-      if (base < end && base + KEYS > first) {
-        f32x4 s[NG];
-#pragma unroll
-        for (int t = 0; t < NG; ++t) {
-          s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int x = 0; x < QW; ++x) {
-            const u32x4 kf = *(const u32x4*)((const unsigned char*)(tile + (16 * t + c) * LD) + 64 * x + 16 * g);
-            if constexpr (sizeof(T) == 4) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                    __uint_as_float(kf[e]), __uint_as_float(qf[x][e]), s[t], 0, 0, 0);
-            } else {
-              s[t] = Elem<T>::mma(kf, qf[x], s[t]);
-            }
+            for (int e = 0; e < 4; ++e)
+              s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[e]),
+                                                          __uint_as_float(qf[x][e]), s[t], 0, 0, 0);
+          } else {
+            s[t] = Elem<T>::mma(kf, qf[x], s[t]);
           }
         }
-        float p[NK], peak = -__builtin_inff();
-        const bool whole = base >= first && base + KEYS <= end && __ballot(bad != 0) == 0;
+      }
+      float p[NK], peak = -__builtin_inff();
+      const bool whole = base >= first && base + KEYS <= end && __ballot(bad != 0) == 0;
 #pragma unroll
-        for (int j = 0; j < NK; ++j) p[j] = s[j / 4][j % 4] * a.scale;
-        if (!whole) {
-#pragma unroll
-          for (int j = 0; j < NK; ++j) {
-            const int key = base + 16 * (j / 4) + 4 * g + j % 4;
-            const bool live = key >= first && key < end;
-            const bool lost = bad >> (FOURS ? j / 4 : j) & 1;
-            p[j] = live ? (lost ? __builtin_nanf("") : p[j]) : -__builtin_inff();
-            // 0 times a value that is not finite would be a NaN.
-#pragma unroll
-            for (int w = 0; w < C::W; ++w) vr[j].w[w] = live ? vr[j].w[w] : 0u;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < NK; ++j) peak = fmaxf(peak, p[j]);
-        peak = fmaxf(pa_max(peak), top);
-        const float from = peak == -__builtin_inff() ? 0.f : peak;
-        if (__ballot(peak > top) != 0) {
-          const float down = pa_exp2(top - from);
-          sum *= down;
-#pragma unroll
-          for (int e = 0; e < E; ++e) o[e] *= down;
-          top = peak;
-        }
+      for (int j = 0; j < NK; ++j) p[j] = s[j / 4][j % 4] * a.scale;
+      if (!whole) {
 #pragma unroll
         for (int j = 0; j < NK; ++j) {
-          p[j] = pa_exp2(p[j] - from);
-          sum += p[j];
-        }
-        if constexpr (sizeof(T) == 4) {
+          const int key = base + 16 * (j / 4) + 4 * g + j % 4;
+          const bool live = key >= first && key < end;
+          const bool lost = bad >> (FOURS ? j / 4 : j) & 1;
+          p[j] = live ? (lost ? __builtin_nanf("") : p[j]) : -__builtin_inff();
+          // 0 times a value that is not finite would be a NaN.
 #pragma unroll
-          for (int j = 0; j < NK; ++j)
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-              o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[j].w[e]), p[j], o[e],
-                                                          0, 0, 0);
-        } else {
-          u32x4 hi, lo;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            hi[j] = Elem<T>::pack(p[2 * j], p[2 * j + 1]);
-            lo[j] = Elem<T>::pack(p[2 * j] - Elem<T>::low(hi[j]), p[2 * j + 1] - Elem<T>::high(hi[j]));
-          }
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            u32x4 vf;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)  // element e of tokens 2 j and 2 j + 1
-              vf[j] = __builtin_amdgcn_perm(vr[2 * j + 1].w[e / 2], vr[2 * j].w[e / 2],
-                                            e & 1 ? 0x07060302u : 0x05040100u);
-            o[e] = Elem<T>::mma(vf, hi, o[e]);
-            o[e] = Elem<T>::mma(vf, lo, o[e]);
-          }
+          for (int w = 0; w < CV::W; ++w) vr[j].w[w] = live ? vr[j].w[w] : 0u;
         }
       }
-      values();
-      __builtin_amdgcn_wave_barrier();
-    }
-
-    // The waves' sums, in LDS where the keys were.
-    sum = pa_sum(sum);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+      for (int j = 0; j < NK; ++j) peak = fmaxf(peak, p[j]);
+      peak = fmaxf(pa_max(peak), top);
+      const float from = peak == -__builtin_inff() ? 0.f : peak;
+      if (__ballot(peak > top) != 0) {
+        const float down = pa_exp2(top - from);
+        sum *= down;
 #pragma unroll
-      for (int e = 0; e < E; e += 4)
-        *(f32x4*)(sums + c * OLD + E * (4 * g + i) + e) =
-            f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
-    }
-    if (lane < PA_ROWS) s_max[wave][lane] = top, s_sum[wave][lane] = sum;
-    __syncthreads();
-    const bool done = here == seq.steps;
-    const int64_t slot = 2 * (int64_t)blockIdx.x + (head ? 0 : 1);
-    for (int n = threadIdx.x; n < rows * (D / 4); n += PA_NT) {
-      const int r = n / (D / 4), x = 4 * (n - r * (D / 4));
-      if (x >= a.dv) continue;
-      float m = s_max[0][r];
-      for (int w = 1; w < PA_NW; ++w) m = fmaxf(m, s_max[w][r]);
-      const float from = m == -__builtin_inff() ? 0.f : m;
-      f32x4 v = {0.f, 0.f, 0.f, 0.f};
-      float l = 0.f;
-      for (int w = 0; w < PA_NW; ++w) {
-        const float down = pa_exp2(s_max[w][r] - from);
-        l += down * s_sum[w][r];
-        v += down * *(const f32x4*)((const float*)s_tile[w] + r * OLD + x);
+        for (int e = 0; e < EV; ++e) o[e] *= down;
+        top = peak;
       }
-      if (done) {
-        T* dst = (T*)a.o + (b * a.H + hk * a.group + q0 + r) * (int64_t)a.dv;
-        const float inv = seq.bad ? __builtin_nanf("") : 1.f / l;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (x + e < a.dv) dst[x + e] = pg_round<T>(v[e] * inv);
+      for (int j = 0; j < NK; ++j) {
+        p[j] = pa_exp2(p[j] - from);
+        sum += p[j];
+      }
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < NK; ++j)
+#pragma unroll
+          for (int e = 0; e < EV; ++e)
+            o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[j].w[e]), p[j], o[e], 0,
+                                                        0, 0);
       } else {
-        float* dst = a.part + (slot * a.rows + r) * a.dv;
+        u32x4 hi, lo;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (x + e < a.dv) dst[x + e] = v[e];
-        if (x == 0) {
-          float* stat = a.part + 2 * (int64_t)a.shares * a.rows * a.dv + (slot * a.rows + r) * 2;
-          stat[0] = m, stat[1] = l;
+        for (int j = 0; j < 4; ++j) {
+          hi[j] = Elem<T>::pack(p[2 * j], p[2 * j + 1]);
+          lo[j] = Elem<T>::pack(p[2 * j] - Elem<T>::low(hi[j]), p[2 * j + 1] - Elem<T>::high(hi[j]));
+        }
+#pragma unroll
+        for (int e = 0; e < EV; ++e) {
+          u32x4 vf;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // element e of tokens 2 j and 2 j + 1
+            vf[j] = __builtin_amdgcn_perm(vr[2 * j + 1].w[e / 2], vr[2 * j].w[e / 2],
+                                          e & 1 ? 0x07060302u : 0x05040100u);
+          o[e] = Elem<T>::mma(vf, hi, o[e]);
+          o[e] = Elem<T>::mma(vf, lo, o[e]);
         }
       }
     }
-    __syncthreads();
-    at += here;
-    head = false;
+    __builtin_amdgcn_sched_barrier(0);
+    values();
+    __builtin_amdgcn_wave_barrier();
+    if (now.todo == 1) {
+      // The piece's end: the waves' sums meet in LDS, where the keys were.
+      if (next.valid) queries(next);
+      sum = pa_sum(sum);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int e = 0; e < EV; e += 4)
+          *(f32x4*)(sums + c * OLD + EV * (4 * g + i) + e) =
+              f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
+      }
+      if (lane < PA_ROWS) s_max[wave][lane] = top, s_sum[wave][lane] = sum;
+      __syncthreads();
+      const bool done = now.here == now.seq.steps;
+      const int q0 = now.tile_q * PA_ROWS, rows = a.group - q0 < PA_ROWS ? a.group - q0 : PA_ROWS;
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (head ? 0 : 1);
+      for (int n = threadIdx.x; n < rows * (DV / 4); n += PA_NT) {
+        const int r = n / (DV / 4), x = 4 * (n - r * (DV / 4));
+        if (x >= a.dv) continue;
+        float m = s_max[0][r];
+#pragma unroll
+        for (int w = 1; w < PA_NW; ++w) m = fmaxf(m, s_max[w][r]);
+        const float from = m == -__builtin_inff() ? 0.f : m;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
+#pragma unroll
+        for (int w = 0; w < PA_NW; ++w) {
+          const float down = pa_exp2(s_max[w][r] - from);
+          l += down * s_sum[w][r];
+          v += down * *(const f32x4*)((const float*)s_tile[w] + r * OLD + x);
+        }
+        if (done) {
+          T* dst = (T*)a.o + (now.b * a.H + now.hk * a.group + q0 + r) * (int64_t)a.dv;
+          const float inv = now.seq.bad ? __builtin_nanf("") : 1.f / l;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (x + e < a.dv) dst[x + e] = pg_round<T>(v[e] * inv);
+        } else {
+          float* dst = a.part + (slot * a.rows + r) * a.dv;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (x + e < a.dv) dst[x + e] = v[e];
+          if (x == 0) {
+            float* stat = a.part + 2 * (int64_t)a.shares * a.rows * a.dv + (slot * a.rows + r) * 2;
+            stat[0] = m, stat[1] = l;
+          }
+        }
+      }
+      if (!next.valid) return;
+      __syncthreads();
+      head = false;
+      top = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < EV; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    now = next, next = far;
+    if (far.valid) advance(far);
   }
 }
 
 // Joins the pieces of one query head: a workgroup each.
-constexpr int PA_MOST = 512;  // shares
+constexpr int PA_MOST = 1024;  // shares
 template <typename T, int SPAN>
 __global__ __launch_bounds__(PA_NT) void paged_attention_join(PaArgs a) {
-  __shared__ int64_t s_find[PA_NW + 1];
   __shared__ float s_weight[PA_MOST], s_red[2 * PA_NW];
   __shared__ f32x4 s_part[PA_NT];
   const int lane = threadIdx.x & (MG_WAVE - 1), wave = threadIdx.x / MG_WAVE;
@@ -545,25 +611,17 @@ __global__ __launch_bounds__(PA_NT) void paged_attention_join(PaArgs a) {
       dst[x] = pg_round<T>(seq.bad ? __builtin_nanf("") : 0.f);
     return;
   }
-  const PaRow row = pa_row<SPAN>(a, s_find);
-  int64_t before = 0;
-  if (a.B > 1) {
-    if (b >= row.first && b < row.first + row.run) {
-      before = row.from;
-      for (int64_t i = row.first; i < b; ++i)
-        before += pa_seq<SPAN>(a, i).steps * (int64_t)a.Hk * a.tiles_q;
-      s_find[PA_NW] = before;
-    }
-    __syncthreads();
-    before = s_find[PA_NW];
-  }
-  const int shares = pa_shares_used(a, row.all);
+  const int64_t pairs = (int64_t)a.Hk * a.tiles_q;
+  int64_t steps, run;
+  const int64_t all = pa_all<SPAN>(a, pairs, steps, run);
+  const int64_t before = pa_find<SPAN, false>(a, pairs, steps, run, b, 0).before;
+  const int shares = pa_shares_used(a, all);
   const int64_t from = before + ((int64_t)hk * a.tiles_q + in / PA_ROWS) * seq.steps;
-  const int w0 = (int)pa_holder(from, row.all, shares);
-  const int n = (int)pa_holder(from + seq.steps - 1, row.all, shares) - w0 + 1;
+  const int w0 = pa_holder(from, all, shares);
+  const int n = pa_holder(from + seq.steps - 1, all, shares) - w0 + 1;
   if (n == 1) return;  // one share held it and has written it
   // The pieces are the first or second one of w0, then the first ones of w0 + 1 .. w0 + n - 1.
-  const int second = pa_share(w0, row.all, shares) == from ? 0 : 1;
+  const int second = pa_share(w0, all, shares) == from ? 0 : 1;
   const float* const stat = a.part + 2 * (int64_t)a.shares * a.rows * a.dv;
   auto place = [&](int i) { return ((int64_t)2 * (w0 + i) + (i ? 0 : second)) * a.rows + r; };
   float m[PA_MOST / PA_NT], l[PA_MOST / PA_NT], top = -__builtin_inff(), sum = 0.f;
@@ -624,7 +682,7 @@ __global__ __launch_bounds__(PA_NT) void paged_attention_join(PaArgs a) {
 
 // ---- host --------------------------------------------------------------------------------
 // Shares: as many as the chip's 256 CUs hold workgroups at once.
-int pa_most(int dk, int dv) { return 256 * (dk > 128 || dv > 128 ? 1 : 2); }
+int pa_most(int dk, int dv) { return 256 * pa_groups(dk > dv ? dk : dv); }
 
 bool pa_ok(int dtype, int64_t B, int H, int Hk, int dk, int dv, int64_t M, int64_t P) {
   return dtype >= 0 && dtype <= 2 && B >= 1 && H >= 1 && Hk >= 1 && H % Hk == 0 && dk >= 1 &&
@@ -632,7 +690,7 @@ bool pa_ok(int dtype, int64_t B, int H, int Hk, int dk, int dv, int64_t M, int64
          M < 1ll << 31 && M * P < (1ll << 31) - 1024 && B < 1ll << 24 && H < 1 << 24 &&
          B * H < 1ll << 24;
 }
-int pa_span(int dtype) { return dtype == 0 ? PaShape<float, 64>::SPAN : PaShape<Bf16, 64>::SPAN; }
+int pa_span(int dtype) { return dtype == 0 ? PaShape<float, 64, 64>::SPAN : PaShape<Bf16, 64, 64>::SPAN; }
 // Workgroups: no more than there can be steps.
 int pa_shares(int dtype, int64_t B, int H, int Hk, int dk, int dv, int64_t M, int64_t P) {
   const int64_t span = pa_span(dtype), tiles = (H / Hk + PA_ROWS - 1) / PA_ROWS;
@@ -642,29 +700,32 @@ int pa_shares(int dtype, int64_t B, int H, int Hk, int dk, int dv, int64_t M, in
 }
 int pa_rows(int H, int Hk) { return H / Hk < PA_ROWS ? H / Hk : PA_ROWS; }
 
-template <typename T, int D>
-void pa_launch(const PaArgs& a, bool vec, bool fours, hipStream_t stream) {
+template <typename T, int DK, int DV>
+void pa_launch(const PaArgs& a, hipStream_t stream) {
+  // Vectors of a chunk: 16 bytes, 8 where a chunk is no more.
+  const int e = sizeof(T), bk = DK * e / 16 < 16 ? 8 : 16, bv = DV * e / 16 < 16 ? 8 : 16;
+  bool vec = a.dk * e % bk == 0 && a.dv * e % bv == 0 && ((uintptr_t)a.k & (bk - 1)) == 0 &&
+             ((uintptr_t)a.v & (bv - 1)) == 0;
+  for (int i = 0; i < 3; ++i) vec = vec && a.ks[i] * e % bk == 0 && a.vs[i] * e % bv == 0;
   const dim3 grid(a.shares), nt(PA_NT);
-  if (vec && fours) hipLaunchKernelGGL((paged_attention<T, D, true, true>), grid, nt, 0, stream, a);
-  else if (vec) hipLaunchKernelGGL((paged_attention<T, D, true, false>), grid, nt, 0, stream, a);
-  else hipLaunchKernelGGL((paged_attention<T, D, false, false>), grid, nt, 0, stream, a);
+  if (vec && a.P.d % 4 == 0)
+    hipLaunchKernelGGL((paged_attention<T, DK, DV, true, true>), grid, nt, 0, stream, a);
+  else if (vec)
+    hipLaunchKernelGGL((paged_attention<T, DK, DV, true, false>), grid, nt, 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_attention<T, DK, DV, false, false>), grid, nt, 0, stream, a);
 }
 template <typename T>
 int pa_run(const PaArgs& a, hipStream_t stream) {
-  const int d = a.dk > a.dv ? a.dk : a.dv, D = d <= 64 ? 64 : (d <= 128 ? 128 : 256);
-  // Vectors of a chunk: 16 bytes, 8 where a chunk is no more.
-  const int bytes = D * (int)sizeof(T) / 16 < 16 ? 8 : 16, e = sizeof(T);
-  bool vec = a.dk * e % bytes == 0 && a.dv * e % bytes == 0 &&
-             (((uintptr_t)a.k | (uintptr_t)a.v) & (bytes - 1)) == 0;
-  for (int i = 0; i < 3; ++i)
-    vec = vec && (a.ks[i] * e) % bytes == 0 && (a.vs[i] * e) % bytes == 0;
-  const bool fours = a.P.d % 4 == 0;
-  if (D == 64) pa_launch<T, 64>(a, vec, fours, stream);
-  else if (D == 128) pa_launch<T, 128>(a, vec, fours, stream);
-  else pa_launch<T, 256>(a, vec, fours, stream);
+  const int dk = a.dk > a.dv ? a.dk : a.dv;
+  if (dk <= 64) pa_launch<T, 64, 64>(a, stream);
+  else if (dk <= 128 && a.dv <= 64) pa_launch<T, 128, 64>(a, stream);
+  else if (dk <= 128) pa_launch<T, 128, 128>(a, stream);
+  else if (a.dv <= 128) pa_launch<T, 256, 128>(a, stream);
+  else pa_launch<T, 256, 256>(a, stream);
   if (hipGetLastError() != hipSuccess) return MG_ERR_LAUNCH;
-  hipLaunchKernelGGL((paged_attention_join<T, PaShape<T, 64>::SPAN>), dim3((unsigned)(a.B * a.H)),
-                     dim3(PA_NT), 0, stream, a);
+  hipLaunchKernelGGL((paged_attention_join<T, PaShape<T, 64, 64>::SPAN>),
+                     dim3((unsigned)(a.B * a.H)), dim3(PA_NT), 0, stream, a);
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
 
