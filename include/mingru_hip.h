@@ -526,7 +526,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
  *
  * mg_paged_append: new tokens k (B, T, Hk, dk), v (B, T, Hk, dv), token t of sequence b at
  * position start[b] + t, go into the caches; q (B, T, H, dk) or NULL goes to q_out, dense.  With
- * n > 0 frequencies (fp32, or fp64 for freq_dtype 1), 2 n <= dk, n <= 2048, elements i and i + n
+ * n > 0 frequencies (fp32, or fp64 for freq_dtype 1), 2 n <= dk, n <= 1024, elements i and i + n
  * (2 i and 2 i + 1 if interleaved) of q and k turn by position times freq[i] radians.  lengths
  * (B) or NULL: tokens of right-padded sequences; the rest has no effect but queries of 0.  A
  * token of a negative page is not kept; one outside of its row of M pages, or of a page from N

@@ -11,7 +11,7 @@
 // the lanes.  Of the keys that a lane each offers, those that beat the W-th of them are put in
 // one by one where they are few, or sorted and merged (bitonic, over the lanes).  A long row has
 // few such keys: after n of them a new one comes with W / n, so that most elements cost a
-// comparison.  The lanes' largest elements of the first tile, sorted, are the first best.
+// comparison of values.  A first bar is the W-th of the lanes' largest values of the first tile.
 // Lanes exchange keys by row operations and swaps of half rows, without LDS.
 // Keys are whole numbers that order as (value, lower index first), no two alike: the result
 // does not depend on the order of arrival, and ties fall as they are defined.
@@ -60,37 +60,51 @@ __device__ __forceinline__ unsigned bs_prev(unsigned x) {  // of the lane before
 }
 
 // A key orders as (value, lower index first); 0 is below every key.  Key32's value is of 32
-// bits, above its inverted index; Key64's of 64.
+// bits, above its inverted index; Key64's of 64.  Words by name, not in an array: a choice
+// between two arrays' elements becomes one between their addresses, in memory.
+__device__ __forceinline__ unsigned long long bs_join(unsigned hi, unsigned lo) {
+  return (unsigned long long)hi << 32 | lo;
+}
 struct Key32 {
-  unsigned w[2];
-  __device__ __forceinline__ unsigned long long all() const {
-    return (unsigned long long)w[1] << 32 | w[0];
+  unsigned index, value;
+  __device__ __forceinline__ unsigned long long all() const { return bs_join(value, index); }
+  __device__ __forceinline__ bool above(Key32 o) const { return all() > o.all(); }
+  template <typename F>
+  __device__ __forceinline__ Key32 map(F&& f) const {
+    return Key32{f(index), f(value)};
   }
-  __device__ __forceinline__ bool above(const Key32& o) const { return all() > o.all(); }
+  __device__ __forceinline__ Key32 pick(bool first, Key32 o) const {
+    return Key32{first ? index : o.index, first ? value : o.value};
+  }
+};
+struct Value32 {  // no index: for a bar
+  unsigned value;
+  __device__ __forceinline__ bool above(Value32 o) const { return value > o.value; }
+  template <typename F>
+  __device__ __forceinline__ Value32 map(F&& f) const {
+    return Value32{f(value)};
+  }
+  __device__ __forceinline__ Value32 pick(bool first, Value32 o) const {
+    return Value32{first ? value : o.value};
+  }
 };
 struct Key64 {
-  unsigned w[3];
-  __device__ __forceinline__ unsigned long long value() const {
-    return (unsigned long long)w[2] << 32 | w[1];
+  unsigned index, lo, hi;
+  __device__ __forceinline__ unsigned long long value() const { return bs_join(hi, lo); }
+  __device__ __forceinline__ bool above(Key64 o) const {
+    return value() > o.value() || (value() == o.value() && index > o.index);
   }
-  __device__ __forceinline__ bool above(const Key64& o) const {
-    return value() > o.value() || (value() == o.value() && w[0] > o.w[0]);
+  template <typename F>
+  __device__ __forceinline__ Key64 map(F&& f) const {
+    return Key64{f(index), f(lo), f(hi)};
+  }
+  __device__ __forceinline__ Key64 pick(bool first, Key64 o) const {
+    return Key64{first ? index : o.index, first ? lo : o.lo, first ? hi : o.hi};
   }
 };
-template <typename K, typename F>
-__device__ __forceinline__ K bs_map(const K& x, F&& f) {
-  K y;
-#pragma unroll
-  for (int i = 0; i < (int)(sizeof(K) / 4); ++i) y.w[i] = f(x.w[i], i);
-  return y;
-}
 template <typename K>
-__device__ __forceinline__ K bs_pick(bool first, const K& x, const K& y) {
-  return bs_map(x, [&](unsigned w, int i) { return first ? w : y.w[i]; });
-}
-template <typename K>
-__device__ __forceinline__ K bs_from(const K& x, int lane) {  // the same lane for all
-  return bs_map(x, [&](unsigned w, int) { return bs_read(w, lane); });
+__device__ __forceinline__ K bs_from(K x, int lane) {  // the same lane for all
+  return x.map([=](unsigned w) { return bs_read(w, lane); });
 }
 
 __device__ __forceinline__ unsigned bs_order(float x) {
@@ -110,45 +124,46 @@ __device__ __forceinline__ double bs_value(unsigned long long o) {
 
 // One exchange with lane ^ D: the larger key stays where `up` holds.
 template <int D, typename K>
-__device__ __forceinline__ void bs_swap(K& x, bool up) {
-  const K o = bs_map(x, [](unsigned w, int) { return bs_xor<D>(w); });
-  x = bs_pick(x.above(o) == up, x, o);
+__device__ __forceinline__ K bs_swap(K x, bool up) {
+  const K o = x.map([](unsigned w) { return bs_xor<D>(w); });
+  return x.pick(x.above(o) == up, o);
 }
 // A bitonic row of 2 D lanes becomes falling (up) or rising.
 template <int D, typename K>
-__device__ __forceinline__ void bs_settle(K& x, bool up) {
-  bs_swap<D>(x, ((bs_lane() & D) == 0) == up);
-  if constexpr (D > 1) bs_settle<D / 2>(x, up);
+__device__ __forceinline__ K bs_settle(K x, bool up) {
+  x = bs_swap<D>(x, ((bs_lane() & D) == 0) == up);
+  if constexpr (D > 1) x = bs_settle<D / 2>(x, up);
+  return x;
 }
 // Falling over the lanes.
 template <typename K>
-__device__ __forceinline__ void bs_sort(K& x) {
+__device__ __forceinline__ K bs_sort(K x) {
   const int lane = bs_lane();
-  bs_settle<1>(x, (lane & 2) == 0);
-  bs_settle<2>(x, (lane & 4) == 0);
-  bs_settle<4>(x, (lane & 8) == 0);
-  bs_settle<8>(x, (lane & 16) == 0);
-  bs_settle<16>(x, (lane & 32) == 0);
-  bs_settle<32>(x, true);
+  x = bs_settle<1>(x, (lane & 2) == 0);
+  x = bs_settle<2>(x, (lane & 4) == 0);
+  x = bs_settle<4>(x, (lane & 8) == 0);
+  x = bs_settle<8>(x, (lane & 16) == 0);
+  x = bs_settle<16>(x, (lane & 32) == 0);
+  return bs_settle<32>(x, true);
 }
 // The 64 largest of two falling lists.
 template <typename K>
-__device__ __forceinline__ void bs_merge(K& best, const K& more) {
-  const K o = bs_map(more, [](unsigned w, int) { return bs_mirror(w); });
-  best = bs_pick(o.above(best), o, best);
-  bs_settle<32>(best, true);
+__device__ __forceinline__ K bs_merge(K best, K more) {
+  const K o = more.map([](unsigned w) { return bs_mirror(w); });
+  return bs_settle<32>(o.pick(o.above(best), best), true);
 }
 
 // The W largest of what is offered.
 template <typename K>
 struct Best {
-  K best, bar;  // falling over the lanes, and the W-th of them
+  K best, bar;  // falling over the lanes; the W-th of them, or floor where that is above
+  K floor;      // a key that W of all keys reach, here or elsewhere
   int last;     // W - 1
-  __device__ __forceinline__ void start(const K& x, int W) {
-    best = x, last = W - 1;
-    bs_sort(best);
-    bar = bs_from(best, last);
+  __device__ __forceinline__ void settle() {
+    const K x = bs_from(best, last);
+    bar = floor.pick(floor.above(x), x);
   }
+  __device__ __forceinline__ void start(int W) { best = K{}, bar = K{}, floor = K{}, last = W - 1; }
   // One key of each lane, 0 for none.
   __device__ __forceinline__ void offer(K x) {
     const bool in = x.above(bar);
@@ -156,19 +171,17 @@ struct Best {
     if (who == 0) return;
     // Where a sort's 27 exchanges cost less.
     if (__popcll(who) > 8) {
-      x = bs_pick(in, x, K{});
-      bs_sort(x);
-      bs_merge(best, x);
+      best = bs_merge(best, bs_sort(x.pick(in, K{})));
     } else {
       do {
         const K one = bs_from(x, __ffsll(who) - 1);
         who &= who - 1;
         const int at = __popcll(__ballot(best.above(one)));
-        const K up = bs_map(best, [](unsigned w, int) { return bs_prev(w); });
-        best = bs_pick(bs_lane() < at, best, bs_pick(bs_lane() == at, one, up));
+        const K up = best.map([](unsigned w) { return bs_prev(w); });
+        best = best.pick(bs_lane() < at, one.pick(bs_lane() == at, up));
       } while (who);
     }
-    bar = bs_from(best, last);
+    settle();
   }
 };
 
@@ -183,18 +196,21 @@ struct BsArgs {
   int K, V, W, end;
   int parts, per;                 // of a row; elements of a part, a multiple of a tile's
   float2* stats;                  // (B, K, parts): maximum, sum
-  unsigned long long* keys;       // (B, K, parts, W)
+  unsigned long long* keys;       // (B, W, K, parts)
   float* out;
   int64_t *parents, *tokens;
   unsigned char* done;            // or null
 };
 
 constexpr int BS_NW = 4, BS_NT = BS_NW * MG_WAVE;
-constexpr int BS_VECTORS = 4;  // of 16 bytes, of a lane in a tile
+constexpr int BS_EACH = 32;    // elements of a lane in a tile
+constexpr int BS_HITS = 512;   // elements that are kept to be offered
+constexpr int BS_READY = 32;   // more are offered
 
 __device__ __forceinline__ bool bs_finished(const BsArgs& a, int64_t b, int k) {
   return a.finished && a.finished[b * a.fs[0] + k * a.fs[1]];
 }
+__device__ __forceinline__ float bs_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 __device__ __forceinline__ bool bs_finite(float x) { return fabsf(x) < __builtin_inff(); }
 
 template <typename T>
@@ -203,8 +219,9 @@ struct BsVec {
 };
 
 template <typename T>
-__global__ __launch_bounds__(BS_NT) void beam_rows(BsArgs a) {
-  constexpr int N = BsVec<T>::N, ALL = N * BS_VECTORS, TILE = ALL * MG_WAVE;
+__global__ __launch_bounds__(BS_NT, 4) void beam_rows(BsArgs a) {
+  constexpr int N = BsVec<T>::N, VECTORS = BS_EACH / N, ALL = BS_EACH, TILE = ALL * MG_WAVE;
+  __shared__ int s_place[BS_NW][BS_HITS];  // elements that reach the bar
   const int lane = bs_lane(), wave = (int)mg_uniform(threadIdx.x / MG_WAVE);
   const int64_t id = (int64_t)blockIdx.x * BS_NW + wave;
   const int64_t row = id / a.parts;
@@ -212,7 +229,6 @@ __global__ __launch_bounds__(BS_NT) void beam_rows(BsArgs a) {
   const int part = (int)(id - row * a.parts);
   const int64_t b = row / a.K;
   const int k = (int)(row - b * a.K);
-  if (bs_finished(a, b, k) || !bs_finite(a.scores[b * a.ss[0] + k * a.ss[1]])) return;
   const T* const x = (const T*)a.logits + b * a.sb + k * a.sk;
   // Vectors start at the 16-byte line that holds the row's first element: what lies before it
   // in that line, and behind the row's end in the last, is in the same page and not used.
@@ -222,24 +238,29 @@ __global__ __launch_bounds__(BS_NT) void beam_rows(BsArgs a) {
   const int begin = part * a.per, stop = all - begin < a.per ? all : begin + a.per;
 
   Best<Key32> list;
+  list.start(a.W);
   // No maximum is below the lowest number, so that a lane of -inf alone, or without an element,
   // has a sum of 0.
   float top = -3.402823466e38f, sum = 0.f;
-  uint4 raw[BS_VECTORS];
+  // A tile ahead; the first is on its way before it is known whether the row counts.
+  uint4 raw[VECTORS];
   auto load = [&](int at) {
 #pragma unroll
-    for (int i = 0; i < BS_VECTORS; ++i) {
+    for (int i = 0; i < VECTORS; ++i) {
       const int e = at + (i * MG_WAVE + lane) * N;
       raw[i] = lines[(e < stop ? e : begin) / N];
     }
   };
+  int kept = 0;
   if (begin < stop) load(begin);
+  const float score = a.scores[b * a.ss[0] + k * a.ss[1]];
+  if (bs_finished(a, b, k) || !bs_finite(score)) return;
   for (int at = begin; at < stop; at += TILE) {
     float v[ALL];
     float peak = -__builtin_inff();
     const bool whole = at >= skew && at + TILE <= stop;
 #pragma unroll
-    for (int i = 0; i < BS_VECTORS; ++i) {
+    for (int i = 0; i < VECTORS; ++i) {
       const T* p = (const T*)&raw[i];
 #pragma unroll
       for (int j = 0; j < N; ++j) v[i * N + j] = pg_float(p[j]);
@@ -252,49 +273,82 @@ __global__ __launch_bounds__(BS_NT) void beam_rows(BsArgs a) {
         v[i] = e >= skew && e < stop ? v[i] : -__builtin_inff();
       }
     }
+    float peaks[VECTORS];
 #pragma unroll
-    for (int i = 0; i < ALL; ++i) peak = fmaxf(peak, v[i]);
+    for (int i = 0; i < VECTORS; ++i) {
+      peaks[i] = v[i * N];
+#pragma unroll
+      for (int j = 1; j < N; ++j) peaks[i] = fmaxf(peaks[i], v[i * N + j]);
+      peak = fmaxf(peak, peaks[i]);
+    }
     const float next = fmaxf(top, peak);
-    sum *= __expf(top - next);
-    float add = 0.f;
+    sum *= bs_exp(top - next);
+    float add[2] = {0.f, 0.f};
+    if (__ballot(next < -1e38f) == 0) {
+      // exp(v - next) as 2^(v L - c), L = log2 e, one operation less: c is next L rounded, and what
+      // that rounds off, r, the same for all of them, is put back once.
+      const float c = next * 1.44269504f, r = __builtin_fmaf(next, 1.44269504f, -c);
 #pragma unroll
-    for (int i = 0; i < ALL; ++i) add += __expf(v[i] - next);
-    sum += add;
+      for (int i = 0; i < ALL; ++i)
+        add[i & 1] += __builtin_amdgcn_exp2f(__builtin_fmaf(v[i], 1.44269504f, -c));
+      sum += (add[0] + add[1]) * __builtin_amdgcn_exp2f(-r);
+    } else {  // where next L may be out of range
+#pragma unroll
+      for (int i = 0; i < ALL; ++i) add[i & 1] += bs_exp(v[i] - next);
+      sum += add[0] + add[1];
+    }
     top = next;
-    auto key = [&](int i) {
-      const int e = at + ((i / N) * MG_WAVE + lane) * N + i % N;
-      const bool in = e >= skew && e < stop;
-      return Key32{{in ? ~(unsigned)(e - skew) : 0u, in ? bs_order(v[i]) : 0u}};
-    };
-    int own = -1;  // this lane's element among the first best
     if (at == begin) {
-      Key32 most = {};
-#pragma unroll
-      for (int i = 0; i < ALL; ++i) {
-        const Key32 x = key(i);
-        const bool more = x.above(most);
-        most = bs_pick(more, x, most);
-        own = more ? i : own;
-      }
-      list.start(most, a.W);
+      const Value32 bar = bs_from(bs_sort(Value32{bs_order(peak)}), a.W - 1);
+      list.floor = Key32{0, bar.value};  // below every key of that value
+      list.settle();
     }
-    // By values first: most elements are below the W-th best.
-    float bar = bs_value(list.bar.w[1]);
-    if (list.bar.all() == 0) bar = -__builtin_inff();
-    if (__ballot(peak >= bar) == 0) continue;
+    const float bar = bs_value(list.bar.value);
+    // A bit for each element that does; then each lane's first one, its second, and so on go to the
+    // list.  (A test of the whole wave for each element is a chain of some thirty round trips
+    // between the vector and the scalar unit: 8 us of 28 at 512 rows of 50257 in bf16.)
+    int hits = kept;
+    unsigned bits = 0;
 #pragma unroll
-    for (int i = 0; i < ALL; ++i) {
-      if (__ballot(v[i] >= bar) == 0) continue;
-      list.offer(bs_pick(i == own, Key32{}, key(i)));
-      bar = list.bar.all() == 0 ? -__builtin_inff() : bs_value(list.bar.w[1]);
+    for (int g = 0; g < VECTORS; ++g) {
+      if (__ballot(peaks[g] >= bar) == 0) continue;
+#pragma unroll
+      for (int i = g * N; i < g * N + N; ++i) bits |= v[i] >= bar ? 1u << i : 0u;
     }
+    for (unsigned long long who; (who = __ballot(bits != 0)) != 0; bits &= bits - 1) {
+      const int i = __ffs(bits) - 1, to = hits + (int)__builtin_amdgcn_mbcnt_hi(
+          (unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0));
+      if (bits != 0 && to < BS_HITS)
+        s_place[wave][to] = at + (i / N * MG_WAVE + lane) * N + i % N;
+      hits += __popcll(who);
+    }
+    // They are offered when there are many, or no more to come.  Where a tile has more than there
+    // is room for (rows full of ties, rising rows), those of the tiles before, then the whole tile.
+    const bool again = hits > BS_HITS;
+    const int ready = again ? kept : (hits > BS_READY || at + TILE >= stop ? hits : 0);
+    kept = ready || again ? 0 : hits;
+    const int chunks = (ready + MG_WAVE - 1) / MG_WAVE, every = chunks + (again ? ALL : 0);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    for (int n = 0; n < every; ++n) {
+      const bool from = n < chunks;
+      const int i = n * MG_WAVE + lane;
+      const int e = from ? s_place[wave][i < ready ? i : 0] : at + i - chunks * MG_WAVE;
+      const bool in = (!from || i < ready) && e >= skew && e < stop;
+      const float value = pg_float(x[in ? e - skew : 0]);
+      list.offer(Key32{in ? ~(unsigned)(e - skew) : 0u, in ? bs_order(value) : 0u});
+    }
+    __builtin_amdgcn_wave_barrier();
   }
   float m = top;
 #pragma unroll
   for (int d = 1; d < MG_WAVE; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-  const float total = mg_group_sum<64>(sum * __expf(top - m));
+  const float total = mg_group_sum<64>(sum * bs_exp(top - m));
   if (lane == 0) a.stats[id] = make_float2(m, total);
-  if (lane < a.W) a.keys[id * a.W + lane] = begin < stop ? list.best.all() : 0ull;
+  if (lane < a.W) {
+    const int64_t lists = (int64_t)a.K * a.parts;
+    a.keys[(b * a.W + lane) * lists + (id - b * lists)] = begin < stop ? list.best.all() : 0ull;
+  }
 }
 
 // ---- the selection -----------------------------------------------------------------------
@@ -316,7 +370,7 @@ __device__ __forceinline__ double bs_row_sum(double x) {  // over 16 lanes
 
 template <int NW>
 __global__ __launch_bounds__(NW* MG_WAVE) void beam_pick(BsArgs a) {
-  __shared__ Key64 s_list[NW / 2][MG_WAVE];
+  __shared__ Key64 s_list[NW / 2][MG_WAVE], s_bar;
   __shared__ double s_norm[BS_MAX_K], s_score[BS_MAX_K];
   __shared__ unsigned char s_kind[BS_MAX_K];
   enum { LIVE = 0, FINISHED = 1, DEAD = 2 };
@@ -337,7 +391,7 @@ __global__ __launch_bounds__(NW* MG_WAVE) void beam_pick(BsArgs a) {
       m = fmaxf(m, mg_row_ror<4>(m));
       m = fmaxf(m, mg_row_ror<2>(m));
       m = fmaxf(m, mg_row_ror<1>(m));
-      for (int i = in; i < a.parts; i += 16) sum += (double)st[i].y * (double)__expf(st[i].x - m);
+      for (int i = in; i < a.parts; i += 16) sum += (double)st[i].y * (double)bs_exp(st[i].x - m);
       sum = bs_row_sum(sum);
     }
     if (in == 0 && k < a.K) {
@@ -349,21 +403,24 @@ __global__ __launch_bounds__(NW* MG_WAVE) void beam_pick(BsArgs a) {
   __syncthreads();
 
   Best<Key64> list;
-  const int each = a.parts * a.W, all = a.K * each;
+  // Every part's first candidates come before any part's second ones, so that the first ones that
+  // are looked at set a high bar.
+  const int lists = a.K * a.parts, all = lists * a.W;
   auto key = [&](double score, unsigned index) {
     const unsigned long long o = bs_order(score);
-    return Key64{{~index, (unsigned)o, (unsigned)(o >> 32)}};
+    return Key64{~index, (unsigned)o, (unsigned)(o >> 32)};
   };
-  auto candidate = [&](int n) {
+  const unsigned long long* const keys = a.keys + b * all;
+  auto raw = [&](int n) { return keys[n < all ? n : 0]; };
+  auto candidate = [&](int n, unsigned long long from) {
     Key64 x = {};
     if (n < all) {
-      const int k = n / each, r = n - k * each;
+      const int r = n / lists, at = n - r * lists, k = at / a.parts;
       if (s_kind[k] == LIVE) {
-        const unsigned long long from = a.keys[(b * a.K + k) * each + r];
         if (from)
           x = key(s_score[k] + ((double)bs_value((unsigned)(from >> 32)) - s_norm[k]),
                   (unsigned)k * (unsigned)a.V + ~(unsigned)from);
-      } else if (r < a.W) {  // no part of the row: its end, and the first tokens at -inf
+      } else if (at == k * a.parts) {  // in place of its parts: its end, and the first tokens at -inf
         const bool over = s_kind[k] == FINISHED, first = over && r == 0;
         int token = first ? a.end : r - (over ? 1 : 0);
         if (over && !first && token >= a.end) ++token;
@@ -373,18 +430,37 @@ __global__ __launch_bounds__(NW* MG_WAVE) void beam_pick(BsArgs a) {
     }
     return x;
   };
-  list.start(candidate(wave * MG_WAVE + lane), a.W);
-  for (int at = (wave + NW) * MG_WAVE; at < all; at += NW * MG_WAVE) list.offer(candidate(at + lane));
+  // A bar that W candidates reach: of 64 parts' first ones, all over the beams, the W-th.  The
+  // candidates that reach it are few more than W.
+  int at = wave * MG_WAVE;
+  unsigned long long next = raw(at + lane);
+  if (wave == 0) {
+    const int n = lists > MG_WAVE ? (int)((int64_t)lane * lists / MG_WAVE) : lane;
+    const Key64 x = bs_sort(n < all ? candidate(n, raw(n)) : Key64{});
+    const Key64 bar = bs_from(x, a.W - 1);
+    if (lane == 0) s_bar = bar;
+  }
+  __syncthreads();
+  // Just below that candidate: the inverted index of a key is above 0.
+  list.start(a.W);
+  list.floor = s_bar;
+  if (list.floor.above(Key64{})) list.floor.index -= 1;
+  list.settle();
+  for (; at < all; at += NW * MG_WAVE) {
+    const unsigned long long now = next;
+    next = raw(at + NW * MG_WAVE + lane);
+    list.offer(candidate(at + lane, now));
+  }
   // The waves' lists, by halves.
 #pragma unroll
   for (int half = NW / 2; half > 0; half /= 2) {
     if (wave >= half && wave < 2 * half) s_list[wave - half][lane] = list.best;
     __syncthreads();
-    if (wave < half) bs_merge(list.best, s_list[wave][lane]);
+    if (wave < half) list.best = bs_merge(list.best, s_list[wave][lane]);
     __syncthreads();
   }
   if (wave == 0 && lane < a.W) {
-    const unsigned flat = ~list.best.w[0];
+    const unsigned flat = ~list.best.index;
     const int k = (int)(flat / (unsigned)a.V), token = (int)(flat - (unsigned)k * (unsigned)a.V);
     const int64_t n = b * a.W + lane;
     a.out[n] = (float)bs_value(list.best.value());
@@ -393,13 +469,15 @@ __global__ __launch_bounds__(NW* MG_WAVE) void beam_pick(BsArgs a) {
   }
 }
 
-// Waves of a row: enough to fill the chip's 256 CUs with 16 waves each, no less than a tile each.
+// Waves of a row: two for each of the chip's 1024 vector units over all rows, none with less than
+// a tile.  (64 x 8 rows of 50257 in bf16, both launches in a graph: 24.6 us; four for each, with
+// more first tiles and candidates, 25.8, one 33.  16 x 16 of 32771 in fp32, 32 wide: 32, four 38.)
 int bs_parts(int64_t rows, int V, int tile) {
-  int64_t want = (4096 + rows - 1) / rows;
+  const int64_t want = (2048 + rows - 1) / rows;
   const int64_t most = ((int64_t)V + 8 + tile - 1) / tile;
   return (int)(want < most ? want : most);
 }
-int bs_tile(int dtype) { return (dtype == 0 ? 4 : 8) * BS_VECTORS * MG_WAVE; }
+constexpr int BS_TILE = BS_EACH * MG_WAVE;
 bool bs_ok(int dtype, int64_t B, int64_t K, int64_t V, int W) {
   return dtype >= 0 && dtype <= 2 && B >= 1 && K >= 1 && V >= 1 && K <= BS_MAX_K && W >= 1 &&
          W <= MG_WAVE && V < 1ll << 30 && K * V < 1ll << 31 && W <= K * V && B < 1ll << 22 &&
@@ -480,7 +558,7 @@ extern "C" {
 
 size_t mg_beam_select_workspace_bytes(int dtype, int64_t B, int64_t K, int64_t V, int W) {
   if (!bs_ok(dtype, B, K, V, W)) return 0;
-  const size_t parts = (size_t)B * K * bs_parts(B * K, (int)V, bs_tile(dtype));
+  const size_t parts = (size_t)B * K * bs_parts(B * K, (int)V, BS_TILE);
   return parts * (sizeof(float2) + W * sizeof(unsigned long long));
 }
 
@@ -497,7 +575,7 @@ int mg_beam_select(int dtype, const void* logits, const float* scores, const voi
   a.sb = strides[0], a.sk = strides[1];
   for (int i = 0; i < 2; ++i) a.ss[i] = strides[2 + i], a.fs[i] = strides[4 + i];
   a.B = B, a.K = (int)K, a.V = (int)V, a.W = W, a.end = (int)end;
-  const int tile = bs_tile(dtype);
+  const int tile = BS_TILE;
   a.parts = bs_parts(B * K, (int)V, tile);
   const int64_t per = (V + 8 + a.parts - 1) / a.parts;
   a.per = (int)((per + tile - 1) / tile * tile);

@@ -38,6 +38,22 @@ __device__ __forceinline__ float pg_round<float>(float v) {
   return v;
 }
 
+// Two values as a word of two elements.
+template <typename T>
+__device__ __forceinline__ unsigned pg_pack(float x, float y);
+template <>
+__device__ __forceinline__ unsigned pg_pack<Bf16>(float x, float y) {
+  const bf16x2 h = {(__bf16)x, (__bf16)y};
+  unsigned u = __builtin_bit_cast(unsigned, h);
+  asm("" : "+v"(u));  // keeps the pair one packed conversion
+  return u;
+}
+template <>
+__device__ __forceinline__ unsigned pg_pack<Fp16>(float x, float y) {
+  const f16x2 h = {(_Float16)x, (_Float16)y};
+  return __builtin_bit_cast(unsigned, h);
+}
+
 // Integers of a caller: int32, or int64 where wide.
 struct Ints {
   const void* p;

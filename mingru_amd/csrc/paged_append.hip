@@ -6,7 +6,9 @@
 //
 // Bound by memory: q, k and v are read and written once.  A workgroup takes a few tokens of a
 // sequence, all their heads: the angles' sines and cosines are formed once a token, in LDS, and
-// serve every head.  A thread moves units of 16 bytes, or two of them that turn together.
+// serve every head.  A thread moves units of 16 bytes, or two of them that turn together, the
+// same ones of one token after another: what they are and where they lie is worked out once, not
+// for each (which took more of the vector units' time than the memory's).
 //
 // Angles are products in fp64, reduced to a part of a turn there: at position 2^20 a product in
 // fp32 is off by 2^-4 radians.  Sines and cosines of the reduced angle are fp32.
@@ -27,11 +29,16 @@ struct ApArgs {
   int64_t parts;                // workgroups of a sequence
   int P, H, Hk, dk, dv, n;      // n: frequencies
   int tokens;                   // of a workgroup
+  // units: of a head of q and k and of v (ku, vu), those of them that turn, of all q, of all k,
+  // of a token
+  int turning, ku, vu, qn, kn, all;
+  int abreast;                  // tokens that the workgroup's threads take at a time
 };
 
 constexpr int AP_NT = 256;
-constexpr int AP_TABLE = 2048;  // sine and cosine pairs of a workgroup's tokens in LDS
+constexpr int AP_TABLE = 1024;  // sine and cosine pairs of a workgroup's tokens in LDS
 constexpr int AP_MOST = 16;     // tokens of a workgroup
+constexpr int AP_AHEAD = 2;     // tokens whose loads a thread has on their way
 
 template <typename T, int VE>
 struct alignas(sizeof(T) * VE) ApVec {
@@ -45,116 +52,146 @@ struct ApPlace {
 };
 enum { AP_PADDING = 0, AP_KEPT = 1, AP_DROPPED = 2, AP_BAD = 3 };
 
+template <typename T, int VE>
+__device__ __forceinline__ void ap_get(const ApVec<T, VE>& v, float (&f)[VE]) {
+#pragma unroll
+  for (int e = 0; e < VE; ++e) f[e] = pg_float(v.e[e]);
+}
+template <typename T, int VE>
+__device__ __forceinline__ void ap_set(ApVec<T, VE>& v, const float (&f)[VE]) {
+  if constexpr (sizeof(T) == 2 && VE > 1) {
+    unsigned w[VE / 2];
+#pragma unroll
+    for (int e = 0; e < VE; e += 2) w[e / 2] = pg_pack<T>(f[e], f[e + 1]);
+    v = __builtin_bit_cast(ApVec<T, VE>, w);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v.e[e] = pg_round<T>(f[e]);
+  }
+}
+
 // VE elements are a unit: 16 bytes, or 1 where sizes, strides or pointers do not allow it.
 template <typename T, int VE>
 __global__ __launch_bounds__(AP_NT) void paged_append(ApArgs a) {
-  __shared__ float2 s_turn[AP_TABLE];
+  __shared__ alignas(16) float2 s_turn[AP_TABLE];
   __shared__ ApPlace s_place[AP_MOST];
+  typedef ApVec<T, VE> V;
   const int64_t b = blockIdx.x / a.parts, part = blockIdx.x - b * a.parts;
   const int64_t t0 = part * a.tokens;
-  const int64_t left = a.T - t0;
-  const int count = (int)(left < a.tokens ? left : a.tokens);
-  const int64_t start = a.start[b];
-  if ((int)threadIdx.x < count) {
-    const int64_t t = t0 + threadIdx.x, p = start + t;
-    ApPlace at = {0, 0, AP_KEPT};
-    if (a.lengths.p && t >= a.lengths[b]) {
-      at.kind = AP_PADDING;
-    } else if (p < 0 || p / a.P >= a.M) {
-      at.kind = AP_BAD;
-    } else {
-      const int64_t row = p / a.P, slot = p - row * a.P, page = a.pages[b * a.page_stride + row];
-      at.kind = page < 0 ? AP_DROPPED : (page >= a.N ? AP_BAD : AP_KEPT);
-      at.k = page * a.kcs[0] + slot * a.kcs[2];
-      at.v = page * a.vcs[0] + slot * a.vcs[2];
-    }
-    s_place[threadIdx.x] = at;
+  const int count = (int)(a.T - t0 < a.tokens ? a.T - t0 : a.tokens);
+  int live = count;  // tokens that are there
+  if (a.lengths.p) {
+    const int64_t n = a.lengths[b] - t0;
+    live = n < 0 ? 0 : (n < count ? (int)n : count);
   }
-  for (int i = threadIdx.x; i < count * a.n; i += AP_NT) {
-    const int t = i / a.n, f = i - t * a.n;
-    const double w = a.wide_freq ? ((const double*)a.freq)[f] : (double)((const float*)a.freq)[f];
-    // In turns, of which whole ones do not matter.
-    const double turns = (double)(start + t0 + t) * w * 0.15915494309189533577;
-    float sin, cos;
-    sincospif(2.f * (float)(turns - rint(turns)), &sin, &cos);
-    s_turn[i] = make_float2(cos, sin);
+  {
+    const int64_t start = a.start[b];
+    if ((int)threadIdx.x < count) {
+      const int64_t p = start + t0 + threadIdx.x;
+      ApPlace at = {0, 0, AP_KEPT};
+      if ((int)threadIdx.x >= live) {
+        at.kind = AP_PADDING;
+      } else if (p < 0 || p / a.P >= a.M) {
+        at.kind = AP_BAD;
+      } else {
+        const int64_t row = p / a.P, slot = p - row * a.P, page = a.pages[b * a.page_stride + row];
+        at.kind = page < 0 ? AP_DROPPED : (page >= a.N ? AP_BAD : AP_KEPT);
+        at.k = page * a.kcs[0] + slot * a.kcs[2];
+        at.v = page * a.vcs[0] + slot * a.vcs[2];
+      }
+      s_place[threadIdx.x] = at;
+    }
+    for (int i = threadIdx.x; i < live * a.n; i += AP_NT) {
+      const int t = i / a.n, f = i - t * a.n;
+      const double w = a.wide_freq ? ((const double*)a.freq)[f] : (double)((const float*)a.freq)[f];
+      // In turns, of which whole ones do not matter.
+      const double turns = (double)(start + t0 + t) * w * 0.15915494309189533577;
+      float sin, cos;
+      sincospif(2.f * (float)(turns - rint(turns)), &sin, &cos);
+      s_turn[i] = make_float2(cos, sin);
+    }
   }
   __syncthreads();
 
   // A head's units: pairs of units that turn together (n elements each; neighbours turn within
   // a unit), then single ones.
-  typedef ApVec<T, VE> V;
-  const bool within = a.interleaved != 0;
-  const int turning = within ? 2 * a.n / VE : a.n / VE;
-  const int ku = turning + (a.dk - 2 * a.n) / VE, vu = a.dv / VE;
-  const int qn = a.q ? a.H * ku : 0, kn = a.Hk * ku, all = qn + kn + a.Hk * vu;
-  for (int64_t i = threadIdx.x; i < (int64_t)count * all; i += AP_NT) {
-    const int t = (int)(i / all);
-    int u = (int)(i - (int64_t)t * all);
-    const ApPlace at = s_place[t];
-    const bool query = u < qn;
-    if (!query && at.kind != AP_KEPT) continue;
+  const int lead = a.abreast > 1 ? (int)threadIdx.x / a.all : 0;
+  if (lead >= a.abreast) return;
+  for (int i = (int)threadIdx.x - lead * a.all; i < a.all; i += AP_NT) {
+    const bool query = i < a.qn, value = i >= a.qn + a.kn;
+    const int j = query ? i : (value ? i - a.qn - a.kn : i - a.qn);
+    const int h = j / (value ? a.vu : a.ku), in = j - h * (value ? a.vu : a.ku);
+    const bool turns = !value && in < a.turning, two = turns && !a.interleaved;
+    const int c = value || turns ? in * VE : 2 * a.n + (in - a.turning) * VE;
     const T* src;
     T* dst;
-    if (!query && u >= qn + kn) {
-      u -= qn + kn;
-      const int h = u / vu, c = (u - h * vu) * VE;
-      src = (const T*)a.v + b * a.vs[0] + (t0 + t) * a.vs[1] + h * a.vs[2] + c;
-      dst = (T*)a.vc + at.v + h * a.vcs[1] + c;
-      *(V*)dst = *(const V*)src;
-      continue;
-    }
-    if (!query) u -= qn;
-    const int h = u / ku;
-    int c = u - h * ku;
+    int64_t step;
     if (query) {
-      src = (const T*)a.q + b * a.qs[0] + (t0 + t) * a.qs[1] + h * a.qs[2];
-      dst = (T*)a.qo + ((b * a.T + t0 + t) * a.H + h) * a.dk;
+      src = (const T*)a.q + b * a.qs[0] + h * a.qs[2], step = a.qs[1];
+      dst = (T*)a.qo + ((b * a.T + t0) * a.H + h) * a.dk;
+    } else if (value) {
+      src = (const T*)a.v + b * a.vs[0] + h * a.vs[2], step = a.vs[1];
+      dst = (T*)a.vc + h * a.vcs[1];
     } else {
-      src = (const T*)a.k + b * a.ks[0] + (t0 + t) * a.ks[1] + h * a.ks[2];
-      dst = (T*)a.kc + at.k + h * a.kcs[1];
+      src = (const T*)a.k + b * a.ks[0] + h * a.ks[2], step = a.ks[1];
+      dst = (T*)a.kc + h * a.kcs[1];
     }
-    const bool turns = c < turning, two = turns && !within;
-    c = turns ? c * VE : 2 * a.n + (c - turning) * VE;
-    V x, y;
-    if (at.kind == AP_PADDING || at.kind == AP_BAD) {  // a query's row of no place
-      const T fill = pg_round<T>(at.kind == AP_BAD ? __builtin_nanf("") : 0.f);
+    src += t0 * step + c, dst += c;
+    const int64_t row = (int64_t)a.H * a.dk;
+    // The other half of what turns: n elements on, or (one element a unit) the neighbour, which its
+    // own thread writes.
+    const int other = two ? a.n : (VE == 1 && turns ? (c & 1 ? -1 : 1) : 0);
+    for (int t1 = lead; t1 < count; t1 += AP_AHEAD * a.abreast) {
+      V x[AP_AHEAD], y[AP_AHEAD];
 #pragma unroll
-      for (int e = 0; e < VE; ++e) x.e[e] = fill;
-      *(V*)(dst + c) = x;
-      if (two) *(V*)(dst + a.n + c) = x;
-      continue;
-    }
-    x = *(const V*)(src + c);
-    if (!turns) {
-      *(V*)(dst + c) = x;
-      continue;
-    }
-    const float2* turn = s_turn + t * a.n;
-    if (two) {
-      y = *(const V*)(src + a.n + c);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float2 w = turn[c + e];
-        const float p = pg_float(x.e[e]), r = pg_float(y.e[e]);
-        x.e[e] = pg_round<T>(p * w.x - r * w.y);
-        y.e[e] = pg_round<T>(r * w.x + p * w.y);
+      for (int r = 0; r < AP_AHEAD; ++r) {
+        const int t = t1 + r * a.abreast;
+        if (t >= live) continue;  // padding is not read
+        x[r] = *(const V*)(src + t * step);
+        if (other) y[r] = *(const V*)(src + t * step + other);
       }
-      *(V*)(dst + c) = x;
-      *(V*)(dst + a.n + c) = y;
-    } else if constexpr (VE > 1) {
 #pragma unroll
-      for (int e = 0; e < VE; e += 2) {
-        const float2 w = turn[(c + e) / 2];
-        const float p = pg_float(x.e[e]), r = pg_float(x.e[e + 1]);
-        x.e[e] = pg_round<T>(p * w.x - r * w.y);
-        x.e[e + 1] = pg_round<T>(r * w.x + p * w.y);
+      for (int r = 0; r < AP_AHEAD; ++r) {
+        const int t = t1 + r * a.abreast;
+        if (t >= count) continue;
+        const int kind = s_place[t].kind;
+        if (!query && kind != AP_KEPT) continue;
+        T* const to = dst + (query ? t * row : (value ? s_place[t].v : s_place[t].k));
+        if (turns && t < live) {
+          float p[VE], q[VE];
+          ap_get(x[r], p), ap_get(y[r], q);
+          const float2* const turn = s_turn + t * a.n;
+          if (two) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+              const float2 w = turn[c + e];
+              const float s = p[e] * w.x - q[e] * w.y;
+              q[e] = q[e] * w.x + p[e] * w.y, p[e] = s;
+            }
+            ap_set(y[r], q);
+          } else if constexpr (VE > 1) {
+#pragma unroll
+            for (int e = 0; e < VE; e += 2) {
+              const float2 w = turn[(c + e) / 2];
+              const float s = p[e] * w.x - p[e + 1] * w.y;
+              p[e + 1] = p[e + 1] * w.x + p[e] * w.y, p[e] = s;
+            }
+          } else {
+            const float2 w = turn[c / 2];
+            p[0] = c & 1 ? p[0] * w.x + q[0] * w.y : p[0] * w.x - q[0] * w.y;
+          }
+          ap_set(x[r], p);
+        }
+        if (kind == AP_PADDING || kind == AP_BAD) {  // a query's row of no place
+          float f[VE];
+#pragma unroll
+          for (int e = 0; e < VE; ++e) f[e] = kind == AP_BAD ? __builtin_nanf("") : 0.f;
+          ap_set(x[r], f);
+          y[r] = x[r];
+        }
+        *(V*)to = x[r];
+        if (two) *(V*)(to + a.n) = y[r];
       }
-      *(V*)(dst + c) = x;
-    } else {  // one element a thread: its neighbour is read here and written by its own thread
-      const float2 w = turn[c / 2];
-      const float p = pg_float(x.e[0]), r = pg_float(src[c ^ 1]);
-      *(dst + c) = pg_round<T>(c & 1 ? p * w.x + r * w.y : p * w.x - r * w.y);
     }
   }
 }
@@ -175,14 +212,19 @@ int ap_run(ApArgs& a, int64_t B, hipStream_t stream) {
                    (!a.q || (ap_aligned(a.q, a.qs, e) && ((uintptr_t)a.qo & 15) == 0)) &&
                    ap_aligned(a.k, a.ks, e) && ap_aligned(a.v, a.vs, e) &&
                    ap_aligned(a.kc, a.kcs, e) && ap_aligned(a.vc, a.vcs, e);
-  // Tokens of a workgroup: two rounds of its threads' units, as many angles as LDS holds.
-  const int64_t heads = (int64_t)((a.q ? a.H : 0) + a.Hk) * a.dk + (int64_t)a.Hk * a.dv;
-  const int64_t units = heads / (vec ? VE : 1);
-  int64_t n = 2 * AP_NT / (units > 1 ? units : 1);
+  const int ve = vec ? VE : 1;
+  a.turning = (a.interleaved ? 2 * a.n : a.n) / ve;
+  a.ku = a.turning + (a.dk - 2 * a.n) / ve, a.vu = a.dv / ve;
+  a.qn = a.H * a.ku, a.kn = a.Hk * a.ku, a.all = a.qn + a.kn + a.Hk * a.vu;
+  a.abreast = a.all < AP_NT ? AP_NT / a.all : 1;
+  // Tokens of a workgroup: as many as leave the chip's 256 CUs eight workgroups each, and as many
+  // angles as LDS holds.
+  int64_t n = a.abreast * ((B * a.T) / (2048 * (int64_t)a.abreast));
+  if (n < a.abreast) n = a.abreast;
   if (n > AP_MOST) n = AP_MOST;
   if (a.n && n > AP_TABLE / a.n) n = AP_TABLE / a.n;
   if (n > a.T) n = a.T;
-  if (n < 1) n = 1;
+  if (a.abreast > n) a.abreast = (int)n;
   a.tokens = (int)n;
   a.parts = (a.T + n - 1) / n;
   const int64_t grid = B * a.parts;

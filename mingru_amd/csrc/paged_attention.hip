@@ -48,6 +48,7 @@ struct PaArgs {
   int shares;
   float* part;            // (2 shares, rows, dv) sums, then (2 shares, rows, 2) maxima and sums
   int rows;
+  int few_steps;          // whether the sequences' steps cannot pass 2^31
 };
 
 // ---- element types ---------------------------------------------------------------------
@@ -61,12 +62,6 @@ struct Elem<Bf16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ unsigned pack(float x, float y) {
-    const bf16x2 h = {(__bf16)x, (__bf16)y};
-    unsigned u = __builtin_bit_cast(unsigned, h);
-    asm("" : "+v"(u));  // keeps the pair one packed conversion
-    return u;
-  }
   static __device__ __forceinline__ float low(unsigned u) { return __uint_as_float(u << 16); }
   static __device__ __forceinline__ float high(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
 };
@@ -77,10 +72,6 @@ struct Elem<Fp16> {
   static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ unsigned pack(float x, float y) {
-    const f16x2 h = {(_Float16)x, (_Float16)y};
-    return __builtin_bit_cast(unsigned, h);
   }
   static __device__ __forceinline__ float low(unsigned u) {
     return (float)__builtin_bit_cast(f16x2, u)[0];
@@ -162,6 +153,12 @@ __device__ __forceinline__ float pa_max(float x) {
   r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+__device__ __forceinline__ float pa_wave_max(float x) {
+  x = fmaxf(x, mg_row_ror<8>(x));
+  x = fmaxf(x, mg_row_ror<4>(x));
+  x = fmaxf(x, mg_row_ror<2>(x));
+  return pa_max(fmaxf(x, mg_row_ror<1>(x)));
+}
 __device__ __forceinline__ float pa_sum(float x) { return mg_pair_sum<32>(mg_pair_sum<16>(x)); }
 
 // ---- the division of work --------------------------------------------------------------
@@ -201,6 +198,16 @@ __device__ __forceinline__ int64_t pa_steps(const PaArgs& a, int64_t b0, int64_t
   const int lane = threadIdx.x & (MG_WAVE - 1);
   int64_t sum = 0;
   for (int64_t i = lane * run; i < (lane + 1) * run && i < n; ++i) sum += pa_seq<SPAN>(a, b0 + i).steps;
+  if (a.few_steps) {  // 32 bits hold them all
+    int x = (int)sum;
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    const int t0 = __builtin_amdgcn_readlane(x, 15), t1 = __builtin_amdgcn_readlane(x, 31);
+    const int t2 = __builtin_amdgcn_readlane(x, 47), row = lane >> 4;
+    return x + (row > 0 ? t0 : 0) + (row > 1 ? t1 : 0) + (row > 2 ? t2 : 0);
+  }
 #pragma unroll
   for (int d = 1; d < MG_WAVE; d *= 2) {
     const int64_t up = __shfl_up(sum, d);
@@ -255,12 +262,8 @@ __device__ __forceinline__ int pa_holder(int64_t step, int64_t all, int n) {
 }
 
 // ---- the main kernel -------------------------------------------------------------------
-#ifndef G128
-#define G128 2
-#define G64 3
-#endif
-// Workgroups that a CU holds: at 256 a tile, its successor, queries and outputs take 300 registers.
-constexpr int pa_groups(int dk) { return dk > 128 ? 1 : (dk > 64 ? G128 : G64); }
+// Workgroups that a CU holds: at 256 a step, its successor, queries and outputs take 300 registers.
+constexpr int pa_groups(int dk, int dv) { return dv > 128 ? 1 : (dk > 64 ? 2 : 3); }
 template <typename T, int DK, int DV>
 struct PaShape {
   static constexpr int KEYS = Elem<T>::KEYS;      // tokens of a tile
@@ -271,7 +274,7 @@ struct PaShape {
   static constexpr int OLD = DV + 4;              // floats of an output row in LDS
   static constexpr int BYTES = KEYS * LD * sizeof(T);  // of a wave
   // Workgroups of a CU.
-  static constexpr int GROUPS = pa_groups(DK);
+  static constexpr int GROUPS = pa_groups(DK, DV);
   static_assert(DV <= DK && PA_ROWS * OLD * 4 <= BYTES, "the outputs lie where the keys were");
 };
 
@@ -414,10 +417,21 @@ __global__ __launch_bounds__(PA_NT, (PaShape<T, DK, DV>::GROUPS)) void paged_att
     asm volatile("" : "+v"(chunk));
 #pragma unroll
     for (int s = 0; s < QW; ++s) {
-      Chunk<T, VE> x;
-      pa_load<T, VE, false>(row, 4 * s + chunk, a.dk, x);
-      pa_clear<T, VE>(4 * s + chunk, a.dk, x);
-      qf[s] = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
+      const int at = (4 * s + chunk) * VE;
+      if constexpr (VEC && CK::W == 2) {  // a row is a multiple of 8 bytes
+        const u32x2 x = *(const u32x2*)(row + (at < a.dk ? at : 0));
+        const u32x2 y = *(const u32x2*)(row + (at + VE / 2 < a.dk ? at + VE / 2 : 0));
+        const bool in = at < a.dk, all = at + VE / 2 < a.dk;
+        qf[s] = u32x4{in ? x[0] : 0, in ? x[1] : 0, all ? y[0] : 0, all ? y[1] : 0};
+      } else if constexpr (VEC) {
+        const u32x4 x = *(const u32x4*)(row + (at < a.dk ? at : 0));
+        qf[s] = at < a.dk ? x : u32x4{0, 0, 0, 0};
+      } else {
+        Chunk<T, VE> x;
+        pa_load<T, VE, false>(row, 4 * s + chunk, a.dk, x);
+        pa_clear<T, VE>(4 * s + chunk, a.dk, x);
+        qf[s] = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
+      }
     }
   };
 
@@ -516,8 +530,8 @@ __global__ __launch_bounds__(PA_NT, (PaShape<T, DK, DV>::GROUPS)) void paged_att
         u32x4 hi, lo;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          hi[j] = Elem<T>::pack(p[2 * j], p[2 * j + 1]);
-          lo[j] = Elem<T>::pack(p[2 * j] - Elem<T>::low(hi[j]), p[2 * j + 1] - Elem<T>::high(hi[j]));
+          hi[j] = pg_pack<T>(p[2 * j], p[2 * j + 1]);
+          lo[j] = pg_pack<T>(p[2 * j] - Elem<T>::low(hi[j]), p[2 * j + 1] - Elem<T>::high(hi[j]));
         }
 #pragma unroll
         for (int e = 0; e < EV; ++e) {
@@ -595,25 +609,23 @@ __global__ __launch_bounds__(PA_NT, (PaShape<T, DK, DV>::GROUPS)) void paged_att
 }
 
 // Joins the pieces of one query head: a workgroup each.
-constexpr int PA_MOST = 1024;  // shares
 template <typename T, int SPAN>
 __global__ __launch_bounds__(PA_NT) void paged_attention_join(PaArgs a) {
-  __shared__ float s_weight[PA_MOST], s_red[2 * PA_NW];
   __shared__ f32x4 s_part[PA_NT];
-  const int lane = threadIdx.x & (MG_WAVE - 1), wave = threadIdx.x / MG_WAVE;
+  const int lane = threadIdx.x & (MG_WAVE - 1);
   const int64_t b = blockIdx.x / a.H;
   const int h = (int)(blockIdx.x - b * a.H), hk = h / a.group, in = h - hk * a.group;
   const int r = in % PA_ROWS;
+  const int64_t pairs = (int64_t)a.Hk * a.tiles_q;
+  int64_t steps, run;
   const PaSeq seq = pa_seq<SPAN>(a, b);
+  const int64_t all = pa_all<SPAN>(a, pairs, steps, run);
   T* const dst = (T*)a.o + (b * a.H + h) * (int64_t)a.dv;
   if (seq.steps == 0) {
     for (int x = threadIdx.x; x < a.dv; x += PA_NT)
       dst[x] = pg_round<T>(seq.bad ? __builtin_nanf("") : 0.f);
     return;
   }
-  const int64_t pairs = (int64_t)a.Hk * a.tiles_q;
-  int64_t steps, run;
-  const int64_t all = pa_all<SPAN>(a, pairs, steps, run);
   const int64_t before = pa_find<SPAN, false>(a, pairs, steps, run, b, 0).before;
   const int shares = pa_shares_used(a, all);
   const int64_t from = before + ((int64_t)hk * a.tiles_q + in / PA_ROWS) * seq.steps;
@@ -622,53 +634,58 @@ __global__ __launch_bounds__(PA_NT) void paged_attention_join(PaArgs a) {
   if (n == 1) return;  // one share held it and has written it
   // The pieces are the first or second one of w0, then the first ones of w0 + 1 .. w0 + n - 1.
   const int second = pa_share(w0, all, shares) == from ? 0 : 1;
-  const float* const stat = a.part + 2 * (int64_t)a.shares * a.rows * a.dv;
+  const float2* const stat = (const float2*)(a.part + 2 * (int64_t)a.shares * a.rows * a.dv);
   auto place = [&](int i) { return ((int64_t)2 * (w0 + i) + (i ? 0 : second)) * a.rows + r; };
-  float m[PA_MOST / PA_NT], l[PA_MOST / PA_NT], top = -__builtin_inff(), sum = 0.f;
-#pragma unroll
-  for (int j = 0; j < PA_MOST / PA_NT; ++j) {
-    const int i = threadIdx.x + j * PA_NT;
-    const float2 st = *(const float2*)(stat + 2 * place(i < n ? i : 0));
-    m[j] = i < n ? st.x : -__builtin_inff(), l[j] = i < n ? st.y : 0.f;
-    top = fmaxf(top, m[j]);
-  }
-#pragma unroll
-  for (int d = 1; d < MG_WAVE; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-  if (lane == 0) s_red[wave] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < PA_NW; ++w) top = fmaxf(top, s_red[w]);
-  const float base = top == -__builtin_inff() ? 0.f : top;
-#pragma unroll
-  for (int j = 0; j < PA_MOST / PA_NT; ++j) {
-    const int i = threadIdx.x + j * PA_NT;
-    const float down = pa_exp2(m[j] - base);
-    if (i < n) s_weight[i] = down;
-    sum += i < n ? down * l[j] : 0.f;
-  }
-  sum = mg_group_sum<64>(sum);
-  if (lane == 0) s_red[PA_NW + wave] = sum;
-  __syncthreads();
-  sum = 0.f;
-#pragma unroll
-  for (int w = 0; w < PA_NW; ++w) sum += s_red[PA_NW + w];
-  // Threads side by side take four elements each, groups of them every n-th piece.
+  // Threads side by side take four elements each, groups of them every n-th piece.  Each thread's
+  // first pieces are on their way before the maximum is known.
   int wide = 1;
   while (4 * wide < a.dv) wide *= 2;
   const int groups = PA_NT / wide, mine = threadIdx.x / wide, x = 4 * (threadIdx.x - mine * wide);
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  auto add = [&](int i) {
-    const float* p = a.part + place(i) * a.dv;
-    const float down = s_weight[i];
+  const bool whole = a.dv % 4 == 0 && x < a.dv;
+  auto load = [&](int i) {
+    const float* p = a.part + place(i < n ? i : 0) * a.dv;
+    if (whole) return *(const f32x4*)(p + x);
+    f32x4 v;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += down * p[x + e < a.dv ? x + e : 0];
+    for (int e = 0; e < 4; ++e) v[e] = p[x + e < a.dv ? x + e : 0];
+    return v;
   };
-  int i = mine;
-  for (; i + 3 * groups < n; i += 4 * groups) {
+  constexpr int AHEAD = 4;
+  f32x4 ahead[AHEAD];
+  float peak[AHEAD];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) add(i + j * groups);
+  for (int j = 0; j < AHEAD; ++j) {
+    const int i = mine + j * groups;
+    ahead[j] = load(i);
+    peak[j] = i < n ? stat[place(i)].x : -__builtin_inff();
   }
-  for (; i < n; i += groups) add(i);
+  // Each wave looks at all pieces' maxima and sums.
+  float2 st = lane < n ? stat[place(lane)] : make_float2(-__builtin_inff(), 0.f);
+  float top = st.x;
+  for (int i = lane + MG_WAVE; i < n; i += MG_WAVE) top = fmaxf(top, stat[place(i)].x);
+  top = pa_wave_max(top);
+  const float base = top == -__builtin_inff() ? 0.f : top;
+  float sum = pa_exp2(st.x - base) * st.y;
+  for (int i = lane + MG_WAVE; i < n; i += MG_WAVE) {
+    st = stat[place(i)];
+    sum += pa_exp2(st.x - base) * st.y;
+  }
+  sum = mg_group_sum<64>(sum);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j)
+    if (mine + j * groups < n) v += pa_exp2(peak[j] - base) * ahead[j];
+  for (int i = mine + AHEAD * groups; i < n; i += AHEAD * groups) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int at = i + j * groups;
+      ahead[j] = load(at);
+      peak[j] = at < n ? stat[place(at)].x : -__builtin_inff();
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (i + j * groups < n) v += pa_exp2(peak[j] - base) * ahead[j];
+  }
   s_part[threadIdx.x] = v;
   __syncthreads();
   if (mine == 0) {
@@ -682,7 +699,7 @@ __global__ __launch_bounds__(PA_NT) void paged_attention_join(PaArgs a) {
 
 // ---- host --------------------------------------------------------------------------------
 // Shares: as many as the chip's 256 CUs hold workgroups at once.
-int pa_most(int dk, int dv) { return 256 * pa_groups(dk > dv ? dk : dv); }
+int pa_most(int dk, int dv) { return 256 * pa_groups(dk > dv ? dk : dv, dv); }
 
 bool pa_ok(int dtype, int64_t B, int H, int Hk, int dk, int dv, int64_t M, int64_t P) {
   return dtype >= 0 && dtype <= 2 && B >= 1 && H >= 1 && Hk >= 1 && H % Hk == 0 && dk >= 1 &&
@@ -705,7 +722,8 @@ void pa_launch(const PaArgs& a, hipStream_t stream) {
   // Vectors of a chunk: 16 bytes, 8 where a chunk is no more.
   const int e = sizeof(T), bk = DK * e / 16 < 16 ? 8 : 16, bv = DV * e / 16 < 16 ? 8 : 16;
   bool vec = a.dk * e % bk == 0 && a.dv * e % bv == 0 && ((uintptr_t)a.k & (bk - 1)) == 0 &&
-             ((uintptr_t)a.v & (bv - 1)) == 0;
+             ((uintptr_t)a.v & (bv - 1)) == 0 && ((uintptr_t)a.q & (bk - 1)) == 0 &&
+             a.qs[0] * e % bk == 0 && a.qs[1] * e % bk == 0;
   for (int i = 0; i < 3; ++i) vec = vec && a.ks[i] * e % bk == 0 && a.vs[i] * e % bv == 0;
   const dim3 grid(a.shares), nt(PA_NT);
   if (vec && a.P.d % 4 == 0)
@@ -758,6 +776,7 @@ int mg_paged_attention_step(int dtype, const void* q, const void* k_cache, const
   a.B = B, a.N = N, a.room = M * P, a.window = window, a.P = pg_divisor(P);
   a.H = H, a.Hk = Hk, a.group = H / Hk, a.tiles_q = (a.group + PA_ROWS - 1) / PA_ROWS;
   a.dk = dk, a.dv = dv;
+  a.few_steps = B * (M * P / pa_span(dtype) + 2) < 1ll << 31;
   a.scale = scale * 1.4426950408889634f;
   a.shares = pa_shares(dtype, B, H, Hk, dk, dv, M, P), a.part = (float*)ws, a.rows = pa_rows(H, Hk);
   if (dtype == 0) return pa_run<float>(a, stream);

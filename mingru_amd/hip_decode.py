@@ -62,8 +62,8 @@ def paged_cache_append_impl(k, v, k_cache, v_cache, pages, start, q, lengths, fr
     _cache(what, "k_cache", k_cache), _cache(what, "v_cache", v_cache)
     H = 0 if q is None else q.shape[2]
     if N >= 2**31 or P >= 2**31 or Hk * (dk + dv) + H * dk >= 2**26 or \
-            (frequencies is not None and frequencies.numel() > 2048):
-        raise ScanFallback(f"{what} kernels take tokens of fewer than 2^26 elements, up to 2048 "
+            (frequencies is not None and frequencies.numel() > 1024):
+        raise ScanFallback(f"{what} kernels take tokens of fewer than 2^26 elements, up to 1024 "
                            f"frequencies and fewer than 2^31 pages (got {N} of {P} tokens)")
     if q is not None:
         q = _last_dense(q)
@@ -101,6 +101,9 @@ def paged_attention_step_impl(q, k_cache, v_cache, pages, lengths, scale, window
                            f"sequences, tables of fewer than 2^31 - 1024 tokens and fewer than 2^31 "
                            f"pages (got {dk} and {dv}, {B} x {H}, {M} x {P} and {N})")
     q = _last_dense(q)
+    if q.data_ptr() % 16 or not q.is_contiguous():
+        # Small, and the kernels load the caches by vectors only together with the queries.
+        q = q.clone(memory_format=torch.contiguous_format)
     wide, pages, lengths = _ints(pages, lengths)
     o = torch.empty(B, H, dv, dtype=q.dtype, device=q.device)
     ws = _workspace(nbytes, q.device)
