@@ -38,7 +38,6 @@ struct ApArgs {
 constexpr int AP_NT = 256;
 constexpr int AP_TABLE = 1024;  // sine and cosine pairs of a workgroup's tokens in LDS
 constexpr int AP_MOST = 16;     // tokens of a workgroup
-constexpr int AP_AHEAD = 2;     // tokens whose loads a thread has on their way
 
 template <typename T, int VE>
 struct alignas(sizeof(T) * VE) ApVec {
@@ -68,6 +67,15 @@ __device__ __forceinline__ void ap_set(ApVec<T, VE>& v, const float (&f)[VE]) {
 #pragma unroll
     for (int e = 0; e < VE; ++e) v.e[e] = pg_round<T>(f[e]);
   }
+}
+
+// Past the caches: 96 us with ordinary stores in place of 82 at 16 x 2048 tokens.
+template <typename T, int VE>
+__device__ __forceinline__ void ap_store(T* to, const ApVec<T, VE>& v) {
+  if constexpr (sizeof(v) == 16)
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (u32x4*)to);
+  else
+    *(ApVec<T, VE>*)to = v;
 }
 
 // VE elements are a unit: 16 bytes, or 1 where sizes, strides or pointers do not allow it.
@@ -141,57 +149,49 @@ __global__ __launch_bounds__(AP_NT) void paged_append(ApArgs a) {
     // The other half of what turns: n elements on, or (one element a unit) the neighbour, which its
     // own thread writes.
     const int other = two ? a.n : (VE == 1 && turns ? (c & 1 ? -1 : 1) : 0);
-    for (int t1 = lead; t1 < count; t1 += AP_AHEAD * a.abreast) {
-      V x[AP_AHEAD], y[AP_AHEAD];
-#pragma unroll
-      for (int r = 0; r < AP_AHEAD; ++r) {
-        const int t = t1 + r * a.abreast;
-        if (t >= live) continue;  // padding is not read
-        x[r] = *(const V*)(src + t * step);
-        if (other) y[r] = *(const V*)(src + t * step + other);
+    for (int t = lead; t < count; t += a.abreast) {
+      V x, y;
+      if (t < live) {  // padding is not read
+        x = *(const V*)(src + t * step);
+        if (other) y = *(const V*)(src + t * step + other);
       }
+      const int kind = s_place[t].kind;
+      if (!query && kind != AP_KEPT) continue;
+      T* const to = dst + (query ? t * row : (value ? s_place[t].v : s_place[t].k));
+      if (turns && t < live) {
+        float p[VE], q[VE];
+        ap_get(x, p), ap_get(y, q);
+        const float2* const turn = s_turn + t * a.n;
+        if (two) {
 #pragma unroll
-      for (int r = 0; r < AP_AHEAD; ++r) {
-        const int t = t1 + r * a.abreast;
-        if (t >= count) continue;
-        const int kind = s_place[t].kind;
-        if (!query && kind != AP_KEPT) continue;
-        T* const to = dst + (query ? t * row : (value ? s_place[t].v : s_place[t].k));
-        if (turns && t < live) {
-          float p[VE], q[VE];
-          ap_get(x[r], p), ap_get(y[r], q);
-          const float2* const turn = s_turn + t * a.n;
-          if (two) {
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-              const float2 w = turn[c + e];
-              const float s = p[e] * w.x - q[e] * w.y;
-              q[e] = q[e] * w.x + p[e] * w.y, p[e] = s;
-            }
-            ap_set(y[r], q);
-          } else if constexpr (VE > 1) {
-#pragma unroll
-            for (int e = 0; e < VE; e += 2) {
-              const float2 w = turn[(c + e) / 2];
-              const float s = p[e] * w.x - p[e + 1] * w.y;
-              p[e + 1] = p[e + 1] * w.x + p[e] * w.y, p[e] = s;
-            }
-          } else {
-            const float2 w = turn[c / 2];
-            p[0] = c & 1 ? p[0] * w.x + q[0] * w.y : p[0] * w.x - q[0] * w.y;
+          for (int e = 0; e < VE; ++e) {
+            const float2 w = turn[c + e];
+            const float s = p[e] * w.x - q[e] * w.y;
+            q[e] = q[e] * w.x + p[e] * w.y, p[e] = s;
           }
-          ap_set(x[r], p);
-        }
-        if (kind == AP_PADDING || kind == AP_BAD) {  // a query's row of no place
-          float f[VE];
+          ap_set(y, q);
+        } else if constexpr (VE > 1) {
 #pragma unroll
-          for (int e = 0; e < VE; ++e) f[e] = kind == AP_BAD ? __builtin_nanf("") : 0.f;
-          ap_set(x[r], f);
-          y[r] = x[r];
+          for (int e = 0; e < VE; e += 2) {
+            const float2 w = turn[(c + e) / 2];
+            const float s = p[e] * w.x - p[e + 1] * w.y;
+            p[e + 1] = p[e + 1] * w.x + p[e] * w.y, p[e] = s;
+          }
+        } else {
+          const float2 w = turn[c / 2];
+          p[0] = c & 1 ? p[0] * w.x + q[0] * w.y : p[0] * w.x - q[0] * w.y;
         }
-        *(V*)to = x[r];
-        if (two) *(V*)(to + a.n) = y[r];
+        ap_set(x, p);
       }
+      if (kind == AP_PADDING || kind == AP_BAD) {  // a query's row of no place
+        float f[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) f[e] = kind == AP_BAD ? __builtin_nanf("") : 0.f;
+        ap_set(x, f);
+        y = x;
+      }
+      ap_store(to, x);
+      if (two) ap_store(to + a.n, y);
     }
   }
 }
@@ -217,9 +217,10 @@ int ap_run(ApArgs& a, int64_t B, hipStream_t stream) {
   a.ku = a.turning + (a.dk - 2 * a.n) / ve, a.vu = a.dv / ve;
   a.qn = a.H * a.ku, a.kn = a.Hk * a.ku, a.all = a.qn + a.kn + a.Hk * a.vu;
   a.abreast = a.all < AP_NT ? AP_NT / a.all : 1;
-  // Tokens of a workgroup: as many as leave the chip's 256 CUs eight workgroups each, and as many
-  // angles as LDS holds.
-  int64_t n = a.abreast * ((B * a.T) / (2048 * (int64_t)a.abreast));
+  // Tokens of a workgroup: as many as leave the chip's 256 CUs 32 workgroups each, and as many
+  // angles as LDS holds.  (16 x 2048 ragged tokens of 16 and 8 heads of 128 in bf16: 66 us, with 64
+  // workgroups each 72, with 8 82.)
+  int64_t n = a.abreast * ((B * a.T) / (8192 * (int64_t)a.abreast));
   if (n < a.abreast) n = a.abreast;
   if (n > AP_MOST) n = AP_MOST;
   if (a.n && n > AP_TABLE / a.n) n = AP_TABLE / a.n;

@@ -135,7 +135,8 @@ def test_repeats_bitwise(cuda):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16, torch.int32,
                                    torch.int64, torch.bool, torch.uint8, torch.float64,
                                    torch.complex64])
-@pytest.mark.parametrize("shape", [(), (1,), (3,), (8, 5), (1024,), (1025,), (3, 1000), (0, 4)])
+@pytest.mark.parametrize("shape", [(), (1,), (3,), (8, 5), (1024,), (1025,), (3, 1000), (0, 4),
+                                   (17,), (4099,), (20001,)])
 def test_reorder(cuda, dtype, shape):
     g = torch.Generator().manual_seed(0)
     x = (torch.randn(6 * 4, *shape, generator=g) * 20).to(dtype).to(cuda)
