@@ -675,11 +675,31 @@ int mg_reorder_rows(int count, const void* const* src, void* const* dst, const i
     return MG_ERR_ARG;
   for (int i = 0; i < count; ++i)
     if (!src[i] || !dst[i] || bytes[i] < 1 || bytes[i] >= 1ll << 40) return MG_ERR_ARG;
+  // How a tensor's rows go: log2 of a unit's bytes, or across the rows' ends.  The latter where few
+  // vectors hold an end: rows of 19137 elements of 2 bytes take 23 us in place of 71 (6 layers of
+  // 256 rows), rows of 36 bytes 10 in place of 7.
+  auto shift_of = [&](int i) {
+    const uint64_t odd = (uint64_t)(uintptr_t)src[i] | (uint64_t)(uintptr_t)dst[i] |
+                         (uint64_t)strides[i] | (uint64_t)bytes[i];
+    int shift = 0;
+    while (shift < 4 && !(odd >> shift & 1)) ++shift;
+    return shift;
+  };
+  auto across_of = [&](int i) {
+    return shift_of(i) < 4 && bytes[i] >= 256 && ((uintptr_t)dst[i] & 15) == 0;
+  };
+  auto units_of = [&](int i) {
+    return across_of(i) ? (B * W * bytes[i] + 15) / 16 : B * W * (bytes[i] >> shift_of(i));
+  };
+  int64_t units = 0;
+  for (int i = 0; i < count; ++i) {
+    if (bytes[i] >= (1ll << 62) / (B * W)) return MG_ERR_TOO_LARGE;
+    units += units_of(i) + RO_NT * RO_UNITS;
+    if (units >= (int64_t)(RO_NT * RO_UNITS) << 24) return MG_ERR_TOO_LARGE;  // 2^32 threads
+  }
   // Two chunks of a workgroup where they are many: its start costs less (168 us in place of 177 at
   // 537 MB), one where they are few.
-  int64_t all = 0;
-  for (int i = 0; i < count; ++i) all += bytes[i] < 1ll << 20 ? bytes[i] : 1ll << 20;
-  const int chunks = all * (B * W) >= 128ll << 20 ? 2 : 1;
+  const int chunks = units >= 8ll << 20 ? 2 : 1;
   for (int across = 0; across < 2; ++across) {
     RoArgs a = {};
     a.parents = Ints{parents, wide}, a.ps[0] = pb, a.ps[1] = pw;
@@ -687,21 +707,14 @@ int mg_reorder_rows(int count, const void* const* src, void* const* dst, const i
     a.chunks = chunks;
     int64_t groups = 0;
     for (int i = 0; i < count; ++i) {
-      const uint64_t odd = (uint64_t)(uintptr_t)src[i] | (uint64_t)(uintptr_t)dst[i] |
-                           (uint64_t)strides[i] | (uint64_t)bytes[i];
-      int shift = 0;
-      while (shift < 4 && !(odd >> shift & 1)) ++shift;
-      // Where few vectors hold an end: rows of 19137 elements of 2 bytes take 23 us in place of 71
-      // (6 layers of 256 rows), rows of 36 bytes 10 in place of 7.
-      if ((shift < 4 && bytes[i] >= 256 && ((uintptr_t)dst[i] & 15) == 0) == (across != 0)) {
+      if (across_of(i) == (across != 0)) {
         RoTensor& t = a.t[a.count];
         t.src = (const unsigned char*)src[i], t.dst = (unsigned char*)dst[i], t.stride = strides[i];
-        t.units = across ? bytes[i] : bytes[i] >> shift;
-        a.shift[a.count] = (unsigned char)shift;
+        t.units = across ? bytes[i] : bytes[i] >> shift_of(i);
+        a.shift[a.count] = (unsigned char)shift_of(i);
         a.first[a.count++] = (unsigned)groups;
-        const int64_t units = across ? (a.rows * t.units + 15) / 16 : a.rows * t.units;
-        groups += (units + RO_NT * RO_UNITS * a.chunks - 1) / (RO_NT * RO_UNITS * a.chunks);
-        if (groups >= 1ll << 24) return MG_ERR_TOO_LARGE;  // 2^32 threads
+        const int64_t each = RO_NT * RO_UNITS * chunks;
+        groups += (units_of(i) + each - 1) / each;
       }
       if (a.count == 0 || (a.count < RO_MOST && i + 1 < count)) continue;
       for (int j = a.count; j < RO_MOST; ++j) a.first[j] = ~0u;

@@ -212,6 +212,7 @@ int ap_run(ApArgs& a, int64_t B, hipStream_t stream) {
                    (!a.q || (ap_aligned(a.q, a.qs, e) && ((uintptr_t)a.qo & 15) == 0)) &&
                    ap_aligned(a.k, a.ks, e) && ap_aligned(a.v, a.vs, e) &&
                    ap_aligned(a.kc, a.kcs, e) && ap_aligned(a.vc, a.vcs, e);
+  if (B >= 1ll << 24 || a.T >= 1ll << 38) return MG_ERR_TOO_LARGE;
   const int ve = vec ? VE : 1;
   a.turning = (a.interleaved ? 2 * a.n : a.n) / ve;
   a.ku = a.turning + (a.dk - 2 * a.n) / ve, a.vu = a.dv / ve;
@@ -229,7 +230,7 @@ int ap_run(ApArgs& a, int64_t B, hipStream_t stream) {
   a.tokens = (int)n;
   a.parts = (a.T + n - 1) / n;
   const int64_t grid = B * a.parts;
-  if (grid >= 1ll << 24) return MG_ERR_TOO_LARGE;  // 2^32 threads
+  if (a.parts >= 1ll << 24 || grid >= 1ll << 24) return MG_ERR_TOO_LARGE;  // 2^32 threads
   if (vec)
     hipLaunchKernelGGL((paged_append<T, VE>), dim3((unsigned)grid), dim3(AP_NT), 0, stream, a);
   else

@@ -1,6 +1,7 @@
 """A small language model of the operators in :mod:`mingru_amd.sequence_ops`, as an example of
 using them together: blocks of decaying linear attention and an MLP between fused norms, trained
-with the vocabulary loss and generating through the one-token forms.
+with the vocabulary loss and generating through the one-token forms, greedily or by the beam
+search of :mod:`mingru_amd.decode_ops`.
 
 ``python -m mingru_amd.decay_lm`` trains it on a synthetic task (a random pattern repeated, which
 a model can only continue by recalling it) and prints the losses and a generated continuation.
@@ -14,6 +15,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .decode_ops import beam_select, reorder_states
 from .sequence_ops import (
     linear_attention,
     linear_attention_step,
@@ -108,28 +110,59 @@ class DecayLM(nn.Module):
         y, _ = self(inputs)
         return linear_cross_entropy(y, self.head.weight, tokens[:, 1:], ignore_index=ignore_index)
 
+    def _step(self, token, state):
+        """The next rows (B, d_model) after one token (B) of each sequence, and the new states."""
+        x, y = self._enter(token)
+        new = []
+        for block, h in zip(self.blocks, state):
+            x, y, h = block.step(x, y, h)
+            new.append(h)
+        return y, new
+
+    def _search(self, y, state, n: int, beams: int, end):
+        """The best of ``beams`` continuations that are kept from token to token."""
+        B, V = len(y), self.head.out_features
+        scores = y.new_zeros(B, 1, dtype=torch.promote_types(y.dtype, torch.float32))
+        finished, chosen = None, []
+        for i in range(n):
+            logits = self.head(y).view(B, scores.shape[1], V)
+            width = min(beams, logits.shape[1] * V)  # one token alone has V continuations
+            scores, parent, token, *rest = beam_select(logits, scores, width, end=end,
+                                                       finished=finished)
+            finished = rest[0] if rest else None
+            chosen.append((parent, token))
+            if i + 1 < n:
+                y, state = self._step(token.flatten(), reorder_states(state, parent))
+        beam = torch.zeros(B, 1, dtype=torch.int64, device=y.device)
+        out = []
+        for parent, token in reversed(chosen):
+            out.append(token.gather(1, beam))
+            beam = parent.gather(1, beam)
+        return torch.cat(out[::-1], 1)
+
     @torch.no_grad()
-    def generate(self, prompt, n: int, lengths=None):
-        """The ``n`` likeliest next tokens, one after another, after each prompt (B, T), whose
-        ``lengths`` (B), of 1 to T tokens, leave off padding at the end."""
+    def generate(self, prompt, n: int, lengths=None, beams: int = 1, end: int | None = None):
+        """``n`` tokens after each prompt (B, T), whose ``lengths`` (B), of 1 to T tokens, leave
+        off padding at the end: the likeliest, one after another, or with ``beams`` the likeliest
+        continuation of a search that keeps so many.  After the token ``end`` a continuation goes
+        on by that token alone, at no cost."""
         T = prompt.shape[1]
         if T == 0:
             raise ValueError("the prompt has no token to go on from")
+        if beams < 1:
+            raise ValueError(f"beams is at least 1 (got {beams})")
         if lengths is not None and bool(((lengths < 1) | (lengths > T)).any()):
             raise ValueError(f"lengths are from 1 to the prompt's {T} tokens (got {lengths.tolist()})")
         y, state = self(prompt, lengths=lengths)
         rows = torch.arange(len(prompt), device=prompt.device)
         y = y[:, -1] if lengths is None else y[rows, lengths.long() - 1]
+        if beams != 1 or end is not None:
+            return self._search(y, state, n, beams, end)
         out = []
         for _ in range(n):
             token = self.head(y).argmax(-1)
             out.append(token)
-            x, y = self._enter(token)
-            new = []
-            for block, h in zip(self.blocks, state):
-                x, y, h = block.step(x, y, h)
-                new.append(h)
-            state = new
+            y, state = self._step(token, state)
         return torch.stack(out, 1)
 
 
