@@ -220,7 +220,7 @@ __device__ __forceinline__ int64_t pa_lane(int64_t x, int lane) {  // the same l
                    (unsigned)__builtin_amdgcn_readlane((int)x, lane));
 }
 // All sequences' steps as one row, a sequence's pairs of a key head and 16 of its queries one
-// after another.  Sequence b's first step, or (by_step) the sequence that holds step `at`.
+// after another.  The sequence that holds step `at`, and its first step.
 struct PaPlace {
   int64_t b, before;
 };
@@ -230,14 +230,14 @@ __device__ __forceinline__ int64_t pa_all(const PaArgs& a, int64_t pairs, int64_
   sums = pa_steps<SPAN>(a, 0, a.B, run);
   return pa_lane(sums, MG_WAVE - 1) * pairs;
 }
-template <int SPAN, bool BY_STEP>
+template <int SPAN>
 __device__ __forceinline__ PaPlace pa_find(const PaArgs& a, int64_t pairs, int64_t sums, int64_t run,
-                                           int64_t b, int64_t at) {
+                                           int64_t at) {
   PaPlace p = {0, 0};
   int64_t n = a.B;
   for (;;) {
     // The run that holds it: the lanes before have all theirs before it.
-    const int lane = BY_STEP ? __popcll(__ballot(p.before + sums * pairs <= at)) : (int)((b - p.b) / run);
+    const int lane = __popcll(__ballot(p.before + sums * pairs <= at));
     if (lane > 0) p.before += pa_lane(sums, lane - 1) * pairs;
     p.b += lane * run;
     if (run == 1) return p;
@@ -245,6 +245,16 @@ __device__ __forceinline__ PaPlace pa_find(const PaArgs& a, int64_t pairs, int64
     run = (run + MG_WAVE - 1) / MG_WAVE;
     sums = pa_steps<SPAN>(a, p.b, n, run);
   }
+}
+
+// A step of a sequence's: its pair, and which of that.
+struct PaPair {
+  int pair, step;
+};
+__device__ __forceinline__ PaPair pa_pair(int64_t in, int steps) {
+  in = pa_uniform(in);
+  const int pair = in >> 32 ? (int)(in / steps) : (int)((unsigned)in / (unsigned)steps);
+  return PaPair{pair, (int)(in - (int64_t)pair * steps)};
 }
 
 // Share w of n holds the steps [w all / n, (w + 1) all / n); no share is empty, as n <= all.
@@ -308,6 +318,17 @@ __global__ __launch_bounds__(PA_NT, (PaShape<T, DK, DV>::GROUPS)) void paged_att
   float* const sums = (float*)s_tile[wave];
   const bool short_k = DK != a.dk;
 
+  // The outputs of sequences without a token.
+  for (int64_t b0 = blockIdx.x; b0 < a.B; b0 += (int64_t)gridDim.x * PA_NT) {
+    const int64_t b = b0 + (int64_t)gridDim.x * threadIdx.x;
+    unsigned long long empty = __ballot(b < a.B && a.lengths[b < a.B ? b : b0] <= 0);
+    for (; empty != 0; empty &= empty - 1) {
+      const int64_t at = b0 + (int64_t)gridDim.x * (wave * MG_WAVE + __ffsll(empty) - 1);
+      T* const dst = (T*)a.o + at * a.H * (int64_t)a.dv;
+      for (int x = lane; x < a.H * a.dv; x += MG_WAVE) dst[x] = pg_round<T>(0.f);
+    }
+  }
+
   // This share's first step.
   PaStep now;
   {
@@ -318,13 +339,12 @@ __global__ __launch_bounds__(PA_NT, (PaShape<T, DK, DV>::GROUPS)) void paged_att
     if ((int)blockIdx.x >= shares) return;
     const int64_t at = pa_share(blockIdx.x, all, shares);
     now.left = pa_share(blockIdx.x + 1, all, shares) - at;
-    const PaPlace p = pa_find<SPAN, true>(a, pairs, steps, run, 0, at);
+    const PaPlace p = pa_find<SPAN>(a, pairs, steps, run, at);
     now.b = pa_uniform(p.b);
     now.seq = pa_seq_uniform<SPAN>(a, now.b);
-    const int64_t in = pa_uniform(at - p.before);
-    const int pair = in >> 32 ? (int)(in / now.seq.steps) : (int)((unsigned)in / (unsigned)now.seq.steps);
-    now.hk = pair / a.tiles_q, now.tile_q = pair - now.hk * a.tiles_q;
-    now.todo = (int)(in - (int64_t)pair * now.seq.steps);  // the step, for now
+    const PaPair pair = pa_pair(at - p.before, now.seq.steps);
+    now.hk = pair.pair / a.tiles_q, now.tile_q = pair.pair - now.hk * a.tiles_q;
+    now.todo = pair.step;  // for now
     now.valid = true;
   }
   auto open = [&](PaStep& s, int step) {  // a piece from that step of its pair on
@@ -608,28 +628,45 @@ __global__ __launch_bounds__(PA_NT, (PaShape<T, DK, DV>::GROUPS)) void paged_att
   }
 }
 
-// Joins the pieces of one query head: a workgroup each.
-template <typename T, int SPAN>
+// Joins the pieces of the pairs that are cut in two or more.  Where pairs are few and pieces many, a
+// workgroup for each pair and query head (BY_PAIR, at most 64 sequences); else a wave for each start
+// of a share, which cuts a pair or does not, and query head.  (A workgroup for each of all heads,
+// most of which are whole, took 131 us for 1024 sequences of 256 tokens and 16 heads, where the
+// main kernel takes 104 and this 6.)
+template <typename T, int SPAN, bool BY_PAIR>
 __global__ __launch_bounds__(PA_NT) void paged_attention_join(PaArgs a) {
   __shared__ f32x4 s_part[PA_NT];
-  const int lane = threadIdx.x & (MG_WAVE - 1);
-  const int64_t b = blockIdx.x / a.H;
-  const int h = (int)(blockIdx.x - b * a.H), hk = h / a.group, in = h - hk * a.group;
-  const int r = in % PA_ROWS;
+  constexpr int TPR = BY_PAIR ? PA_NT : MG_WAVE;  // threads of a query head
+  const int lane = threadIdx.x & (MG_WAVE - 1), tid = threadIdx.x % TPR;
+  const int r = (int)mg_uniform(blockIdx.y * (PA_NT / TPR) + threadIdx.x / TPR);
   const int64_t pairs = (int64_t)a.Hk * a.tiles_q;
   int64_t steps, run;
-  const PaSeq seq = pa_seq<SPAN>(a, b);
   const int64_t all = pa_all<SPAN>(a, pairs, steps, run);
-  T* const dst = (T*)a.o + (b * a.H + h) * (int64_t)a.dv;
-  if (seq.steps == 0) {
-    for (int x = threadIdx.x; x < a.dv; x += PA_NT)
-      dst[x] = pg_round<T>(seq.bad ? __builtin_nanf("") : 0.f);
-    return;
-  }
-  const int64_t before = pa_find<SPAN, false>(a, pairs, steps, run, b, 0).before;
   const int shares = pa_shares_used(a, all);
-  const int64_t from = before + ((int64_t)hk * a.tiles_q + in / PA_ROWS) * seq.steps;
-  const int w0 = pa_holder(from, all, shares);
+  int64_t b, from;
+  PaSeq seq;
+  int pair, w0;
+  if constexpr (BY_PAIR) {
+    b = blockIdx.x / pairs, pair = (int)(blockIdx.x - b * pairs);
+    seq = pa_seq_uniform<SPAN>(a, b);
+    if (seq.steps == 0) return;
+    from = (b ? pa_lane(steps, (int)b - 1) * pairs : 0) + (int64_t)pair * seq.steps;
+    w0 = pa_holder(from, all, shares);
+  } else {
+    const int w = blockIdx.x + 1;
+    if (w >= shares) return;
+    const int64_t start = pa_share(w, all, shares);
+    const PaPlace p = pa_find<SPAN>(a, pairs, steps, run, start);
+    b = pa_uniform(p.b);
+    seq = pa_seq_uniform<SPAN>(a, b);
+    const PaPair at = pa_pair(start - p.before, seq.steps);
+    if (at.step == 0) return;  // a pair starts here
+    from = start - at.step, pair = at.pair, w0 = w - 1;
+    if (pa_share(w0, all, shares) > from) return;  // an earlier start cuts it, too
+  }
+  const int hk = pair / a.tiles_q, tile_q = pair - hk * a.tiles_q;
+  if (r >= a.rows || tile_q * PA_ROWS + r >= a.group) return;
+  T* const dst = (T*)a.o + (b * a.H + hk * a.group + tile_q * PA_ROWS + r) * (int64_t)a.dv;
   const int n = pa_holder(from + seq.steps - 1, all, shares) - w0 + 1;
   if (n == 1) return;  // one share held it and has written it
   // The pieces are the first or second one of w0, then the first ones of w0 + 1 .. w0 + n - 1.
@@ -640,7 +677,7 @@ __global__ __launch_bounds__(PA_NT) void paged_attention_join(PaArgs a) {
   // first pieces are on their way before the maximum is known.
   int wide = 1;
   while (4 * wide < a.dv) wide *= 2;
-  const int groups = PA_NT / wide, mine = threadIdx.x / wide, x = 4 * (threadIdx.x - mine * wide);
+  const int groups = TPR / wide, mine = tid / wide, x = 4 * (tid - mine * wide);
   const bool whole = a.dv % 4 == 0 && x < a.dv;
   auto load = [&](int i) {
     const float* p = a.part + place(i < n ? i : 0) * a.dv;
@@ -650,7 +687,7 @@ __global__ __launch_bounds__(PA_NT) void paged_attention_join(PaArgs a) {
     for (int e = 0; e < 4; ++e) v[e] = p[x + e < a.dv ? x + e : 0];
     return v;
   };
-  constexpr int AHEAD = 4;
+  constexpr int AHEAD = BY_PAIR ? 16 : 4;
   f32x4 ahead[AHEAD];
   float peak[AHEAD];
 #pragma unroll
@@ -686,10 +723,16 @@ __global__ __launch_bounds__(PA_NT) void paged_attention_join(PaArgs a) {
     for (int j = 0; j < AHEAD; ++j)
       if (i + j * groups < n) v += pa_exp2(peak[j] - base) * ahead[j];
   }
-  s_part[threadIdx.x] = v;
-  __syncthreads();
+  f32x4* const part = s_part + (threadIdx.x - tid);
+  part[tid] = v;
+  if constexpr (TPR == MG_WAVE) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
+  }
   if (mine == 0) {
-    for (int j = 1; j < groups; ++j) v += s_part[j * wide + threadIdx.x];
+    for (int j = 1; j < groups; ++j) v += part[j * wide + tid];
     const float inv = seq.bad ? __builtin_nanf("") : 1.f / sum;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -742,8 +785,19 @@ int pa_run(const PaArgs& a, hipStream_t stream) {
   else if (a.dv <= 128) pa_launch<T, 256, 128>(a, stream);
   else pa_launch<T, 256, 256>(a, stream);
   if (hipGetLastError() != hipSuccess) return MG_ERR_LAUNCH;
-  hipLaunchKernelGGL((paged_attention_join<T, PaShape<T, 64, 64>::SPAN>),
-                     dim3((unsigned)(a.B * a.H)), dim3(PA_NT), 0, stream, a);
+  // Where no pair can have two steps, or all are one share, none is cut.
+  constexpr int SPAN = PaShape<T, 64, 64>::SPAN;
+  if (a.shares == 1 || a.room <= SPAN) return MG_OK;
+  // By pair where one has more than some eight pieces.  (64 x 4096 tokens, one key head, both
+  // launches: 33 us by starts, 41 with a workgroup in a wave's place.  262144 tokens of one key head:
+  // the join takes 26 us by starts, nearly all of which cut the same pair.)
+  const int64_t all = a.B * a.Hk * a.tiles_q;
+  if (all * 8 >= a.shares || a.B > MG_WAVE)
+    hipLaunchKernelGGL((paged_attention_join<T, SPAN, false>),
+                       dim3(a.shares - 1, (a.rows + PA_NW - 1) / PA_NW), dim3(PA_NT), 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_attention_join<T, SPAN, true>), dim3((unsigned)all, a.rows),
+                       dim3(PA_NT), 0, stream, a);
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
 
