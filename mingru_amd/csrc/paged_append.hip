@@ -89,8 +89,8 @@ __global__ __launch_bounds__(AP_NT) void paged_append(ApArgs a) {
   const int count = (int)(a.T - t0 < a.tokens ? a.T - t0 : a.tokens);
   int live = count;  // tokens that are there
   if (a.lengths.p) {
-    const int64_t n = a.lengths[b] - t0;
-    live = n < 0 ? 0 : (n < count ? (int)n : count);
+    const int64_t n = a.lengths[b];
+    live = n <= t0 ? 0 : (n - t0 < count ? (int)(n - t0) : count);
   }
   {
     const int64_t start = a.start[b];

@@ -11,6 +11,7 @@ import ctypes
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from .hip_scans import ScanFallback, _call, _funnel, _ptr, _size, _stream, _workspace
 from .hip_sequence import _array, _last_dense, _no_tangents
@@ -30,6 +31,14 @@ def _tag(what, t) -> int:
     if tag is None:
         raise ScanFallback(f"{what} kernels take float32, bfloat16 and float16 (got {t.dtype})")
     return tag
+
+
+def _launch(what, t, name, *args):
+    """``name`` of the C ABI on ``t``'s device, whose default stream is another device's otherwise."""
+    if torch.cuda.current_device() != t.device.index:
+        with torch.cuda.device(t.device):
+            return _funnel(what, _call, name, *args, _stream(t))
+    return _funnel(what, _call, name, *args, _stream(t))
 
 
 def _ints(*ts):
@@ -80,10 +89,13 @@ def paged_cache_append_impl(k, v, k_cache, v_cache, pages, start, q, lengths, fr
     strides = (*qs, *k.stride()[:3], *v.stride()[:3], *k_cache.stride()[:3], *v_cache.stride()[:3],
                pages.stride(0))
     n = 0 if frequencies is None else frequencies.numel()
-    _funnel(what, _call, "mg_paged_append", tag, _ptr(q), _ptr(k), _ptr(v), _ptr(k_cache),
+    _launch(what, k, "mg_paged_append", tag, _ptr(q), _ptr(k), _ptr(v), _ptr(k_cache),
             _ptr(v_cache), _ptr(out), _array(strides), wide, _ptr(pages), _ptr(start),
             _ptr(lengths), int(n > 0 and frequencies.dtype == torch.float64), _ptr(frequencies), n,
-            int(bool(interleaved)), B, T, H, Hk, dk, dv, N, pages.shape[1], P, _stream(k))
+            int(bool(interleaved)), B, T, H, Hk, dk, dv, N, pages.shape[1], P)
+    for cache in (k_cache, v_cache):
+        if not cache.is_inference():
+            increment_version(cache)  # as torch's own writes do, for what autograd may have saved
     return (out,)
 
 
@@ -101,7 +113,9 @@ def paged_attention_step_impl(q, k_cache, v_cache, pages, lengths, scale, window
                            f"sequences, tables of fewer than 2^31 - 1024 tokens and fewer than 2^31 "
                            f"pages (got {dk} and {dv}, {B} x {H}, {M} x {P} and {N})")
     q = _last_dense(q)
-    if q.data_ptr() % 16 or not q.is_contiguous():
+    size = q.element_size()
+    row = 16 if dk * size % 16 == 0 else 8
+    if dk * size % row == 0 and (q.data_ptr() | (q.stride(0) | q.stride(1)) * size) % row:
         # Small, and the kernels load the caches by vectors only together with the queries.
         q = q.clone(memory_format=torch.contiguous_format)
     wide, pages, lengths = _ints(pages, lengths)
@@ -110,9 +124,9 @@ def paged_attention_step_impl(q, k_cache, v_cache, pages, lengths, scale, window
     strides = (*q.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3], pages.stride(0))
     # A window that no sequence outgrows is none.
     window = 0 if window is None or window >= M * P else window
-    _funnel(what, _call, "mg_paged_attention_step", tag, _ptr(q), _ptr(k_cache), _ptr(v_cache),
+    _launch(what, q, "mg_paged_attention_step", tag, _ptr(q), _ptr(k_cache), _ptr(v_cache),
             _array(strides), wide, _ptr(pages), _ptr(lengths), _ptr(o), B, H, Hk, dk, dv, N, M, P,
-            window, scale, _ptr(ws), ws.numel(), _stream(q))
+            window, scale, _ptr(ws), ws.numel())
     return o
 
 
@@ -141,9 +155,9 @@ def beam_select_impl(logits, scores, width, end, finished):
     ws = _workspace(nbytes, dev)
     strides = (*logits.stride()[:2], *scores.stride(),
                *((0, 0) if finished is None else finished.stride()))
-    _funnel(what, _call, "mg_beam_select", tag, _ptr(logits), _ptr(scores), _ptr(finished),
+    _launch(what, logits, "mg_beam_select", tag, _ptr(logits), _ptr(scores), _ptr(finished),
             _array(strides), -1 if end is None else int(end), _ptr(out), _ptr(parents),
-            _ptr(tokens), _ptr(done), B, K, V, width, _ptr(ws), ws.numel(), _stream(logits))
+            _ptr(tokens), _ptr(done), B, K, V, width, _ptr(ws), ws.numel())
     return (out, parents, tokens) if done is None else (out, parents, tokens, done)
 
 
@@ -164,6 +178,8 @@ def reorder_states_impl(tensors, parents, K):
     out, src, dst, strides, sizes = [], [], [], [], []
     rows = B * K
     for t in tensors:
+        if t.is_conj() or t.is_neg():
+            t = t.resolve_conj().resolve_neg()
         dense = t.is_contiguous()
         if dense and W == K:
             new = torch.empty_like(t)
@@ -184,7 +200,7 @@ def reorder_states_impl(tensors, parents, K):
         dst.append(new)
         sizes.append(size)
     if src:
-        _funnel(what, _call, "mg_reorder_rows", len(src), _pointers(src), _pointers(dst),
+        _launch(what, parents, "mg_reorder_rows", len(src), _pointers(src), _pointers(dst),
                 _array(strides), _array(sizes), int(parents.dtype == torch.int64), _ptr(parents),
-                *parents.stride(), B, K, W, _stream(parents))
+                *parents.stride(), B, K, W)
     return out

@@ -86,6 +86,7 @@ def test_tangents_leave_the_kernels(monkeypatch, name):
     monkeypatch.setattr(hip_scans, "available", lambda: True)
     real = sequence_ops._dispatch
     monkeypatch.setattr(decode_ops, "_dispatch", lambda what, is_cuda, *rest: real(what, True, *rest))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)  # the CPU's index
     monkeypatch.setattr(hip_decode, "_stream", lambda t: 0)
     monkeypatch.setattr(hip_decode, "_size", lambda *a: 256)
     calls = []
@@ -97,3 +98,31 @@ def test_tangents_leave_the_kernels(monkeypatch, name):
             out = f(forward_ad.make_dual(x, torch.ones_like(x)))
         assert forward_ad.unpack_dual(out).tangent is not None
     assert len(calls) == 1
+
+
+def test_calls_run_on_their_tensors_device(monkeypatch):
+    """The default stream is a number that means the current device's."""
+    import contextlib
+
+    from mingru_amd import hip_decode
+
+    class Tensor:
+        device = torch.device("cuda", 1)
+
+    current = [0]
+
+    @contextlib.contextmanager
+    def device(d):
+        old, current[0] = current[0], d.index
+        yield
+        current[0] = old
+
+    seen = []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(hip_decode, "_stream", lambda t: 0)
+    monkeypatch.setattr(hip_decode, "_call", lambda *a: seen.append((current[0], a)))
+    hip_decode._launch("what", Tensor(), "name", 3)
+    current[0] = 1
+    hip_decode._launch("what", Tensor(), "name", 3)
+    assert seen == [(1, ("name", 3, 0))] * 2 and current == [1]

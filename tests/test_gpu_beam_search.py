@@ -217,3 +217,12 @@ def test_on_another_stream(cuda):
         got = [beam_select(logits, scores) for _ in range(3)]
     stream.synchronize()
     assert all(torch.equal(a, b) for one in got for a, b in zip(one, want))
+
+
+def test_reorder_resolves_views(cuda):
+    """Conjugates and negatives that are only marked as such."""
+    x = torch.randn(6, 5, dtype=torch.complex64, device=cuda)
+    parents = torch.tensor([[2, 0], [1, 1]], device=cuda)
+    at = torch.tensor([2, 0, 4, 4], device=cuda)
+    for t in (x.conj(), x.conj().imag):
+        assert torch.equal(reorder_states(t, parents), t.resolve_conj().resolve_neg()[at])

@@ -124,6 +124,25 @@ def test_append_padding_is_not_read(cuda):
     check_append(cuda, s)
 
 
+@pytest.mark.parametrize("n", [-(2**63), -1, 2**40, 2**63 - 1])
+def test_append_lengths_of_64_bits(cuda, n):
+    s = append_inputs(2, 5, 2, 1, 8, 8, 2, 4, 4, dtype=torch.float32)
+    s["lengths"] = torch.tensor([n, 3])
+    check_append(cuda, s)
+
+
+def test_append_marks_the_caches_as_written(cuda):
+    s = to(append_inputs(2, 5, 2, 1, 8, 8, 2, 4, 4, dtype=torch.float32), cuda)
+    w = torch.ones((), device=cuda, requires_grad=True)
+    y = (w * s["k_cache"]).sum()  # keeps the cache for its gradient
+    paged_cache_append(**s)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        s = to(append_inputs(2, 5, 2, 1, 8, 8, 2, 4, 4, dtype=torch.float32), cuda)
+        paged_cache_append(**s)
+
+
 def test_append_far_positions(cuda):
     """Angles of positions whose product with a frequency has no more bits in fp32 left."""
     far, n = 3 * 10**6, 64
@@ -279,6 +298,15 @@ def test_attend_strides(cuda, dtype):
     both = torch.cat([dev["k_cache"], dev["v_cache"]], -1)  # keys and values side by side
     dev["k_cache"], dev["v_cache"] = both.split((64, 48), -1)
     check_attend(cuda, s, dev=dev)
+
+
+def test_attend_queries_of_a_joined_projection(cuda):
+    s = attend_inputs(4, 6, 2, 64, 64, 16, 20, dtype=torch.bfloat16)
+    for pad in (0, 1, 4, 8):  # aligned or not
+        dev = to(s, cuda)
+        joined = torch.cat([dev["q"].flatten(1), dev["q"].flatten(1)[:, : 64 + pad]], 1)
+        dev["q"] = joined[:, : 6 * 64].unflatten(1, (6, 64))
+        check_attend(cuda, s, dev=dev)
 
 
 def test_attend_unaligned(cuda):
