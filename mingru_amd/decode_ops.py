@@ -37,22 +37,36 @@ def _check_whole(what: str, device, **tensors) -> None:
             raise ValueError(f"{what}: {name} is on {t.device}, the first input on {device}")
 
 
-def _check_cache(what: str, k_cache, v_cache, pages, B: int) -> None:
-    if k_cache.dim() != 4 or v_cache.dim() != 4 or k_cache.shape[:3] != v_cache.shape[:3]:
+def _check_cache(what: str, k_cache, v_cache, pages, B: int) -> tuple:
+    """N, Hk, P, dk and dv of the caches."""
+    ks, vs = k_cache.shape, v_cache.shape
+    if len(ks) != 4 or ks[:3] != vs[:3] or len(vs) != 4:
         raise ValueError(f"{what}: k_cache is (N, Hk, P, dk) and v_cache (N, Hk, P, dv) (got "
-                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)})")
-    if 0 in k_cache.shape[1:] or v_cache.shape[3] == 0:
-        raise ValueError(f"{what}: a size of the caches is 0 (got {tuple(k_cache.shape)} and "
-                         f"{tuple(v_cache.shape)})")
-    if pages.dim() != 2 or pages.shape[0] != B:
+                         f"{tuple(ks)} and {tuple(vs)})")
+    if 0 in ks[1:] or vs[3] == 0:
+        raise ValueError(f"{what}: a size of the caches is 0 (got {tuple(ks)} and {tuple(vs)})")
+    if pages.dim() != 2 or len(pages) != B:
         raise ValueError(f"{what}: pages is (B, M) with B = {B} (got {tuple(pages.shape)})")
+    return *ks, vs[3]
 
 
-def _check_types(what: str, **tensors) -> None:
-    names = [n for n, t in tensors.items() if t is not None]
-    if len({tensors[n].dtype for n in names}) > 1:
-        raise TypeError(f"{what}: {', '.join(names)} have one type (got "
-                        f"{', '.join(str(tensors[n].dtype) for n in names)})")
+def _check_one_type(what: str, **tensors) -> None:
+    """Floating-point tensors of one type on one device."""
+    dtype = device = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: {name} must be a floating-point tensor (got "
+                            f"{type(t).__name__})")
+        if dtype is None:
+            first, dtype, device = name, t.dtype, t.device
+            if not dtype.is_floating_point:
+                raise TypeError(f"{what}: {name} must be a floating-point tensor (got {dtype})")
+        elif t.dtype is not dtype:
+            raise TypeError(f"{what}: {name} has {first}'s type (got {t.dtype} and {dtype})")
+        elif t.device != device:
+            raise ValueError(f"{what}: {name} is on {t.device}, the first input on {device}")
 
 
 # ---------------------------------------------------------------------------
@@ -107,20 +121,19 @@ def paged_cache_append(k, v, k_cache, v_cache, pages, start, *, q=None, lengths=
     looking would wait for it, it is not kept and its queries are NaN.
     """
     what = "paged_cache_append"
-    _check_floats(what, k=k, v=v, k_cache=k_cache, v_cache=v_cache, q=q, frequencies=frequencies)
+    _check_one_type(what, k=k, v=v, k_cache=k_cache, v_cache=v_cache, q=q)
+    _check_floats(what, k=k, frequencies=frequencies)
     _check_whole(what, k.device, pages=pages, start=start, lengths=lengths)
-    _check_types(what, k=k, v=v, k_cache=k_cache, v_cache=v_cache, q=q)
-    if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3]:
+    shape = k.shape
+    if len(shape) != 4 or v.dim() != 4 or shape[:3] != v.shape[:3]:
         raise ValueError(f"{what}: k is (B, T, Hk, dk) and v (B, T, Hk, dv) (got "
-                         f"{tuple(k.shape)} and {tuple(v.shape)})")
-    B, T, Hk, dk = k.shape
-    _check_cache(what, k_cache, v_cache, pages, B)
-    N, _, P, dv = v_cache.shape
-    if k_cache.shape[1] != Hk or k_cache.shape[3] != dk or v.shape[3] != dv:
-        raise ValueError(f"{what}: the caches hold heads {tuple(k_cache.shape[1::2])} and "
-                         f"{tuple(v_cache.shape[1::2])}, k and v are {tuple(k.shape)} and "
-                         f"{tuple(v.shape)}")
-    if q is not None and (q.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != dk):
+                         f"{tuple(shape)} and {tuple(v.shape)})")
+    B, T, Hk, dk = shape
+    N, heads, P, *sizes = _check_cache(what, k_cache, v_cache, pages, B)
+    if heads != Hk or sizes != [dk, v.shape[3]]:
+        raise ValueError(f"{what}: the caches hold {heads} heads of sizes {sizes}, k and v are "
+                         f"{tuple(shape)} and {tuple(v.shape)}")
+    if q is not None and (q.dim() != 4 or q.shape[:2] != shape[:2] or q.shape[3] != dk):
         raise ValueError(f"{what}: q is (B, T, H, dk) = ({B}, {T}, H, {dk}) (got {tuple(q.shape)})")
     for name, t in (("start", start), ("lengths", lengths)):
         if t is not None and t.shape != (B,):
@@ -130,7 +143,7 @@ def paged_cache_append(k, v, k_cache, v_cache, pages, start, *, q=None, lengths=
         raise ValueError(f"{what}: frequencies is (n,) with n from 1 to dk / 2 = {dk // 2} (got "
                          f"{tuple(frequencies.shape)})")
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        if 0 in t.stride() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
             raise ValueError(f"{what}: {name} is written, so it must not be an expanded view")
     if B * T and N and pages.shape[1]:
         done = _dispatch(what, k.is_cuda, lambda backend: backend.paged_cache_append_impl(
@@ -202,17 +215,15 @@ def paged_attention_step(q, k_cache, v_cache, pages, lengths, *, scale=None, win
     sequence's ``o`` is NaN.
     """
     what = "paged_attention_step"
-    _check_floats(what, q=q, k_cache=k_cache, v_cache=v_cache)
+    _check_one_type(what, q=q, k_cache=k_cache, v_cache=v_cache)
     _check_whole(what, q.device, pages=pages, lengths=lengths)
-    _check_types(what, q=q, k_cache=k_cache, v_cache=v_cache)
     if q.dim() != 3:
         raise ValueError(f"{what}: q is (B, H, dk) (got {tuple(q.shape)})")
     B, H, dk = q.shape
-    _check_cache(what, k_cache, v_cache, pages, B)
-    N, Hk, P, dv = v_cache.shape
-    if k_cache.shape[3] != dk or H < 1 or H % Hk:
-        raise ValueError(f"{what}: q is {tuple(q.shape)}, the keys' heads {Hk} of size "
-                         f"{k_cache.shape[3]}; their number divides q's, their size is q's")
+    N, Hk, P, size, dv = _check_cache(what, k_cache, v_cache, pages, B)
+    if size != dk or H < 1 or H % Hk:
+        raise ValueError(f"{what}: q is {tuple(q.shape)}, the keys' heads {Hk} of size {size}; their "
+                         "number divides q's, their size is q's")
     if lengths.shape != (B,):
         raise ValueError(f"{what}: lengths is (B,) = ({B},) (got {tuple(lengths.shape)})")
     if window is not None and (isinstance(window, bool) or int(window) != window or window < 1):

@@ -46,10 +46,10 @@ def _ints(*ts):
     wide, out = 0, []
     for i, t in enumerate(ts):
         if t is not None:
-            if t.dtype not in (torch.int32, torch.int64):
+            if t.dtype is not torch.int32:
                 t = t.to(torch.int64)
+                wide |= 1 << i
             t = _last_dense(t)
-            wide |= (t.dtype == torch.int64) << i
         out.append(t)
     return (wide, *out)
 
@@ -66,32 +66,30 @@ def paged_cache_append_impl(k, v, k_cache, v_cache, pages, start, q, lengths, fr
     what = "paged_cache_append"
     _no_tangents(what, k, v, k_cache, v_cache, q, frequencies)
     tag = _tag(what, k)
-    (B, T, Hk, dk), dv = k.shape, v.shape[3]
-    N, _, P, _ = k_cache.shape
+    (B, T, Hk, dk), (N, _, P, dv) = k.shape, v_cache.shape
     _cache(what, "k_cache", k_cache), _cache(what, "v_cache", v_cache)
     H = 0 if q is None else q.shape[2]
-    if N >= 2**31 or P >= 2**31 or Hk * (dk + dv) + H * dk >= 2**26 or \
-            (frequencies is not None and frequencies.numel() > 1024):
+    n = 0 if frequencies is None else len(frequencies)
+    if N >= 2**31 or P >= 2**31 or Hk * (dk + dv) + H * dk >= 2**26 or n > 1024:
         raise ScanFallback(f"{what} kernels take tokens of fewer than 2^26 elements, up to 1024 "
                            f"frequencies and fewer than 2^31 pages (got {N} of {P} tokens)")
-    if q is not None:
-        q = _last_dense(q)
     k, v = _last_dense(k), _last_dense(v)
-    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if H == 0:
-        q = None
+    out, turned, qs = None, 0, (0, 0, 0)
+    if q is not None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        q = _last_dense(q)
+        turned, qs = out.data_ptr(), q.stride()[:3]
     wide, pages, start, lengths = _ints(pages, start, lengths)
-    if frequencies is not None:
+    if n:
         if frequencies.dtype not in (torch.float32, torch.float64):
             frequencies = frequencies.float()
         frequencies = frequencies.contiguous()
-    qs = (0, 0, 0) if q is None else q.stride()[:3]
     strides = (*qs, *k.stride()[:3], *v.stride()[:3], *k_cache.stride()[:3], *v_cache.stride()[:3],
                pages.stride(0))
-    n = 0 if frequencies is None else frequencies.numel()
-    _launch(what, k, "mg_paged_append", tag, _ptr(q), _ptr(k), _ptr(v), _ptr(k_cache),
-            _ptr(v_cache), _ptr(out), _array(strides), wide, _ptr(pages), _ptr(start),
-            _ptr(lengths), int(n > 0 and frequencies.dtype == torch.float64), _ptr(frequencies), n,
+    _launch(what, k, "mg_paged_append", tag, _ptr(q) if H else 0, k.data_ptr(), v.data_ptr(),
+            k_cache.data_ptr(), v_cache.data_ptr(), turned, _array(strides), wide,
+            pages.data_ptr(), start.data_ptr(), _ptr(lengths),
+            int(n > 0 and frequencies.dtype is torch.float64), _ptr(frequencies), n,
             int(bool(interleaved)), B, T, H, Hk, dk, dv, N, pages.shape[1], P)
     for cache in (k_cache, v_cache):
         if not cache.is_inference():
