@@ -290,15 +290,16 @@ __global__ __launch_bounds__(BS_NT, 4) void beam_rows(BsArgs a) {
     const float next = fmaxf(top, peak);
     sum *= bs_exp(top - next);
     float add[2] = {0.f, 0.f};
-    if (__ballot(next < -1e38f) == 0) {
+    if (__ballot(!(fabsf(next) < 1048576.f)) == 0) {
       // exp(v - next) as 2^(v L - c), L = log2 e, one operation less: c is next L rounded, and what
-      // that rounds off, r, the same for all of them, is put back once.
+      // that rounds off, r, the same for all of them, is put back once.  Below 2^20 it is 2^-4 at
+      // most; without a bound it would grow with next until 2^r is out of range.
       const float c = next * 1.44269504f, r = __builtin_fmaf(next, 1.44269504f, -c);
 #pragma unroll
       for (int i = 0; i < ALL; ++i)
         add[i & 1] += __builtin_amdgcn_exp2f(__builtin_fmaf(v[i], 1.44269504f, -c));
       sum += (add[0] + add[1]) * __builtin_amdgcn_exp2f(-r);
-    } else {  // where next L may be out of range
+    } else {
 #pragma unroll
       for (int i = 0; i < ALL; ++i) add[i & 1] += bs_exp(v[i] - next);
       sum += add[0] + add[1];
@@ -377,7 +378,8 @@ __device__ __forceinline__ double bs_row_sum(double x) {  // over 16 lanes
 template <int NW>
 __global__ __launch_bounds__(NW* MG_WAVE) void beam_pick(BsArgs a) {
   __shared__ Key64 s_list[NW / 2][MG_WAVE], s_bar;
-  __shared__ double s_norm[BS_MAX_K], s_score[BS_MAX_K];
+  __shared__ double s_log[BS_MAX_K], s_score[BS_MAX_K];  // of the sum over exp(x - top)
+  __shared__ float s_top[BS_MAX_K];
   __shared__ unsigned char s_kind[BS_MAX_K];
   enum { LIVE = 0, FINISHED = 1, DEAD = 2 };
   const int lane = bs_lane(), wave = (int)mg_uniform(threadIdx.x / MG_WAVE);
@@ -401,9 +403,10 @@ __global__ __launch_bounds__(NW* MG_WAVE) void beam_pick(BsArgs a) {
       sum = bs_row_sum(sum);
     }
     if (in == 0 && k < a.K) {
-      const double norm = (double)m + log(sum);
-      s_score[k] = score, s_norm[k] = over ? 0.0 : norm;
-      s_kind[k] = !finite ? DEAD : (over ? FINISHED : (fabs(norm) < __builtin_inf() ? LIVE : DEAD));
+      const double part = log(sum);
+      const bool live = bs_finite(m) && fabs(part) < __builtin_inf();
+      s_score[k] = score, s_top[k] = m, s_log[k] = part;
+      s_kind[k] = !finite ? DEAD : (over ? FINISHED : (live ? LIVE : DEAD));
     }
   }
   __syncthreads();
@@ -424,7 +427,8 @@ __global__ __launch_bounds__(NW* MG_WAVE) void beam_pick(BsArgs a) {
       const int r = n / lists, at = n - r * lists, k = at / a.parts;
       if (s_kind[k] == LIVE) {
         if (from)
-          x = key(s_score[k] + ((double)bs_value((unsigned)(from >> 32)) - s_norm[k]),
+          // The difference first: a large top would swallow the logarithm.
+          x = key(s_score[k] + ((double)bs_value((unsigned)(from >> 32)) - (double)s_top[k] - s_log[k]),
                   (unsigned)k * (unsigned)a.V + ~(unsigned)from);
       } else if (at == k * a.parts) {  // in place of its parts: its end, and the first tokens at -inf
         const bool over = s_kind[k] == FINISHED, first = over && r == 0;

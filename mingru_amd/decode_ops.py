@@ -337,12 +337,12 @@ def _eager_select(logits, scores, width, end, finished):
     V = logits.shape[2]
     wide = torch.promote_types(torch.promote_types(logits.dtype, scores.dtype), torch.float32)
     x, s = logits.double(), scores.double()
-    total = torch.logsumexp(x, -1)
     if finished is not None:
         only = torch.full((V,), -torch.inf, dtype=x.dtype, device=x.device)
         only[int(end)] = 0.0
         x = torch.where(finished[..., None], only, x)
-        total = torch.where(finished, torch.zeros_like(total), total)
+    x = x - x.amax(-1, keepdim=True)  # first of all: a large maximum would swallow the logarithm
+    total = x.exp().sum(-1).log()
     dead = ~(torch.isfinite(total) & torch.isfinite(s))[..., None]
     score = (s[..., None] + (x - total[..., None])).masked_fill(dead, -torch.inf)
     score, order = torch.sort(score.flatten(1), dim=-1, descending=True, stable=True)

@@ -74,6 +74,17 @@ def test_ties_go_to_the_lower_beam_then_the_lower_token():
     assert got[0].dtype == torch.float32
 
 
+@pytest.mark.parametrize("size", [1.0, 1e9, 3e37, 1e300])
+def test_large_logits_keep_their_rows_weight(size):
+    """Beams that differ only in how many tokens share a row."""
+    logits = torch.full((1, 3, 8), -math.inf, dtype=torch.float64)
+    logits[0, 0, :4], logits[0, 1, 5:7], logits[0, 2] = size, -size, size
+    score, parent, token = beam_select(logits, torch.tensor([[0.0, -0.1, 0.0]]), 7)
+    assert parent.tolist() == [[1, 1, 0, 0, 0, 0, 2]] and token.tolist() == [[5, 6, 0, 1, 2, 3, 0]]
+    want = torch.tensor([-0.1 - math.log(2)] * 2 + [-math.log(4)] * 4 + [-math.log(8)])
+    assert torch.allclose(score[0], want.double(), atol=1e-6)  # the scores are of 32 bits
+
+
 def odd_beams(K=8, V=13, width=20, seed=1):
     """Beams that have ended, that have no finite score or sum, and masked tokens."""
     logits, scores = beam_inputs(1, K, V, seed)

@@ -99,6 +99,18 @@ def test_orders(cuda, dtype, kind, V):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e4, 1e6, 1.2e6, 3e9, 1e20, 3e37, 3e38])
+def test_large_logits(cuda, dtype, size):
+    """Up to where a logit times log2 e leaves the type's range; equal ones share a row's weight."""
+    g = torch.Generator().manual_seed(2)
+    x = size * torch.randint(-1, 2, (2, 3, 5000), generator=g).float()
+    x[0, 0] = size
+    x[0, 1] = -size
+    x[1, 2, 7:] = -size
+    check(x.to(dtype).to(cuda), -torch.rand(2, 3, generator=g).to(cuda), 8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_rows_that_start_anywhere(cuda, dtype):
     logits, scores = inputs(cuda, 3, 4, 3001, dtype)
     wide = torch.full((3, 4, 3040), math.nan, dtype=dtype, device=cuda)
