@@ -537,7 +537,7 @@ int mg_vocab_loss_bwd(int dtype, const void* w, const void* bias, const float* d
  * `window` (0: all) of lengths[b] tokens, for dk, dv <= 256, B H < 2^24, M P < 2^31 - 1024.  A
  * length of 0 gives 0; one above M P, or a page that is needed and not in the cache, NaN.
  * strides: q (sequence, head), k_cache, v_cache (page, head, slot), pages (sequence).  ints: bit
- * 0 pages, 1 lengths. */
+ * 0 pages, 1 lengths.  ws is 16-byte aligned, here and below. */
 int mg_paged_append(int dtype, const void* q, const void* k, const void* v, void* k_cache,
                     void* v_cache, void* q_out, const int64_t* strides, int ints,
                     const void* pages, const void* start, const void* lengths, int freq_dtype,

@@ -198,7 +198,8 @@ def paged_attention_step(q, k_cache, v_cache, pages, lengths, *, scale=None, win
     v_cache : (N, Hk, P, dv)
         ``Hk`` divides ``H``; each key head serves ``H / Hk`` heads in a row.  What lies in pages
         behind a sequence's last token, or before its window, has no part in the result,
-        whatever it is.  One type for ``q`` and the caches.
+        whatever it is; an infinity among the values that do have makes it infinite or NaN.  One
+        type for ``q`` and the caches.
     pages : (B, M) integers
         Only the entries of tokens that are attended to are looked at.
     lengths : (B) integers

@@ -244,6 +244,24 @@ def test_attend_batches(cuda, B, longest, dtype):
     check_attend(cuda, s)
 
 
+@pytest.mark.parametrize("B", [64, 65, 4097, 9000])
+def test_attend_many_sequences(cuda, B):
+    """More than a wave's lanes find at once, and than their runs; nearly all of them empty."""
+    s = attend_inputs(B, 2, 1, 16, 16, 16, 20, dtype=torch.float32)
+    some = torch.rand(B, generator=torch.Generator().manual_seed(4)) < 60 / B
+    s["lengths"] = torch.where(some, s["lengths"], torch.zeros_like(s["lengths"]))
+    s["lengths"][-1] = 320
+    check_attend(cuda, s)
+
+
+def test_attend_to_nothing(cuda):
+    s = attend_inputs(70, 2, 1, 16, 16, 16, 20, dtype=torch.float32)
+    s["lengths"] = torch.zeros(70, dtype=torch.int64)
+    for M in (20, 3):
+        s["pages"] = s["pages"][:, :M]
+        check_attend(cuda, s)
+
+
 @pytest.mark.parametrize("window", [None, 5, 70])
 @pytest.mark.parametrize("P", [4, 7, 64])
 @pytest.mark.parametrize("dtype", TYPES)
