@@ -1,9 +1,9 @@
 """``paged_cache_append`` and ``paged_attention_step`` kernels against the definition in float64.
 
-Tolerances.  Append, element by element: the reduced angle is rounded to 2^-25 of a turn at most
-half a turn wide, 2 pi 2^-26 = 1.6 * 2^-24 radians; its sine and cosine, two products and a sum
-are five more roundings of 2^-24: 2^-21 of the pair's sum of magnitudes is more than all of them.
-Then one rounding of the result, ``eps / 2``.
+Tolerances.  Append, element by element: the angle, reduced to an eighth of a turn or less, is
+rounded to fp32 (below 1, by 2^-25 at most); its sine and cosine, two products and a sum are five
+more roundings of 2^-24: 2^-21 of the pair's sum of magnitudes is more than all of them.  Then one
+rounding of the result, ``eps / 2``.
 
 Attention, as the 2-norm of the difference over that of the result: a score is a sum of up to 256
 products, whose rounding is that of as many partial sums of its size, in disorder, sqrt(256) =
@@ -252,6 +252,21 @@ def test_attend_many_sequences(cuda, B):
     s["lengths"] = torch.where(some, s["lengths"], torch.zeros_like(s["lengths"]))
     s["lengths"][-1] = 320
     check_attend(cuda, s)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("e", [3, 8, 14, 30, 60])
+def test_attend_large_scores(cuda, dtype, e):
+    """Scores of 2^(2 e - 3), as exact as sums, so that equal keys share the weight exactly."""
+    if dtype == torch.float16 and e > 14:
+        pytest.skip("out of the type's range")
+    s = attend_inputs(6, 6, 2, 64, 64, 16, 60, dtype=dtype)
+    g = torch.Generator().manual_seed(1)
+    s["q"] = torch.zeros_like(s["q"])
+    s["q"][..., 5] = 2.0**e * (torch.arange(6) % 3 - 1)
+    s["k_cache"][..., 5] = 2.0**e * torch.randint(-1, 2, s["k_cache"].shape[:-1], generator=g)
+    check_attend(cuda, s)
+    check_attend(cuda, s, window=77)
 
 
 def test_attend_to_nothing(cuda):
