@@ -31,6 +31,12 @@ namespace {
 // ---- sorted lists over a wave -----------------------------------------------------------
 __device__ __forceinline__ int bs_lane() { return threadIdx.x & (MG_WAVE - 1); }
 
+// Lanes of `who` before this one.
+__device__ __forceinline__ int bs_before(unsigned long long who) {
+  return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32),
+                                        __builtin_amdgcn_mbcnt_lo((unsigned)who, 0));
+}
+
 // x of lane ^ D.
 template <int CTRL>
 __device__ __forceinline__ unsigned bs_dpp(unsigned x) {
@@ -99,10 +105,6 @@ struct Key64 {
   __device__ __forceinline__ unsigned long long value() const { return bs_join(hi, lo); }
   __device__ __forceinline__ bool above(Key64 o) const {
     return value() > o.value() || (value() == o.value() && index > o.index);
-  }
-  template <typename F>
-  __device__ __forceinline__ Key64 map(F&& f) const {
-    return Key64{f(index), f(lo), f(hi)};
   }
   __device__ __forceinline__ Key64 pick(bool first, Key64 o) const {
     return Key64{first ? index : o.index, first ? lo : o.lo, first ? hi : o.hi};
@@ -200,6 +202,7 @@ struct BsArgs {
   int64_t ss[2], fs[2];           // of the scores and of finished
   int64_t B;
   int K, V, W, end;
+  Divisor by_lists, by_parts;     // K parts and parts
   int parts, per;                 // of a row; elements of a part, a multiple of a tile's
   float2* stats;                  // (B, K, parts): maximum, sum
   unsigned long long* keys;       // (B, W, K, parts)
@@ -323,8 +326,7 @@ __global__ __launch_bounds__(BS_NT, 4) void beam_rows(BsArgs a) {
       for (int i = g * N; i < g * N + N; ++i) bits |= v[i] >= bar ? 1u << i : 0u;
     }
     for (unsigned long long who; (who = __ballot(bits != 0)) != 0; bits &= bits - 1) {
-      const int i = __ffs(bits) - 1, to = hits + (int)__builtin_amdgcn_mbcnt_hi(
-          (unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0));
+      const int i = __ffs(bits) - 1, to = hits + bs_before(who);
       if (bits != 0 && to < BS_HITS)
         s_place[wave][to] = at + (i / N * MG_WAVE + lane) * N + i % N;
       hits += __popcll(who);
@@ -375,113 +377,260 @@ __device__ __forceinline__ double bs_row_sum(double x) {  // over 16 lanes
   return x;
 }
 
-template <int NW>
-__global__ __launch_bounds__(NW* MG_WAVE) void beam_pick(BsArgs a) {
-  __shared__ Key64 s_list[NW / 2][MG_WAVE], s_bar;
-  __shared__ double s_log[BS_MAX_K], s_score[BS_MAX_K];  // of the sum over exp(x - top)
-  __shared__ float s_top[BS_MAX_K];
-  __shared__ unsigned char s_kind[BS_MAX_K];
+// The candidates lie by their ranks in their lists (a part's), all lists' first ones ahead.  A first
+// pass counts them by steps of how far they lie below the best score that a beam can give, and ends
+// where all lists have fallen behind the steps that hold the W best; a second one puts those within
+// reach, W and few more, into LDS, where each one's place is the number of those above it.  No chain
+// is long: sorted lists over the waves' lanes, as for the rows, took 15 us of 31 for 16 searches of 16
+// beams of 32771, 32 wide, where this takes 10 of 26; one search of 256 beams of 50257, 64 wide, took
+// 151 us with both launches in place of 63.
+// Eight waves and two candidates a thread: sixteen and four take 25.7 us in place of 26.0 for the former,
+// but 13.1 in place of 10.8 for 4 beams of 50257, 4 wide.
+constexpr int BP_NW = 8, BP_NT = BP_NW * MG_WAVE, BP_HELD = 2, BP_CHUNK = BP_HELD * BP_NT;
+constexpr int BP_STEPS = 256;
+constexpr int BP_MOST = 256;  // keys in LDS before others come
+
+// The candidates that may be among the W best, and how many of them are above each.
+struct Pool {
+  static constexpr int ROOM = BP_MOST + BP_NT;
+  unsigned long long value[ROOM];
+  unsigned index[ROOM];
+  int rank[ROOM];
+  int steps[BP_STEPS];
+  int count, reach;
+  int few;    // no more than BP_MOST are within reach
+  int fresh;  // the last chunk, from 1, that has had some
+  Key64 bar;  // the W-th of all before, once there have been more
+
+  __device__ __forceinline__ Key64 at(int i) const {
+    return Key64{index[i], (unsigned)value[i], (unsigned)(value[i] >> 32)};
+  }
+  __device__ __forceinline__ void put(int i, Key64 x) {
+    value[i] = x.value(), index[i] = x.index, rank[i] = 0;
+  }
+  // All threads.  A wave takes 64 keys and those that it compares them with: all, or where there
+  // are fewer keys than threads a part.
+  __device__ __forceinline__ void order(int n) {
+    const int wave = (int)mg_uniform(threadIdx.x / MG_WAVE);
+    const int blocks = (n + MG_WAVE - 1) / MG_WAVE, cuts = blocks < BP_NW ? BP_NW / blocks : 1;
+    const int each = (n + cuts - 1) / cuts;
+    for (int u = wave; u < blocks * cuts; u += BP_NW) {
+      const int cut = u / blocks, i = (u - cut * blocks) * MG_WAVE + bs_lane();
+      const int end = (cut + 1) * each < n ? (cut + 1) * each : n;
+      const Key64 x = at(i < n ? i : 0);
+      int above = 0;
+#pragma unroll 4
+      for (int j = cut * each; j < end; ++j) above += at(j).above(x) ? 1 : 0;
+      if (i < n) atomicAdd(&rank[i], above);
+    }
+    __syncthreads();
+  }
+};
+
+__global__ __launch_bounds__(BP_NT) void beam_pick(BsArgs a) {
+  constexpr int EACH = BP_STEPS / MG_WAVE;
+  __shared__ Pool pool;
   enum { LIVE = 0, FINISHED = 1, DEAD = 2 };
-  const int lane = bs_lane(), wave = (int)mg_uniform(threadIdx.x / MG_WAVE);
+  struct alignas(8) Beam {
+    double score, log;  // log of the sum over exp(x - top)
+    float top;
+    int kind;
+  };
+  __shared__ Beam s_beam[BS_MAX_K];
+  const int lane = bs_lane(), me = threadIdx.x;
   const int64_t b = blockIdx.x;
+  const int lists = a.K * a.parts, all = lists * a.W;
+  const unsigned long long* const keys = a.keys + b * all;
+  // On their way together with all else: what other parts of the chip have just written is far away.
+  unsigned long long raw[BP_HELD];
+  auto load = [&](int at) {
+#pragma unroll
+    for (int i = 0; i < BP_HELD; ++i) raw[i] = keys[at + i * BP_NT + me < all ? at + i * BP_NT + me : 0];
+  };
+  load(0);
   // Sixteen lanes a row.
-  for (int k0 = 0; k0 < a.K; k0 += NW * 4) {
+  for (int k0 = 0; k0 < a.K; k0 += BP_NW * 4) {
     const int k = k0 + (int)threadIdx.x / 16, in = threadIdx.x & 15;
     const int at = k < a.K ? k : a.K - 1;
     const float score = a.scores[b * a.ss[0] + at * a.ss[1]];
-    const bool finite = bs_finite(score), over = bs_finished(a, b, at);
     const float2* st = a.stats + (b * a.K + at) * a.parts;
-    float m = -__builtin_inff();
+    // On their way before it is known whether the first launch has written them.
+    const float2 none = make_float2(-__builtin_inff(), 0.f);
+    const float2 x = in < a.parts ? st[in] : none, y = in + 16 < a.parts ? st[in + 16] : none;
+    const bool finite = bs_finite(score), over = bs_finished(a, b, at);
+    float m = fmaxf(x.x, y.x);
     double sum = 0.0;
-    if (finite && !over) {  // written by the first launch
-      for (int i = in; i < a.parts; i += 16) m = fmaxf(m, st[i].x);
+    if (finite && !over) {
+      for (int i = in + 32; i < a.parts; i += 16) m = fmaxf(m, st[i].x);
       m = fmaxf(m, mg_row_ror<8>(m));
       m = fmaxf(m, mg_row_ror<4>(m));
       m = fmaxf(m, mg_row_ror<2>(m));
       m = fmaxf(m, mg_row_ror<1>(m));
-      for (int i = in; i < a.parts; i += 16) sum += (double)st[i].y * (double)bs_exp(st[i].x - m);
+      sum = (double)x.y * (double)bs_exp(x.x - m) + (double)y.y * (double)bs_exp(y.x - m);
+      for (int i = in + 32; i < a.parts; i += 16) sum += (double)st[i].y * (double)bs_exp(st[i].x - m);
       sum = bs_row_sum(sum);
     }
     if (in == 0 && k < a.K) {
       const double part = log(sum);
       const bool live = bs_finite(m) && fabs(part) < __builtin_inf();
-      s_score[k] = score, s_top[k] = m, s_log[k] = part;
-      s_kind[k] = !finite ? DEAD : (over ? FINISHED : (live ? LIVE : DEAD));
+      s_beam[k] = Beam{score, part, m, !finite ? DEAD : (over ? FINISHED : (live ? LIVE : DEAD))};
     }
   }
+  for (int i = me; i < BP_STEPS; i += BP_NT) pool.steps[i] = 0;
+  if (me == 0) pool.count = pool.fresh = pool.few = 0, pool.reach = BP_STEPS - 1, pool.bar = Key64{};
   __syncthreads();
-
-  Best<Key64> list;
-  // Every part's first candidates come before any part's second ones, so that the first ones that
-  // are looked at set a high bar.
-  const int lists = a.K * a.parts, all = lists * a.W;
+  double most = -__builtin_inf();
+  for (int k = lane; k < a.K; k += MG_WAVE) {
+    const Beam beam = s_beam[k];
+    if (beam.kind != DEAD) most = fmax(most, beam.kind == LIVE ? beam.score - beam.log : beam.score);
+  }
+#pragma unroll
+  for (int d = 1; d < MG_WAVE; d *= 2) most = fmax(most, __shfl_xor(most, d));
   auto key = [&](double score, unsigned index) {
     const unsigned long long o = bs_order(score);
     return Key64{~index, (unsigned)o, (unsigned)(o >> 32)};
   };
-  const unsigned long long* const keys = a.keys + b * all;
-  auto raw = [&](int n) { return keys[n < all ? n : 0]; };
   auto candidate = [&](int n, unsigned long long from) {
-    Key64 x = {};
-    if (n < all) {
-      const int r = n / lists, at = n - r * lists, k = at / a.parts;
-      if (s_kind[k] == LIVE) {
-        if (from)
-          // The difference first: a large top would swallow the logarithm.
-          x = key(s_score[k] + ((double)bs_value((unsigned)(from >> 32)) - (double)s_top[k] - s_log[k]),
-                  (unsigned)k * (unsigned)a.V + ~(unsigned)from);
-      } else if (at == k * a.parts) {  // in place of its parts: its end, and the first tokens at -inf
-        const bool over = s_kind[k] == FINISHED, first = over && r == 0;
-        int token = first ? a.end : r - (over ? 1 : 0);
-        if (over && !first && token >= a.end) ++token;
-        if (token < a.V)
-          x = key(first ? s_score[k] : -__builtin_inf(), (unsigned)k * (unsigned)a.V + (unsigned)token);
+    const int r = (int)pg_div((unsigned)n, a.by_lists), at = n - r * lists;
+    const int k = (int)pg_div((unsigned)at, a.by_parts);
+    const Beam beam = s_beam[k];
+    const bool live = beam.kind == LIVE, over = beam.kind == FINISHED;
+    // In place of the parts of a beam that is not: its end, and the first tokens at -inf.
+    const int token = over ? (r == 0 ? a.end : r - (r <= a.end ? 1 : 0)) : r;
+    const bool there = live ? from != 0 : at == k * a.parts && token < a.V;
+    // The difference first: a large top would swallow the logarithm.
+    const double value = (double)bs_value((unsigned)(from >> 32)) - (double)beam.top - beam.log;
+    const Key64 x = key(live || (over && r == 0) ? beam.score + (live ? value : 0.0) : -__builtin_inf(),
+                        (unsigned)k * (unsigned)a.V + (live ? ~(unsigned)from : (unsigned)token));
+    return x.pick(there, Key64{});
+  };
+  // How far below the beams' best scores a candidate lies, in steps of an eighth of an octave from
+  // 2^-8 on: the W best are in the first steps that hold W, and those hold few more.
+  auto step = [&](Key64 x) {
+    const float d = (float)(most - bs_value(x.value()));
+    const int s = (int)(__float_as_uint(d) >> 20) - ((127 - 8) << 3);
+    return d < 0.00390625f ? 0 : (s < BP_STEPS ? s : BP_STEPS - 1);
+  };
+  Key64 held[BP_HELD];
+  auto value_all = [&](int at) {
+#pragma unroll
+    for (int i = 0; i < BP_HELD; ++i) {
+      const int n = at + i * BP_NT + me;
+      held[i] = candidate(n < all ? n : 0, raw[i]);
+      held[i] = held[i].pick(n < all, Key64{});
+    }
+  };
+  int end = 0, reach = BP_STEPS - 1;
+  bool few = false;
+  for (int at = 0; at < all; at += BP_CHUNK) {
+    if (at) load(at);
+    value_all(at);
+    bool fresh = false;
+#pragma unroll
+    for (int i = 0; i < BP_HELD; ++i) {
+      const int s = step(held[i]);
+      if (held[i].index == 0 || s >= BP_STEPS - 1 || s > reach) continue;
+      atomicAdd(&pool.steps[s], 1);
+      fresh = true;
+    }
+    if (fresh) pool.fresh = at + 1;
+    __syncthreads();
+    // Nothing new within reach among as many candidates as there are lists: some rank of every list,
+    // so that none behind it is.
+    if (reach < BP_STEPS - 1 && pool.fresh != at + 1) {
+      if (at + BP_CHUNK - end >= lists) break;
+      continue;
+    }
+    end = at + BP_CHUNK;
+    if (me < MG_WAVE) {
+      int n[EACH], sum = 0;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) sum += n[i] = pool.steps[me * EACH + i];
+      int before = sum;
+#pragma unroll
+      for (int d = 1; d < MG_WAVE; d *= 2) {
+        const int o = __shfl_up(before, d);
+        before += lane >= d ? o : 0;
+      }
+      // The step at which W are reached; the last one, whose are not counted, if none is.
+      const unsigned long long who = __ballot(before >= a.W);
+      if (who && me == __ffsll(who) - 1) {
+        before -= sum;
+        int s = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const bool on = before < a.W;
+          before += on ? n[i] : 0, s += on ? 1 : 0;
+        }
+        pool.reach = me * EACH + s - 1, pool.few = before <= BP_MOST;
       }
     }
-    return x;
-  };
-  // A bar that W candidates reach: of 64 parts' first ones, all over the beams, the W-th.  The
-  // candidates that reach it are few more than W.
-  int at = wave * MG_WAVE;
-  unsigned long long next = raw(at + lane);
-  if (wave == 0) {
-    const int n = lists > MG_WAVE ? (int)((int64_t)lane * lists / MG_WAVE) : lane;
-    const Key64 x = bs_sort(n < all ? candidate(n, raw(n)) : Key64{});
-    const Key64 bar = bs_from(x, a.W - 1);
-    if (lane == 0) s_bar = bar;
+    __syncthreads();
+    reach = pool.reach, few = pool.few != 0;
   }
-  __syncthreads();
-  // Just below that candidate: the inverted index of a key is above 0.
-  list.start(a.W);
-  list.floor = s_bar;
-  if (list.floor.above(Key64{})) list.floor.index -= 1;
-  list.settle();
-  for (; at < all; at += NW * MG_WAVE) {
-    const unsigned long long now = next;
-    next = raw(at + NW * MG_WAVE + lane);
-    list.offer(candidate(at + lane, now));
-  }
-  // The waves' lists, by halves.
+  end = end < all ? end : all;
+#pragma unroll 1
+  for (int at = 0;; at += BP_NT) {
+    const int i = at / BP_NT % BP_HELD;
+    if (i == 0 && all > BP_CHUNK) load(at), value_all(at);
+    Key64 one = held[0];
 #pragma unroll
-  for (int half = NW / 2; half > 0; half /= 2) {
-    if (wave >= half && wave < 2 * half) s_list[wave - half][lane] = list.best;
+    for (int j = 1; j < BP_HELD; ++j) one = held[j].pick(i == j, one);
+    const bool in = one.above(pool.bar) && step(one) <= reach;
+    const unsigned long long who = __ballot(in);
+    if (who) {
+      int to = 0;
+      if (lane == 0) to = atomicAdd(&pool.count, __popcll(who));
+      to = (int)bs_read((unsigned)to, 0) + bs_before(who);
+      if (in) pool.put(to, one);
+    }
+    const bool more = at + BP_NT < end;
+    if (more && few) continue;
     __syncthreads();
-    if (wave < half) list.best = bs_merge(list.best, s_list[wave][lane]);
+    const int n = pool.count;
+    if (more && n <= BP_MOST) {
+      __syncthreads();
+      continue;
+    }
+    pool.order(n);
+    Key64 x[Pool::ROOM / BP_NT + 1];
+    int rank[Pool::ROOM / BP_NT + 1];
+#pragma unroll
+    for (int i = 0; i <= Pool::ROOM / BP_NT; ++i) {
+      const int from = me + i * BP_NT;
+      rank[i] = from < n ? pool.rank[from] : a.W;
+      x[i] = pool.at(from < n ? from : 0);
+    }
+    if (!more) {
+#pragma unroll
+      for (int i = 0; i <= Pool::ROOM / BP_NT; ++i) {
+        if (rank[i] >= a.W) continue;
+        const unsigned flat = ~x[i].index;
+        const int k = (int)(flat / (unsigned)a.V), token = (int)(flat - (unsigned)k * (unsigned)a.V);
+        const int64_t to = b * a.W + rank[i];
+        a.out[to] = (float)bs_value(x[i].value());
+        a.parents[to] = k, a.tokens[to] = token;
+        if (a.done) a.done[to] = token == a.end || bs_finished(a, b, k);
+      }
+      return;
+    }
+    // The W best go on, and the last of them is the bar.
     __syncthreads();
-  }
-  if (wave == 0 && lane < a.W) {
-    const unsigned flat = ~list.best.index;
-    const int k = (int)(flat / (unsigned)a.V), token = (int)(flat - (unsigned)k * (unsigned)a.V);
-    const int64_t n = b * a.W + lane;
-    a.out[n] = (float)bs_value(list.best.value());
-    a.parents[n] = k, a.tokens[n] = token;
-    if (a.done) a.done[n] = token == a.end || bs_finished(a, b, k);
+#pragma unroll
+    for (int i = 0; i <= Pool::ROOM / BP_NT; ++i) {
+      if (rank[i] >= a.W) continue;
+      pool.put(rank[i], x[i]);
+      if (rank[i] == a.W - 1) pool.bar = x[i];
+    }
+    if (me == 0) pool.count = a.W;
+    __syncthreads();
   }
 }
 
 // Waves of a row: two for each of the chip's 1024 vector units over all rows, none with less than
-// a tile.  (64 x 8 rows of 50257 in bf16, both launches in a graph: 24.6 us; four for each, with
-// more first tiles and candidates, 25.8, one 33.  16 x 16 of 32771 in fp32, 32 wide: 32, four 38.)
+// a tile.  (64 x 8 rows of 50257 in bf16, both launches in a graph: 24.0 us; four for each 24.2, one
+// 27.4.  16 x 16 of 32771 in fp32, 32 wide: 26.0, four, with more first tiles and candidates, 30.5, one
+// 27.0.)
 int bs_parts(int64_t rows, int V, int tile) {
   const int64_t want = (2048 + rows - 1) / rows;
   const int64_t most = ((int64_t)V + 8 + tile - 1) / tile;
@@ -658,6 +807,7 @@ int mg_beam_select(int dtype, const void* logits, const float* scores, const voi
   const int64_t per = (V + 8 + a.parts - 1) / a.parts;
   a.per = (int)((per + tile - 1) / tile * tile);
   a.parts = (int)((V + 8 + a.per - 1) / a.per);
+  a.by_lists = pg_divisor(K * a.parts), a.by_parts = pg_divisor(a.parts);
   a.keys = (unsigned long long*)ws;
   a.stats = (float2*)(a.keys + B * K * a.parts * W);
   a.out = out, a.parents = parents, a.tokens = tokens, a.done = (unsigned char*)done;
@@ -666,13 +816,7 @@ int mg_beam_select(int dtype, const void* logits, const float* scores, const voi
   else if (dtype == 1) hipLaunchKernelGGL(beam_rows<Bf16>, grid, nt, 0, stream, a);
   else hipLaunchKernelGGL(beam_rows<Fp16>, grid, nt, 0, stream, a);
   if (hipGetLastError() != hipSuccess) return MG_ERR_LAUNCH;
-  // Eight waves where four would have more than two rounds of candidates: 8 x 8 beams of 31633 take
-  // 13.9 us with both launches, with four 14.5; 16 x 16 of 32771, 32 wide, 31.2, four 32.8, sixteen
-  // 31.9.
-  if (K * a.parts * W <= 2 * 4 * MG_WAVE)
-    hipLaunchKernelGGL(beam_pick<4>, dim3((unsigned)B), dim3(4 * MG_WAVE), 0, stream, a);
-  else
-    hipLaunchKernelGGL(beam_pick<8>, dim3((unsigned)B), dim3(8 * MG_WAVE), 0, stream, a);
+  hipLaunchKernelGGL(beam_pick, dim3((unsigned)B), dim3(BP_NT), 0, stream, a);
   return hipGetLastError() == hipSuccess ? MG_OK : MG_ERR_LAUNCH;
 }
 

@@ -31,6 +31,20 @@ def exact(logits, scores, width, end=None, finished=None):
                            finished=None if finished is None else finished.cpu())
 
 
+def check_near(logits, scores, width):
+    """As ``check`` where scores of two beams may be nearer than the roundings of their rows' sums,
+    2^-24 of each or more: such candidates may change places.  Each is then a candidate of its own,
+    with its own score, which is also that of its place."""
+    want = exact(logits, scores, width)
+    score, parent, token = (t.cpu() for t in beam_select(logits, scores, width))
+    x = torch.log_softmax(logits.cpu().double(), -1) + scores.cpu().double()[..., None]
+    own = x.flatten(1).gather(1, parent * logits.shape[2] + token)
+    for other in (own, want[0]):
+        assert not bool(((score.double() - other).abs() > TOL * other.abs().clamp(min=1.0)).any())
+    assert not bool((score[:, 1:] > score[:, :-1]).any())
+    assert all(len(set(zip(p, t))) == width for p, t in zip(parent.tolist(), token.tolist()))
+
+
 def check(logits, scores, width, end=None, finished=None):
     want = exact(logits, scores, width, end, finished)
     got = beam_select(logits, scores, width, end=end, finished=finished)
@@ -96,6 +110,40 @@ def test_orders(cuda, dtype, kind, V):
     scores = -torch.rand(2, 3, generator=g)
     for width in (1, 6, 64):
         check(x.to(dtype).to(cuda), scores.to(cuda), width)
+
+
+@pytest.mark.parametrize("kind", ["level", "ahead", "equal", "close", "finished", "dead", "spread"])
+@pytest.mark.parametrize("B, K, V, width", [(1, 256, 3001, 64), (3, 64, 5000, 64), (2, 33, 9001, 50),
+                                            (1, 200, 70, 64)])
+def test_many_beams(cuda, kind, B, K, V, width):
+    """Candidates of one beam alone, of all, and far more of one score than are kept."""
+    logits, scores = beam_inputs(B, K, V, 3)
+    logits, scores, finished = logits.float(), scores.float(), None
+    g = torch.Generator().manual_seed(5)
+    if kind == "level":
+        scores[:] = -1.0
+    elif kind == "ahead":
+        scores -= 100.0
+        scores[:, K // 2] = -1.0
+    elif kind == "equal":
+        logits[:], scores[:] = 0.25, -2.0
+    elif kind == "close":  # steps of a few roundings
+        logits = torch.randint(0, 9, logits.shape, generator=g) * 2.0**-20
+        scores[:] = -3.0
+    elif kind == "finished":
+        finished = torch.rand(B, K, generator=g) < 0.9
+        scores -= 50.0 * torch.rand(B, K, generator=g)
+    elif kind == "dead":  # fewer candidates than are kept
+        logits[..., 3:] = -math.inf
+        scores[:, 5:] = -math.inf
+    elif kind == "spread":
+        scores *= torch.logspace(-3, 9, K)
+    end = None if finished is None else 11
+    finished = None if finished is None else finished.to(cuda)
+    if kind == "close":
+        check_near(logits.to(cuda), scores.to(cuda), width)
+    else:
+        check(logits.to(cuda), scores.to(cuda), width, end, finished)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
