@@ -417,11 +417,13 @@ def reorder_states(states, parents):
     tensors = _leaves(states, [])
     if not tensors:
         return _rebuilt(states, iter(()))
-    rows, device = len(tensors[0]) if tensors[0].dim() else -1, parents.device
+    rows, device = tensors[0].shape[0] if tensors[0].dim() else -1, parents.device
+    uneven = rows % B if B else rows
     for t in tensors:
         if t.device != device:
             raise ValueError(f"{what}: a state is on {t.device}, parents on {device}")
-        if t.dim() < 1 or len(t) != rows or (rows % B if B else rows):
+        shape = t.shape
+        if uneven or not shape or shape[0] != rows:
             raise ValueError(f"{what}: each state has B K rows, the same for all, with B = {B} (got "
                              f"{tuple(t.shape)})")
     K = rows // B if B else 0

@@ -159,10 +159,6 @@ def beam_select_impl(logits, scores, width, end, finished):
     return (out, parents, tokens) if done is None else (out, parents, tokens, done)
 
 
-def _pointers(ts):
-    return (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
-
-
 def reorder_states_impl(tensors, parents, K):
     """``reorder_states`` on checked arguments: a list of tensors, of ``K`` rows a search."""
     what = "reorder_states"
@@ -173,32 +169,35 @@ def reorder_states_impl(tensors, parents, K):
         raise ScanFallback(f"{what} kernels write fewer than 2^31 rows (got {B} x {W})")
     if parents.dtype not in (torch.int32, torch.int64):
         parents = parents.to(torch.int64)
-    out, src, dst, strides, sizes = [], [], [], [], []
-    rows = B * K
+    out, src, dst, strides, sizes, kept = [], [], [], [], [], []
+    rows, same = B * K, W == K
     for t in tensors:
         if t.is_conj() or t.is_neg():
             t = t.resolve_conj().resolve_neg()
+            kept.append(t)  # until the launch
         dense = t.is_contiguous()
-        if dense and W == K:
+        if dense and same:
             new = torch.empty_like(t)
         else:
             new = torch.empty((B * W, *t.shape[1:]), dtype=t.dtype, device=t.device)
         out.append(new)
-        size = t.nbytes // rows
+        size = stride = t.nbytes // rows
         if size == 0:
             continue
-        if dense:
-            strides.append(size)
-        elif t[0].is_contiguous():
-            strides.append(t.stride(0) * t.element_size())
-        else:
-            t = t.contiguous()
-            strides.append(size)
-        src.append(t)
-        dst.append(new)
+        if not dense:
+            if t[0].is_contiguous():
+                stride = t.stride(0) * t.element_size()
+            else:
+                t = t.contiguous()
+            kept.append(t)  # until the launch
+        src.append(t.data_ptr())
+        dst.append(new.data_ptr())
+        strides.append(stride)
         sizes.append(size)
     if src:
-        _launch(what, parents, "mg_reorder_rows", len(src), _pointers(src), _pointers(dst),
-                _array(strides), _array(sizes), int(parents.dtype == torch.int64), _ptr(parents),
+        n = len(src)
+        pointers, longs = ctypes.c_void_p * n, ctypes.c_int64 * n
+        _launch(what, parents, "mg_reorder_rows", n, pointers(*src), pointers(*dst),
+                longs(*strides), longs(*sizes), int(parents.dtype == torch.int64), _ptr(parents),
                 *parents.stride(), B, K, W)
     return out
