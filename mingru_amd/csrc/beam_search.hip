@@ -17,8 +17,8 @@
 // does not depend on the order of arrival, and ties fall as they are defined.
 //
 // 64 x 8 rows of 50257 in bf16, a fifth of them not read: 17 us for 41 MB and 6 for the selection.
-// What is left above the memory's 8 is the exponentials and comparisons (the vector units issue
-// half of the time) and a wave's two sorts, each a chain of 21 exchanges.
+// Of a wave's 12 us 1.5 are its first load, 1 the first bar's sort, 7 six tiles (a tile's exponentials
+// and comparisons keep the vector units busy most of 1.1), 2 one or two sorts of what reached the bar.
 //
 // reorder_states: rows of up to 32 tensors a launch, in vectors of 16 bytes of the output, whose rows
 // follow one another.  A vector lies in one row, read from wherever that starts, or holds the end of
@@ -242,7 +242,9 @@ __global__ __launch_bounds__(BS_NT, 4) void beam_rows(BsArgs a) {
   // Vectors start at the 16-byte line that holds the row's first element: what lies before it
   // in that line, and behind the row's end in the last, is in the same page and not used.
   const int skew = (int)(((uintptr_t)x & 15) / sizeof(T));
-  const uint4* const lines = (const uint4*)((uintptr_t)x & ~(uintptr_t)15);
+  // (By subtraction: of an integer, the compiler would not know that it points to global memory,
+  // and its loads would be waited for wherever LDS is.)
+  const uint4* const lines = (const uint4*)(x - skew);
   const int all = a.V + skew;  // elements from the first line on
   const int begin = part * a.per, stop = all - begin < a.per ? all : begin + a.per;
 
@@ -382,9 +384,9 @@ __device__ __forceinline__ double bs_row_sum(double x) {  // over 16 lanes
 // where all lists have fallen behind the steps that hold the W best; a second one puts those within
 // reach, W and few more, into LDS, where each one's place is the number of those above it.  No chain
 // is long: sorted lists over the waves' lanes, as for the rows, took 15 us of 31 for 16 searches of 16
-// beams of 32771, 32 wide, where this takes 10 of 26; one search of 256 beams of 50257, 64 wide, took
+// beams of 32771, 32 wide, where this takes 10 of 25; one search of 256 beams of 50257, 64 wide, took
 // 151 us with both launches in place of 63.
-// Eight waves and two candidates a thread: sixteen and four take 25.7 us in place of 26.0 for the former,
+// Eight waves and two candidates a thread: sixteen and four take 0.3 us less for the former,
 // but 13.1 in place of 10.8 for 4 beams of 50257, 4 wide.
 constexpr int BP_NW = 8, BP_NT = BP_NW * MG_WAVE, BP_HELD = 2, BP_CHUNK = BP_HELD * BP_NT;
 constexpr int BP_STEPS = 256;
