@@ -25,12 +25,15 @@ from .sequence_ops import _check_floats, _dispatch, _wide
 __all__ = ["beam_select", "paged_attention_step", "paged_cache_append", "reorder_states"]
 
 
+_INTEGERS = {torch.int8, torch.int16, torch.int32, torch.int64, torch.uint8, torch.uint16,
+             torch.uint32, torch.uint64}
+
+
 def _check_whole(what: str, device, **tensors) -> None:
     for name, t in tensors.items():
         if t is None:
             continue
-        if not torch.is_tensor(t) or t.dtype.is_floating_point or t.dtype.is_complex or \
-                t.dtype == torch.bool:
+        if not isinstance(t, torch.Tensor) or t.dtype not in _INTEGERS:
             raise TypeError(f"{what}: {name} must be a tensor of integers (got "
                             f"{t.dtype if torch.is_tensor(t) else type(t).__name__})")
         if t.device != device:
@@ -39,15 +42,16 @@ def _check_whole(what: str, device, **tensors) -> None:
 
 def _check_cache(what: str, k_cache, v_cache, pages, B: int) -> tuple:
     """N, Hk, P, dk and dv of the caches."""
-    ks, vs = k_cache.shape, v_cache.shape
-    if len(ks) != 4 or ks[:3] != vs[:3] or len(vs) != 4:
+    ks, vs, table = k_cache.shape, v_cache.shape, pages.shape
+    if len(ks) != 4 or len(vs) != 4 or (ks[0], ks[1], ks[2]) != (vs[0], vs[1], vs[2]):
         raise ValueError(f"{what}: k_cache is (N, Hk, P, dk) and v_cache (N, Hk, P, dv) (got "
                          f"{tuple(ks)} and {tuple(vs)})")
-    if 0 in ks[1:] or vs[3] == 0:
+    N, Hk, P, dk = ks
+    if not (Hk and P and dk and vs[3]):
         raise ValueError(f"{what}: a size of the caches is 0 (got {tuple(ks)} and {tuple(vs)})")
-    if pages.dim() != 2 or len(pages) != B:
-        raise ValueError(f"{what}: pages is (B, M) with B = {B} (got {tuple(pages.shape)})")
-    return *ks, vs[3]
+    if len(table) != 2 or table[0] != B:
+        raise ValueError(f"{what}: pages is (B, M) with B = {B} (got {tuple(table)})")
+    return N, Hk, P, dk, vs[3]
 
 
 def _check_one_type(what: str, **tensors) -> None:
@@ -122,26 +126,29 @@ def paged_cache_append(k, v, k_cache, v_cache, pages, start, *, q=None, lengths=
     """
     what = "paged_cache_append"
     _check_one_type(what, k=k, v=v, k_cache=k_cache, v_cache=v_cache, q=q)
-    _check_floats(what, k=k, frequencies=frequencies)
     _check_whole(what, k.device, pages=pages, start=start, lengths=lengths)
-    shape = k.shape
-    if len(shape) != 4 or v.dim() != 4 or shape[:3] != v.shape[:3]:
+    shape, vs = k.shape, v.shape
+    if len(shape) != 4 or len(vs) != 4 or (shape[0], shape[1], shape[2]) != (vs[0], vs[1], vs[2]):
         raise ValueError(f"{what}: k is (B, T, Hk, dk) and v (B, T, Hk, dv) (got "
-                         f"{tuple(shape)} and {tuple(v.shape)})")
+                         f"{tuple(shape)} and {tuple(vs)})")
     B, T, Hk, dk = shape
     N, heads, P, *sizes = _check_cache(what, k_cache, v_cache, pages, B)
-    if heads != Hk or sizes != [dk, v.shape[3]]:
+    if heads != Hk or sizes != [dk, vs[3]]:
         raise ValueError(f"{what}: the caches hold {heads} heads of sizes {sizes}, k and v are "
-                         f"{tuple(shape)} and {tuple(v.shape)}")
-    if q is not None and (q.dim() != 4 or q.shape[:2] != shape[:2] or q.shape[3] != dk):
-        raise ValueError(f"{what}: q is (B, T, H, dk) = ({B}, {T}, H, {dk}) (got {tuple(q.shape)})")
+                         f"{tuple(shape)} and {tuple(vs)}")
+    if q is not None:
+        qs = q.shape
+        if len(qs) != 4 or qs[0] != B or qs[1] != T or qs[3] != dk:
+            raise ValueError(f"{what}: q is (B, T, H, dk) = ({B}, {T}, H, {dk}) (got {tuple(qs)})")
     for name, t in (("start", start), ("lengths", lengths)):
         if t is not None and t.shape != (B,):
             raise ValueError(f"{what}: {name} is (B,) = ({B},) (got {tuple(t.shape)})")
-    if frequencies is not None and (frequencies.dim() != 1
-                                    or not 1 <= frequencies.numel() <= dk // 2):
-        raise ValueError(f"{what}: frequencies is (n,) with n from 1 to dk / 2 = {dk // 2} (got "
-                         f"{tuple(frequencies.shape)})")
+    if frequencies is not None:
+        _check_floats(what, k=k, frequencies=frequencies)
+        n = frequencies.shape
+        if len(n) != 1 or not 1 <= n[0] <= dk // 2:
+            raise ValueError(f"{what}: frequencies is (n,) with n from 1 to dk / 2 = {dk // 2} (got "
+                             f"{tuple(n)})")
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if 0 in t.stride() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
             raise ValueError(f"{what}: {name} is written, so it must not be an expanded view")
@@ -218,12 +225,13 @@ def paged_attention_step(q, k_cache, v_cache, pages, lengths, *, scale=None, win
     what = "paged_attention_step"
     _check_one_type(what, q=q, k_cache=k_cache, v_cache=v_cache)
     _check_whole(what, q.device, pages=pages, lengths=lengths)
-    if q.dim() != 3:
-        raise ValueError(f"{what}: q is (B, H, dk) (got {tuple(q.shape)})")
-    B, H, dk = q.shape
+    qs = q.shape
+    if len(qs) != 3:
+        raise ValueError(f"{what}: q is (B, H, dk) (got {tuple(qs)})")
+    B, H, dk = qs
     N, Hk, P, size, dv = _check_cache(what, k_cache, v_cache, pages, B)
     if size != dk or H < 1 or H % Hk:
-        raise ValueError(f"{what}: q is {tuple(q.shape)}, the keys' heads {Hk} of size {size}; their "
+        raise ValueError(f"{what}: q is {tuple(qs)}, the keys' heads {Hk} of size {size}; their "
                          "number divides q's, their size is q's")
     if lengths.shape != (B,):
         raise ValueError(f"{what}: lengths is (B,) = ({B},) (got {tuple(lengths.shape)})")
@@ -308,10 +316,11 @@ def beam_select(logits, scores, width=None, *, end=None, finished=None):
     """
     what = "beam_select"
     _check_floats(what, logits=logits, scores=scores)
-    if logits.dim() != 3 or scores.shape != logits.shape[:2] or 0 in logits.shape[1:]:
+    shape = logits.shape
+    if len(shape) != 3 or scores.shape != shape[:2] or not (shape[1] and shape[2]):
         raise ValueError(f"{what}: logits is (B, K, V) and scores (B, K) (got "
-                         f"{tuple(logits.shape)} and {tuple(scores.shape)})")
-    B, K, V = logits.shape
+                         f"{tuple(shape)} and {tuple(scores.shape)})")
+    B, K, V = shape
     width = K if width is None else width
     if isinstance(width, bool) or int(width) != width or not 1 <= width <= K * V:
         raise ValueError(f"{what}: width is a whole number from 1 to K V = {K * V} (got {width!r})")

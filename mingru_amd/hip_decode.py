@@ -69,7 +69,7 @@ def paged_cache_append_impl(k, v, k_cache, v_cache, pages, start, q, lengths, fr
     (B, T, Hk, dk), (N, _, P, dv) = k.shape, v_cache.shape
     _cache(what, "k_cache", k_cache), _cache(what, "v_cache", v_cache)
     H = 0 if q is None else q.shape[2]
-    n = 0 if frequencies is None else len(frequencies)
+    n = 0 if frequencies is None else frequencies.shape[0]
     if N >= 2**31 or P >= 2**31 or Hk * (dk + dv) + H * dk >= 2**26 or n > 1024:
         raise ScanFallback(f"{what} kernels take tokens of fewer than 2^26 elements, up to 1024 "
                            f"frequencies and fewer than 2^31 pages (got {N} of {P} tokens)")
@@ -91,9 +91,8 @@ def paged_cache_append_impl(k, v, k_cache, v_cache, pages, start, q, lengths, fr
             pages.data_ptr(), start.data_ptr(), _ptr(lengths),
             int(n > 0 and frequencies.dtype is torch.float64), _ptr(frequencies), n,
             int(bool(interleaved)), B, T, H, Hk, dk, dv, N, pages.shape[1], P)
-    for cache in (k_cache, v_cache):
-        if not cache.is_inference():
-            increment_version(cache)  # as torch's own writes do, for what autograd may have saved
+    # As torch's own writes do, for what autograd may have saved.
+    increment_version([c for c in (k_cache, v_cache) if not c.is_inference()])
     return (out,)
 
 
