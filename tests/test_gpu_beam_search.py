@@ -65,7 +65,7 @@ def inputs(cuda, B, K, V, dtype, seed=0):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("B, K, V, width", [
     (1, 1, 1, 1), (1, 1, 5, 3), (2, 3, 11, 33), (3, 4, 2047, 4), (1, 4, 2048, 8), (2, 8, 2049, 64),
-    (1, 2, 50257, 2), (1, 1, 131071, 64), (40, 5, 1000, 5), (3, 64, 700, 64), (1, 256, 300, 40),
+    (1, 2, 50257, 2), (1, 1, 131071, 64), (1, 1, 300007, 64), (40, 5, 1000, 5), (3, 64, 700, 64), (1, 256, 300, 40),
     (700, 1, 33, 7), (1, 1, 64, 64), (2, 2, 40, 64), (9, 16, 4096, 32)])
 def test_sizes(cuda, dtype, B, K, V, width):
     check(*inputs(cuda, B, K, V, dtype), width)
@@ -114,7 +114,7 @@ def test_orders(cuda, dtype, kind, V):
 
 @pytest.mark.parametrize("kind", ["level", "ahead", "equal", "close", "finished", "dead", "spread"])
 @pytest.mark.parametrize("B, K, V, width", [(1, 256, 3001, 64), (3, 64, 5000, 64), (2, 33, 9001, 50),
-                                            (1, 200, 70, 64)])
+                                            (1, 200, 70, 64), (1, 256, 20011, 64)])
 def test_many_beams(cuda, kind, B, K, V, width):
     """Candidates of one beam alone, of all, and far more of one score than are kept."""
     logits, scores = beam_inputs(B, K, V, 3)
