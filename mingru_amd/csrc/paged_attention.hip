@@ -18,7 +18,9 @@
 //   all chunks c at one e (E elements a chunk), a fragment of them is a lane's element e of
 //   each of its tokens.
 // * Half types' probabilities are two summands of their type, so that their rounding is 2^-16
-//   (bf16) of them: one of 2^-9 is as large as the result's own.
+//   (bf16) or 2^-22 (fp16) of them: one's is as large as the result's own.  In fp16, which has nothing
+//   below 2^-24, they and their sum are 2^15 times as large: weights down to 2^-40 of the largest
+//   count in the products as they do in the sum.
 // Maxima, sums and O are fp32, with O scaled again only where a maximum rises.
 //
 // Work is divided on the device, where the lengths are: the steps (four tiles, one for each wave
@@ -62,6 +64,7 @@ struct Elem;
 template <>
 struct Elem<Bf16> {
   static constexpr int KEYS = 32, PAD = 8;
+  static constexpr float WEIGHT = 1.f;
   typedef bf16x8 Frag;
   static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
@@ -73,6 +76,7 @@ struct Elem<Bf16> {
 template <>
 struct Elem<Fp16> {
   static constexpr int KEYS = 32, PAD = 8;
+  static constexpr float WEIGHT = 32768.f;  // of a score that is the maximum
   typedef f16x8 Frag;
   static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
@@ -88,6 +92,7 @@ struct Elem<Fp16> {
 template <>
 struct Elem<float> {
   static constexpr int KEYS = 16, PAD = 4;
+  static constexpr float WEIGHT = 1.f;
 };
 
 // A lane's chunk of a row: E elements in registers of 32 bits.
@@ -541,7 +546,7 @@ __global__ __launch_bounds__(PA_NT, (PaShape<T, DK, DV>::GROUPS)) void paged_att
       }
 #pragma unroll
       for (int j = 0; j < NK; ++j) {
-        p[j] = pa_exp2(p[j] - from);
+        p[j] = Elem<T>::WEIGHT * pa_exp2(p[j] - from);
         sum += p[j];
       }
       if constexpr (sizeof(T) == 4) {
