@@ -28,6 +28,8 @@
 
 namespace {
 
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+
 // ---- sorted lists over a wave -----------------------------------------------------------
 __device__ __forceinline__ int bs_lane() { return threadIdx.x & (MG_WAVE - 1); }
 
@@ -239,14 +241,15 @@ __global__ __launch_bounds__(BS_NT, 4) void beam_rows(BsArgs a) {
   const int64_t b = row / a.K;
   const int k = (int)(row - b * a.K);
   const T* const x = (const T*)a.logits + b * a.sb + k * a.sk;
-  // Vectors start at the 16-byte line that holds the row's first element: what lies before it
-  // in that line, and behind the row's end in the last, is in the same page and not used.
-  const int skew = (int)(((uintptr_t)x & 15) / sizeof(T));
+  // Vectors start at the row's first element, wherever that lies: who adds which elements, in which
+  // order, then goes by their places in the row alone, so that equal rows have equal sums and their
+  // candidates tie.  The last vector ends with the row; what it shares with the one before is that one's.
   // (By subtraction: of an integer, the compiler would not know that it points to global memory,
   // and its loads would be waited for wherever LDS is.)
-  const uint4* const lines = (const uint4*)(x - skew);
-  const int all = a.V + skew;  // elements from the first line on
-  const int begin = part * a.per, stop = all - begin < a.per ? all : begin + a.per;
+  const int last = a.V < N ? 0 : a.V - N;
+  // A row of less than a vector is read by elements; loads stay in the 16-byte line of its first.
+  const T* const vectors = a.V < N ? x - (int)(((uintptr_t)x & 15) / sizeof(T)) : x;
+  const int begin = part * a.per, stop = a.V - begin < a.per ? a.V : begin + a.per;
 
   Best<Key32> list;
   list.start(a.W);
@@ -254,12 +257,12 @@ __global__ __launch_bounds__(BS_NT, 4) void beam_rows(BsArgs a) {
   // has a sum of 0.
   float top = -3.402823466e38f, sum = 0.f;
   // A tile ahead; the first is on its way before it is known whether the row counts.
-  uint4 raw[VECTORS];
+  u32x4 raw[VECTORS];
   auto load = [&](int at) {
 #pragma unroll
     for (int i = 0; i < VECTORS; ++i) {
       const int e = at + (i * MG_WAVE + lane) * N;
-      raw[i] = lines[(e < stop ? e : begin) / N];
+      raw[i] = *(const u32x4_any*)(vectors + (e < last ? e : last));
     }
   };
   int kept = 0;
@@ -269,7 +272,7 @@ __global__ __launch_bounds__(BS_NT, 4) void beam_rows(BsArgs a) {
   for (int at = begin; at < stop; at += TILE) {
     float v[ALL];
     float peak = -__builtin_inff();
-    const bool whole = at >= skew && at + TILE <= stop;
+    const bool whole = at + TILE <= stop;
 #pragma unroll
     for (int i = 0; i < VECTORS; ++i) {
       const T* p = (const T*)&raw[i];
@@ -277,11 +280,18 @@ __global__ __launch_bounds__(BS_NT, 4) void beam_rows(BsArgs a) {
       for (int j = 0; j < N; ++j) v[i * N + j] = pg_float(p[j]);
     }
     load(at + TILE < stop ? at + TILE : begin);
-    if (!whole) {  // what is not in the row adds nothing
+    unsigned there = ~0u;
+    if (!whole) {  // what is not in the row, or is there twice, adds nothing
+      if (a.V < N) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = pg_float(x[j < a.V ? j : 0]);
+      }
 #pragma unroll
       for (int i = 0; i < ALL; ++i) {
-        const int e = at + ((i / N) * MG_WAVE + lane) * N + i % N;
-        v[i] = e >= skew && e < stop ? v[i] : -__builtin_inff();
+        const int from = at + ((i / N) * MG_WAVE + lane) * N;
+        const int e = (from < last ? from : last) + i % N;
+        if (e >= from && e < stop) continue;
+        v[i] = -__builtin_inff(), there &= ~(1u << i);
       }
     }
     float peaks[VECTORS];
@@ -327,10 +337,11 @@ __global__ __launch_bounds__(BS_NT, 4) void beam_rows(BsArgs a) {
 #pragma unroll
       for (int i = g * N; i < g * N + N; ++i) bits |= v[i] >= bar ? 1u << i : 0u;
     }
+    bits &= there;
     for (unsigned long long who; (who = __ballot(bits != 0)) != 0; bits &= bits - 1) {
       const int i = __ffs(bits) - 1, to = hits + bs_before(who);
-      if (bits != 0 && to < BS_HITS)
-        s_place[wave][to] = at + (i / N * MG_WAVE + lane) * N + i % N;
+      const int from = at + (i / N * MG_WAVE + lane) * N;
+      if (bits != 0 && to < BS_HITS) s_place[wave][to] = (from < last ? from : last) + i % N;
       hits += __popcll(who);
     }
     // They are offered when there are many, or no more to come.  Where a tile has more than there
@@ -345,9 +356,9 @@ __global__ __launch_bounds__(BS_NT, 4) void beam_rows(BsArgs a) {
       const bool from = n < chunks;
       const int i = n * MG_WAVE + lane;
       const int e = from ? s_place[wave][i < ready ? i : 0] : at + i - chunks * MG_WAVE;
-      const bool in = (!from || i < ready) && e >= skew && e < stop;
-      const float value = pg_float(x[in ? e - skew : 0]);
-      list.offer(Key32{in ? ~(unsigned)(e - skew) : 0u, in ? bs_order(value) : 0u});
+      const bool in = from ? i < ready : e < stop;
+      const float value = pg_float(x[in ? e : 0]);
+      list.offer(Key32{in ? ~(unsigned)e : 0u, in ? bs_order(value) : 0u});
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -635,7 +646,7 @@ __global__ __launch_bounds__(BP_NT) void beam_pick(BsArgs a) {
 // 27.0.)
 int bs_parts(int64_t rows, int V, int tile) {
   const int64_t want = (2048 + rows - 1) / rows;
-  const int64_t most = ((int64_t)V + 8 + tile - 1) / tile;
+  const int64_t most = ((int64_t)V + tile - 1) / tile;
   return (int)(want < most ? want : most);
 }
 constexpr int BS_TILE = BS_EACH * MG_WAVE;
@@ -700,8 +711,6 @@ __device__ __forceinline__ void ro_copy(const RoTensor& t, const RoArgs& a, int6
     if (n < all) __builtin_nontemporal_store(v[i], (U*)(t.dst + n * (int64_t)sizeof(U)));
   }
 }
-
-typedef u32x4 u32x4_any __attribute__((aligned(1)));
 
 // The same with vectors that hold 16 bytes of the rows one after another, each of 16 or more (units:
 // bytes of a row).
@@ -806,9 +815,9 @@ int mg_beam_select(int dtype, const void* logits, const float* scores, const voi
   a.B = B, a.K = (int)K, a.V = (int)V, a.W = W, a.end = (int)end;
   const int tile = BS_TILE;
   a.parts = bs_parts(B * K, (int)V, tile);
-  const int64_t per = (V + 8 + a.parts - 1) / a.parts;
+  const int64_t per = (V + a.parts - 1) / a.parts;
   a.per = (int)((per + tile - 1) / tile * tile);
-  a.parts = (int)((V + 8 + a.per - 1) / a.per);
+  a.parts = (int)((V + a.per - 1) / a.per);
   a.by_lists = pg_divisor(K * a.parts), a.by_parts = pg_divisor(a.parts);
   a.keys = (unsigned long long*)ws;
   a.stats = (float2*)(a.keys + B * K * a.parts * W);

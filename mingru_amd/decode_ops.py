@@ -310,7 +310,9 @@ def beam_select(logits, scores, width=None, *, end=None, finished=None):
     ``scores`` (B, width) in 32 bits (64 for float64 inputs), falling; ``parents`` and
     ``tokens`` (B, width) in int64; and, with ``end``, ``finished`` (B, width): whether the
     candidate's parent had ended or its token is ``end``.  Candidates are ranked by their scores
-    in 64 bits, equal ones by the lower beam, then by the lower token.  All candidates of a beam
+    in 64 bits, equal ones by the lower beam, then by the lower token.  On the GPU a beam's sum of
+    exponentials is in 32 bits, some 2^-24 of it off and the same for beams of equal logits:
+    candidates of other beams whose scores are that close may change places.  All candidates of a beam
     whose score or whose logits' sum is not finite (a NaN or ``inf`` among the logits, or only
     ``-inf``) have the score ``-inf``.
     """
