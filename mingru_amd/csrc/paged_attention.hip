@@ -334,8 +334,9 @@ __global__ __launch_bounds__(PA_NT, (PaShape<T, DK, DV>::GROUPS)) void paged_att
     unsigned long long empty = __ballot(b < a.B && a.lengths[b < a.B ? b : b0] <= 0);
     for (; empty != 0; empty &= empty - 1) {
       const int64_t at = b0 + (int64_t)gridDim.x * (wave * MG_WAVE + __ffsll(empty) - 1);
-      T* const dst = (T*)a.o + at * a.H * (int64_t)a.dv;
-      for (int x = lane; x < a.H * a.dv; x += MG_WAVE) dst[x] = pg_round<T>(0.f);
+      const int64_t n = a.H * (int64_t)a.dv;
+      T* const dst = (T*)a.o + at * n;
+      for (int64_t x = lane; x < n; x += MG_WAVE) dst[x] = pg_round<T>(0.f);
     }
   }
 
