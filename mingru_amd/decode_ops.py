@@ -121,8 +121,8 @@ def paged_cache_append(k, v, k_cache, v_cache, pages, start, *, q=None, lengths=
     Returns
     -------
     The rotated ``q``, or ``None`` without one.  A token that lies behind its row of ``pages``,
-    or whose page is not in the cache, raises ``IndexError`` on the CPU; on the GPU, where
-    looking would wait for it, it is not kept and its queries are NaN.
+    or whose page is not in the cache, raises ``IndexError`` in the eager body, on either device;
+    with the kernels, where looking would wait for the GPU, it is not kept and its queries are NaN.
     """
     what = "paged_cache_append"
     _check_one_type(what, k=k, v=v, k_cache=k_cache, v_cache=v_cache, q=q)
@@ -152,7 +152,7 @@ def paged_cache_append(k, v, k_cache, v_cache, pages, start, *, q=None, lengths=
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if 0 in t.stride() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
             raise ValueError(f"{what}: {name} is written, so it must not be an expanded view")
-    if B * T and N and pages.shape[1]:
+    if B * T:
         done = _dispatch(what, k.is_cuda, lambda backend: backend.paged_cache_append_impl(
             k, v, k_cache, v_cache, pages, start, q, lengths, frequencies, interleaved),
             "hip_decode")
@@ -219,8 +219,8 @@ def paged_attention_step(q, k_cache, v_cache, pages, lengths, *, scale=None, win
     Returns
     -------
     ``o`` (B, H, dv) in ``q``'s type.  A length beyond M pages, or a page that is not in the
-    cache, raises ``IndexError`` on the CPU; on the GPU, where looking would wait for it, that
-    sequence's ``o`` is NaN.
+    cache, raises ``IndexError`` in the eager body, on either device; with the kernels, where
+    looking would wait for the GPU, that sequence's ``o`` is NaN.
     """
     what = "paged_attention_step"
     _check_one_type(what, q=q, k_cache=k_cache, v_cache=v_cache)
@@ -239,7 +239,7 @@ def paged_attention_step(q, k_cache, v_cache, pages, lengths, *, scale=None, win
         raise ValueError(f"{what}: window is a whole number of at least 1 (got {window!r})")
     window = None if window is None else int(window)
     scale = dk**-0.5 if scale is None else float(scale)
-    if B and N and pages.shape[1]:
+    if B:
         out = _dispatch(what, q.is_cuda, lambda backend: backend.paged_attention_step_impl(
             q, k_cache, v_cache, pages, lengths, scale, window), "hip_decode")
         if out is not None:
@@ -415,8 +415,8 @@ def reorder_states(states, parents):
     Returns
     -------
     The same structure of new tensors (B W, ...): row ``b W + w`` is row ``b K + parents[b, w]``.
-    A parent outside of 0 to K - 1 raises ``IndexError`` on the CPU; on the GPU, where looking
-    would wait for it, that row is 0.
+    A parent outside of 0 to K - 1 raises ``IndexError`` in the eager body, on either device; with
+    the kernels, where looking would wait for the GPU, that row is 0.
     """
     what = "reorder_states"
     if not torch.is_tensor(parents):

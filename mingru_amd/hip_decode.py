@@ -68,6 +68,13 @@ def paged_cache_append_impl(k, v, k_cache, v_cache, pages, start, q, lengths, fr
     tag = _tag(what, k)
     (B, T, Hk, dk), (N, _, P, dv) = k.shape, v_cache.shape
     _cache(what, "k_cache", k_cache), _cache(what, "v_cache", v_cache)
+    if not (N and pages.shape[1]):
+        # No token has a place: every page from 0 on is 1 of a cache of one, which nothing is written to.
+        if q is None:
+            return (None,)
+        k_cache, v_cache = (c.new_empty(1, *c.shape[1:]) for c in (k_cache, v_cache))
+        N, pages = 1, (torch.where(pages.long() < 0, -1, 1) if pages.shape[1]
+                       else pages.new_ones(B, 1, dtype=torch.int64))
     H = 0 if q is None else q.shape[2]
     n = 0 if frequencies is None else frequencies.shape[0]
     if N >= 2**31 or P >= 2**31 or Hk * (dk + dv) + H * dk >= 2**26 or n > 1024:
@@ -103,6 +110,9 @@ def paged_attention_step_impl(q, k_cache, v_cache, pages, lengths, scale, window
     tag = _tag(what, q)
     (B, H, dk), (N, Hk, P, dv) = q.shape, v_cache.shape
     M = pages.shape[1]
+    if not (N and M):  # no token has a place
+        lost = torch.where(lengths.long() > 0, torch.nan, 0.0).to(q.dtype)
+        return lost[:, None, None].expand(B, H, dv).contiguous()
     _cache(what, "k_cache", k_cache), _cache(what, "v_cache", v_cache)
     nbytes = _size("mg_paged_attention_workspace_bytes", tag, B, H, Hk, dk, dv, M, P)
     if not nbytes or N >= 2**31:
