@@ -438,7 +438,7 @@ def reorder_states(states, parents):
             raise ValueError(f"{what}: each state has B K rows, the same for all, with B = {B} (got "
                              f"{tuple(t.shape)})")
     K = rows // B if B else 0
-    if B * W and K:
+    if B * W:
         out = _dispatch(what, parents.is_cuda, lambda backend: backend.reorder_states_impl(
             tensors, parents, K), "hip_decode")
         if out is not None:

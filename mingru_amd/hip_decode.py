@@ -174,6 +174,8 @@ def reorder_states_impl(tensors, parents, K):
     if getattr(forward_ad, "_current_level", 0) >= 0:
         _no_tangents(what, *[t for t in tensors if t.dtype.is_floating_point])
     B, W = parents.shape
+    if K == 0:  # no parent is one of them
+        return [t.new_zeros(B * W, *t.shape[1:]) for t in tensors]
     if B * W >= 2**31 or K >= 2**31:
         raise ScanFallback(f"{what} kernels write fewer than 2^31 rows (got {B} x {W})")
     if parents.dtype not in (torch.int32, torch.int64):
