@@ -17,10 +17,11 @@
 //   it loaded, so neither moves between lanes: the product's rows are the elements E c + e of
 //   all chunks c at one e (E elements a chunk), a fragment of them is a lane's element e of
 //   each of its tokens.
-// * Half types' probabilities are two summands of their type, so that their rounding is 2^-16
-//   (bf16) or 2^-22 (fp16) of them: one's is as large as the result's own.  In fp16, which has nothing
-//   below 2^-24, they and their sum are 2^15 times as large: weights down to 2^-40 of the largest
-//   count in the products as they do in the sum.
+// * Half types' probabilities are summands of their type, three in bf16 and two in fp16, so that the
+//   rounding is 2^-24 or 2^-22 of them: one's is as large as the result's own, and two in bf16 (2^-16)
+//   show where values cancel.  (524287 tokens of 8 key heads in bf16: 368 us, with two 366.)  In fp16,
+//   which has nothing below 2^-24, they and their sum are 2^15 times as large: weights down to 2^-40 of
+//   the largest count in the products as they do in the sum.
 // Maxima, sums and O are fp32, with O scaled again only where a maximum rises.
 //
 // Work is divided on the device, where the lengths are: the steps (four tiles, one for each wave
@@ -65,6 +66,7 @@ template <>
 struct Elem<Bf16> {
   static constexpr int KEYS = 32, PAD = 8;
   static constexpr float WEIGHT = 1.f;
+  static constexpr int PLANES = 3;
   typedef bf16x8 Frag;
   static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
@@ -77,6 +79,7 @@ template <>
 struct Elem<Fp16> {
   static constexpr int KEYS = 32, PAD = 8;
   static constexpr float WEIGHT = 32768.f;  // of a score that is the maximum
+  static constexpr int PLANES = 2;
   typedef f16x8 Frag;
   static __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
@@ -558,11 +561,14 @@ __global__ __launch_bounds__(PA_NT, (PaShape<T, DK, DV>::GROUPS)) void paged_att
             o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[j].w[e]), p[j], o[e], 0,
                                                         0, 0);
       } else {
-        u32x4 hi, lo;
+        u32x4 plane[Elem<T>::PLANES];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          hi[j] = pg_pack<T>(p[2 * j], p[2 * j + 1]);
-          lo[j] = pg_pack<T>(p[2 * j] - Elem<T>::low(hi[j]), p[2 * j + 1] - Elem<T>::high(hi[j]));
+        for (int n = 0; n < Elem<T>::PLANES; ++n) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            plane[n][j] = pg_pack<T>(p[2 * j], p[2 * j + 1]);
+            p[2 * j] -= Elem<T>::low(plane[n][j]), p[2 * j + 1] -= Elem<T>::high(plane[n][j]);
+          }
         }
 #pragma unroll
         for (int e = 0; e < EV; ++e) {
@@ -571,8 +577,8 @@ __global__ __launch_bounds__(PA_NT, (PaShape<T, DK, DV>::GROUPS)) void paged_att
           for (int j = 0; j < 4; ++j)  // element e of tokens 2 j and 2 j + 1
             vf[j] = __builtin_amdgcn_perm(vr[2 * j + 1].w[e / 2], vr[2 * j].w[e / 2],
                                           e & 1 ? 0x07060302u : 0x05040100u);
-          o[e] = Elem<T>::mma(vf, hi, o[e]);
-          o[e] = Elem<T>::mma(vf, lo, o[e]);
+#pragma unroll
+          for (int n = 0; n < Elem<T>::PLANES; ++n) o[e] = Elem<T>::mma(vf, plane[n], o[e]);
         }
       }
     }
