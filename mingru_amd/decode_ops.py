@@ -18,6 +18,8 @@ of one token that is all but the newest, so such beams follow their parents by
 
 from __future__ import annotations
 
+import copy
+
 import torch
 
 from .sequence_ops import _check_floats, _dispatch, _wide
@@ -393,12 +395,23 @@ def _rebuilt(states, new):
     if torch.is_tensor(states):
         return next(new)
     if isinstance(states, dict):
-        return {k: _rebuilt(s, new) for k, s in states.items()}
+        each = {k: _rebuilt(s, new) for k, s in states.items()}
+        if type(states) is dict:
+            return each
+        out = copy.copy(states)  # a class of the caller's, with whatever else it holds
+        for k, s in each.items():
+            out[k] = s
+        return out
     if isinstance(states, (list, tuple)):
         each = [next(new) if isinstance(s, torch.Tensor) else _rebuilt(s, new) for s in states]
-        if hasattr(states, "_fields"):
-            return type(states)(*each)
-        return each if isinstance(states, list) else tuple(each)
+        kind = type(states)
+        if kind is list:
+            return each
+        if isinstance(states, list):
+            out = copy.copy(states)
+            out[:] = each
+            return out
+        return kind(*each) if hasattr(states, "_fields") else kind(each)
     return None
 
 
@@ -414,7 +427,7 @@ def reorder_states(states, parents):
 
     Returns
     -------
-    The same structure of new tensors (B W, ...): row ``b W + w`` is row ``b K + parents[b, w]``.
+    The same structure, of the same classes, of new tensors (B W, ...): row ``b W + w`` is row ``b K + parents[b, w]``.
     A parent outside of 0 to K - 1 raises ``IndexError`` in the eager body, on either device; with
     the kernels, where looking would wait for the GPU, that row is 0.
     """
