@@ -102,6 +102,7 @@ def paged_cache_append(k, v, k_cache, v_cache, pages, start, *, q=None, lengths=
     elements ``x_i`` and ``x_{i+n}`` (n frequencies; ``x_{2i}`` and ``x_{2i+1}`` if
     ``interleaved``) of each key and query become ``x_i cos(p f_i) - x_{i+n} sin(p f_i)`` and
     ``x_{i+n} cos(p f_i) + x_i sin(p f_i)``; angles are in 64 bits.  Elements from 2n on stay.
+    Nothing of it has gradients: not the queries, nor what lies in the caches.
 
     Parameters
     ----------
@@ -197,8 +198,9 @@ def paged_attention_step(q, k_cache, v_cache, pages, lengths, *, scale=None, win
     """Attention of each sequence's newest token over its paged cache.
 
     ``o = sum_j w_j v_j`` with ``w`` the softmax of ``scale * (q . k_j)`` over the sequence's
-    last ``window`` tokens (all without one), for each head.  On the GPU the kernels take head
-    sizes up to 256; larger ones run the eager body, with the warning of a decline.
+    last ``window`` tokens (all without one), for each head; without gradients.  On the GPU the
+    kernels take head sizes up to 256; larger ones run the eager body, with the warning of a
+    decline.
 
     Parameters
     ----------
@@ -290,7 +292,7 @@ def beam_select(logits, scores, width=None, *, end=None, finished=None):
     """A beam search's choice of the best continuations over beams and vocabulary.
 
     The candidate that goes on from beam ``k`` by token ``v`` has the score
-    ``scores[b, k] + logits[b, k, v] - log(sum(exp(logits[b, k])))``.
+    ``scores[b, k] + logits[b, k, v] - log(sum(exp(logits[b, k])))``, without gradients.
 
     Parameters
     ----------
@@ -416,7 +418,7 @@ def _rebuilt(states, new):
 
 
 def reorder_states(states, parents):
-    """Every state's rows in the order of the chosen beams.
+    """Every state's rows in the order of the chosen beams, without gradients.
 
     Parameters
     ----------
