@@ -277,10 +277,11 @@ def _eager_attention(q, k_cache, v_cache, pages, lengths, scale, window):
             for c in (k_cache, v_cache))
     k, v = (_wide(c).transpose(1, 2) for c in (k, v))
     qw = _wide(q).view(B, Hk, H // Hk, dk) * scale
-    scores = (qw @ k.transpose(-1, -2)).masked_fill(~live[:, None, None], -torch.inf)
-    w = torch.softmax(scores, -1)
-    w = w.masked_fill((lengths == 0)[:, None, None, None], 0)
-    return (w @ v).reshape(B, H, dv).to(q.dtype)
+    with torch.autocast(q.device.type, enabled=False):  # it would round both products' operands
+        scores = (qw @ k.transpose(-1, -2)).masked_fill(~live[:, None, None], -torch.inf)
+        w = torch.softmax(scores, -1)
+        w = w.masked_fill((lengths == 0)[:, None, None, None], 0)
+        return (w @ v).reshape(B, H, dv).to(q.dtype)
 
 
 # ---------------------------------------------------------------------------
