@@ -16,7 +16,7 @@
 // Keys are whole numbers that order as (value, lower index first), no two alike: the result
 // does not depend on the order of arrival, and ties fall as they are defined.
 //
-// 64 x 8 rows of 50257 in bf16, a fifth of them not read: 17 us for 41 MB and 6 for the selection.
+// 64 x 8 rows of 50257 in bf16, a fifth of them not read: 18 us for 41 MB and 6 for the selection.
 // Of a wave's 12 us 1.5 are its first load, 1 the first bar's sort, 7 six tiles (a tile's exponentials
 // and comparisons keep the vector units busy most of 1.1), 2 one or two sorts of what reached the bar.
 //
@@ -395,7 +395,7 @@ __device__ __forceinline__ double bs_row_sum(double x) {  // over 16 lanes
 // where all lists have fallen behind the steps that hold the W best; a second one puts those within
 // reach, W and few more, into LDS, where each one's place is the number of those above it.  No chain
 // is long: sorted lists over the waves' lanes, as for the rows, took 15 us of 31 for 16 searches of 16
-// beams of 32771, 32 wide, where this takes 10 of 25; one search of 256 beams of 50257, 64 wide, took
+// beams of 32771, 32 wide, where this takes 10 of 24; one search of 256 beams of 50257, 64 wide, took
 // 151 us with both launches in place of 63.
 // Eight waves and two candidates a thread: sixteen and four take 0.3 us less for the former,
 // but 13.1 in place of 10.8 for 4 beams of 50257, 4 wide.
@@ -641,9 +641,9 @@ __global__ __launch_bounds__(BP_NT) void beam_pick(BsArgs a) {
 }
 
 // Waves of a row: two for each of the chip's 1024 vector units over all rows, none with less than
-// a tile.  (64 x 8 rows of 50257 in bf16, both launches in a graph: 24.0 us; four for each 24.2, one
-// 27.4.  16 x 16 of 32771 in fp32, 32 wide: 26.0, four, with more first tiles and candidates, 30.5, one
-// 27.0.)
+// a tile.  (64 x 8 rows of 50257 in bf16, both launches in a graph: 23.4 us; four for each 24.4, one
+// 25.5.  16 x 16 of 32771 in fp32, 32 wide: 24.2, four, with more first tiles and candidates, 25.2, one
+// 24.8.)
 int bs_parts(int64_t rows, int V, int tile) {
   const int64_t want = (2048 + rows - 1) / rows;
   const int64_t most = ((int64_t)V + tile - 1) / tile;

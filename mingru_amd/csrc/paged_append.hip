@@ -11,9 +11,9 @@
 // for each (which took more of the vector units' time than the memory's).
 //
 // Angles are products in fp64, reduced to an eighth of a turn at most there: at position 2^20 a
-// product in fp32 is off by 2^-4 radians.  Sines and cosines of the rest are fp32.
+// product in fp32 is off by 2^-4 radians, one in fp64 by 2^-33.  Sines and cosines of the rest are fp32.
 //
-// 16 x 2048 ragged tokens of 16 and 8 heads of 128 in bf16: 66 us, 5.2 TB/s with the padding's zeros.
+// 16 x 2048 ragged tokens of 16 and 8 heads of 128 in bf16: 67 us, 5.2 TB/s with the padding's zeros.
 #include "mg_paged.h"
 
 namespace {
@@ -71,7 +71,7 @@ __device__ __forceinline__ void ap_set(ApVec<T, VE>& v, const float (&f)[VE]) {
   }
 }
 
-// Past the caches: 96 us with ordinary stores in place of 82 at 16 x 2048 tokens.
+// Past the caches: 75 us with ordinary stores in place of 67 at 16 x 2048 tokens.
 template <typename T, int VE>
 __device__ __forceinline__ void ap_store(T* to, const ApVec<T, VE>& v) {
   if constexpr (sizeof(v) == 16)
@@ -225,7 +225,7 @@ int ap_run(ApArgs& a, int64_t B, hipStream_t stream) {
   a.qn = a.H * a.ku, a.kn = a.Hk * a.ku, a.all = a.qn + a.kn + a.Hk * a.vu;
   a.abreast = a.all < AP_NT ? AP_NT / a.all : 1;
   // Tokens of a workgroup: as many as leave the chip's 256 CUs 32 workgroups each, and as many
-  // angles as LDS holds.  (16 x 2048 ragged tokens of 16 and 8 heads of 128 in bf16: 66 us, with 64
+  // angles as LDS holds.  (16 x 2048 ragged tokens of 16 and 8 heads of 128 in bf16: 67 us, with 64
   // workgroups each 72, with 8 82.)
   int64_t n = a.abreast * ((B * a.T) / (8192 * (int64_t)a.abreast));
   if (n < a.abreast) n = a.abreast;

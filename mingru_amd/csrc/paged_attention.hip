@@ -3,10 +3,10 @@
 //   s_j = scale q . k_j;  o = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s)
 // over a sequence's last tokens, for each head; the heads of a group share a key head.
 //
-// Bound by memory: every key and value is read once (by each 16 queries of a larger group).  The unit of work is a tile of 32 tokens
-// (16 in fp32) of one key head, held by one wave, for 16 query heads of the group on the matrix
-// cores: rows beyond the group are idle there, but at 16 rows a bf16 tile of 16 KB costs about
-// 260 cycles of matrix instructions, where its share of the memory's rate is 2000.
+// Bound by memory: every key and value is read once (by each 16 queries of a larger group).  The unit of
+// work is a tile of 32 tokens (16 in fp32) of one key head, held by one wave, for 16 query heads of the
+// group on the matrix cores: rows beyond the group are idle there, but at 16 rows a bf16 tile of 16 KB
+// costs a SIMD some 350 cycles of matrix instructions, where its share of the memory's rate is 7000.
 //
 // Sums as the matrix cores take them (lane = 16 g + c, g < 4):
 // * A lane loads its tile's tokens 4 g + j (and 16 + 4 g + j), 1/16 of a row (chunk c) of each, so
@@ -32,8 +32,9 @@
 // A share's loads run on over the ends of its pieces: the next step's keys and values, and the pages
 // of the one after it, are on their way whichever piece they are of.
 //
-// bf16, heads of 128, 4 queries a key head: 64 sequences of up to 8192 tokens (501 MB) 97 us, 5.2 TB/s,
-// and 5 for the join; 524287 tokens of 8 key heads (2.1 GB) 359 us, 6.0 TB/s.  A copy reaches 5.13.
+// bf16, heads of 128, 4 queries a key head: 64 sequences of up to 8192 tokens (501 MB) 97 to 104 us, 5 TB/s,
+// and 5 for the join; 524287 tokens of 8 key heads, 2 queries each (2.1 GB), 358 to 370 us, 5.9 TB/s.  A
+// copy reaches 5.13.
 #include "mg_paged.h"
 
 namespace {
